@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define MDMM_ABI_VERSION 33
+#define MDMM_ABI_VERSION 34
 #define MDMM_MAX_EXPERTS 8 /* observation / filter experts fused per step (dmm.py:387-395) */
 #define MDMM_MAX_PASSES 8  /* ELBO passes swept together: 1 multimodal + M unimodal (dgts.py:119-129) */
 
@@ -36,7 +36,7 @@ extern "C" {
 int mdmm_version(void);
 const char* mdmm_strerror(int code);
 /* sizeof() of an argument struct as the library was compiled, for a binding to check its own
- * declaration against at load time: 0 gtf, 1 expert, 2 sweep, 4 gru, 5 dks, 6 mlp, 7 bn, ... 15 convf; 0 if unknown */
+ * declaration against at load time: 0 gtf, 1 expert, 2 sweep, 4 gru, 5 dks, 6 mlp, 7 bn, ... 15 convf, 16 audio, 17 gated_scan, 18 block_norm, 19 ortho; 0 if unknown */
 size_t mdmm_sizeof(int which);
 /* round n up to the padded width the packed weights use (multiple of 4) */
 int mdmm_pad(int n);
@@ -1062,6 +1062,120 @@ int mdmm_cat_head_nll_fwd(const float* hid, const float* w, const float* bias, c
 int mdmm_cat_head_nll_bwd(const float* hid, const float* w, const float* label, const float* seq_mask, int64_t rows,
                           int64_t label_rows, int H, int n_cat, float scale, const float* scale_dev, int passes,
                           const float* pass_weight, const float* probs, float* g_hid, float* slab, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Gated linear recurrence over time (ABI 34), the recurrence of an inference RNN without a recurrent product: per channel
+ *   h_t = a_t h_{t-1} + (1 - a_t) c_t,   a_t = sigmoid(f_t);   mask[t][b] = 0: h_t = h_{t-1} (f, c of that step not used)
+ * as the skip updates of the GRU above (dks.py:224-227).  gates (T, B, >= 2H): f in columns [0, H), c in [H, 2H), unit
+ * stride along the columns, any strides over t and b (elements); fp32, or bf16 with gates_bf16.  h (T, B, H) contiguous,
+ * time-indexed, fp32 or (with gates_bf16 only) bf16 with h_bf16.  The state is fp32 throughout.  reverse: from the last
+ * step to the first.  h0: row b at b * h0_sb (0: one row for all; NULL: zeros).  h_last (B, H): the state behind the last
+ * step taken (NULL: not wanted).
+ * states: mdmm_gated_scan_states() floats the forward pass leaves for the backward one (NULL in a forward-only call).
+ * ws: mdmm_gated_scan_ws(a, bwd) floats of scratch per call (0: NULL is fine).
+ * backward: g_h (T, B, H) in h's type (NULL: none), g_last (B, H) fp32 (NULL: none); g_gates in the gates' type and
+ * column order with its own strides (every element of its 2H columns is written, 0 where the mask is 0); g_h0 (B, H) fp32
+ * per sequence (NULL: not wanted).  T, B or H of 0: nothing is launched.
+ * --------------------------------------------------------------------------------- */
+typedef struct mdmm_gated_scan {
+  int32_t T, B, H, reverse, gates_bf16, h_bf16;
+  const void* gates;
+  int64_t gates_st, gates_sb;
+  const float* h0;
+  int64_t h0_sb;
+  const uint8_t* mask;
+  int64_t mask_st, mask_sb;
+  void* h;
+  float* h_last;
+  float* states;
+  float* ws;
+  const void* g_h;
+  const float* g_last;
+  void* g_gates;
+  int64_t g_gates_st, g_gates_sb;
+  float* g_h0;
+} mdmm_gated_scan_t;
+int64_t mdmm_gated_scan_states(const mdmm_gated_scan_t* a);
+int64_t mdmm_gated_scan_ws(const mdmm_gated_scan_t* a, int bwd);
+int mdmm_gated_scan_fwd(const mdmm_gated_scan_t* a, void* stream);
+int mdmm_gated_scan_bwd(const mdmm_gated_scan_t* a, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * The norms before and after a residual block with the block's gate and residual scale, one pass each way (ABI 34):
+ *   out = res + scale . silu(gate) . (y rsqrt(mean(y^2) + eps) w)       [gate, scale: NULL = 1]
+ *   n   = out rsqrt(mean(out^2) + eps) w_next                           [w_next NULL: not formed]
+ * y NULL: out = res is not stored and n is the plain norm of res.  Rows of H <= MDMM_NORM_MAX_H columns, each tensor with
+ * its own row stride (elements), unit column stride; out, n and the gradients' strides too.  y, the branch (gate, n) and
+ * res / out are each fp32 or bf16 (y_bf16, branch_bf16, res_bf16); vectors and row statistics fp32.
+ * Supported type combinations (y, branch, res): all fp32; all bf16; bf16, bf16, fp32; fp32, bf16, fp32; fp32, bf16, bf16.
+ * backward: g_out in res's type, g_n in n's (either may be NULL: none) -> d_y, d_gate, d_res (NULL: not wanted) and the
+ * column sums d_w, d_scale, d_w_next (H each; NULL: not wanted) through ws of mdmm_block_norm_ws() floats.
+ * --------------------------------------------------------------------------------- */
+#define MDMM_NORM_MAX_H 8192
+typedef struct mdmm_block_norm {
+  int64_t rows;
+  int32_t H, y_bf16, branch_bf16, res_bf16;
+  float eps;
+  int32_t reserved;
+  const void* y;
+  const void* gate;
+  const void* res;
+  int64_t y_st, gate_st, res_st;
+  const float* w;
+  const float* scale;
+  const float* w_next;
+  void* out;
+  void* n;
+  int64_t out_st, n_st;
+  const void* g_out;
+  const void* g_n;
+  int64_t g_out_st, g_n_st;
+  void* d_y;
+  void* d_gate;
+  void* d_res;
+  int64_t d_y_st, d_gate_st, d_res_st;
+  float* d_w;
+  float* d_scale;
+  float* d_w_next;
+  float* ws;
+} mdmm_block_norm_t;
+int64_t mdmm_block_norm_ws(const mdmm_block_norm_t* a);
+int mdmm_block_norm_fwd(const mdmm_block_norm_t* a, void* stream);
+int mdmm_block_norm_bwd(const mdmm_block_norm_t* a, void* stream);
+/* One time step of the recurrence and its block norm in one launch (T = 1, no gradient): the state of `scan` from h0 to
+ * h_last, h itself not stored; gates and gate come from one row [f | c | g] (norm->gate NULL: no gate), norm->y is not
+ * read.  H <= MDMM_NORM_MAX_H.  */
+int mdmm_gated_block_step(const mdmm_gated_scan_t* scan, const mdmm_block_norm_t* norm, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Orthogonalised updates of weight matrices (ABI 34): for each of n matrices, X = M / (|M|_F + eps) laid down (no more
+ * rows than columns), then `steps` times X <- ca X + (cb A + cc A^2) X with A = X X^T, all in fp32, and
+ *   dst = X                                  (update 0)
+ *   dst = (1 - lr decay) dst - lr gain X     (update 1: one optimizer step on the fp32 parameter dst; lr = *lr_dev, or
+ *                                             the argument where lr_dev is NULL)
+ * M = src (rows, cols) with row stride src_ld, fp32 or bf16 (src_bf16); with mom (contiguous fp32 rows x cols): first
+ * mom = momentum mom + src, then M = mom, or src + momentum mom with nesterov.  No two matrices' mom or dst overlap.  dst has src's shape, its own row stride,
+ * and type (dst_bf16, update 0 only).  ws: mdmm_ortho_ws() bytes, 256-byte aligned.
+ * --------------------------------------------------------------------------------- */
+#define MDMM_ORTHO_MAX 24
+typedef struct mdmm_ortho_item {
+  const void* src;
+  float* mom;
+  void* dst;
+  int64_t src_ld, dst_ld;
+  int32_t rows, cols;
+  float gain;
+  int32_t reserved;
+} mdmm_ortho_item_t;
+typedef struct mdmm_ortho {
+  int32_t n, steps, src_bf16, dst_bf16, nesterov, update;
+  float eps, ca, cb, cc, momentum, decay, lr, reserved;
+  const float* lr_dev;
+  void* ws;
+  mdmm_ortho_item_t item[MDMM_ORTHO_MAX];
+} mdmm_ortho_t;
+int64_t mdmm_ortho_ws(const mdmm_ortho_t* a);
+int mdmm_ortho(const mdmm_ortho_t* a, void* stream);
 
 #ifdef __cplusplus
 }

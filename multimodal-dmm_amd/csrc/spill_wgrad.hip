@@ -142,6 +142,9 @@ extern "C" size_t mdmm_sizeof(int which) {
     case 14: return sizeof(mdmm_spill_wgrad_batch_t);
     case 15: return sizeof(mdmm_convf_t);
     case 16: return sizeof(mdmm_audio_t);
+    case 17: return sizeof(mdmm_gated_scan_t);
+    case 18: return sizeof(mdmm_block_norm_t);
+    case 19: return sizeof(mdmm_ortho_t);
     default: return 0;
   }
 }

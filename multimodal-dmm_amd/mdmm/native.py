@@ -12,7 +12,7 @@ LIB_PATH = os.environ.get('MDMM_LIB') or os.path.join(_HERE, 'lib', 'libmdmm_hip
 
 MAX_EXPERTS = 8
 MAX_PASSES = 8
-ABI_VERSION = 33
+ABI_VERSION = 34
 PREC_F32, PREC_BF16 = 0, 1
 
 SYMBOLS = [
@@ -47,6 +47,9 @@ SYMBOLS = [
     'mdmm_collate_pad', 'mdmm_delete_steps', 'mdmm_decollate_pack', 'mdmm_sqerr_steps', 'mdmm_time_avg', 'mdmm_time_acc',
     'mdmm_ssim_ws_floats', 'mdmm_ssim',
     'mdmm_cat_head_supported', 'mdmm_cat_head_slabs', 'mdmm_cat_head_nll_fwd', 'mdmm_cat_head_nll_bwd',
+    'mdmm_gated_scan_states', 'mdmm_gated_scan_ws', 'mdmm_gated_scan_fwd', 'mdmm_gated_scan_bwd',
+    'mdmm_block_norm_ws', 'mdmm_block_norm_fwd', 'mdmm_block_norm_bwd', 'mdmm_gated_block_step',
+    'mdmm_ortho_ws', 'mdmm_ortho',
 ]
 
 _P = C.c_void_p
@@ -250,6 +253,42 @@ class Gemm(C.Structure):
                  ('ldc', C.c_int64), ('ws', _P), ('colsum_a', _P)])
 
 
+class GatedScan(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ('T', 'B', 'H', 'reverse', 'gates_bf16', 'h_bf16')] +
+                [('gates', _P), ('gates_st', C.c_int64), ('gates_sb', C.c_int64), ('h0', _P), ('h0_sb', C.c_int64),
+                 ('mask', _P), ('mask_st', C.c_int64), ('mask_sb', C.c_int64)] +
+                [(n, _P) for n in ('h', 'h_last', 'states', 'ws', 'g_h', 'g_last', 'g_gates')] +
+                [('g_gates_st', C.c_int64), ('g_gates_sb', C.c_int64), ('g_h0', _P)])
+
+
+NORM_MAX_H = 8192
+
+
+class BlockNorm(C.Structure):
+    _fields_ = ([('rows', C.c_int64)] + [(n, C.c_int32) for n in ('H', 'y_bf16', 'branch_bf16', 'res_bf16')] +
+                [('eps', C.c_float), ('reserved', C.c_int32)] + [(n, _P) for n in ('y', 'gate', 'res')] +
+                [(n, C.c_int64) for n in ('y_st', 'gate_st', 'res_st')] +
+                [(n, _P) for n in ('w', 'scale', 'w_next', 'out', 'n')] + [('out_st', C.c_int64), ('n_st', C.c_int64)] +
+                [('g_out', _P), ('g_n', _P), ('g_out_st', C.c_int64), ('g_n_st', C.c_int64)] +
+                [(n, _P) for n in ('d_y', 'd_gate', 'd_res')] +
+                [(n, C.c_int64) for n in ('d_y_st', 'd_gate_st', 'd_res_st')] +
+                [(n, _P) for n in ('d_w', 'd_scale', 'd_w_next', 'ws')])
+
+
+ORTHO_MAX = 24
+
+
+class OrthoItem(C.Structure):
+    _fields_ = [('src', _P), ('mom', _P), ('dst', _P), ('src_ld', C.c_int64), ('dst_ld', C.c_int64),
+                ('rows', C.c_int32), ('cols', C.c_int32), ('gain', C.c_float), ('reserved', C.c_int32)]
+
+
+class Ortho(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ('n', 'steps', 'src_bf16', 'dst_bf16', 'nesterov', 'update')] +
+                [(n, C.c_float) for n in ('eps', 'ca', 'cb', 'cc', 'momentum', 'decay', 'lr', 'reserved')] +
+                [('lr_dev', _P), ('ws', _P), ('item', OrthoItem * ORTHO_MAX)])
+
+
 class MdmmError(RuntimeError):
     pass
 
@@ -413,10 +452,22 @@ def lib():
         L.mdmm_cat_head_slabs.argtypes = [i64]
         L.mdmm_cat_head_nll_fwd.argtypes = [_P, _P, _P, _P, _P, i64, i64, i32, i32, f32, i32, C.POINTER(C.c_float), _P, _P, _P]
         L.mdmm_cat_head_nll_bwd.argtypes = [_P, _P, _P, _P, i64, i64, i32, i32, f32, _P, i32, C.POINTER(C.c_float), _P, _P, _P, _P]
+        for st, names in ((GatedScan, ('mdmm_gated_scan_fwd', 'mdmm_gated_scan_bwd')),
+                          (BlockNorm, ('mdmm_block_norm_fwd', 'mdmm_block_norm_bwd')), (Ortho, ('mdmm_ortho',))):
+            for name in names:
+                getattr(L, name).argtypes = [C.POINTER(st), _P]
+        L.mdmm_gated_block_step.argtypes = [C.POINTER(GatedScan), C.POINTER(BlockNorm), _P]
+        L.mdmm_gated_scan_states.argtypes = [C.POINTER(GatedScan)]
+        L.mdmm_gated_scan_ws.argtypes = [C.POINTER(GatedScan), C.c_int]
+        L.mdmm_block_norm_ws.argtypes = [C.POINTER(BlockNorm)]
+        L.mdmm_ortho_ws.argtypes = [C.POINTER(Ortho)]
+        for name in ('mdmm_gated_scan_states', 'mdmm_gated_scan_ws', 'mdmm_block_norm_ws', 'mdmm_ortho_ws'):
+            getattr(L, name).restype = C.c_int64
         L.mdmm_sizeof.argtypes = [C.c_int]
         L.mdmm_sizeof.restype = C.c_size_t
         for which, st in ((0, Gtf), (1, Expert), (2, Sweep), (4, Gru), (5, Dks), (6, Mlp), (7, Bn), (8, Conv),
-                          (9, FragLayers), (10, Gemm), (11, Conv1d), (12, Vrnn), (13, VrnnLayout), (14, SpillWgradBatch), (15, ConvF), (16, Audio)):
+                          (9, FragLayers), (10, Gemm), (11, Conv1d), (12, Vrnn), (13, VrnnLayout), (14, SpillWgradBatch), (15, ConvF), (16, Audio),
+                          (17, GatedScan), (18, BlockNorm), (19, Ortho)):
             if L.mdmm_sizeof(which) != C.sizeof(st):
                 raise MdmmError('struct %s: library %d bytes, binding %d bytes'
                                 % (st.__name__, L.mdmm_sizeof(which), C.sizeof(st)))

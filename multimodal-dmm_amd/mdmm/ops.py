@@ -3480,3 +3480,11 @@ def vrnn_scan(spec, eps, xs, params):
     (T,B,dims[m]) inputs or None.  Returns (infer_mean, infer_std, prior_mean, prior_std,
     rec_mean per modality ..., rec_std per modality ...)."""
     return _VrnnFn.apply(spec, _f32c(eps) if eps is not None else None, xs, *params)
+
+
+# ------------------------------------------------------------------------------------
+# Gated linear recurrence, block norms (mdmm.recurrent) and orthogonalised updates (mdmm.ortho)
+# ------------------------------------------------------------------------------------
+from .recurrent import (block_norm, gated_block, gated_block_step, gated_scan, gated_scan_step,  # noqa: F401,E402
+                        rms_norm)
+from .ortho import orthogonalise  # noqa: F401,E402

@@ -1,0 +1,523 @@
+"""The gated linear recurrence, the norms around its block, and the layer that joins them (csrc/gated_scan.hip,
+csrc/block_norm.hip): autograd nodes and the single-step forms.  Public through mdmm.ops.
+
+One layer of a recurrent residual block (models.common.GatedLinearRNN stacks them):
+
+    n    = rms_norm(x, w_0)                                         the norm before the first block
+    proj = n W^T + b            (T, B, 3H) = [f | c | g]            one time-parallel product
+    h_t  = a_t h_{t-1} + (1 - a_t) c_t,  a = sigmoid(f)             gated_scan
+    x'   = x + s silu(g) rms_norm(h, w);  n' = rms_norm(x', w')     block_norm (w': the next block's norm)
+
+States, row statistics and sums are fp32 whatever the tensors' type; every stored tensor is rounded once.
+"""
+import ctypes as C
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import native, ops
+
+_TYPES = (torch.float32, torch.bfloat16)
+
+
+def _check_type(name, *tensors):
+    for t in tensors:
+        if t is not None and t.dtype not in _TYPES:
+            raise ValueError('%s: fp32 or bf16 tensors, got %s' % (name, t.dtype))
+
+
+def _check_device(name, first, *tensors):
+    ops._need_gpu(first, *tensors)
+    for t in tensors:
+        if t is not None and t.device != first.device:
+            raise ValueError('%s: tensors on %s and %s' % (name, first.device, t.device))
+
+
+def _vector(name, what, t, H):
+    """An fp32 weight vector of H elements as the kernels read it."""
+    if t is None:
+        return None
+    if not torch.is_tensor(t) or t.dim() != 1 or t.shape[0] != H:
+        raise ValueError('%s: %s must be a vector of %d elements, got %s'
+                         % (name, what, H, tuple(t.shape) if torch.is_tensor(t) else t))
+    if t.dtype != torch.float32:
+        raise ValueError('%s: %s must be fp32, got %s' % (name, what, t.dtype))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _vectors(name, weight, scale, next_weight, H):
+    if weight is None:
+        raise ValueError('%s: weight is not optional' % name)
+    return [_vector(name, k, t, H) for k, t in (('weight', weight), ('scale', scale), ('next_weight', next_weight))]
+
+
+class _on:
+    """The device of the operands as the current one (a caller may have another one current)."""
+
+    def __init__(self, device):
+        self.ctx = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def _mask_bytes(name, mask, lead):
+    """(T,B[,1]) mask (bool, bytes or floats; 0 = left out) as a byte tensor."""
+    if mask is None:
+        return None
+    if mask.dim() == len(lead) + 1 and mask.shape[-1] == 1:
+        mask = mask.squeeze(-1)
+    if tuple(mask.shape) != tuple(lead):
+        raise ValueError('%s: mask must be %s, got %s' % (name, tuple(lead), tuple(mask.shape)))
+    return mask if mask.dtype in (torch.bool, torch.uint8) else mask.detach() != 0
+
+
+def _unit_cols(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _check_h0(name, h0, B, H):
+    if h0 is None:
+        return None
+    if tuple(h0.shape) not in ((H,), (B, H)):
+        raise ValueError('%s: h0 must be (%d,) or (%d, %d), got %s' % (name, H, B, H, tuple(h0.shape)))
+    return _unit_cols(h0.float())
+
+
+def _fill_scan(a, x, H, h0, mask, reverse):
+    T, B = x.shape[:2]
+    a.T, a.B, a.H, a.reverse, a.gates_bf16 = T, B, H, int(reverse), int(x.dtype == torch.bfloat16)
+    a.gates, a.gates_st, a.gates_sb = x.data_ptr(), x.stride(0), x.stride(1)
+    if h0 is not None:
+        a.h0, a.h0_sb = h0.data_ptr(), (h0.stride(0) if h0.dim() == 2 else 0)
+    if mask is not None:
+        a.mask, a.mask_st, a.mask_sb = mask.data_ptr(), mask.stride(0), mask.stride(1)
+
+
+def _scan_ws(a, bwd, device):
+    n = native.lib().mdmm_gated_scan_ws(C.byref(a), bwd)
+    if n <= 0:
+        return None
+    ws = torch.empty(n, dtype=torch.float32, device=device)
+    a.ws = ws.data_ptr()
+    return ws
+
+
+def _scan_forward(x, H, h0, mask, reverse, h_dtype, keep):
+    """-> (h, h_last, states)."""
+    T, B = x.shape[:2]
+    dev = x.device
+    h = torch.empty(T, B, H, device=dev, dtype=h_dtype)
+    if T == 0:
+        last = torch.zeros(B, H, device=dev) if h0 is None else h0.detach().expand(B, H).clone()
+        return h, last, None
+    last = torch.empty(B, H, device=dev, dtype=torch.float32)
+    a = native.GatedScan()
+    _fill_scan(a, x, H, h0, mask, reverse)
+    a.h, a.h_last, a.h_bf16 = h.data_ptr(), last.data_ptr(), int(h_dtype == torch.bfloat16)
+    states = None
+    if keep:
+        states = torch.empty(native.lib().mdmm_gated_scan_states(C.byref(a)), device=dev, dtype=torch.float32)
+        a.states = states.data_ptr()
+    ws = _scan_ws(a, 0, dev)
+    ops._call('mdmm_gated_scan_fwd', C.byref(a), tag='gated_scan_fwd[H=%d]' % H)
+    del ws
+    return h, last, states
+
+
+def _scan_backward(x, H, h0, mask, reverse, h_dtype, states, g_h, g_last, g_x):
+    """Writes columns [0, 2H) of g_x; -> gradient of h0 in its shape (None without h0)."""
+    T, B = x.shape[:2]
+    dev = x.device
+    if T == 0:
+        g0 = g_last.float() if g_last is not None else None
+    else:
+        a = native.GatedScan()
+        _fill_scan(a, x, H, h0, mask, reverse)
+        a.h_bf16 = int(h_dtype == torch.bfloat16)
+        a.states, a.g_h, a.g_last = ops._ptr(states), ops._ptr(g_h), ops._ptr(g_last)
+        a.g_gates, a.g_gates_st, a.g_gates_sb = g_x.data_ptr(), g_x.stride(0), g_x.stride(1)
+        g0 = None
+        if h0 is not None:
+            g0 = torch.empty(B, H, device=dev, dtype=torch.float32)
+            a.g_h0 = g0.data_ptr()
+        ws = _scan_ws(a, 1, dev)
+        ops._call('mdmm_gated_scan_bwd', C.byref(a), tag='gated_scan_bwd[H=%d]' % H)
+        del ws
+    if h0 is None:
+        return None
+    if g0 is None:
+        return torch.zeros_like(h0)
+    return g0 if h0.dim() == 2 else _row_sum(g0)
+
+
+def _row_sum(g):
+    """(B, H) -> (H,), on the column-sum kernel where it takes the width (a fixed order, and safe in a captured graph)."""
+    if g.shape[0] == 0:
+        return g.new_zeros(g.shape[1])
+    return g[0] if g.shape[0] == 1 else ops.colsum(g)
+
+
+class _GatedScanFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gates, h0, mask, reverse):
+        ctx.set_materialize_grads(False)
+        H = gates.shape[-1] // 2
+        keep = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        with _on(gates.device):
+            h, last, states = _scan_forward(gates, H, h0, mask, reverse, gates.dtype, keep)
+        if keep:
+            ctx.save_for_backward(gates, h0, mask, states)
+            ctx.reverse = reverse
+        return h, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_h, g_last):
+        if g_h is None and g_last is None:
+            return None, None, None, None
+        gates, h0, mask, states = ctx.saved_tensors
+        T, B, H2 = gates.shape
+        with _on(gates.device):
+            g_h = None if g_h is None else g_h.contiguous()
+            g_last = None if g_last is None else g_last.contiguous()
+            g_x = torch.empty(T, B, H2, device=gates.device, dtype=gates.dtype)
+            g0 = _scan_backward(gates, H2 // 2, h0, mask, ctx.reverse, gates.dtype, states, g_h, g_last, g_x)
+        return g_x, g0, None, None
+
+
+def gated_scan(gates, h0=None, mask=None, reverse=False):
+    """h_t = a_t h_{t-1} + (1 - a_t) c_t with a = sigmoid(f) over dim 0 of gates (T,B,2H) = [f | c], fp32 or bf16.
+
+    h0: the state in front of the first step, (H,) for every sequence or (B,H); zeros by default.  mask (T,B): a step with
+    0 leaves the state as it is, its f and c are not used (they may be NaN) and get zero gradients.  reverse: from the last
+    step to the first.  -> (h (T,B,H) in the gates' type, the state behind the last step taken (B,H) in fp32).
+    Differentiable in gates and h0, once."""
+    if gates.dim() != 3 or gates.shape[2] % 2:
+        raise ValueError('gated_scan: gates must be (T, B, 2H), got %s' % (tuple(gates.shape),))
+    _check_type('gated_scan', gates)
+    T, B, H2 = gates.shape
+    h0, mask = _check_h0('gated_scan', h0, B, H2 // 2), _mask_bytes('gated_scan', mask, (T, B))
+    _check_device('gated_scan', gates, h0, mask)
+    return _GatedScanFn.apply(_unit_cols(gates), h0, mask, bool(reverse))
+
+
+def _no_grad_only(name, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError('%s has no gradient: call it under torch.no_grad(), or %s for training'
+                         % (name, name.replace('_step', '')))
+
+
+def _check_state(name, state, new_state, B, H):
+    for what, t in (('state', state), ('new_state', new_state)):
+        if t is None and what == 'new_state':
+            continue
+        if not torch.is_tensor(t) or t.dtype != torch.float32 or tuple(t.shape) != (B, H) or not t.is_contiguous():
+            raise ValueError('%s: %s must be contiguous fp32 (%d, %d), got %s'
+                             % (name, what, B, H, (t.dtype, tuple(t.shape)) if torch.is_tensor(t) else t))
+
+
+def gated_scan_step(gates, state, mask=None, new_state=None):
+    """One time step of gated_scan for streams whose state the caller keeps: gates (B,2H), state (B,H) fp32, mask (B,).
+    -> (h (B,H) in the gates' type, new state (B,H) fp32).  new_state: where the state goes; `state` itself updates it in
+    place, None allocates.  No gradient."""
+    if gates.dim() != 2 or gates.shape[1] % 2:
+        raise ValueError('gated_scan_step: gates must be (B, 2H), got %s' % (tuple(gates.shape),))
+    _check_type('gated_scan_step', gates)
+    B, H = gates.shape[0], gates.shape[1] // 2
+    mask = _mask_bytes('gated_scan_step', mask, (B,))
+    _no_grad_only('gated_scan_step', gates, state)
+    _check_state('gated_scan_step', state, new_state, B, H)
+    _check_device('gated_scan_step', gates, state, mask, new_state)
+    new_state = torch.empty_like(state) if new_state is None else new_state
+    with _on(gates.device):
+        h = torch.empty(B, H, device=gates.device, dtype=gates.dtype)
+        if B and H:
+            a = native.GatedScan()
+            _fill_scan(a, _unit_cols(gates).unsqueeze(0), H, state, None if mask is None else mask.unsqueeze(0), False)
+            a.h, a.h_last, a.h_bf16 = h.data_ptr(), new_state.data_ptr(), a.gates_bf16
+            ops._call('mdmm_gated_scan_fwd', C.byref(a), tag='gated_scan_step[H=%d]' % H)
+    return h, new_state
+
+
+# ---- norms -------------------------------------------------------------------------------------------------------
+
+def _as_rows(t, H):
+    """(rows, H) view with unit column stride: rows of any one stride without a copy."""
+    return _unit_cols(t.reshape(-1, H))
+
+
+def _combo(name, y, branch, res):
+    key = tuple(d == torch.bfloat16 for d in (y, branch, res))
+    if key not in ((False, False, False), (True, True, True), (True, True, False), (False, True, False), (False, True, True)):
+        raise ValueError('%s: types (y, gate / norm output, residual) = (%s, %s, %s) are not supported together' % (name, y, branch, res))
+    return key
+
+
+def _row(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _fill_norm(p, y, gate, res, w, s, w_next, branch, eps):
+    p.rows, p.H, p.eps = res.shape[0], res.shape[1], eps
+    p.branch_bf16, p.res_bf16 = int(branch == torch.bfloat16), int(res.dtype == torch.bfloat16)
+    p.res, p.res_st = res.data_ptr(), _row(res)
+    if y is not None:
+        p.y, p.y_st, p.y_bf16 = y.data_ptr(), _row(y), int(y.dtype == torch.bfloat16)
+    if gate is not None:
+        p.gate, p.gate_st = gate.data_ptr(), _row(gate)
+    p.w, p.scale, p.w_next = ops._ptr(w), ops._ptr(s), ops._ptr(w_next)
+
+
+def _norm_forward(y, gate, res, w, s, w_next, branch, eps):
+    """Row-major (rows, H) operands -> (out or None, n or None)."""
+    rows, H = res.shape
+    out = torch.empty(rows, H, device=res.device, dtype=res.dtype) if y is not None else None
+    n = torch.empty(rows, H, device=res.device, dtype=branch) if w_next is not None else None
+    p = native.BlockNorm()
+    _fill_norm(p, y, gate, res, w, s, w_next, branch, eps)
+    if out is not None:
+        p.out, p.out_st = out.data_ptr(), H
+    if n is not None:
+        p.n, p.n_st = n.data_ptr(), H
+    ops._call('mdmm_block_norm_fwd', C.byref(p), tag='block_norm_fwd[H=%d]' % H)
+    return out, n
+
+
+def _norm_backward(y, gate, res, w, s, w_next, branch, eps, g_out, g_n, d_y, d_gate, d_res, want):
+    """Writes d_y, d_gate, d_res (row-major views, None: not wanted); want = (d_w, d_scale, d_w_next) flags -> the three
+    column sums (None where not wanted)."""
+    H, dev = res.shape[1], res.device
+    p = native.BlockNorm()
+    _fill_norm(p, y, gate, res, w, s, w_next, branch, eps)
+    for f, t in (('g_out', g_out), ('g_n', g_n), ('d_y', d_y), ('d_gate', d_gate), ('d_res', d_res)):
+        if t is not None:
+            setattr(p, f, t.data_ptr())
+            setattr(p, f + '_st', _row(t))
+    sums = [torch.empty(H, device=dev, dtype=torch.float32) if k else None for k in want]
+    if res.shape[0] == 0:
+        return [None if t is None else t.zero_() for t in sums]
+    p.d_w, p.d_scale, p.d_w_next = (ops._ptr(t) for t in sums)
+    ws = torch.empty(native.lib().mdmm_block_norm_ws(C.byref(p)), device=dev, dtype=torch.float32)
+    p.ws = ws.data_ptr()
+    ops._call('mdmm_block_norm_bwd', C.byref(p), tag='block_norm_bwd[H=%d]' % H)
+    return sums
+
+
+class _RmsNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, eps, dtype):
+        ctx.set_materialize_grads(False)
+        rows = _as_rows(x, x.shape[-1])
+        ctx.save_for_backward(rows, w)
+        ctx.eps, ctx.branch = eps, dtype
+        with _on(x.device):
+            n = _norm_forward(None, None, rows, None, None, w, dtype, eps)[1]
+        return n.view(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        if g is None:
+            return None, None, None, None
+        x, w = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        with _on(x.device):
+            d_x = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
+            sums = _norm_backward(None, None, x, None, None, w, ctx.branch, ctx.eps, None, _as_rows(g, x.shape[1]), None, None,
+                                  d_x, (False, False, need_w))
+        return None if d_x is None else d_x.view(g.shape), sums[2], None, None
+
+
+def _check_width(name, H):
+    if not 1 <= H <= native.NORM_MAX_H:
+        raise ValueError('%s: rows of 1 to %d columns, got %d' % (name, native.NORM_MAX_H, H))
+
+
+def rms_norm(x, weight, eps=1e-6, dtype=None):
+    """x rsqrt(mean(x^2) + eps) weight over the last dimension: the norm before a block.  x fp32 or bf16, weight (H,) fp32;
+    dtype: the output's type (x's by default; bf16 from fp32 is the other one there is).  Differentiable, once."""
+    if x.dim() < 1:
+        raise ValueError('rms_norm: a tensor with rows, got a scalar')
+    H = x.shape[-1]
+    dtype = x.dtype if dtype is None else dtype
+    _check_type('rms_norm', x)
+    _check_width('rms_norm', H)
+    if dtype not in _TYPES or (x.dtype == torch.bfloat16 and dtype != torch.bfloat16):
+        raise ValueError('rms_norm: %s rows to %s' % (x.dtype, dtype))
+    weight = _vector('rms_norm', 'weight', weight, H)
+    _check_device('rms_norm', x, weight)
+    return _RmsNormFn.apply(x, weight, float(eps), dtype)
+
+
+class _BlockNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, res, w, gate, s, w_next, eps):
+        ctx.set_materialize_grads(False)
+        H = res.shape[-1]
+        rows = [None if t is None else _as_rows(t, H) for t in (y, gate, res)]
+        ctx.save_for_backward(*rows, w, s, w_next)
+        ctx.eps, ctx.shape = eps, res.shape
+        with _on(res.device):
+            out, n = _norm_forward(*rows, w, s, w_next, y.dtype, eps)
+        out = out.view(res.shape)
+        return out if n is None else (out, n.view(res.shape))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_out, g_n=None):
+        if g_out is None and g_n is None:
+            return (None,) * 7
+        y, gate, res, w, s, w_next = ctx.saved_tensors
+        need = ctx.needs_input_grad                     # y, res, w, gate, s, w_next
+        H, dev = res.shape[1], res.device
+        with _on(dev):
+            g_out = None if g_out is None else _as_rows(g_out, H)
+            g_n = None if g_n is None else _as_rows(g_n, H)
+            empty = lambda like: torch.empty(res.shape, device=dev, dtype=like.dtype)      # noqa: E731
+            d_y = empty(y) if need[0] else None
+            d_gate = empty(gate) if need[3] else None
+            d_res = empty(res) if need[1] and g_n is not None else None      # (without a next norm it is g_out itself)
+            sums = _norm_backward(y, gate, res, w, s, w_next, y.dtype, ctx.eps, g_out, g_n, d_y, d_gate, d_res,
+                                  (need[2], need[4], need[5]))
+            if need[1] and d_res is None:
+                d_res = g_out
+        view = lambda t: None if t is None else t.reshape(ctx.shape)                       # noqa: E731
+        return view(d_y), view(d_res), sums[0], view(d_gate), sums[1], sums[2], None
+
+
+def block_norm(y, residual, weight, gate=None, scale=None, next_weight=None, eps=1e-6):
+    """The end of a residual block and the norm of the next one in one pass each way:
+
+        out = residual + scale * silu(gate) * rms_norm(y, weight)          (gate, scale: None = 1)
+        n   = rms_norm(out, next_weight)
+
+    -> out, or (out, n) with next_weight.  y, gate and n fp32 or bf16 (one type), residual and out that type or fp32; weight,
+    scale and next_weight (H,) fp32; any leading dimensions.  Differentiable in every tensor, once."""
+    name = 'block_norm'
+    if y.shape != residual.shape or (gate is not None and gate.shape != y.shape) or y.dim() < 1:
+        raise ValueError('%s: y %s, residual %s and gate %s must have one shape'
+                         % (name, tuple(y.shape), tuple(residual.shape), None if gate is None else tuple(gate.shape)))
+    H = y.shape[-1]
+    _check_type(name, y, residual, gate)
+    _check_width(name, H)
+    if gate is not None and gate.dtype != y.dtype:
+        raise ValueError('%s: gate %s beside y %s' % (name, gate.dtype, y.dtype))
+    _combo(name, y.dtype, y.dtype, residual.dtype)
+    weight, scale, next_weight = _vectors(name, weight, scale, next_weight, H)
+    _check_device(name, y, residual, weight, gate, scale, next_weight)
+    return _BlockNormFn.apply(y, residual, weight, gate, scale, next_weight, float(eps))
+
+
+# ---- the layer ---------------------------------------------------------------------------------------------------
+
+class _GatedBlockFn(torch.autograd.Function):
+    """gated_scan and block_norm on one projection: the state stays fp32 between them, and their gradients land in one
+    (T,B,3H) buffer instead of being joined by copies."""
+
+    @staticmethod
+    def forward(ctx, proj, res, h0, w, s, w_next, mask, reverse, eps):
+        ctx.set_materialize_grads(False)
+        T, B, H = res.shape
+        keep = any(ctx.needs_input_grad)
+        with _on(proj.device):
+            h, last, states = _scan_forward(proj, H, h0, mask, reverse, torch.float32, keep)
+            rows, flat = _as_rows(res, H), _as_rows(proj, 3 * H)
+            out, n = _norm_forward(h.view(-1, H), flat[:, 2 * H:], rows, w, s, w_next, proj.dtype, eps)
+        if keep:
+            ctx.save_for_backward(proj, rows, h0, w, s, w_next, mask, states, h)
+            ctx.reverse, ctx.eps = reverse, eps
+        out = out.view(T, B, H)
+        return (out, last) if n is None else (out, n.view(T, B, H), last)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        proj, res, h0, w, s, w_next, mask, states, h = ctx.saved_tensors
+        g_out, g_last = grads[0], grads[-1]
+        g_n = grads[1] if len(grads) == 3 else None
+        need = ctx.needs_input_grad                    # proj, res, h0, w, s, w_next
+        T, B, H3 = proj.shape
+        H, dev = H3 // 3, proj.device
+        if g_out is None and g_n is None and g_last is None:
+            return (None,) * 9
+        with _on(dev):
+            g_out = None if g_out is None else _as_rows(g_out, H)
+            g_n = None if g_n is None else _as_rows(g_n, H)
+            g_last = None if g_last is None else g_last.contiguous()
+            g_x = torch.empty(T, B, H3, device=dev, dtype=proj.dtype)
+            d_res = d_h = None
+            sums = [None, None, None]
+            if g_out is None and g_n is None:
+                g_x[..., 2 * H:].zero_()
+            else:
+                d_h = torch.empty(T * B, H, device=dev, dtype=torch.float32)
+                d_res = torch.empty(T * B, H, device=dev, dtype=res.dtype) if need[1] and g_n is not None else None
+                sums = _norm_backward(h.view(-1, H), _as_rows(proj, H3)[:, 2 * H:], res, w, s, w_next, proj.dtype, ctx.eps,
+                                      g_out, g_n, d_h, g_x.view(-1, H3)[:, 2 * H:], d_res, (need[3], need[4], need[5]))
+                if need[1] and d_res is None:
+                    d_res = g_out
+            g0 = _scan_backward(proj, H, h0, mask, ctx.reverse, torch.float32, states, d_h, g_last, g_x)
+        return (g_x, None if d_res is None else d_res.reshape(T, B, H), g0, *sums, None, None, None)
+
+
+def _check_block(name, proj, residual, lead):
+    H = residual.shape[-1]
+    if tuple(proj.shape[:-1]) != tuple(residual.shape[:-1]) or proj.shape[-1] != 3 * H or proj.dim() != lead + 1:
+        raise ValueError('%s: proj %s must be %s with three times the residual\'s columns, residual %s'
+                         % (name, tuple(proj.shape), '(T, B, 3H)' if lead == 2 else '(B, 3H)', tuple(residual.shape)))
+    _check_type(name, proj, residual)
+    _check_width(name, H)
+    _combo(name, torch.float32, proj.dtype, residual.dtype)
+    return H
+
+
+def gated_block(proj, residual, h0, weight, scale=None, next_weight=None, mask=None, reverse=False, eps=1e-6):
+    """A recurrent residual block behind its projection proj (T,B,3H) = [f | c | g]:
+
+        h   = gated_scan([f | c], h0, mask, reverse)                        kept in fp32
+        out = residual + scale * silu(g) * rms_norm(h, weight);  n = rms_norm(out, next_weight)
+
+    -> (out, h_last) or, with next_weight, (out, n, h_last).  The mask concerns the state alone: a step that is left out
+    still gives an output, from the state it leaves unchanged, so its g must be finite.  proj and n fp32 or bf16, residual
+    and out that type or fp32.  Differentiable in every floating tensor, once."""
+    name = 'gated_block'
+    H = _check_block(name, proj, residual, 2)
+    T, B = proj.shape[:2]
+    weight, scale, next_weight = _vectors(name, weight, scale, next_weight, H)
+    h0, mask = _check_h0(name, h0, B, H), _mask_bytes(name, mask, (T, B))
+    _check_device(name, proj, residual, h0, weight, scale, next_weight, mask)
+    return _GatedBlockFn.apply(_unit_cols(proj), residual, h0, weight, scale, next_weight, mask, bool(reverse), float(eps))
+
+
+def gated_block_step(proj, residual, state, weight, scale=None, next_weight=None, mask=None, eps=1e-6, new_state=None):
+    """One time step of gated_block in one launch: proj (B,3H), residual (B,H), state (B,H) fp32, mask (B,) ->
+    (out, new state) or (out, n, new state).  new_state as in gated_scan_step.  No gradient."""
+    name = 'gated_block_step'
+    H = _check_block(name, proj, residual, 1)
+    B = proj.shape[0]
+    w, s, w_next = _vectors(name, weight, scale, next_weight, H)
+    mask = _mask_bytes(name, mask, (B,))
+    _no_grad_only(name, proj, residual, state, w, s, w_next)
+    _check_state(name, state, new_state, B, H)
+    _check_device(name, proj, residual, state, w, s, w_next, mask, new_state)
+    new_state = torch.empty_like(state) if new_state is None else new_state
+    with _on(proj.device):
+        proj, residual = _unit_cols(proj), _unit_cols(residual)
+        out = torch.empty(B, H, device=proj.device, dtype=residual.dtype)
+        n = torch.empty(B, H, device=proj.device, dtype=proj.dtype) if w_next is not None else None
+        if B:
+            a, p = native.GatedScan(), native.BlockNorm()
+            _fill_scan(a, proj.unsqueeze(0), H, state, None if mask is None else mask.unsqueeze(0), False)
+            a.h_last = new_state.data_ptr()
+            _fill_norm(p, None, proj[:, 2 * H:], residual, w, s, w_next, proj.dtype, float(eps))
+            p.out, p.out_st = out.data_ptr(), H
+            if n is not None:
+                p.n, p.n_st = n.data_ptr(), H
+            ops._call('mdmm_gated_block_step', C.byref(a), C.byref(p), tag='gated_block_step[H=%d]' % H)
+    return (out, new_state) if n is None else (out, n, new_state)
