@@ -1,7 +1,7 @@
 #!/bin/bash
 # usage: tools/kernel_regs.sh file.hip [grep-pattern]   -- registers / occupancy per kernel (gfx950)
 cd "$(dirname "$0")/../multimodal-dmm_amd/csrc"
-/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -c "$1" -o /tmp/_kr.o \
+/opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -c "$1" -o /tmp/_kr.o \
   -Rpass-analysis=kernel-resource-usage 2>&1 |
 python3 -c "
 import re, sys
