@@ -10,19 +10,47 @@
 namespace mdmm {
 namespace {
 
-template <int VEC> __device__ __forceinline__ void load_v(const float* p, float* v) {
-  if constexpr (VEC == 4) {
-    const float4 x = *(const float4*)p;
-    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-  } else v[0] = *p;
+// VEC columns as loaded
+template <typename T, int VEC> struct Raw { T x; };
+template <> struct Raw<float, 4> { float4 x; };
+template <> struct Raw<__bf16, 4> { uint2 x; };
+
+template <int VEC> __device__ __forceinline__ void widen(const Raw<float, VEC>& r, float* v) {
+  if constexpr (VEC == 4) { v[0] = r.x.x; v[1] = r.x.y; v[2] = r.x.z; v[3] = r.x.w; }
+  else v[0] = r.x;
 }
-template <int VEC> __device__ __forceinline__ void load_v(const __bf16* p, float* v) {
+template <int VEC> __device__ __forceinline__ void widen(const Raw<__bf16, VEC>& r, float* v) {
   if constexpr (VEC == 4) {
-    const uint2 x = *(const uint2*)p;
-    v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xffff0000u);
-    v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xffff0000u);
-  } else v[0] = (float)*p;
+    v[0] = __uint_as_float(r.x.x << 16); v[1] = __uint_as_float(r.x.x & 0xffff0000u);
+    v[2] = __uint_as_float(r.x.y << 16); v[3] = __uint_as_float(r.x.y & 0xffff0000u);
+  } else v[0] = (float)r.x;
 }
+template <int VEC> __device__ __forceinline__ void load_v(const float* p, float* v) { widen(*(const Raw<float, VEC>*)p, v); }
+
+// A thread's pieces of a vector over the columns, kept in registers over all rows (read again for each row, the three vectors
+// in fp32 are more bytes than a bf16 row); `none` where it is not there
+template <int VEC, int NV>
+__device__ __forceinline__ void keep(float (&v)[NV][VEC], const float* base, float none, int lane, int tpr, int H) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * tpr + lane) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[k][e] = none;
+    if (base && c < H) load_v<VEC>(base + c, v[k]);
+  }
+}
+
+// A row's pieces of one tensor; columns past the end (and a tensor that is not there) are zeros
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void fetch(Raw<T, VEC> (&r)[NV], const void* base, int64_t at, int lane, int tpr, int H) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * tpr + lane) * VEC;
+    r[k] = Raw<T, VEC>{};
+    if (base && c < H) r[k] = *(const Raw<T, VEC>*)((const T*)base + at + c);
+  }
+}
+
 template <int VEC> __device__ __forceinline__ void store_v(float* p, const float* v) {
   if constexpr (VEC == 4) *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
   else *p = v[0];
@@ -36,57 +64,92 @@ template <int VEC> __device__ __forceinline__ void store_v(__bf16* p, const floa
   } else *p = (__bf16)v[0];
 }
 
-// sum over the TPR threads of a row, in every one of them
-template <int TPR> __device__ __forceinline__ float row_sum(float v, float* lds, int& slot) {
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  if constexpr (TPR > 64) {
-    constexpr int W = TPR / 64;
-    float* s = lds + (slot ^= 1) * W;
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.0f;
-    for (int w = 0; w < W; ++w) v += s[w];
-  }
-  return v;
+// sum over the wave, in every lane: rows of 16 by DPP moves (no LDS round trip), then across the four rows
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float wave_total(float v) {
+  v = dpp_add<0xb1, 0xf>(v);        // neighbours
+  v = dpp_add<0x4e, 0xf>(v);        // pairs
+  v = dpp_add<0x141, 0xf>(v);       // half rows mirrored
+  v = dpp_add<0x140, 0xf>(v);       // rows mirrored: every lane holds its row's sum
+  v = dpp_add<0x142, 0xa>(v);       // row 0 into row 1, row 2 into row 3
+  v = dpp_add<0x143, 0xc>(v);       // rows 0 and 1 into rows 2 and 3: lane 63 holds the sum
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
-template <typename Y, typename Br, typename R, int VEC, int NV, int TPR>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(mdmm_block_norm_t p) {
-  constexpr int NT = TPR > 256 ? TPR : 256, RPW = NT / TPR;
-  __shared__ float lds[2 * (TPR / 64)];
+// N sums over a row's threads (a wave, or WIDE the workgroup), in every one of them
+template <bool WIDE, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float* lds, int& slot) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = wave_total(v[i]);
+  if constexpr (WIDE) {
+    const int W = blockDim.x >> 6;
+    float* s = lds + (slot ^= 1) * 2 * W;       // (two sets: a wave that runs ahead writes the other one)
+    if ((threadIdx.x & 63) == 0)
+      for (int i = 0; i < N; ++i) s[i * W + (threadIdx.x >> 6)] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.0f;
+      for (int w = 0; w < W; ++w) v[i] += s[i * W + w];
+    }
+  }
+}
+template <bool WIDE> __device__ __forceinline__ float row_sum(float v, float* lds, int& slot) {
+  float a[1] = {v};
+  row_sums<WIDE, 1>(a, lds, slot);
+  return a[0];
+}
+
+template <typename Y, typename Br, typename R, int VEC, int NV, int MAXT>
+__global__ __launch_bounds__(MAXT) void norm_fwd_kernel(mdmm_block_norm_t p) {
+  constexpr bool WIDE = MAXT > 256;
+  constexpr int RPW = WIDE ? 1 : 4;
+  __shared__ float lds[WIDE ? MAXT / 16 : 1];
   int slot = 0;
-  const int lane = threadIdx.x % TPR;
+  const int tpr = WIDE ? (int)blockDim.x : 64, lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x & 63);
   const float inv = 1.0f / (float)p.H;
-  for (int64_t row = (int64_t)blockIdx.x * RPW + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * RPW) {
+  const int64_t step = (int64_t)gridDim.x * RPW;
+  int64_t row = (int64_t)blockIdx.x * RPW + (WIDE ? 0 : threadIdx.x >> 6);
+  float w[NV][VEC], s[NV][VEC], wn[NV][VEC];
+  keep<VEC, NV>(w, p.w, 0.0f, lane, tpr, p.H);
+  keep<VEC, NV>(s, p.scale, 1.0f, lane, tpr, p.H);
+  keep<VEC, NV>(wn, p.w_next, 0.0f, lane, tpr, p.H);
+  Raw<R, VEC> res[NV];
+  Raw<Y, VEC> ry[NV];
+  Raw<Br, VEC> rg[NV];
+  if (row < p.rows) {
+    fetch<R, VEC, NV>(res, p.res, row * p.res_st, lane, tpr, p.H);
+    fetch<Y, VEC, NV>(ry, p.y, row * p.y_st, lane, tpr, p.H);
+    fetch<Br, VEC, NV>(rg, p.gate, row * p.gate_st, lane, tpr, p.H);
+  }
+  for (; row < p.rows; row += step) {
     float o[NV][VEC], y[NV][VEC], g[NV][VEC];
     float ss = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (k * TPR + lane) * VEC;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) o[k][e] = y[k][e] = g[k][e] = 0.0f;
-      if (c < p.H) {
-        load_v<VEC>((const R*)p.res + row * p.res_st + c, o[k]);
-        if (p.y) load_v<VEC>((const Y*)p.y + row * p.y_st + c, y[k]);
-        if (p.gate) load_v<VEC>((const Br*)p.gate + row * p.gate_st + c, g[k]);
-      }
+      widen(res[k], o[k]);
+      widen(ry[k], y[k]);
+      widen(rg[k], g[k]);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) ss += y[k][e] * y[k][e];
     }
+    if (row + step < p.rows) {           // the next row's pieces, in flight behind this one's arithmetic
+      fetch<R, VEC, NV>(res, p.res, (row + step) * p.res_st, lane, tpr, p.H);
+      fetch<Y, VEC, NV>(ry, p.y, (row + step) * p.y_st, lane, tpr, p.H);
+      fetch<Br, VEC, NV>(rg, p.gate, (row + step) * p.gate_st, lane, tpr, p.H);
+    }
     if (p.y) {
-      const float r = rsqrtf(row_sum<TPR>(ss, lds, slot) * inv + p.eps);
+      const float r = rsqrtf(row_sum<WIDE>(ss, lds, slot) * inv + p.eps);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * TPR + lane) * VEC;
+        const int c = (k * tpr + lane) * VEC;
         if (c < p.H) {
-          float w[VEC], s[VEC];
-          load_v<VEC>(p.w + c, w);
-          if (p.scale) load_v<VEC>(p.scale + c, s);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            float u = y[k][e] * r * w[e];
+            float u = y[k][e] * r * w[k][e];
             if (p.gate) u *= g[k][e] * sigmoid_(g[k][e]);
-            o[k][e] = p.scale ? fmaf(s[e], u, o[k][e]) : o[k][e] + u;
+            o[k][e] = fmaf(s[k][e], u, o[k][e]);
           }
           store_v<VEC>((R*)p.out + row * p.out_st + c, o[k]);
         }
@@ -98,15 +161,13 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(mdmm_bl
       for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) ss += o[k][e] * o[k][e];
-      const float r = rsqrtf(row_sum<TPR>(ss, lds, slot) * inv + p.eps);
+      const float r = rsqrtf(row_sum<WIDE>(ss, lds, slot) * inv + p.eps);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * TPR + lane) * VEC;
+        const int c = (k * tpr + lane) * VEC;
         if (c < p.H) {
-          float w[VEC];
-          load_v<VEC>(p.w_next + c, w);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) o[k][e] *= r * w[e];
+          for (int e = 0; e < VEC; ++e) o[k][e] *= r * wn[k][e];
           store_v<VEC>((Br*)p.n + row * p.n_st + c, o[k]);
         }
       }
@@ -114,69 +175,86 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_fwd_kernel(mdmm_bl
   }
 }
 
-template <typename Y, typename Br, typename R, int VEC, int NV, int TPR>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(mdmm_block_norm_t p) {
-  constexpr int NT = TPR > 256 ? TPR : 256, RPW = NT / TPR;
-  __shared__ float lds[2 * (TPR / 64)];
-  __shared__ float fold[RPW > 1 ? RPW * TPR * VEC : 1];
+template <typename Y, typename Br, typename R, int VEC, int NV, int MAXT>
+__global__ __launch_bounds__(MAXT) void norm_bwd_kernel(mdmm_block_norm_t p) {
+  constexpr bool WIDE = MAXT > 256;
+  constexpr int RPW = WIDE ? 1 : 4;
+  __shared__ float lds[WIDE ? MAXT / 16 : 1];
+  __shared__ float fold[WIDE ? 1 : 256 * VEC];
   int slot = 0;
-  const int lane = threadIdx.x % TPR;
+  const int tpr = WIDE ? (int)blockDim.x : 64, lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x & 63);
   const float inv = 1.0f / (float)p.H;
+  const int64_t step = (int64_t)gridDim.x * RPW;
+  int64_t row = (int64_t)blockIdx.x * RPW + (WIDE ? 0 : threadIdx.x >> 6);
   float aw[NV][VEC] = {}, as[NV][VEC] = {}, an[NV][VEC] = {};
-  for (int64_t row = (int64_t)blockIdx.x * RPW + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * RPW) {
-    float o[NV][VEC], y[NV][VEC], g[NV][VEC], d[NV][VEC], q[NV][VEC];
+  float w[NV][VEC], s[NV][VEC], wn[NV][VEC];
+  keep<VEC, NV>(w, p.w, 0.0f, lane, tpr, p.H);
+  keep<VEC, NV>(s, p.scale, 1.0f, lane, tpr, p.H);
+  keep<VEC, NV>(wn, p.w_next, 0.0f, lane, tpr, p.H);
+  Raw<R, VEC> res[NV], rd[NV];
+  Raw<Y, VEC> ry[NV];
+  Raw<Br, VEC> rg[NV], rq[NV];
+  auto fetch_row = [&](int64_t at) {
+    fetch<Y, VEC, NV>(ry, p.y, at * p.y_st, lane, tpr, p.H);
+    fetch<Br, VEC, NV>(rg, p.gate, at * p.gate_st, lane, tpr, p.H);
+    if (p.g_n) fetch<R, VEC, NV>(res, p.res, at * p.res_st, lane, tpr, p.H);      // (read for the next norm alone)
+    fetch<Br, VEC, NV>(rq, p.g_n, at * p.g_n_st, lane, tpr, p.H);
+    fetch<R, VEC, NV>(rd, p.g_out, at * p.g_out_st, lane, tpr, p.H);
+  };
+  if (row < p.rows) fetch_row(row);
+  for (; row < p.rows; row += step) {
+    float x[NV][VEC], g[NV][VEC], sg[NV][VEC], o[NV][VEC], q[NV][VEC], d[NV][VEC];
     float ss = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (k * TPR + lane) * VEC;
+      widen(ry[k], x[k]);
+      widen(rg[k], g[k]);
+      if (p.g_n) widen(res[k], o[k]);
+      widen(rq[k], q[k]);
+      widen(rd[k], d[k]);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o[k][e] = y[k][e] = g[k][e] = d[k][e] = q[k][e] = 0.0f;
-      if (c < p.H) {
-        load_v<VEC>((const R*)p.res + row * p.res_st + c, o[k]);
-        if (p.y) load_v<VEC>((const Y*)p.y + row * p.y_st + c, y[k]);
-        if (p.gate) load_v<VEC>((const Br*)p.gate + row * p.gate_st + c, g[k]);
-        if (p.g_out) load_v<VEC>((const R*)p.g_out + row * p.g_out_st + c, d[k]);
-        if (p.g_n) load_v<VEC>((const Br*)p.g_n + row * p.g_n_st + c, q[k]);
-      }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) ss += y[k][e] * y[k][e];
+      for (int e = 0; e < VEC; ++e) ss += x[k][e] * x[k][e];
     }
+    if (row + step < p.rows) fetch_row(row + step);       // in flight behind this row's arithmetic
     float r = 0.0f;
-    if (p.y) r = rsqrtf(row_sum<TPR>(ss, lds, slot) * inv + p.eps);
+    if (p.y) {
+      r = rsqrtf(row_sum<WIDE>(ss, lds, slot) * inv + p.eps);
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          x[k][e] *= r;
+          sg[k][e] = p.gate ? sigmoid_(g[k][e]) : 1.0f;
+        }
+    }
     if (p.g_n) {
-      float s2 = 0.0f, sq = 0.0f;
+      float sums[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * TPR + lane) * VEC;
+        const int c = (k * tpr + lane) * VEC;
         if (c < p.H) {
-          float w[VEC], s[VEC], wn[VEC];
-          if (p.y) load_v<VEC>(p.w + c, w);
-          if (p.scale) load_v<VEC>(p.scale + c, s);
-          load_v<VEC>(p.w_next + c, wn);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             if (p.y) {
-              float u = y[k][e] * r * w[e];
-              if (p.gate) u *= g[k][e] * sigmoid_(g[k][e]);
-              o[k][e] = p.scale ? fmaf(s[e], u, o[k][e]) : o[k][e] + u;
+              float u = x[k][e] * w[k][e];
+              if (p.gate) u *= g[k][e] * sg[k][e];
+              o[k][e] = fmaf(s[k][e], u, o[k][e]);
             }
-            s2 += o[k][e] * o[k][e];
-            sq += q[k][e] * wn[e] * o[k][e];
+            sums[0] += o[k][e] * o[k][e];
+            sums[1] += q[k][e] * wn[k][e] * o[k][e];
           }
         }
       }
-      const float r2 = rsqrtf(row_sum<TPR>(s2, lds, slot) * inv + p.eps);
-      const float m = row_sum<TPR>(sq, lds, slot) * inv * r2 * r2;
+      row_sums<WIDE, 2>(sums, lds, slot);
+      const float r2 = rsqrtf(sums[0] * inv + p.eps), m = sums[1] * inv * r2 * r2;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * TPR + lane) * VEC;
+        const int c = (k * tpr + lane) * VEC;
         if (c < p.H) {
-          float wn[VEC];
-          load_v<VEC>(p.w_next + c, wn);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             an[k][e] += q[k][e] * o[k][e] * r2;
-            d[k][e] += r2 * (q[k][e] * wn[e] - o[k][e] * m);
+            d[k][e] += r2 * (q[k][e] * wn[k][e] - o[k][e] * m);
           }
         }
       }
@@ -184,7 +262,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(mdmm_bl
     if (p.d_res) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * TPR + lane) * VEC;
+        const int c = (k * tpr + lane) * VEC;
         if (c < p.H) store_v<VEC>((R*)p.d_res + row * p.d_res_st + c, d[k]);
       }
     }
@@ -192,40 +270,33 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(mdmm_bl
       float sm = 0.0f;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * TPR + lane) * VEC;
+        const int c = (k * tpr + lane) * VEC;
         if (c < p.H) {
-          float w[VEC], s[VEC], dg[VEC];
-          load_v<VEC>(p.w + c, w);
-          if (p.scale) load_v<VEC>(p.scale + c, s);
+          float dg[VEC];
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            const float x = y[k][e] * r, u = x * w[e], sc = p.scale ? s[e] : 1.0f;
-            float act = 1.0f, slope = 0.0f;
-            if (p.gate) {
-              const Gate sg(g[k][e]);
-              act = g[k][e] * sg.a;
-              slope = sg.a * fmaf(g[k][e], sg.k, 1.0f);
-            }
+            // act = silu(g) = g sg, slope = silu'(g) = sg + act (1 - sg)
+            const float act = p.gate ? g[k][e] * sg[k][e] : 1.0f;
+            const float u = x[k][e] * w[k][e], ds = d[k][e] * s[k][e];
             as[k][e] += d[k][e] * act * u;
-            dg[e] = d[k][e] * sc * u * slope;
-            const float t = d[k][e] * sc * act;
-            aw[k][e] += t * x;
-            y[k][e] = x;
-            d[k][e] = t * w[e];
-            sm += d[k][e] * x;
+            dg[e] = ds * u * fmaf(-act, sg[k][e], sg[k][e] + act);
+            const float t = ds * act;
+            aw[k][e] += t * x[k][e];
+            d[k][e] = t * w[k][e];
+            sm += d[k][e] * x[k][e];
           }
           if (p.d_gate) store_v<VEC>((Br*)p.d_gate + row * p.d_gate_st + c, dg);
         }
       }
-      sm = row_sum<TPR>(sm, lds, slot) * inv;
+      sm = row_sum<WIDE>(sm, lds, slot) * inv;
       if (p.d_y) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-          const int c = (k * TPR + lane) * VEC;
+          const int c = (k * tpr + lane) * VEC;
           if (c < p.H) {
             float dy[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) dy[e] = r * (d[k][e] - y[k][e] * sm);
+            for (int e = 0; e < VEC; ++e) dy[e] = r * (d[k][e] - x[k][e] * sm);
             store_v<VEC>((Y*)p.d_y + row * p.d_y_st + c, dy);
           }
         }
@@ -242,18 +313,18 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(mdmm_bl
       if constexpr (RPW > 1) {
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) fold[(threadIdx.x / TPR * TPR + lane) * VEC + e] = acc[e];
+        for (int e = 0; e < VEC; ++e) fold[threadIdx.x * VEC + e] = acc[e];
         __syncthreads();
-        for (int i = threadIdx.x; i < TPR * VEC; i += NT) {
-          const int c = k * TPR * VEC + i;
+        for (int i = threadIdx.x; i < 64 * VEC; i += 256) {
+          const int c = k * 64 * VEC + i;
           if (c < p.H) {
             float s = 0.0f;
-            for (int w = 0; w < RPW; ++w) s += fold[w * TPR * VEC + i];
+            for (int w = 0; w < RPW; ++w) s += fold[w * 64 * VEC + i];
             slab[which * p.H + c] = s;
           }
         }
       } else {
-        const int c = (k * TPR + lane) * VEC;
+        const int c = (k * tpr + lane) * VEC;
         if (c < p.H)
           for (int e = 0; e < VEC; ++e) slab[which * p.H + c + e] = acc[e];
       }
@@ -263,7 +334,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_bwd_kernel(mdmm_bl
 // One time step of the recurrence with its block norm: a row b of the state, TPR threads
 template <typename Br, typename R, int NV, int TPR>
 __global__ __launch_bounds__(TPR) void step_kernel(mdmm_gated_scan_t q, mdmm_block_norm_t p) {
-  __shared__ float lds[2 * (TPR / 64)];
+  constexpr bool WIDE = TPR > 64;
+  __shared__ float lds[4 * (TPR / 64)];
   int slot = 0;
   const int64_t b = blockIdx.x;
   const float inv = 1.0f / (float)p.H;
@@ -286,7 +358,7 @@ __global__ __launch_bounds__(TPR) void step_kernel(mdmm_gated_scan_t q, mdmm_blo
     }
     ss += h[k] * h[k];
   }
-  float r = rsqrtf(row_sum<TPR>(ss, lds, slot) * inv + p.eps);
+  float r = rsqrtf(row_sum<WIDE>(ss, lds, slot) * inv + p.eps);
   ss = 0.0f;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -303,7 +375,7 @@ __global__ __launch_bounds__(TPR) void step_kernel(mdmm_gated_scan_t q, mdmm_blo
     ss += o[k] * o[k];
   }
   if (!p.w_next) return;
-  r = rsqrtf(row_sum<TPR>(ss, lds, slot) * inv + p.eps);
+  r = rsqrtf(row_sum<WIDE>(ss, lds, slot) * inv + p.eps);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = k * TPR + threadIdx.x;
@@ -320,15 +392,23 @@ int launch_step(const mdmm_gated_scan_t* q, const mdmm_block_norm_t* p, hipStrea
   return (int)hipGetLastError();
 }
 
-// column sums of the slabs: 16 columns a workgroup, 16 threads down each column, joined in a fixed order
-__global__ __launch_bounds__(256) void norm_fold_kernel(const float* __restrict__ ws, int slabs, int H, float* d_w, float* d_s,
-                                                        float* d_n) {
-  __shared__ float part[16][17];
+// column sums of the slabs: 16 columns (64 bytes of a slab) and 64 threads down each a workgroup, joined in a fixed order;
+// at 1024 slabs a thread has 16 loads, all in flight (with 16 threads down a column the launch took 20 us at H = 256)
+__global__ __launch_bounds__(1024) void norm_fold_kernel(const float* __restrict__ ws, int slabs, int H, float* d_w, float* d_s,
+                                                         float* d_n) {
+  __shared__ float part[64][17];
   const int c = blockIdx.x * 16 + (threadIdx.x & 15), r = threadIdx.x >> 4;
   float s = 0.0f;
-  if (c < 3 * H)
-    for (int i = r; i < slabs; i += 16) s += ws[(int64_t)i * 3 * H + c];
+  if (c < 3 * H) {
+#pragma unroll 16
+    for (int i = r; i < slabs; i += 64) s += ws[(int64_t)i * 3 * H + c];
+  }
   part[r][threadIdx.x & 15] = s;
+  __syncthreads();
+  if (threadIdx.x < 256) {
+    const int q = threadIdx.x >> 4, k = threadIdx.x & 15;
+    part[q][k] = (part[q][k] + part[q + 16][k]) + (part[q + 32][k] + part[q + 48][k]);
+  }
   __syncthreads();
   if (r == 0 && c < 3 * H) {
     s = 0.0f;
@@ -338,7 +418,7 @@ __global__ __launch_bounds__(256) void norm_fold_kernel(const float* __restrict_
   }
 }
 
-struct Plan { int vec, nv, tpr; };
+struct Plan { int vec, nv, maxt, threads; };
 
 bool aligned(const void* p, int64_t st, int bf16) {
   return !p || (((uintptr_t)p & (bf16 ? 7 : 15)) == 0 && (st & 3) == 0);
@@ -351,25 +431,24 @@ Plan plan(const mdmm_block_norm_t* a) {
                   aligned(a->g_n, a->g_n_st, a->branch_bf16) && aligned(a->d_y, a->d_y_st, a->y_bf16) &&
                   aligned(a->d_gate, a->d_gate_st, a->branch_bf16) && aligned(a->d_res, a->d_res_st, a->res_bf16) &&
                   aligned(a->w, 0, 0) && aligned(a->scale, 0, 0) && aligned(a->w_next, 0, 0);
+  const int h = a->H, w4 = (h + 255) / 256 * 64, w8 = (h + 511) / 512 * 64;
   if (v4) {
-    if (a->H <= 256) return {4, 1, 64};
-    if (a->H <= 512) return {4, 2, 64};
-    if (a->H <= 1024) return {4, 4, 64};
-    if (a->H <= 2048) return {4, 2, 256};
-    if (a->H <= 4096) return {4, 4, 256};
-    return {4, 2, 1024};
+    if (h <= 256) return {4, 1, 256, 256};
+    if (h <= 2048) return {4, 1, 512, w4};
+    if (h <= 4096) return {4, 2, 512, w8};
+    return {4, 2, 1024, w8};
   }
-  if (a->H <= 256) return {1, 4, 64};
-  if (a->H <= 1024) return {1, 4, 256};
-  if (a->H <= 4096) return {1, 4, 1024};
-  return {1, 8, 1024};
+  const int u4 = (h + 255) / 256 * 64, u8 = (h + 511) / 512 * 64;
+  if (h <= 256) return {1, 4, 256, 256};
+  if (h <= 2048) return {1, 4, 512, u4};
+  if (h <= 4096) return {1, 4, 1024, u4};
+  return {1, 8, 1024, u8};
 }
 
 int64_t grid_of(const mdmm_block_norm_t* a, const Plan& q) {
-  const int rpw = q.tpr >= 256 ? 1 : 256 / q.tpr;
+  const int rpw = q.maxt == 256 ? 4 : 1;
   const int64_t g = (a->rows + rpw - 1) / rpw;
-  const int64_t top = q.tpr > 256 ? 512 : 1024;
-  return g < top ? g : top;
+  return g < 1024 ? g : 1024;
 }
 
 int check(const mdmm_block_norm_t* a) {
@@ -384,11 +463,10 @@ int check(const mdmm_block_norm_t* a) {
   return 0;
 }
 
-template <typename Y, typename Br, typename R, int VEC, int NV, int TPR>
-int launch(const mdmm_block_norm_t* a, int64_t grid, bool bwd, hipStream_t s) {
-  constexpr int NT = TPR > 256 ? TPR : 256;
-  if (bwd) hipLaunchKernelGGL((norm_bwd_kernel<Y, Br, R, VEC, NV, TPR>), dim3((unsigned)grid), dim3(NT), 0, s, *a);
-  else hipLaunchKernelGGL((norm_fwd_kernel<Y, Br, R, VEC, NV, TPR>), dim3((unsigned)grid), dim3(NT), 0, s, *a);
+template <typename Y, typename Br, typename R, int VEC, int NV, int MAXT>
+int launch(const mdmm_block_norm_t* a, int64_t grid, int threads, bool bwd, hipStream_t s) {
+  if (bwd) hipLaunchKernelGGL((norm_bwd_kernel<Y, Br, R, VEC, NV, MAXT>), dim3((unsigned)grid), dim3(threads), 0, s, *a);
+  else hipLaunchKernelGGL((norm_fwd_kernel<Y, Br, R, VEC, NV, MAXT>), dim3((unsigned)grid), dim3(threads), 0, s, *a);
   return (int)hipGetLastError();
 }
 
@@ -396,9 +474,9 @@ template <typename Y, typename Br, typename R>
 int dispatch(const mdmm_block_norm_t* a, bool bwd, hipStream_t s) {
   const Plan q = plan(a);
   const int64_t g = grid_of(a, q);
-#define CASE(v, n, t) if (q.vec == v && q.nv == n && q.tpr == t) return launch<Y, Br, R, v, n, t>(a, g, bwd, s)
-  CASE(4, 1, 64); CASE(4, 2, 64); CASE(4, 4, 64); CASE(4, 2, 256); CASE(4, 4, 256); CASE(4, 2, 1024);
-  CASE(1, 4, 64); CASE(1, 4, 256); CASE(1, 4, 1024); CASE(1, 8, 1024);
+#define CASE(v, n, t) if (q.vec == v && q.nv == n && q.maxt == t) return launch<Y, Br, R, v, n, t>(a, g, q.threads, bwd, s)
+  CASE(4, 1, 256); CASE(4, 1, 512); CASE(4, 2, 512); CASE(4, 2, 1024);
+  CASE(1, 4, 256); CASE(1, 4, 512); CASE(1, 4, 1024); CASE(1, 8, 1024);
 #undef CASE
   return MDMM_E_ARG;
 }
@@ -436,7 +514,7 @@ extern "C" int mdmm_block_norm_bwd(const mdmm_block_norm_t* a, void* stream) {
   const int e = run(a, true, (hipStream_t)stream);
   if (e) return e;
   if (!a->d_w && !a->d_scale && !a->d_w_next) return 0;
-  hipLaunchKernelGGL(norm_fold_kernel, dim3((3 * a->H + 15) / 16), dim3(256), 0, (hipStream_t)stream, a->ws,
+  hipLaunchKernelGGL(norm_fold_kernel, dim3((3 * a->H + 15) / 16), dim3(1024), 0, (hipStream_t)stream, a->ws,
                      (int)grid_of(a, plan(a)), a->H, a->d_w, a->d_scale, a->d_w_next);
   return (int)hipGetLastError();
 }
