@@ -10,89 +10,101 @@
 namespace mdmm {
 namespace {
 
-// VEC columns as loaded
-template <typename T, int VEC> struct Raw { T x; };
-template <> struct Raw<float, 4> { float4 x; };
-template <> struct Raw<__bf16, 4> { uint2 x; };
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-template <int VEC> __device__ __forceinline__ void widen(const Raw<float, VEC>& r, float* v) {
-  if constexpr (VEC == 4) { v[0] = r.x.x; v[1] = r.x.y; v[2] = r.x.z; v[3] = r.x.w; }
-  else v[0] = r.x;
+// VEC columns as loaded
+template <typename T, int VEC> struct Raw;
+template <> struct Raw<float, 4> { u32x4 x; };
+template <> struct Raw<float, 1> { unsigned x; };
+template <> struct Raw<__bf16, 4> { u32x2 x; };
+template <> struct Raw<__bf16, 1> { unsigned short x; };
+
+template <int VEC> __device__ __forceinline__ void widen(const Raw<float, VEC>& r, float* v) { __builtin_memcpy(v, &r, sizeof r); }
+__device__ __forceinline__ void widen(const Raw<__bf16, 4>& r, float* v) {
+  v[0] = __uint_as_float(r.x[0] << 16); v[1] = __uint_as_float(r.x[0] & 0xffff0000u);
+  v[2] = __uint_as_float(r.x[1] << 16); v[3] = __uint_as_float(r.x[1] & 0xffff0000u);
 }
-template <int VEC> __device__ __forceinline__ void widen(const Raw<__bf16, VEC>& r, float* v) {
-  if constexpr (VEC == 4) {
-    v[0] = __uint_as_float(r.x.x << 16); v[1] = __uint_as_float(r.x.x & 0xffff0000u);
-    v[2] = __uint_as_float(r.x.y << 16); v[3] = __uint_as_float(r.x.y & 0xffff0000u);
-  } else v[0] = (float)r.x;
-}
-template <int VEC> __device__ __forceinline__ void load_v(const float* p, float* v) { widen(*(const Raw<float, VEC>*)p, v); }
+__device__ __forceinline__ void widen(const Raw<__bf16, 1>& r, float* v) { v[0] = __uint_as_float((unsigned)r.x << 16); }
+
+// One row of a tensor as a buffer of its H columns (none: H = 0): a read past the end gives 0 and a write there is dropped by
+// the address check, so no piece needs a branch -- with branches around the stores the compiler waits for ALL memory
+// operations before it uses the row fetched ahead, the present row's stores among them
+template <typename T, int VEC> struct Row {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ Row(const void* base, int64_t at, int H)
+      : r(__builtin_amdgcn_make_buffer_rsrc((void*)((T*)base + at), 0, base ? H * (int)sizeof(T) : 0, 0x00020000)) {}
+  __device__ __forceinline__ void get(Raw<T, VEC>& v, int c) const {
+    if constexpr (sizeof(v) == 16) v.x = __builtin_amdgcn_raw_buffer_load_b128(r, c * (int)sizeof(T), 0, 0);
+    else if constexpr (sizeof(v) == 8) v.x = __builtin_amdgcn_raw_buffer_load_b64(r, c * (int)sizeof(T), 0, 0);
+    else if constexpr (sizeof(v) == 4) v.x = __builtin_amdgcn_raw_buffer_load_b32(r, c * (int)sizeof(T), 0, 0);
+    else v.x = __builtin_amdgcn_raw_buffer_load_b16(r, c * (int)sizeof(T), 0, 0);
+  }
+  __device__ __forceinline__ void put(const float* f, int c) const {
+    Raw<T, VEC> v;
+    T t[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) t[e] = (T)f[e];          // (bf16: to nearest, ties to even)
+    __builtin_memcpy(&v, t, sizeof v);
+    if constexpr (sizeof(v) == 16) __builtin_amdgcn_raw_buffer_store_b128(v.x, r, c * (int)sizeof(T), 0, 0);
+    else if constexpr (sizeof(v) == 8) __builtin_amdgcn_raw_buffer_store_b64(v.x, r, c * (int)sizeof(T), 0, 0);
+    else if constexpr (sizeof(v) == 4) __builtin_amdgcn_raw_buffer_store_b32(v.x, r, c * (int)sizeof(T), 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(v.x, r, c * (int)sizeof(T), 0, 0);
+  }
+};
 
 // A thread's pieces of a vector over the columns, kept in registers over all rows (read again for each row, the three vectors
 // in fp32 are more bytes than a bf16 row); `none` where it is not there
 template <int VEC, int NV>
-__device__ __forceinline__ void keep(float (&v)[NV][VEC], const float* base, float none, int lane, int tpr, int H) {
+__device__ __forceinline__ void keep(float (&v)[NV][VEC], const float* base, float none, const int (&c)[NV], int H) {
+  const Row<float, VEC> row(base, 0, H);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int c = (k * tpr + lane) * VEC;
+    Raw<float, VEC> x;
+    row.get(x, c[k]);
+    widen(x, v[k]);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) v[k][e] = none;
-    if (base && c < H) load_v<VEC>(base + c, v[k]);
+    for (int e = 0; e < VEC; ++e) v[k][e] = base ? v[k][e] : none;
   }
 }
 
-// A row's pieces of one tensor; columns past the end (and a tensor that is not there) are zeros
 template <typename T, int VEC, int NV>
-__device__ __forceinline__ void fetch(Raw<T, VEC> (&r)[NV], const void* base, int64_t at, int lane, int tpr, int H) {
+__device__ __forceinline__ void fetch(Raw<T, VEC> (&r)[NV], const void* base, int64_t at, const int (&c)[NV], int H) {
+  const Row<T, VEC> row(base, at, H);
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (k * tpr + lane) * VEC;
-    r[k] = Raw<T, VEC>{};
-    if (base && c < H) r[k] = *(const Raw<T, VEC>*)((const T*)base + at + c);
-  }
+  for (int k = 0; k < NV; ++k) row.get(r[k], c[k]);
 }
 
-template <int VEC> __device__ __forceinline__ void store_v(float* p, const float* v) {
-  if constexpr (VEC == 4) *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
-  else *p = v[0];
-}
-template <int VEC> __device__ __forceinline__ void store_v(__bf16* p, const float* v) {
-  if constexpr (VEC == 4) {
-    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-    bf16x4 x;
-    x[0] = (__bf16)v[0]; x[1] = (__bf16)v[1]; x[2] = (__bf16)v[2]; x[3] = (__bf16)v[3];
-    *(bf16x4*)p = x;
-  } else *p = (__bf16)v[0];
-}
-
-// sum over the wave, in every lane: rows of 16 by DPP moves (no LDS round trip), then across the four rows
+// sum over rows of 16 lanes by DPP moves (no LDS round trip), in each of them
 template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_add(float v) {
   return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false));
 }
-__device__ __forceinline__ float wave_total(float v) {
+__device__ __forceinline__ float row16_total(float v) {
   v = dpp_add<0xb1, 0xf>(v);        // neighbours
   v = dpp_add<0x4e, 0xf>(v);        // pairs
   v = dpp_add<0x141, 0xf>(v);       // half rows mirrored
-  v = dpp_add<0x140, 0xf>(v);       // rows mirrored: every lane holds its row's sum
+  return dpp_add<0x140, 0xf>(v);    // rows mirrored
+}
+__device__ __forceinline__ float wave_total(float v) {
+  v = row16_total(v);
   v = dpp_add<0x142, 0xa>(v);       // row 0 into row 1, row 2 into row 3
   v = dpp_add<0x143, 0xc>(v);       // rows 0 and 1 into rows 2 and 3: lane 63 holds the sum
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
-// N sums over a row's threads (a wave, or WIDE the workgroup), in every one of them
+// N sums over a row's threads (a wave, or WIDE the workgroup of up to 16 waves), in every one of them.  lds: 2 sets of
+// 2 x 16 words, the words past the last wave zero (a wave that runs ahead writes the other set)
 template <bool WIDE, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float* lds, int& slot) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = wave_total(v[i]);
   if constexpr (WIDE) {
-    const int W = blockDim.x >> 6;
-    float* s = lds + (slot ^= 1) * 2 * W;       // (two sets: a wave that runs ahead writes the other one)
+    float* s = lds + (slot ^= 1) * 32;
     if ((threadIdx.x & 63) == 0)
-      for (int i = 0; i < N; ++i) s[i * W + (threadIdx.x >> 6)] = v[i];
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i * 16 + (threadIdx.x >> 6)] = v[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[i] = 0.0f;
-      for (int w = 0; w < W; ++w) v[i] += s[i * W + w];
-    }
+    for (int i = 0; i < N; ++i) v[i] = row16_total(s[i * 16 + (threadIdx.x & 15)]);
   }
 }
 template <bool WIDE> __device__ __forceinline__ float row_sum(float v, float* lds, int& slot) {
@@ -100,205 +112,201 @@ template <bool WIDE> __device__ __forceinline__ float row_sum(float v, float* ld
   row_sums<WIDE, 1>(a, lds, slot);
   return a[0];
 }
+template <bool WIDE> __device__ __forceinline__ void clear_sums(float* lds) {
+  if constexpr (WIDE) {
+    if (threadIdx.x < 64) lds[threadIdx.x] = 0.0f;
+    __syncthreads();
+  }
+}
 
-template <typename Y, typename Br, typename R, int VEC, int NV, int MAXT>
+template <typename Y, typename Br, typename R, int VEC, int NV, int MAXT, bool ALL>
 __global__ __launch_bounds__(MAXT) void norm_fwd_kernel(mdmm_block_norm_t p) {
   constexpr bool WIDE = MAXT > 256;
-  constexpr int RPW = WIDE ? 1 : 4;
-  __shared__ float lds[WIDE ? MAXT / 16 : 1];
-  int slot = 0;
-  const int tpr = WIDE ? (int)blockDim.x : 64, lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x & 63);
+  __shared__ float lds[64];
+  clear_sums<WIDE>(lds);
+  int slot = 0, c[NV];
+  const int lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x & 63), tpr = WIDE ? (int)blockDim.x : 64;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) c[k] = (k * tpr + lane) * VEC;
   const float inv = 1.0f / (float)p.H;
-  const int64_t step = (int64_t)gridDim.x * RPW;
-  int64_t row = (int64_t)blockIdx.x * RPW + (WIDE ? 0 : threadIdx.x >> 6);
+  const int wave = WIDE ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t step = (int64_t)gridDim.x * (WIDE ? 1 : 4);
+  int64_t row = (int64_t)blockIdx.x * (WIDE ? 1 : 4) + wave;
   float w[NV][VEC], s[NV][VEC], wn[NV][VEC];
-  keep<VEC, NV>(w, p.w, 0.0f, lane, tpr, p.H);
-  keep<VEC, NV>(s, p.scale, 1.0f, lane, tpr, p.H);
-  keep<VEC, NV>(wn, p.w_next, 0.0f, lane, tpr, p.H);
+  keep<VEC, NV>(w, p.w, 0.0f, c, p.H);
+  keep<VEC, NV>(s, p.scale, 1.0f, c, p.H);
+  keep<VEC, NV>(wn, p.w_next, 0.0f, c, p.H);
   Raw<R, VEC> res[NV];
   Raw<Y, VEC> ry[NV];
   Raw<Br, VEC> rg[NV];
-  if (row < p.rows) {
-    fetch<R, VEC, NV>(res, p.res, row * p.res_st, lane, tpr, p.H);
-    fetch<Y, VEC, NV>(ry, p.y, row * p.y_st, lane, tpr, p.H);
-    fetch<Br, VEC, NV>(rg, p.gate, row * p.gate_st, lane, tpr, p.H);
-  }
+  auto fetch_row = [&](int64_t at) {         // (past the last row: empty rows)
+    const int H = at < p.rows ? p.H : 0;
+    if (ALL || p.y) fetch<Y, VEC, NV>(ry, p.y, at * p.y_st, c, H);
+    if (ALL || p.gate) fetch<Br, VEC, NV>(rg, p.gate, at * p.gate_st, c, H);
+    fetch<R, VEC, NV>(res, p.res, at * p.res_st, c, H);
+  };
+  fetch_row(row);
   for (; row < p.rows; row += step) {
     float o[NV][VEC], y[NV][VEC], g[NV][VEC];
     float ss = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       widen(res[k], o[k]);
-      widen(ry[k], y[k]);
-      widen(rg[k], g[k]);
+      if (ALL || p.y) widen(ry[k], y[k]);
+      if (ALL || p.gate) widen(rg[k], g[k]);
+      if (ALL || p.y)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) ss += y[k][e] * y[k][e];
+        for (int e = 0; e < VEC; ++e) ss += y[k][e] * y[k][e];
     }
-    if (row + step < p.rows) {           // the next row's pieces, in flight behind this one's arithmetic
-      fetch<R, VEC, NV>(res, p.res, (row + step) * p.res_st, lane, tpr, p.H);
-      fetch<Y, VEC, NV>(ry, p.y, (row + step) * p.y_st, lane, tpr, p.H);
-      fetch<Br, VEC, NV>(rg, p.gate, (row + step) * p.gate_st, lane, tpr, p.H);
-    }
-    if (p.y) {
+    fetch_row(row + step);                   // in flight behind this row's arithmetic
+    if (ALL || p.y) {
       const float r = rsqrtf(row_sum<WIDE>(ss, lds, slot) * inv + p.eps);
+      const Row<R, VEC> out(p.out, row * p.out_st, p.H);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * tpr + lane) * VEC;
-        if (c < p.H) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            float u = y[k][e] * r * w[k][e];
-            if (p.gate) u *= g[k][e] * sigmoid_(g[k][e]);
-            o[k][e] = fmaf(s[k][e], u, o[k][e]);
-          }
-          store_v<VEC>((R*)p.out + row * p.out_st + c, o[k]);
+        for (int e = 0; e < VEC; ++e) {
+          float u = y[k][e] * r * w[k][e];
+          if (ALL || p.gate) u *= g[k][e] * sigmoid_(g[k][e]);
+          o[k][e] = fmaf(s[k][e], u, o[k][e]);
         }
+        out.put(o[k], c[k]);
       }
     }
-    if (p.w_next) {
+    if (ALL || p.w_next) {
       ss = 0.0f;
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) ss += o[k][e] * o[k][e];
       const float r = rsqrtf(row_sum<WIDE>(ss, lds, slot) * inv + p.eps);
+      const Row<Br, VEC> n(p.n, row * p.n_st, p.H);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * tpr + lane) * VEC;
-        if (c < p.H) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) o[k][e] *= r * wn[k][e];
-          store_v<VEC>((Br*)p.n + row * p.n_st + c, o[k]);
-        }
+        for (int e = 0; e < VEC; ++e) o[k][e] *= r * wn[k][e];
+        n.put(o[k], c[k]);
       }
     }
   }
 }
 
-template <typename Y, typename Br, typename R, int VEC, int NV, int MAXT>
-__global__ __launch_bounds__(MAXT) void norm_bwd_kernel(mdmm_block_norm_t p) {
+template <typename Y, typename Br, typename R, int VEC, int NV, int MAXT, bool ALL>
+__global__ __launch_bounds__(MAXT, MAXT == 512 && NV * VEC == 4 ? (sizeof(Y) + sizeof(R) == 4 ? 5 : 4) : 1)
+void norm_bwd_kernel(mdmm_block_norm_t p) {
   constexpr bool WIDE = MAXT > 256;
-  constexpr int RPW = WIDE ? 1 : 4;
-  __shared__ float lds[WIDE ? MAXT / 16 : 1];
+  __shared__ float lds[64];
   __shared__ float fold[WIDE ? 1 : 256 * VEC];
-  int slot = 0;
-  const int tpr = WIDE ? (int)blockDim.x : 64, lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x & 63);
+  clear_sums<WIDE>(lds);
+  int slot = 0, c[NV];
+  const int lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x & 63), tpr = WIDE ? (int)blockDim.x : 64;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) c[k] = (k * tpr + lane) * VEC;
   const float inv = 1.0f / (float)p.H;
-  const int64_t step = (int64_t)gridDim.x * RPW;
-  int64_t row = (int64_t)blockIdx.x * RPW + (WIDE ? 0 : threadIdx.x >> 6);
+  const int wave = WIDE ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t step = (int64_t)gridDim.x * (WIDE ? 1 : 4);
+  int64_t row = (int64_t)blockIdx.x * (WIDE ? 1 : 4) + wave;
   float aw[NV][VEC] = {}, as[NV][VEC] = {}, an[NV][VEC] = {};
   float w[NV][VEC], s[NV][VEC], wn[NV][VEC];
-  keep<VEC, NV>(w, p.w, 0.0f, lane, tpr, p.H);
-  keep<VEC, NV>(s, p.scale, 1.0f, lane, tpr, p.H);
-  keep<VEC, NV>(wn, p.w_next, 0.0f, lane, tpr, p.H);
+  keep<VEC, NV>(w, p.w, 0.0f, c, p.H);
+  keep<VEC, NV>(s, p.scale, 1.0f, c, p.H);
+  keep<VEC, NV>(wn, p.w_next, 0.0f, c, p.H);
   Raw<R, VEC> res[NV], rd[NV];
   Raw<Y, VEC> ry[NV];
   Raw<Br, VEC> rg[NV], rq[NV];
-  auto fetch_row = [&](int64_t at) {
-    fetch<Y, VEC, NV>(ry, p.y, at * p.y_st, lane, tpr, p.H);
-    fetch<Br, VEC, NV>(rg, p.gate, at * p.gate_st, lane, tpr, p.H);
-    if (p.g_n) fetch<R, VEC, NV>(res, p.res, at * p.res_st, lane, tpr, p.H);      // (read for the next norm alone)
-    fetch<Br, VEC, NV>(rq, p.g_n, at * p.g_n_st, lane, tpr, p.H);
-    fetch<R, VEC, NV>(rd, p.g_out, at * p.g_out_st, lane, tpr, p.H);
+  auto fetch_row = [&](int64_t at) {         // (past the last row: empty rows)
+    const int H = at < p.rows ? p.H : 0;
+    if (ALL || p.y) fetch<Y, VEC, NV>(ry, p.y, at * p.y_st, c, H);
+    if (ALL || p.gate) fetch<Br, VEC, NV>(rg, p.gate, at * p.gate_st, c, H);
+    if (ALL || p.g_n) fetch<R, VEC, NV>(res, p.res, at * p.res_st, c, H);      // (read for the next norm alone)
+    if (ALL || p.g_n) fetch<Br, VEC, NV>(rq, p.g_n, at * p.g_n_st, c, H);
+    fetch<R, VEC, NV>(rd, p.g_out, at * p.g_out_st, c, H);
   };
-  if (row < p.rows) fetch_row(row);
+  fetch_row(row);
   for (; row < p.rows; row += step) {
     float x[NV][VEC], g[NV][VEC], sg[NV][VEC], o[NV][VEC], q[NV][VEC], d[NV][VEC];
     float ss = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      widen(ry[k], x[k]);
-      widen(rg[k], g[k]);
-      if (p.g_n) widen(res[k], o[k]);
-      widen(rq[k], q[k]);
+      if (ALL || p.y) widen(ry[k], x[k]);
+      if (ALL || p.gate) widen(rg[k], g[k]);
+      if (ALL || p.g_n) widen(res[k], o[k]);
+      if (ALL || p.g_n) widen(rq[k], q[k]);
       widen(rd[k], d[k]);
+      if (ALL || p.y)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) ss += x[k][e] * x[k][e];
+        for (int e = 0; e < VEC; ++e) ss += x[k][e] * x[k][e];
     }
-    if (row + step < p.rows) fetch_row(row + step);       // in flight behind this row's arithmetic
+    fetch_row(row + step);                   // in flight behind this row's arithmetic
     float r = 0.0f;
-    if (p.y) {
+    if (ALL || p.y) {
       r = rsqrtf(row_sum<WIDE>(ss, lds, slot) * inv + p.eps);
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           x[k][e] *= r;
-          sg[k][e] = p.gate ? sigmoid_(g[k][e]) : 1.0f;
+          sg[k][e] = (ALL || p.gate) ? sigmoid_(g[k][e]) : 1.0f;
         }
     }
-    if (p.g_n) {
+    if (ALL || p.g_n) {
       float sums[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (k * tpr + lane) * VEC;
-        if (c < p.H) {
+      for (int k = 0; k < NV; ++k)
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            if (p.y) {
-              float u = x[k][e] * w[k][e];
-              if (p.gate) u *= g[k][e] * sg[k][e];
-              o[k][e] = fmaf(s[k][e], u, o[k][e]);
-            }
-            sums[0] += o[k][e] * o[k][e];
-            sums[1] += q[k][e] * wn[k][e] * o[k][e];
+        for (int e = 0; e < VEC; ++e) {
+          if (ALL || p.y) {
+            float u = x[k][e] * w[k][e];
+            if (ALL || p.gate) u *= g[k][e] * sg[k][e];
+            o[k][e] = fmaf(s[k][e], u, o[k][e]);
           }
+          sums[0] += o[k][e] * o[k][e];
+          sums[1] += q[k][e] * wn[k][e] * o[k][e];
         }
-      }
       row_sums<WIDE, 2>(sums, lds, slot);
       const float r2 = rsqrtf(sums[0] * inv + p.eps), m = sums[1] * inv * r2 * r2;
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (k * tpr + lane) * VEC;
-        if (c < p.H) {
+      for (int k = 0; k < NV; ++k)
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            an[k][e] += q[k][e] * o[k][e] * r2;
-            d[k][e] += r2 * (q[k][e] * wn[k][e] - o[k][e] * m);
-          }
+        for (int e = 0; e < VEC; ++e) {
+          an[k][e] += q[k][e] * o[k][e] * r2;
+          d[k][e] += r2 * (q[k][e] * wn[k][e] - o[k][e] * m);
         }
-      }
     }
-    if (p.d_res) {
+    if (ALL || p.d_res) {
+      const Row<R, VEC> out(p.d_res, row * p.d_res_st, p.H);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (k * tpr + lane) * VEC;
-        if (c < p.H) store_v<VEC>((R*)p.d_res + row * p.d_res_st + c, d[k]);
-      }
+      for (int k = 0; k < NV; ++k) out.put(d[k], c[k]);
     }
-    if (p.y) {
+    if (ALL || p.y) {
       float sm = 0.0f;
+      const Row<Br, VEC> out(p.d_gate, row * p.d_gate_st, p.H);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (k * tpr + lane) * VEC;
-        if (c < p.H) {
-          float dg[VEC];
+        float dg[VEC];
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            // act = silu(g) = g sg, slope = silu'(g) = sg + act (1 - sg)
-            const float act = p.gate ? g[k][e] * sg[k][e] : 1.0f;
-            const float u = x[k][e] * w[k][e], ds = d[k][e] * s[k][e];
-            as[k][e] += d[k][e] * act * u;
-            dg[e] = ds * u * fmaf(-act, sg[k][e], sg[k][e] + act);
-            const float t = ds * act;
-            aw[k][e] += t * x[k][e];
-            d[k][e] = t * w[k][e];
-            sm += d[k][e] * x[k][e];
-          }
-          if (p.d_gate) store_v<VEC>((Br*)p.d_gate + row * p.d_gate_st + c, dg);
+        for (int e = 0; e < VEC; ++e) {
+          // act = silu(g) = g sg, slope = silu'(g) = sg + act (1 - sg)
+          const float act = (ALL || p.gate) ? g[k][e] * sg[k][e] : 1.0f;
+          const float u = x[k][e] * w[k][e], ds = d[k][e] * s[k][e];
+          as[k][e] += d[k][e] * act * u;
+          dg[e] = ds * u * fmaf(-act, sg[k][e], sg[k][e] + act);
+          const float t = ds * act;
+          aw[k][e] += t * x[k][e];
+          d[k][e] = t * w[k][e];
+          sm += d[k][e] * x[k][e];
         }
+        if (ALL || p.d_gate) out.put(dg, c[k]);
       }
       sm = row_sum<WIDE>(sm, lds, slot) * inv;
-      if (p.d_y) {
+      if (ALL || p.d_y) {
+        const Row<Y, VEC> dst(p.d_y, row * p.d_y_st, p.H);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-          const int c = (k * tpr + lane) * VEC;
-          if (c < p.H) {
-            float dy[VEC];
+          float dy[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) dy[e] = r * (d[k][e] - x[k][e] * sm);
-            store_v<VEC>((Y*)p.d_y + row * p.d_y_st + c, dy);
-          }
+          for (int e = 0; e < VEC; ++e) dy[e] = r * (d[k][e] - x[k][e] * sm);
+          dst.put(dy, c[k]);
         }
       }
     }
@@ -310,23 +318,19 @@ __global__ __launch_bounds__(MAXT) void norm_bwd_kernel(mdmm_block_norm_t p) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float (&acc)[VEC] = which == 0 ? aw[k] : which == 1 ? as[k] : an[k];
-      if constexpr (RPW > 1) {
+      if constexpr (!WIDE) {
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < VEC; ++e) fold[threadIdx.x * VEC + e] = acc[e];
         __syncthreads();
-        for (int i = threadIdx.x; i < 64 * VEC; i += 256) {
-          const int c = k * 64 * VEC + i;
-          if (c < p.H) {
-            float s = 0.0f;
-            for (int w = 0; w < RPW; ++w) s += fold[w * 64 * VEC + i];
-            slab[which * p.H + c] = s;
-          }
+        if (threadIdx.x < 64 * VEC) {
+          const int i = threadIdx.x, col = k * 64 * VEC + i;
+          if (col < p.H) slab[which * p.H + col] = fold[i] + fold[64 * VEC + i] + fold[128 * VEC + i] + fold[192 * VEC + i];
         }
       } else {
-        const int c = (k * tpr + lane) * VEC;
-        if (c < p.H)
-          for (int e = 0; e < VEC; ++e) slab[which * p.H + c + e] = acc[e];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (c[k] + e < p.H) slab[which * p.H + c[k] + e] = acc[e];
       }
     }
 }
@@ -335,7 +339,8 @@ __global__ __launch_bounds__(MAXT) void norm_bwd_kernel(mdmm_block_norm_t p) {
 template <typename Br, typename R, int NV, int TPR>
 __global__ __launch_bounds__(TPR) void step_kernel(mdmm_gated_scan_t q, mdmm_block_norm_t p) {
   constexpr bool WIDE = TPR > 64;
-  __shared__ float lds[4 * (TPR / 64)];
+  __shared__ float lds[64];
+  clear_sums<WIDE>(lds);
   int slot = 0;
   const int64_t b = blockIdx.x;
   const float inv = 1.0f / (float)p.H;
@@ -445,10 +450,17 @@ Plan plan(const mdmm_block_norm_t* a) {
   return {1, 8, 1024, u8};
 }
 
-int64_t grid_of(const mdmm_block_norm_t* a, const Plan& q) {
-  const int rpw = q.maxt == 256 ? 4 : 1;
-  const int64_t g = (a->rows + rpw - 1) / rpw;
-  return g < 1024 ? g : 1024;
+// Workgroups: as many as the registers let the chip hold at once (16 or, bf16 backward, 20 waves a CU), each walking over
+// rows -- a few more than that would run as a second, nearly empty round (1024 workgroups where 768 fit: 480 us instead of
+// 383 at 65536 x 1280) -- and no more than one for eight rows beyond 1024 of them (each leaves a slab of 3 H sums)
+int64_t grid_of(const mdmm_block_norm_t* a, const Plan& q, bool bwd) {
+  const int rpw = q.maxt == 256 ? 4 : 1, waves = q.threads / 64;
+  const int64_t need = (a->rows + rpw - 1) / rpw;
+  const int per_cu = ((bwd ? a->y_bf16 && a->res_bf16 && q.maxt == 512 && q.nv * q.vec == 4 : false) ? 20 : 16) / waves;
+  int64_t top = 256 * (int64_t)(per_cu > 0 ? per_cu : 1);
+  if (top > 1024 && top > need / 8) top = need / 8 > 1024 ? need / 8 : 1024;
+  if (top > 2048) top = 2048;
+  return need < top ? need : top;
 }
 
 int check(const mdmm_block_norm_t* a) {
@@ -463,17 +475,26 @@ int check(const mdmm_block_norm_t* a) {
   return 0;
 }
 
+// every operand of a whole block there: a variant without the tests for what is missing
+bool whole(const mdmm_block_norm_t* a, bool bwd) {
+  return a->y && a->gate && a->w_next && (!bwd || (a->g_out && a->g_n && a->d_y && a->d_gate && a->d_res));
+}
+
 template <typename Y, typename Br, typename R, int VEC, int NV, int MAXT>
 int launch(const mdmm_block_norm_t* a, int64_t grid, int threads, bool bwd, hipStream_t s) {
-  if (bwd) hipLaunchKernelGGL((norm_bwd_kernel<Y, Br, R, VEC, NV, MAXT>), dim3((unsigned)grid), dim3(threads), 0, s, *a);
-  else hipLaunchKernelGGL((norm_fwd_kernel<Y, Br, R, VEC, NV, MAXT>), dim3((unsigned)grid), dim3(threads), 0, s, *a);
+  const dim3 g((unsigned)grid), t(threads);
+  const bool all = whole(a, bwd);
+  if (bwd && all) hipLaunchKernelGGL((norm_bwd_kernel<Y, Br, R, VEC, NV, MAXT, true>), g, t, 0, s, *a);
+  else if (bwd) hipLaunchKernelGGL((norm_bwd_kernel<Y, Br, R, VEC, NV, MAXT, false>), g, t, 0, s, *a);
+  else if (all) hipLaunchKernelGGL((norm_fwd_kernel<Y, Br, R, VEC, NV, MAXT, true>), g, t, 0, s, *a);
+  else hipLaunchKernelGGL((norm_fwd_kernel<Y, Br, R, VEC, NV, MAXT, false>), g, t, 0, s, *a);
   return (int)hipGetLastError();
 }
 
 template <typename Y, typename Br, typename R>
 int dispatch(const mdmm_block_norm_t* a, bool bwd, hipStream_t s) {
   const Plan q = plan(a);
-  const int64_t g = grid_of(a, q);
+  const int64_t g = grid_of(a, q, bwd);
 #define CASE(v, n, t) if (q.vec == v && q.nv == n && q.maxt == t) return launch<Y, Br, R, v, n, t>(a, g, q.threads, bwd, s)
   CASE(4, 1, 256); CASE(4, 1, 512); CASE(4, 2, 512); CASE(4, 2, 1024);
   CASE(1, 4, 256); CASE(1, 4, 512); CASE(1, 4, 1024); CASE(1, 8, 1024);
@@ -495,7 +516,7 @@ using namespace mdmm;
 
 extern "C" int64_t mdmm_block_norm_ws(const mdmm_block_norm_t* a) {
   if (check(a)) return -1;
-  return (a->rows < 1024 ? a->rows : 1024) * 3 * a->H;       // (the most workgroups any plan takes)
+  return (a->rows < 2048 ? a->rows : 2048) * 3 * a->H;       // (the most workgroups any plan takes)
 }
 
 extern "C" int mdmm_block_norm_fwd(const mdmm_block_norm_t* a, void* stream) {
@@ -515,7 +536,7 @@ extern "C" int mdmm_block_norm_bwd(const mdmm_block_norm_t* a, void* stream) {
   if (e) return e;
   if (!a->d_w && !a->d_scale && !a->d_w_next) return 0;
   hipLaunchKernelGGL(norm_fold_kernel, dim3((3 * a->H + 15) / 16), dim3(1024), 0, (hipStream_t)stream, a->ws,
-                     (int)grid_of(a, plan(a)), a->H, a->d_w, a->d_scale, a->d_w_next);
+                     (int)grid_of(a, plan(a), true), a->H, a->d_w, a->d_scale, a->d_w_next);
   return (int)hipGetLastError();
 }
 

@@ -29,6 +29,9 @@ struct Gate {
   }
 };
 
-__device__ __forceinline__ float sigmoid_(float x) { return Gate(x).a; }
+// sigmoid alone: 1 / (1 + exp(-x)), relative error 6e-8 (1 + |x|); exp may overflow to infinity (then 0)
+__device__ __forceinline__ float sigmoid_(float x) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f));
+}
 
 }  // namespace mdmm
