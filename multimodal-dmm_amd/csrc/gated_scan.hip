@@ -4,7 +4,7 @@
 //
 // Bound by HBM: forward reads f, c and writes h, backward reads f, c, g and writes df, dc; neither keeps h (the backward
 // pass forms it again from one state per tile of time).  A step h -> a h + b composes, (a2, b2)(a1, b1) = (a2 a1, a2 b1 + b2), so time is
-// taken in tiles: a workgroup of up to 8 waves holds 64 VEC channels and a tile of 8 waves x 8 steps in registers, each wave
+// taken in tiles: a workgroup of up to 8 waves holds 64 VEC channels and a tile of 8 steps a wave in registers, each wave
 // composes its 8 steps, the pieces meet in LDS, and every wave then runs its steps from the state in front of them.  Every
 // load of a tile is in flight at once, each tensor passes once, and the next tile's loads are issued before the present
 // tile's are used up.  Where the channels alone do not fill the chip, time is also split over workgroups: a first launch
@@ -15,131 +15,208 @@
 namespace mdmm {
 namespace {
 
-constexpr int S = 8, WMAX = 8, TILE = S * WMAX;      // steps of a wave, waves, steps of a tile
+// steps of a wave; most waves; steps between two states kept for the backward pass (its tiles, above KEEP2 steps)
+constexpr int S = 8, WMAX = 8, KEEP = 32, KEEP2 = 64;
 
-template <typename IO, int VEC> struct Raw;          // VEC elements as loaded
-template <> struct Raw<float, 1> { float x; };
-template <> struct Raw<float, 2> { float2 x; };
-template <> struct Raw<float, 4> { float4 x; };
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T, int VEC> struct Raw;           // VEC elements as loaded
+template <> struct Raw<float, 1> { unsigned x; };
+template <> struct Raw<float, 2> { u32x2 x; };
+template <> struct Raw<float, 4> { u32x4 x; };
 template <> struct Raw<__bf16, 1> { unsigned short x; };
 template <> struct Raw<__bf16, 2> { unsigned x; };
-template <> struct Raw<__bf16, 4> { uint2 x; };
+template <> struct Raw<__bf16, 4> { u32x2 x; };
 
-__device__ __forceinline__ void widen(const Raw<float, 1>& r, float* v) { v[0] = r.x; }
-__device__ __forceinline__ void widen(const Raw<float, 2>& r, float* v) { v[0] = r.x.x; v[1] = r.x.y; }
-__device__ __forceinline__ void widen(const Raw<float, 4>& r, float* v) { v[0] = r.x.x; v[1] = r.x.y; v[2] = r.x.z; v[3] = r.x.w; }
-__device__ __forceinline__ void widen(const Raw<__bf16, 1>& r, float* v) { v[0] = __uint_as_float((unsigned)r.x << 16); }
+template <int VEC> __device__ __forceinline__ void widen(const Raw<float, VEC>& r, float* v) { __builtin_memcpy(v, &r, sizeof r); }
 __device__ __forceinline__ void widen2(unsigned x, float* v) { v[0] = __uint_as_float(x << 16); v[1] = __uint_as_float(x & 0xffff0000u); }
+__device__ __forceinline__ void widen(const Raw<__bf16, 1>& r, float* v) { v[0] = __uint_as_float((unsigned)r.x << 16); }
 __device__ __forceinline__ void widen(const Raw<__bf16, 2>& r, float* v) { widen2(r.x, v); }
-__device__ __forceinline__ void widen(const Raw<__bf16, 4>& r, float* v) { widen2(r.x.x, v); widen2(r.x.y, v + 2); }
+__device__ __forceinline__ void widen(const Raw<__bf16, 4>& r, float* v) { widen2(r.x[0], v); widen2(r.x[1], v + 2); }
 
-template <int VEC> __device__ __forceinline__ void put(float* p, const float* v) {
-  Raw<float, VEC> r;
-  __builtin_memcpy(&r, v, sizeof r);
-  *(Raw<float, VEC>*)p = r;
-}
-template <int VEC> __device__ __forceinline__ void put(__bf16* p, const float* v) {
-  __bf16 t[VEC];
+template <typename T, int VEC> __device__ __forceinline__ Raw<T, VEC> narrow(const float* v) {
+  T t[VEC];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) t[e] = (__bf16)v[e];
-  Raw<__bf16, VEC> r;
+  for (int e = 0; e < VEC; ++e) t[e] = (T)v[e];      // (bf16: to nearest, ties to even)
+  Raw<T, VEC> r;
   __builtin_memcpy(&r, t, sizeof r);
-  *(Raw<__bf16, VEC>*)p = r;
+  return r;
 }
+
+// One time step of a tensor.  BUF: a buffer from its first element on, addressed by 32-bit byte offsets; `live` false makes
+// it empty, an empty step's reads give 0 and its writes are dropped, as are those of a thread without channels (its offset is
+// past every end), so no access needs a branch and the compiler can count what is in flight.  Else (a step's elements 2 GiB
+// apart, as in a long batch-first tensor): pointers, 64-bit offsets, branches.
+template <typename T, int VEC, bool BUF> struct Step;
+template <typename T, int VEC> struct Step<T, VEC, true> {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ Step(const void* base, int64_t at, bool live)
+      : r(__builtin_amdgcn_make_buffer_rsrc((void*)((T*)base + at), 0, live && base ? 0x7fffffff : 0, 0x00020000)) {}
+  __device__ __forceinline__ Raw<T, VEC> get(unsigned o) const {
+    Raw<T, VEC> v;
+    if constexpr (sizeof(v) == 16) v.x = __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0);
+    else if constexpr (sizeof(v) == 8) v.x = __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0);
+    else if constexpr (sizeof(v) == 4) v.x = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
+    else v.x = __builtin_amdgcn_raw_buffer_load_b16(r, o, 0, 0);
+    return v;
+  }
+  __device__ __forceinline__ void put(unsigned o, const float* f) const {
+    const Raw<T, VEC> v = narrow<T, VEC>(f);
+    if constexpr (sizeof(v) == 16) __builtin_amdgcn_raw_buffer_store_b128(v.x, r, o, 0, 0);
+    else if constexpr (sizeof(v) == 8) __builtin_amdgcn_raw_buffer_store_b64(v.x, r, o, 0, 0);
+    else if constexpr (sizeof(v) == 4) __builtin_amdgcn_raw_buffer_store_b32(v.x, r, o, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(v.x, r, o, 0, 0);
+  }
+};
+template <typename T, int VEC> struct Step<T, VEC, false> {
+  char* p;
+  __device__ __forceinline__ Step(const void* base, int64_t at, bool live) : p(live && base ? (char*)((T*)base + at) : nullptr) {}
+  __device__ __forceinline__ Raw<T, VEC> get(int64_t o) const { return p && o >= 0 ? *(const Raw<T, VEC>*)(p + o) : Raw<T, VEC>{}; }
+  __device__ __forceinline__ void put(int64_t o, const float* f) const {
+    if (p && o >= 0) *(Raw<T, VEC>*)(p + o) = narrow<T, VEC>(f);
+  }
+};
+template <bool BUF> struct Off { typedef unsigned type; };
+template <> struct Off<false> { typedef int64_t type; };
 
 struct Plan {
   int vec, waves, splits;
+  bool buf;                    // a time step of every tensor within 2 GiB
   int64_t chunks;              // VEC-wide pieces of a row of H channels
   int64_t wgs;                 // workgroups over the channels
-  int64_t tiles, per;          // tiles of time, tiles of a split
+  int64_t tile, tiles, per;    // steps of a tile, tiles of time, tiles of a split
 };
 
-// A thread's channels: VEC neighbours of one sequence
-struct Lane {
-  int64_t b, j, q;             // sequence, first channel, flat index b H + j
+// A thread's channels: VEC neighbours of one sequence, as byte offsets into a time step of each tensor (-1, which as an
+// unsigned one is past every buffer's end: no channels)
+template <typename IO, typename HO, bool BUF> struct Lane {
+  typedef typename Off<BUF>::type off;
+  int64_t b, j, q;             // sequence, first channel, flat index b H + j (0 for a thread without channels)
+  off gates, h, f32, g_gates, mask;
   bool live;
-  template <int VEC> __device__ __forceinline__ void at(const mdmm_gated_scan_t& p, int64_t chunks, int lane) {
-    int64_t i = (int64_t)blockIdx.x * 64 + lane;
+  __device__ __forceinline__ Lane(const mdmm_gated_scan_t& p, int64_t chunks, int vec) {
+    int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
     live = i < chunks * p.B;
-    if (!live) i = 0;          // (loads stay in bounds; nothing is stored)
+    if (!live) i = 0;
     b = i / chunks;
-    j = (i - b * chunks) * VEC;
+    j = (i - b * chunks) * vec;
     q = b * p.H + j;
+    gates = live ? (off)((b * p.gates_sb + j) * (int64_t)sizeof(IO)) : (off)-1;
+    g_gates = live ? (off)((b * p.g_gates_sb + j) * (int64_t)sizeof(IO)) : (off)-1;
+    h = live ? (off)(q * (int64_t)sizeof(HO)) : (off)-1;
+    f32 = live ? (off)(q * 4) : (off)-1;
+    mask = live ? (off)(b * p.mask_sb) : (off)-1;
   }
 };
 
 __device__ __forceinline__ int64_t time_of(const mdmm_gated_scan_t& p, int64_t i) { return p.reverse ? p.T - 1 - i : i; }
 
-// raw f, c of a wave's 8 steps from step i0 on (steps past the end: the last one's, not used), mask bits in `on`
-template <typename IO, int VEC, bool C>
-__device__ __forceinline__ unsigned fetch(const mdmm_gated_scan_t& p, const Lane& l, int64_t i0, Raw<IO, VEC>* f, Raw<IO, VEC>* c) {
-  unsigned on = 0;
+// f, c and the mask of a wave's S steps from step i0 on as loaded (a step past the end: zeros)
+template <typename IO, typename HO, int VEC, bool BUF> struct Steps {
+  Raw<IO, VEC> f[S], c[S];
+  unsigned char m[S];
+  template <bool C> __device__ __forceinline__ void fetch(const mdmm_gated_scan_t& p, const Lane<IO, HO, BUF>& l, int64_t i0, bool any) {
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    const int64_t i = i0 + s < p.T ? i0 + s : p.T - 1, t = time_of(p, i);
-    const IO* row = (const IO*)p.gates + t * p.gates_st + l.b * p.gates_sb + l.j;
-    f[s] = *(const Raw<IO, VEC>*)row;
-    if (C) c[s] = *(const Raw<IO, VEC>*)(row + p.H);
-    if (i0 + s < p.T && (!p.mask || p.mask[t * p.mask_st + l.b * p.mask_sb])) on |= 1u << s;
+    for (int s = 0; s < S; ++s) {
+      const int64_t t = time_of(p, i0 + s);
+      const bool in = any && i0 + s < p.T;
+      f[s] = Step<IO, VEC, BUF>(p.gates, t * p.gates_st, in).get(l.gates);
+      if (C) c[s] = Step<IO, VEC, BUF>(p.gates, t * p.gates_st + p.H, in).get(l.gates);
+      if constexpr (BUF) {
+        __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(p.mask + t * p.mask_st), 0, in && p.mask ? 0x7fffffff : 0, 0x00020000);
+        m[s] = __builtin_amdgcn_raw_buffer_load_b8(r, l.mask, 0, 0);
+      } else m[s] = in && p.mask && l.live ? p.mask[t * p.mask_st + l.mask] : 0;
+    }
   }
-  return on;
-}
+  // bit s: step s is there and its mask lets it through
+  __device__ __forceinline__ unsigned on(const mdmm_gated_scan_t& p, int64_t i0) const {
+    const int64_t left = p.T - i0;
+    unsigned all = left >= S ? (1u << S) - 1 : left > 0 ? (1u << left) - 1 : 0, some = 0;
+    if (!p.mask) return all;
+#pragma unroll
+    for (int s = 0; s < S; ++s) some |= m[s] ? 1u << s : 0u;
+    return all & some;
+  }
+};
 
-// a state (prefix) in front of split `z`: the composition of the splits before it applied to the start
+// h (from_end: the adjoint) of the start taken through the splits in front of split z: every wave composes its share of
+// them, the shares meet in LDS
 template <int VEC>
-__device__ __forceinline__ void lead_in(const float* ws, int64_t stride, int z, bool from_end, int splits, int64_t q, float* h) {
-  const int n = from_end ? splits - 1 - z : z;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float* a = ws + 2 * stride * (from_end ? splits - 1 - i : i) + q;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) h[e] = fmaf(a[e], h[e], a[stride + e]);
-  }
-}
-
-// Composition of each split: BWD of D -> a (g + D) from its last step to its first, else of h -> a h + k c
-template <typename IO, typename HO, int VEC, bool BWD>
-__global__ __launch_bounds__(64 * WMAX) void scan_split_kernel(mdmm_gated_scan_t p, Plan pl) {
-  __shared__ float sa[WMAX][64 * VEC], sb[WMAX][64 * VEC];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, W = pl.waves;
-  Lane l;
-  l.at<VEC>(p, pl.chunks, lane);
-  const int64_t t0 = blockIdx.y * pl.per, t1 = t0 + pl.per < pl.tiles ? t0 + pl.per : pl.tiles;
-  // a wave composes every step of its own, tile by tile (they interleave with the other waves'), so the order over the split
-  // is kept by giving each wave one run of consecutive tiles
-  const int64_t run = (t1 - t0 + W - 1) / W;
-  const int64_t u0 = t0 + wave * run < t1 ? t0 + wave * run : t1, u1 = u0 + run < t1 ? u0 + run : t1;
+__device__ __forceinline__ void lead_in(const float* ws, int64_t stride, int z, bool from_end, const Plan& pl, int64_t q, float* h,
+                                        float (*sa)[64 * VEC], float (*sb)[64 * VEC]) {
+  if (pl.splits == 1) return;
+  const int n = from_end ? pl.splits - 1 - z : z, W = pl.waves;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float A[VEC], B[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) { A[e] = 1.0f; B[e] = 0.0f; }
-  const int64_t first = u0 * TILE, last = u1 * TILE < p.T ? u1 * TILE : p.T;
-  for (int64_t i = first; i < last; i += S) {
-    const int64_t i0 = BWD ? first + (last - 1 - i) / S * S : i;       // (first + a multiple of S, walked downwards)
-    Raw<IO, VEC> f[S], c[S];
-    Raw<HO, VEC> g[S];
-    const unsigned on = fetch<IO, VEC, !BWD>(p, l, i0, f, c);
-    if (BWD && p.g_h) {
+#pragma unroll 8
+  for (int i = n * wave / W; i < n * (wave + 1) / W; ++i) {
+    const float* a = ws + 2 * stride * (from_end ? pl.splits - 1 - i : i) + q;
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const int64_t t = time_of(p, i0 + s < p.T ? i0 + s : p.T - 1);
-        g[s] = *(const Raw<HO, VEC>*)((const HO*)p.g_h + t * p.B * p.H + l.q);
-      }
+    for (int e = 0; e < VEC; ++e) {
+      B[e] = fmaf(a[e], B[e], a[stride + e]);
+      A[e] *= a[e];
     }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) { sa[wave][e * 64 + lane] = A[e]; sb[wave][e * 64 + lane] = B[e]; }
+  __syncthreads();
+  for (int w = 0; w < W; ++w)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) h[e] = fmaf(sa[w][e * 64 + lane], h[e], sb[w][e * 64 + lane]);
+  __syncthreads();
+}
+
+// Composition of each split: BWD of D -> a (g + D) from its last step to its first, else of h -> a h + k c.  Each wave takes
+// one run of the split's tiles, the runs are joined in LDS
+template <typename IO, typename HO, int VEC, bool BUF, bool BWD>
+__global__ __launch_bounds__(64 * WMAX) void scan_split_kernel(mdmm_gated_scan_t p, Plan pl) {
+  __shared__ float sa[WMAX][64 * VEC], sb[WMAX][64 * VEC];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = pl.waves;
+  const Lane<IO, HO, BUF> l(p, pl.chunks, VEC);
+  const int64_t stride = (int64_t)p.B * p.H;
+  const int64_t t0 = blockIdx.y * pl.per, t1 = t0 + pl.per < pl.tiles ? t0 + pl.per : pl.tiles;
+  const int64_t first_all = t0 * pl.tile, last_all = t1 * pl.tile < p.T ? t1 * pl.tile : p.T;
+  const int64_t run = ((last_all - first_all + W - 1) / W + S - 1) / S * S;
+  const int64_t first = first_all + wave * run < last_all ? first_all + wave * run : last_all;
+  const int64_t last = first + run < last_all ? first + run : last_all;
+  float A[VEC], B[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) { A[e] = 1.0f; B[e] = 0.0f; }
+  Steps<IO, HO, VEC, BUF> x;
+  Raw<HO, VEC> g[S];
+  const int64_t n = (last - first + S - 1) / S;
+  auto fetch = [&](int64_t i) {
+    const int64_t i0 = first + (BWD ? n - 1 - i : i) * S;
+    x.template fetch<!BWD>(p, l, i0, i < n);
+    if (BWD) {
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        g[s] = Step<HO, VEC, BUF>(p.g_h, time_of(p, i0 + s) * stride, i < n && i0 + s < p.T).get(l.h);
+    }
+  };
+  fetch(0);
+  for (int64_t i = 0; i < n; ++i) {
+    const unsigned on = x.on(p, first + (BWD ? n - 1 - i : i) * S);
+    float fv[S][VEC], cv[S][VEC];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      widen(x.f[s], fv[s]);
+      if (BWD) widen(g[s], cv[s]); else widen(x.c[s], cv[s]);
+    }
+    fetch(i + 1);
 #pragma unroll
     for (int s_ = 0; s_ < S; ++s_) {
       const int s = BWD ? S - 1 - s_ : s_;
-      float fv[VEC], cv[VEC], gv[VEC];
-      widen(f[s], fv);
-      if (!BWD) widen(c[s], cv);
-      if (BWD && p.g_h) widen(g[s], gv);
-      const bool in = on >> s & 1, some = i0 + s < last;
+      const bool in = on >> s & 1;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const Gate x(fv[e]);
-        const float a = in ? x.a : 1.0f;
-        if (BWD) {
-          if (some) B[e] = a * ((p.g_h ? gv[e] : 0.0f) + B[e]);
-        } else B[e] = in ? fmaf(x.a, B[e], x.k * cv[e]) : B[e];
+        const Gate y(fv[s][e]);
+        const float a = in ? y.a : 1.0f;
+        if (BWD) B[e] = a * (cv[s][e] + B[e]);            // (a step past the end: its g is 0)
+        else B[e] = in ? fmaf(y.a, B[e], y.k * cv[s][e]) : B[e];
         A[e] *= a;
       }
     }
@@ -148,7 +225,6 @@ __global__ __launch_bounds__(64 * WMAX) void scan_split_kernel(mdmm_gated_scan_t
   for (int e = 0; e < VEC; ++e) { sa[wave][e * 64 + lane] = A[e]; sb[wave][e * 64 + lane] = B[e]; }
   __syncthreads();
   if (wave == 0 && l.live) {
-    const int64_t stride = (int64_t)p.B * p.H;
     float* out = p.ws + 2 * stride * blockIdx.y + l.q;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
@@ -164,48 +240,47 @@ __global__ __launch_bounds__(64 * WMAX) void scan_split_kernel(mdmm_gated_scan_t
   }
 }
 
-template <typename IO, typename HO, int VEC>
-__global__ __launch_bounds__(64 * WMAX) void scan_fwd_kernel(mdmm_gated_scan_t p, Plan pl) {
+template <typename IO, typename HO, int VEC, bool BUF>
+__global__ __launch_bounds__(64 * WMAX, 4) void scan_fwd_kernel(mdmm_gated_scan_t p, Plan pl) {
   __shared__ float sa[2][WMAX][64 * VEC], sb[2][WMAX][64 * VEC];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, W = pl.waves;
-  Lane l;
-  l.at<VEC>(p, pl.chunks, lane);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = pl.waves;
+  const Lane<IO, HO, BUF> l(p, pl.chunks, VEC);
   const int64_t stride = (int64_t)p.B * p.H;
   const int64_t t0 = blockIdx.y * pl.per, t1 = t0 + pl.per < pl.tiles ? t0 + pl.per : pl.tiles;
+  Steps<IO, HO, VEC, BUF> x;
+  x.template fetch<true>(p, l, t0 * pl.tile + wave * S, true);
   float h0[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) h0[e] = p.h0 ? p.h0[l.b * p.h0_sb + l.j + e] : 0.0f;
-  lead_in<VEC>(p.ws, stride, blockIdx.y, false, pl.splits, l.q, h0);
-  Raw<IO, VEC> f[S], c[S];
-  unsigned on = fetch<IO, VEC, true>(p, l, t0 * TILE + wave * S, f, c);
+  lead_in<VEC>(p.ws, stride, blockIdx.y, false, pl, l.q, h0, sa[0], sb[0]);
   for (int64_t tile = t0; tile < t1; ++tile) {
-    const int64_t i0 = tile * TILE + wave * S;
+    const int64_t i0 = tile * pl.tile + wave * S;
+    const unsigned on = x.on(p, i0);
     float a[S][VEC], b[S][VEC], A[VEC], B[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) { A[e] = 1.0f; B[e] = 0.0f; }
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       float fv[VEC], cv[VEC];
-      widen(f[s], fv);
-      widen(c[s], cv);
+      widen(x.f[s], fv);
+      widen(x.c[s], cv);
       const bool in = on >> s & 1;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const Gate x(fv[e]);
-        a[s][e] = in ? x.a : 1.0f;
-        b[s][e] = in ? x.k * cv[e] : 0.0f;
+        const Gate y(fv[e]);
+        a[s][e] = in ? y.a : 1.0f;
+        b[s][e] = in ? y.k * cv[e] : 0.0f;
         B[e] = fmaf(a[s][e], B[e], b[s][e]);
         A[e] *= a[s][e];
       }
     }
-    if (tile + 1 < t1) on = fetch<IO, VEC, true>(p, l, i0 + TILE, f, c);
+    x.template fetch<true>(p, l, i0 + pl.tile, tile + 1 < t1);      // in flight behind the rest of this tile
     const int z = tile & 1;
     if (W > 1) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) { sa[z][wave][e * 64 + lane] = A[e]; sb[z][wave][e * 64 + lane] = B[e]; }
       __syncthreads();         // (two sets of pieces: a wave a tile ahead writes the other one)
     }
-    if (p.states && wave == 0 && l.live) put<VEC>(p.states + tile * stride + l.q, h0);
     float h[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) h[e] = h0[e];
@@ -218,74 +293,78 @@ __global__ __launch_bounds__(64 * WMAX) void scan_fwd_kernel(mdmm_gated_scan_t p
         }
       }
     }
+    if (wave * S % KEEP == 0 && i0 < p.T) Step<float, VEC, BUF>(p.states, i0 / KEEP * stride, true).put(l.f32, h);
 #pragma unroll
     for (int s = 0; s < S; ++s) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) h[e] = fmaf(a[s][e], h[e], b[s][e]);
-      if (i0 + s < p.T && l.live) put<VEC>((HO*)p.h + time_of(p, i0 + s) * stride + l.q, h);
+      Step<HO, VEC, BUF>(p.h, time_of(p, i0 + s) * stride, i0 + s < p.T).put(l.h, h);
     }
     if (W == 1) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) h0[e] = h[e];
     }
   }
-  if (p.h_last && t1 == pl.tiles && wave == 0 && l.live) put<VEC>(p.h_last + l.q, h0);
+  if (t1 == pl.tiles && wave == 0) Step<float, VEC, BUF>(p.h_last, 0, true).put(l.f32, h0);
 }
 
-template <typename IO, typename HO, int VEC>
+template <typename IO, typename HO, int VEC, bool BUF>
 __global__ __launch_bounds__(64 * WMAX) void scan_bwd_kernel(mdmm_gated_scan_t p, Plan pl) {
   __shared__ float sa[2][WMAX][64 * VEC], sb[2][WMAX][64 * VEC], sg[2][WMAX][64 * VEC];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, W = pl.waves;
-  Lane l;
-  l.at<VEC>(p, pl.chunks, lane);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = pl.waves;
+  const Lane<IO, HO, BUF> l(p, pl.chunks, VEC);
   const int64_t stride = (int64_t)p.B * p.H;
   const int64_t t0 = blockIdx.y * pl.per, t1 = t0 + pl.per < pl.tiles ? t0 + pl.per : pl.tiles;
-  float d0[VEC];               // a G of the step behind the present tile
+  Steps<IO, HO, VEC, BUF> x;
+  Raw<HO, VEC> g[S];
+  Raw<float, VEC> start;       // the state in front of the tile
+  auto fetch = [&](int64_t tile) {
+    const bool any = tile >= t0;
+    const int64_t i0 = tile * pl.tile + wave * S;
+    x.template fetch<true>(p, l, i0, any);
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) d0[e] = p.g_last ? p.g_last[l.q + e] : 0.0f;
-  lead_in<VEC>(p.ws, stride, blockIdx.y, true, pl.splits, l.q, d0);
+    for (int s = 0; s < S; ++s) g[s] = Step<HO, VEC, BUF>(p.g_h, time_of(p, i0 + s) * stride, any && i0 + s < p.T).get(l.h);
+    start = Step<float, VEC, BUF>(p.states, tile * stride, any).get(l.f32);
+  };
+  fetch(t1 - 1);
+  float d0[VEC], h00[VEC];     // a G of the step behind the present tile; the state in front of a single tile
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    d0[e] = p.g_last ? p.g_last[l.q + e] : 0.0f;
+    h00[e] = !p.states && p.h0 ? p.h0[l.b * p.h0_sb + l.j + e] : 0.0f;
+  }
+  lead_in<VEC>(p.ws, stride, blockIdx.y, true, pl, l.q, d0, sa[0], sb[0]);
   for (int64_t tile = t1 - 1; tile >= t0; --tile) {
-    const int64_t i0 = tile * TILE + wave * S;
-    Raw<IO, VEC> f[S], c[S];
-    Raw<HO, VEC> g[S];
-    const unsigned on = fetch<IO, VEC, true>(p, l, i0, f, c);
+    const int64_t i0 = tile * pl.tile + wave * S;
+    const unsigned on = x.on(p, i0);
+    float a[S][VEC], k[S][VEC], cv[S][VEC], gv[S][VEC], A[VEC], B[VEC], D[VEC], h[VEC], d[VEC];
+    widen(start, h);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) { A[e] = 1.0f; B[e] = 0.0f; D[e] = 0.0f; if (!p.states) h[e] = h00[e]; }
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      g[s] = Raw<HO, VEC>{};
-      if (p.g_h && i0 + s < p.T) g[s] = *(const Raw<HO, VEC>*)((const HO*)p.g_h + time_of(p, i0 + s) * stride + l.q);
-    }
-    float hs[VEC];             // the state in front of the tile
-#pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      hs[e] = p.states ? p.states[tile * stride + l.q + e] : p.h0 ? p.h0[l.b * p.h0_sb + l.j + e] : 0.0f;
-    float a[S][VEC], k[S][VEC], A[VEC], B[VEC], D[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) { A[e] = 1.0f; B[e] = 0.0f; D[e] = 0.0f; }
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      float fv[VEC], cv[VEC];
-      widen(f[s], fv);
-      widen(c[s], cv);
+      float fv[VEC];
+      widen(x.f[s], fv);
+      widen(x.c[s], cv[s]);
+      widen(g[s], gv[s]);
       const bool in = on >> s & 1;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const Gate x(fv[e]);
-        a[s][e] = in ? x.a : 1.0f;
-        k[s][e] = in ? x.k : 0.0f;
-        B[e] = fmaf(a[s][e], B[e], in ? k[s][e] * cv[e] : 0.0f);
+        const Gate y(fv[e]);
+        a[s][e] = in ? y.a : 1.0f;
+        k[s][e] = in ? y.k : 0.0f;
+        cv[s][e] = in ? cv[s][e] : 0.0f;
+        B[e] = fmaf(a[s][e], B[e], k[s][e] * cv[s][e]);
         A[e] *= a[s][e];
       }
     }
+    fetch(tile - 1);           // in flight behind the rest of this tile
 #pragma unroll
-    for (int s = S - 1; s >= 0; --s) {
-      float gv[VEC];
-      widen(g[s], gv);
+    for (int s = S - 1; s >= 0; --s)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) D[e] = a[s][e] * (gv[e] + D[e]);
-    }
-    float h[VEC], d[VEC];
+      for (int e = 0; e < VEC; ++e) D[e] = a[s][e] * (gv[s][e] + D[e]);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) { h[e] = hs[e]; d[e] = d0[e]; }
+    for (int e = 0; e < VEC; ++e) d[e] = d0[e];
     const int z = tile & 1;
     if (W > 1) {
 #pragma unroll
@@ -295,10 +374,9 @@ __global__ __launch_bounds__(64 * WMAX) void scan_bwd_kernel(mdmm_gated_scan_t p
         sg[z][wave][e * 64 + lane] = D[e];
       }
       __syncthreads();
-      for (int w = 0; w < W; ++w)
+      for (int w = 0; w < wave; ++w)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (w < wave) h[e] = fmaf(sa[z][w][e * 64 + lane], h[e], sb[z][w][e * 64 + lane]);
+        for (int e = 0; e < VEC; ++e) h[e] = fmaf(sa[z][w][e * 64 + lane], h[e], sb[z][w][e * 64 + lane]);
       for (int w = W - 1; w >= 0; --w)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
@@ -309,37 +387,30 @@ __global__ __launch_bounds__(64 * WMAX) void scan_bwd_kernel(mdmm_gated_scan_t p
 #pragma unroll
       for (int e = 0; e < VEC; ++e) d0[e] = fmaf(A[e], d0[e], D[e]);
     }
-    float before[S][VEC];      // h_{t-1} - c_t
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      float cv[VEC];
-      widen(c[s], cv);
-      const bool in = on >> s & 1;
+    for (int s = 0; s < S; ++s)          // cv becomes h_{t-1} - c_t (0 where the mask is: k is 0 there too)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        before[s][e] = in ? h[e] - cv[e] : 0.0f;
-        h[e] = in ? fmaf(a[s][e], h[e], k[s][e] * cv[e]) : h[e];
+        const float before = h[e];
+        h[e] = fmaf(a[s][e], h[e], k[s][e] * cv[s][e]);
+        cv[s][e] = (on >> s & 1) ? before - cv[s][e] : 0.0f;
       }
-    }
 #pragma unroll
     for (int s = S - 1; s >= 0; --s) {
-      float gv[VEC], df[VEC], dc[VEC];
-      widen(g[s], gv);
+      float df[VEC], dc[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float G = gv[e] + d[e];
+        const float G = gv[s][e] + d[e];
         dc[e] = G * k[s][e];
-        df[e] = dc[e] * a[s][e] * before[s][e];
+        df[e] = dc[e] * a[s][e] * cv[s][e];
         d[e] = a[s][e] * G;
       }
-      if (i0 + s < p.T && l.live) {
-        IO* out = (IO*)p.g_gates + time_of(p, i0 + s) * p.g_gates_st + l.b * p.g_gates_sb + l.j;
-        put<VEC>(out, df);
-        put<VEC>(out + p.H, dc);
-      }
+      const int64_t at = time_of(p, i0 + s) * p.g_gates_st;
+      Step<IO, VEC, BUF>(p.g_gates, at, i0 + s < p.T).put(l.g_gates, df);
+      Step<IO, VEC, BUF>(p.g_gates, at + p.H, i0 + s < p.T).put(l.g_gates, dc);
     }
   }
-  if (p.g_h0 && t0 == 0 && wave == 0 && l.live) put<VEC>(p.g_h0 + l.q, d0);
+  if (t0 == 0 && wave == 0) Step<float, VEC, BUF>(p.g_h0, 0, true).put(l.f32, d0);
 }
 
 int check(const mdmm_gated_scan_t* a) {
@@ -363,41 +434,54 @@ Plan plan(const mdmm_gated_scan_t* a, bool bwd) {
   };
   p.vec = fits(2) ? 2 : 1;
   if (!bwd && fits(4) && (int64_t)a->B * a->H >= 64 * 4 * 512) p.vec = 4;
+  auto reach = [&](int64_t sb) { return (sb < 0 ? 0x80000000ll : (a->B - 1) * sb + 2 * (int64_t)a->H) * 4 < 0x7fffffffll; };
+  p.buf = reach(a->gates_sb) && reach(a->g_gates_sb) && reach(a->H) && reach(a->mask_sb);
   p.chunks = a->H / p.vec;
   p.wgs = (p.chunks * a->B + 63) / 64;
+  // up to KEEP2 steps one tile; beyond, forward tiles of 8 waves (at 512 x 256 x 512 in bf16 106 us, of 4 waves 122) and
+  // backward ones of 4 (159 us, of 8 waves 179: three of them, twelve waves, fit a CU's registers, but one of 8)
   const int64_t waves = (a->T + S - 1) / S;
-  p.waves = (int)(waves < WMAX ? waves : WMAX);
-  p.tiles = ((int64_t)a->T + TILE - 1) / TILE;
+  p.waves = (int)(a->T <= KEEP2 ? waves : bwd ? KEEP / S : WMAX);
+  p.tile = p.waves * S;
+  p.tiles = (a->T + p.tile - 1) / p.tile;
+  // fewer than two workgroups a CU: time over workgroups too, two a CU (20011 x 3 x 200 in fp32: 133 us for the four launches
+  // of a training pass, with four a CU 142 -- every split reads through all those before it)
   int64_t splits = 1;
   if (p.wgs < 512 && p.tiles > 1) {
-    splits = (1024 + p.wgs - 1) / p.wgs;
+    splits = (512 + p.wgs - 1) / p.wgs;
     if (splits > p.tiles) splits = p.tiles;
-    if (splits > 64) splits = 64;
+    if (splits > 512) splits = 512;
   }
   p.per = (p.tiles + splits - 1) / splits;
   p.splits = (int)((p.tiles + p.per - 1) / p.per);
   return p;
 }
 
-template <typename IO, typename HO>
+template <typename IO, typename HO, int VEC, bool BUF>
 int launch(const mdmm_gated_scan_t* a, const Plan& pl, bool bwd, hipStream_t s) {
   const dim3 grid((unsigned)pl.wgs, (unsigned)pl.splits), block(64 * pl.waves);
 #define RUN(K) hipLaunchKernelGGL(K, grid, block, 0, s, *a, pl)
   if (bwd) {
-    if (pl.splits > 1) {
-      if (pl.vec == 1) RUN((scan_split_kernel<IO, HO, 1, true>)); else RUN((scan_split_kernel<IO, HO, 2, true>));
+    if constexpr (VEC < 4) {
+      if (pl.splits > 1) RUN((scan_split_kernel<IO, HO, VEC, BUF, true>));
+      RUN((scan_bwd_kernel<IO, HO, VEC, BUF>));
     }
-    if (pl.vec == 1) RUN((scan_bwd_kernel<IO, HO, 1>)); else RUN((scan_bwd_kernel<IO, HO, 2>));
   } else {
-    if (pl.splits > 1) {
-      if (pl.vec == 1) RUN((scan_split_kernel<IO, HO, 1, false>)); else RUN((scan_split_kernel<IO, HO, 2, false>));
+    if constexpr (VEC < 4) {
+      if (pl.splits > 1) RUN((scan_split_kernel<IO, HO, VEC, BUF, false>));
     }
-    if (pl.vec == 1) RUN((scan_fwd_kernel<IO, HO, 1>));
-    else if (pl.vec == 2) RUN((scan_fwd_kernel<IO, HO, 2>));
-    else RUN((scan_fwd_kernel<IO, HO, 4>));
+    RUN((scan_fwd_kernel<IO, HO, VEC, BUF>));
   }
 #undef RUN
   return (int)hipGetLastError();
+}
+
+template <typename IO, typename HO>
+int launch(const mdmm_gated_scan_t* a, const Plan& pl, bool bwd, hipStream_t s) {
+  if (!pl.buf) return pl.vec == 1 ? launch<IO, HO, 1, false>(a, pl, bwd, s) : pl.vec == 2 ? launch<IO, HO, 2, false>(a, pl, bwd, s)
+                                                                             : launch<IO, HO, 4, false>(a, pl, bwd, s);
+  return pl.vec == 1 ? launch<IO, HO, 1, true>(a, pl, bwd, s) : pl.vec == 2 ? launch<IO, HO, 2, true>(a, pl, bwd, s)
+                                                                            : launch<IO, HO, 4, true>(a, pl, bwd, s);
 }
 
 int run(const mdmm_gated_scan_t* a, bool bwd, hipStream_t s) {
@@ -415,8 +499,7 @@ using namespace mdmm;
 
 extern "C" int64_t mdmm_gated_scan_states(const mdmm_gated_scan_t* a) {
   if (check(a)) return -1;
-  const int64_t tiles = ((int64_t)a->T + TILE - 1) / TILE;
-  return tiles > 1 ? tiles * a->B * a->H : 0;         // (a single tile starts at h0)
+  return a->T > KEEP2 ? ((int64_t)a->T + KEEP - 1) / KEEP * a->B * a->H : 0;         // (a single tile starts at h0)
 }
 
 extern "C" int64_t mdmm_gated_scan_ws(const mdmm_gated_scan_t* a, int bwd) {
@@ -438,6 +521,6 @@ extern "C" int mdmm_gated_scan_bwd(const mdmm_gated_scan_t* a, void* stream) {
   const int rc = check(a);
   if (rc) return rc;
   if (none(a)) return 0;
-  if (!a->g_gates || (a->T > TILE && !a->states)) return MDMM_E_ARG;
+  if (!a->g_gates || (a->T > KEEP2 && !a->states)) return MDMM_E_ARG;
   return run(a, true, (hipStream_t)stream);
 }
