@@ -364,7 +364,8 @@ int mdmm_nll_bernoulli_logits_passes_fwd_grad(void* logits, int passes, const fl
 /* torch.optim.Adam's update (the optimizer trainer.py:212 builds; no amsgrad, L2 weight decay added to the gradient) in
  * one streaming launch: gradients and both moments as flat fp32 buffers of n elements in which parameter k owns
  * [offs[k], offs[k + 1]) (offs: n_params + 1 entries, offs[0] = 0, offs[n_params] = n; harness.GradBucket's packing), the
- * parameters where they live (p_ptrs[k] = parameter k's fp32 storage, contiguous) -- both tables in device memory.
+ * parameters where they live (p_ptrs[k] = parameter k's fp32 storage, contiguous; NULL: left alone, as are its moments) --
+ * both tables in device memory.
  *   gr = g + weight_decay p;  m += (1 - beta1)(gr - m);  v = beta2 v + (1 - beta2) gr^2;
  *   p -= lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps),  t = *step
  * (a device scalar holding the count of this update, 1 for the first).  lr_dev (optional device scalar) overrides lr.  */
@@ -1075,7 +1076,8 @@ int mdmm_cat_head_nll_bwd(const float* hid, const float* w, const float* label, 
  * ws: mdmm_gated_scan_ws(a, bwd) floats of scratch per call (0: NULL is fine).
  * backward: g_h (T, B, H) in h's type (NULL: none), g_last (B, H) fp32 (NULL: none); g_gates in the gates' type and
  * column order with its own strides (every element of its 2H columns is written, 0 where the mask is 0); g_h0 (B, H) fp32
- * per sequence (NULL: not wanted).  T, B or H of 0: nothing is launched.
+ * per sequence (NULL: not wanted) and g_h0_sum (H) its sum over the sequences (needs g_h0; the gradient of one row for
+ * all).  T, B or H of 0: nothing is launched.
  * --------------------------------------------------------------------------------- */
 typedef struct mdmm_gated_scan {
   int32_t T, B, H, reverse, gates_bf16, h_bf16;
@@ -1094,6 +1096,7 @@ typedef struct mdmm_gated_scan {
   void* g_gates;
   int64_t g_gates_st, g_gates_sb;
   float* g_h0;
+  float* g_h0_sum;
 } mdmm_gated_scan_t;
 int64_t mdmm_gated_scan_states(const mdmm_gated_scan_t* a);
 int64_t mdmm_gated_scan_ws(const mdmm_gated_scan_t* a, int bwd);
@@ -1142,6 +1145,10 @@ typedef struct mdmm_block_norm {
 int64_t mdmm_block_norm_ws(const mdmm_block_norm_t* a);
 int mdmm_block_norm_fwd(const mdmm_block_norm_t* a, void* stream);
 int mdmm_block_norm_bwd(const mdmm_block_norm_t* a, void* stream);
+/* The layer: mdmm_gated_scan_fwd, then mdmm_block_norm_fwd on its states (norm->y = scan->h); backward the two calls in the
+ * other order (norm->d_y = scan->g_h; norm's part is left out where norm->g_out and g_n are both NULL).  */
+int mdmm_gated_block_fwd(const mdmm_gated_scan_t* scan, const mdmm_block_norm_t* norm, void* stream);
+int mdmm_gated_block_bwd(const mdmm_gated_scan_t* scan, const mdmm_block_norm_t* norm, void* stream);
 /* One time step of the recurrence and its block norm in one launch (T = 1, no gradient): the state of `scan` from h0 to
  * h_last, h itself not stored; gates and gate come from one row [f | c | g] (norm->gate NULL: no gate), norm->y is not
  * read.  H <= MDMM_NORM_MAX_H.  */

@@ -550,3 +550,19 @@ extern "C" int mdmm_gated_block_step(const mdmm_gated_scan_t* q, const mdmm_bloc
   if (!p->branch_bf16) return launch_step<float, float>(q, p, s);
   return p->res_bf16 ? launch_step<__bf16, __bf16>(q, p, s) : launch_step<__bf16, float>(q, p, s);
 }
+
+extern "C" int mdmm_gated_block_fwd(const mdmm_gated_scan_t* q, const mdmm_block_norm_t* p, void* stream) {
+  if (!q || !p || p->y != q->h || p->H != q->H || p->rows != (int64_t)q->T * q->B) return MDMM_E_ARG;
+  const int rc = mdmm_gated_scan_fwd(q, stream);
+  return rc ? rc : mdmm_block_norm_fwd(p, stream);
+}
+
+extern "C" int mdmm_gated_block_bwd(const mdmm_gated_scan_t* q, const mdmm_block_norm_t* p, void* stream) {
+  if (!q || !p || p->H != q->H || p->rows != (int64_t)q->T * q->B) return MDMM_E_ARG;
+  if (p->g_out || p->g_n) {
+    if (p->d_y != q->g_h) return MDMM_E_ARG;
+    const int rc = mdmm_block_norm_bwd(p, stream);
+    if (rc) return rc;
+  }
+  return mdmm_gated_scan_bwd(q, stream);
+}

@@ -413,6 +413,25 @@ __global__ __launch_bounds__(64 * WMAX) void scan_bwd_kernel(mdmm_gated_scan_t p
   if (t0 == 0 && wave == 0) Step<float, VEC, BUF>(p.g_h0, 0, true).put(l.f32, d0);
 }
 
+// sum over the sequences of g_h0: 16 columns and 64 threads down each a workgroup, joined in a fixed order
+__global__ __launch_bounds__(1024) void scan_rows_kernel(const float* __restrict__ g, int64_t rows, int H, float* out) {
+  __shared__ float part[64][17];
+  const int c = blockIdx.x * 16 + (threadIdx.x & 15), r = threadIdx.x >> 4;
+  float s = 0.0f;
+  if (c < H) {
+#pragma unroll 8
+    for (int64_t i = r; i < rows; i += 64) s += g[i * H + c];
+  }
+  part[r][threadIdx.x & 15] = s;
+  __syncthreads();
+  if (r == 0 && c < H) {
+    s = 0.0f;
+#pragma unroll 16
+    for (int i = 0; i < 64; ++i) s += part[i][threadIdx.x & 15];
+    out[c] = s;
+  }
+}
+
 int check(const mdmm_gated_scan_t* a) {
   if (!a || a->T < 0 || a->B < 0 || a->H < 0) return MDMM_E_ARG;
   if (!a->gates_bf16 && a->h_bf16) return MDMM_E_ARG;
@@ -522,5 +541,10 @@ extern "C" int mdmm_gated_scan_bwd(const mdmm_gated_scan_t* a, void* stream) {
   if (rc) return rc;
   if (none(a)) return 0;
   if (!a->g_gates || (a->T > KEEP2 && !a->states)) return MDMM_E_ARG;
-  return run(a, true, (hipStream_t)stream);
+  if (a->g_h0_sum && !a->g_h0) return MDMM_E_ARG;
+  const int e = run(a, true, (hipStream_t)stream);
+  if (e || !a->g_h0_sum) return e;
+  hipLaunchKernelGGL(scan_rows_kernel, dim3((a->H + 15) / 16), dim3(1024), 0, (hipStream_t)stream, a->g_h0, (int64_t)a->B, a->H,
+                     a->g_h0_sum);
+  return (int)hipGetLastError();
 }

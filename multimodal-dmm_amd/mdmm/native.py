@@ -48,7 +48,7 @@ SYMBOLS = [
     'mdmm_ssim_ws_floats', 'mdmm_ssim',
     'mdmm_cat_head_supported', 'mdmm_cat_head_slabs', 'mdmm_cat_head_nll_fwd', 'mdmm_cat_head_nll_bwd',
     'mdmm_gated_scan_states', 'mdmm_gated_scan_ws', 'mdmm_gated_scan_fwd', 'mdmm_gated_scan_bwd',
-    'mdmm_block_norm_ws', 'mdmm_block_norm_fwd', 'mdmm_block_norm_bwd', 'mdmm_gated_block_step',
+    'mdmm_block_norm_ws', 'mdmm_block_norm_fwd', 'mdmm_block_norm_bwd', 'mdmm_gated_block_fwd', 'mdmm_gated_block_bwd', 'mdmm_gated_block_step',
     'mdmm_ortho_ws', 'mdmm_ortho',
 ]
 
@@ -258,7 +258,7 @@ class GatedScan(C.Structure):
                 [('gates', _P), ('gates_st', C.c_int64), ('gates_sb', C.c_int64), ('h0', _P), ('h0_sb', C.c_int64),
                  ('mask', _P), ('mask_st', C.c_int64), ('mask_sb', C.c_int64)] +
                 [(n, _P) for n in ('h', 'h_last', 'states', 'ws', 'g_h', 'g_last', 'g_gates')] +
-                [('g_gates_st', C.c_int64), ('g_gates_sb', C.c_int64), ('g_h0', _P)])
+                [('g_gates_st', C.c_int64), ('g_gates_sb', C.c_int64), ('g_h0', _P), ('g_h0_sum', _P)])
 
 
 NORM_MAX_H = 8192
@@ -456,7 +456,8 @@ def lib():
                           (BlockNorm, ('mdmm_block_norm_fwd', 'mdmm_block_norm_bwd')), (Ortho, ('mdmm_ortho',))):
             for name in names:
                 getattr(L, name).argtypes = [C.POINTER(st), _P]
-        L.mdmm_gated_block_step.argtypes = [C.POINTER(GatedScan), C.POINTER(BlockNorm), _P]
+        for name in ('mdmm_gated_block_fwd', 'mdmm_gated_block_bwd', 'mdmm_gated_block_step'):
+            getattr(L, name).argtypes = [C.POINTER(GatedScan), C.POINTER(BlockNorm), _P]
         L.mdmm_gated_scan_states.argtypes = [C.POINTER(GatedScan)]
         L.mdmm_gated_scan_ws.argtypes = [C.POINTER(GatedScan), C.c_int]
         L.mdmm_block_norm_ws.argtypes = [C.POINTER(BlockNorm)]

@@ -61,9 +61,8 @@ def orthogonalise(mats, steps=5, eps=1e-7, coefficients=COEFFICIENTS):
         ops._need_gpu(m)
         if m.device != mats[0].device:
             raise ValueError('orthogonalise: matrices on %s and %s' % (mats[0].device, m.device))
-    from .recurrent import _on
     dev = mats[0].device
-    with torch.no_grad(), _on(dev):
+    with torch.no_grad(), torch.cuda.device(dev):
         outs = [torch.empty(m.shape, device=dev, dtype=m.dtype) for m in mats]
         for dtype in (torch.float32, torch.bfloat16):
             items = []

@@ -27,10 +27,39 @@ def _check_type(name, *tensors):
 
 
 def _check_device(name, first, *tensors):
-    ops._need_gpu(first, *tensors)
+    """Every tensor on first's GPU -> its index."""
+    i = first.get_device()
+    if i < 0:
+        ops._need_gpu(first)
     for t in tensors:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != i:
+            ops._need_gpu(t)
             raise ValueError('%s: tensors on %s and %s' % (name, first.device, t.device))
+    return i
+
+
+def _apply(device, fn, *args):
+    """fn(*args) with `device` as the current one (a caller may have another one current)."""
+    if device == torch._C._cuda_getDevice():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
+_FN = {}
+
+
+def _launch(name, tag, *structs):
+    """ops._call on the current stream, without its look-ups (they cost as much as the launch itself)."""
+    if ops.TIMER is not None:
+        ops._call(name, *(C.byref(a) for a in structs), tag=tag)
+        return
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(native.lib(), name)
+    rc = fn(*structs, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+    if rc:
+        native.check(rc, name)
 
 
 def _vector(name, what, t, H):
@@ -49,21 +78,6 @@ def _vectors(name, weight, scale, next_weight, H):
     if weight is None:
         raise ValueError('%s: weight is not optional' % name)
     return [_vector(name, k, t, H) for k, t in (('weight', weight), ('scale', scale), ('next_weight', next_weight))]
-
-
-class _on:
-    """The device of the operands as the current one (a caller may have another one current)."""
-
-    def __init__(self, device):
-        self.ctx = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
 
 
 def _mask_bytes(name, mask, lead):
@@ -91,86 +105,96 @@ def _check_h0(name, h0, B, H):
 
 def _fill_scan(a, x, H, h0, mask, reverse):
     T, B = x.shape[:2]
-    a.T, a.B, a.H, a.reverse, a.gates_bf16 = T, B, H, int(reverse), int(x.dtype == torch.bfloat16)
-    a.gates, a.gates_st, a.gates_sb = x.data_ptr(), x.stride(0), x.stride(1)
+    a.T, a.B, a.H, a.reverse, a.gates_bf16 = T, B, H, reverse, x.dtype is torch.bfloat16
+    a.gates = x.data_ptr()
+    a.gates_st, a.gates_sb = x.stride()[:2]
     if h0 is not None:
         a.h0, a.h0_sb = h0.data_ptr(), (h0.stride(0) if h0.dim() == 2 else 0)
     if mask is not None:
         a.mask, a.mask_st, a.mask_sb = mask.data_ptr(), mask.stride(0), mask.stride(1)
 
 
-def _scan_ws(a, bwd, device):
-    n = native.lib().mdmm_gated_scan_ws(C.byref(a), bwd)
+def _size(name, *args):
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(native.lib(), name)
+    return fn(*args)
+
+
+def _scan_ws(a, bwd, dev):
+    """Scratch of a call, to be held until it is launched."""
+    n = _size('mdmm_gated_scan_ws', a, bwd)
     if n <= 0:
         return None
-    ws = torch.empty(n, dtype=torch.float32, device=device)
+    ws = torch.empty(n, dtype=torch.float32, device=dev)
     a.ws = ws.data_ptr()
     return ws
 
 
-def _scan_forward(x, H, h0, mask, reverse, h_dtype, keep):
-    """-> (h, h_last, states)."""
+def _scan_forward(a, x, H, h0, mask, reverse, h, keep):
+    """Fills the struct of a forward call over h.shape -> (h_last, states, scratch)."""
     T, B = x.shape[:2]
     dev = x.device
-    h = torch.empty(T, B, H, device=dev, dtype=h_dtype)
-    if T == 0:
-        last = torch.zeros(B, H, device=dev) if h0 is None else h0.detach().expand(B, H).clone()
-        return h, last, None
-    last = torch.empty(B, H, device=dev, dtype=torch.float32)
-    a = native.GatedScan()
+    last = torch.empty((B, H), device=dev, dtype=torch.float32)
     _fill_scan(a, x, H, h0, mask, reverse)
-    a.h, a.h_last, a.h_bf16 = h.data_ptr(), last.data_ptr(), int(h_dtype == torch.bfloat16)
+    a.h, a.h_last, a.h_bf16 = h.data_ptr(), last.data_ptr(), h.dtype is torch.bfloat16
     states = None
     if keep:
-        states = torch.empty(native.lib().mdmm_gated_scan_states(C.byref(a)), device=dev, dtype=torch.float32)
-        a.states = states.data_ptr()
-    ws = _scan_ws(a, 0, dev)
-    ops._call('mdmm_gated_scan_fwd', C.byref(a), tag='gated_scan_fwd[H=%d]' % H)
-    del ws
-    return h, last, states
+        n = _size('mdmm_gated_scan_states', a)
+        if n:
+            states = torch.empty(n, device=dev, dtype=torch.float32)
+            a.states = states.data_ptr()
+    return last, states, _scan_ws(a, 0, dev)
 
 
-def _scan_backward(x, H, h0, mask, reverse, h_dtype, states, g_h, g_last, g_x):
-    """Writes columns [0, 2H) of g_x; -> gradient of h0 in its shape (None without h0)."""
-    T, B = x.shape[:2]
-    dev = x.device
-    if T == 0:
-        g0 = g_last.float() if g_last is not None else None
-    else:
-        a = native.GatedScan()
-        _fill_scan(a, x, H, h0, mask, reverse)
-        a.h_bf16 = int(h_dtype == torch.bfloat16)
-        a.states, a.g_h, a.g_last = ops._ptr(states), ops._ptr(g_h), ops._ptr(g_last)
-        a.g_gates, a.g_gates_st, a.g_gates_sb = g_x.data_ptr(), g_x.stride(0), g_x.stride(1)
-        g0 = None
-        if h0 is not None:
-            g0 = torch.empty(B, H, device=dev, dtype=torch.float32)
-            a.g_h0 = g0.data_ptr()
-        ws = _scan_ws(a, 1, dev)
-        ops._call('mdmm_gated_scan_bwd', C.byref(a), tag='gated_scan_bwd[H=%d]' % H)
-        del ws
+def _scan_backward(a, x, H, h0, mask, reverse, h_dtype, states, g_h, g_last, g_x, need_h0):
+    """Fills the struct of a backward call that writes columns [0, 2H) of g_x -> (gradient of h0 in its shape or None,
+    tensors to hold until the launch)."""
+    B, dev = x.shape[1], x.device
+    _fill_scan(a, x, H, h0, mask, reverse)
+    a.h_bf16 = h_dtype is torch.bfloat16
+    a.states, a.g_h, a.g_last = ops._ptr(states), ops._ptr(g_h), ops._ptr(g_last)
+    a.g_gates, a.g_gates_st, a.g_gates_sb = g_x.data_ptr(), g_x.stride(0), g_x.stride(1)
+    g0 = per = None
+    if need_h0:
+        g0 = per = torch.empty((B, H), device=dev, dtype=torch.float32)
+        a.g_h0 = per.data_ptr()
+        if h0.dim() == 1:
+            g0 = torch.empty(H, device=dev, dtype=torch.float32)
+            a.g_h0_sum = g0.data_ptr()
+    return g0, (per, _scan_ws(a, 1, dev))
+
+
+def _no_steps_last(h0, B, H, dev):
+    return torch.zeros(B, H, device=dev) if h0 is None else h0.detach().expand(B, H).clone()
+
+
+def _no_steps_grad(h0, g_last):
+    """Gradient of h0 where nothing was launched: T = 0 hands g_last on, B or H = 0 has none."""
     if h0 is None:
         return None
-    if g0 is None:
+    if g_last is None or h0.numel() == 0 or g_last.shape[0] == 0:
         return torch.zeros_like(h0)
-    return g0 if h0.dim() == 2 else _row_sum(g0)
-
-
-def _row_sum(g):
-    """(B, H) -> (H,), on the column-sum kernel where it takes the width (a fixed order, and safe in a captured graph)."""
-    if g.shape[0] == 0:
-        return g.new_zeros(g.shape[1])
-    return g[0] if g.shape[0] == 1 else ops.colsum(g)
+    return g_last if h0.dim() == 2 else ops.colsum(g_last)
 
 
 class _GatedScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gates, h0, mask, reverse):
         ctx.set_materialize_grads(False)
-        H = gates.shape[-1] // 2
-        keep = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-        with _on(gates.device):
-            h, last, states = _scan_forward(gates, H, h0, mask, reverse, gates.dtype, keep)
+        T, B, H2 = gates.shape
+        H = H2 // 2
+        need = ctx.needs_input_grad
+        keep = need[0] or need[1]
+        h = torch.empty((T, B, H), device=gates.device, dtype=gates.dtype)
+        states = None
+        if h.numel() == 0:
+            last = _no_steps_last(h0, B, H, gates.device)
+        else:
+            a = native.GatedScan()
+            last, states, ws = _scan_forward(a, gates, H, h0, mask, reverse, h, keep)
+            _launch('mdmm_gated_scan_fwd', 'gated_scan_fwd', a)
+            del ws
         if keep:
             ctx.save_for_backward(gates, h0, mask, states)
             ctx.reverse = reverse
@@ -182,12 +206,16 @@ class _GatedScanFn(torch.autograd.Function):
         if g_h is None and g_last is None:
             return None, None, None, None
         gates, h0, mask, states = ctx.saved_tensors
-        T, B, H2 = gates.shape
-        with _on(gates.device):
-            g_h = None if g_h is None else g_h.contiguous()
-            g_last = None if g_last is None else g_last.contiguous()
-            g_x = torch.empty(T, B, H2, device=gates.device, dtype=gates.dtype)
-            g0 = _scan_backward(gates, H2 // 2, h0, mask, ctx.reverse, gates.dtype, states, g_h, g_last, g_x)
+        g_h = None if g_h is None else g_h.contiguous()
+        g_last = None if g_last is None else g_last.contiguous()
+        g_x = torch.empty(gates.shape, device=gates.device, dtype=gates.dtype)
+        if g_x.numel() == 0:
+            return g_x, _no_steps_grad(h0, g_last if gates.shape[0] == 0 else None), None, None
+        a = native.GatedScan()
+        g0, hold = _scan_backward(a, gates, gates.shape[2] // 2, h0, mask, ctx.reverse, gates.dtype, states, g_h, g_last, g_x,
+                                  h0 is not None and ctx.needs_input_grad[1])
+        _launch('mdmm_gated_scan_bwd', 'gated_scan_bwd', a)
+        del hold
         return g_x, g0, None, None
 
 
@@ -203,8 +231,8 @@ def gated_scan(gates, h0=None, mask=None, reverse=False):
     _check_type('gated_scan', gates)
     T, B, H2 = gates.shape
     h0, mask = _check_h0('gated_scan', h0, B, H2 // 2), _mask_bytes('gated_scan', mask, (T, B))
-    _check_device('gated_scan', gates, h0, mask)
-    return _GatedScanFn.apply(_unit_cols(gates), h0, mask, bool(reverse))
+    dev = _check_device('gated_scan', gates, h0, mask)
+    return _apply(dev, _GatedScanFn.apply, _unit_cols(gates), h0, mask, bool(reverse))
 
 
 def _no_grad_only(name, *tensors):
@@ -233,16 +261,27 @@ def gated_scan_step(gates, state, mask=None, new_state=None):
     mask = _mask_bytes('gated_scan_step', mask, (B,))
     _no_grad_only('gated_scan_step', gates, state)
     _check_state('gated_scan_step', state, new_state, B, H)
-    _check_device('gated_scan_step', gates, state, mask, new_state)
+    dev = _check_device('gated_scan_step', gates, state, mask, new_state)
+    return _apply(dev, _scan_step, _unit_cols(gates), state, mask, new_state)
+
+
+def _scan_step(gates, state, mask, new_state):
+    B, H = state.shape
     new_state = torch.empty_like(state) if new_state is None else new_state
-    with _on(gates.device):
-        h = torch.empty(B, H, device=gates.device, dtype=gates.dtype)
-        if B and H:
-            a = native.GatedScan()
-            _fill_scan(a, _unit_cols(gates).unsqueeze(0), H, state, None if mask is None else mask.unsqueeze(0), False)
-            a.h, a.h_last, a.h_bf16 = h.data_ptr(), new_state.data_ptr(), a.gates_bf16
-            ops._call('mdmm_gated_scan_fwd', C.byref(a), tag='gated_scan_step[H=%d]' % H)
+    h = torch.empty((B, H), device=gates.device, dtype=gates.dtype)
+    if h.numel():
+        a = native.GatedScan()
+        _fill_step(a, gates, H, state, mask, new_state)
+        a.h, a.h_bf16 = h.data_ptr(), a.gates_bf16
+        _launch('mdmm_gated_scan_fwd', 'gated_scan_step', a)
     return h, new_state
+
+
+def _fill_step(a, x, H, state, mask, new_state):
+    a.T, a.B, a.H, a.gates_bf16 = 1, x.shape[0], H, x.dtype is torch.bfloat16
+    a.gates, a.gates_sb, a.h0, a.h0_sb, a.h_last = x.data_ptr(), x.stride(0), state.data_ptr(), H, new_state.data_ptr()
+    if mask is not None:
+        a.mask, a.mask_sb = mask.data_ptr(), mask.stride(0)
 
 
 # ---- norms -------------------------------------------------------------------------------------------------------
@@ -274,39 +313,41 @@ def _fill_norm(p, y, gate, res, w, s, w_next, branch, eps):
     p.w, p.scale, p.w_next = ops._ptr(w), ops._ptr(s), ops._ptr(w_next)
 
 
-def _norm_forward(y, gate, res, w, s, w_next, branch, eps):
-    """Row-major (rows, H) operands -> (out or None, n or None)."""
-    rows, H = res.shape
-    out = torch.empty(rows, H, device=res.device, dtype=res.dtype) if y is not None else None
-    n = torch.empty(rows, H, device=res.device, dtype=branch) if w_next is not None else None
-    p = native.BlockNorm()
+def _norm_forward(p, y, gate, res, w, s, w_next, branch, eps):
+    """Fills the struct of a forward call on row-major (rows, H) operands -> (out or None, n or None)."""
+    out = n = None
     _fill_norm(p, y, gate, res, w, s, w_next, branch, eps)
-    if out is not None:
-        p.out, p.out_st = out.data_ptr(), H
-    if n is not None:
-        p.n, p.n_st = n.data_ptr(), H
-    ops._call('mdmm_block_norm_fwd', C.byref(p), tag='block_norm_fwd[H=%d]' % H)
+    if y is not None:
+        out = torch.empty(res.shape, device=res.device, dtype=res.dtype)
+        p.out, p.out_st = out.data_ptr(), p.H
+    if w_next is not None:
+        n = torch.empty(res.shape, device=res.device, dtype=branch)
+        p.n, p.n_st = n.data_ptr(), p.H
     return out, n
 
 
-def _norm_backward(y, gate, res, w, s, w_next, branch, eps, g_out, g_n, d_y, d_gate, d_res, want):
-    """Writes d_y, d_gate, d_res (row-major views, None: not wanted); want = (d_w, d_scale, d_w_next) flags -> the three
-    column sums (None where not wanted)."""
+def _norm_backward(p, y, gate, res, w, s, w_next, branch, eps, g_out, g_n, d_y, d_gate, d_res, want):
+    """Fills the struct of a backward call: d_y, d_gate, d_res row-major views (None: not wanted), want = (d_w, d_scale,
+    d_w_next) flags -> (the three column sums, None where not wanted; scratch to hold until the launch)."""
     H, dev = res.shape[1], res.device
-    p = native.BlockNorm()
     _fill_norm(p, y, gate, res, w, s, w_next, branch, eps)
-    for f, t in (('g_out', g_out), ('g_n', g_n), ('d_y', d_y), ('d_gate', d_gate), ('d_res', d_res)):
-        if t is not None:
-            setattr(p, f, t.data_ptr())
-            setattr(p, f + '_st', _row(t))
+    if g_out is not None:
+        p.g_out, p.g_out_st = g_out.data_ptr(), _row(g_out)
+    if g_n is not None:
+        p.g_n, p.g_n_st = g_n.data_ptr(), _row(g_n)
+    if d_y is not None:
+        p.d_y, p.d_y_st = d_y.data_ptr(), _row(d_y)
+    if d_gate is not None:
+        p.d_gate, p.d_gate_st = d_gate.data_ptr(), _row(d_gate)
+    if d_res is not None:
+        p.d_res, p.d_res_st = d_res.data_ptr(), _row(d_res)
     sums = [torch.empty(H, device=dev, dtype=torch.float32) if k else None for k in want]
     if res.shape[0] == 0:
-        return [None if t is None else t.zero_() for t in sums]
+        return [None if t is None else t.zero_() for t in sums], None
     p.d_w, p.d_scale, p.d_w_next = (ops._ptr(t) for t in sums)
-    ws = torch.empty(native.lib().mdmm_block_norm_ws(C.byref(p)), device=dev, dtype=torch.float32)
+    ws = torch.empty(_size('mdmm_block_norm_ws', p), device=dev, dtype=torch.float32)
     p.ws = ws.data_ptr()
-    ops._call('mdmm_block_norm_bwd', C.byref(p), tag='block_norm_bwd[H=%d]' % H)
-    return sums
+    return sums, ws
 
 
 class _RmsNormFn(torch.autograd.Function):
@@ -316,8 +357,9 @@ class _RmsNormFn(torch.autograd.Function):
         rows = _as_rows(x, x.shape[-1])
         ctx.save_for_backward(rows, w)
         ctx.eps, ctx.branch = eps, dtype
-        with _on(x.device):
-            n = _norm_forward(None, None, rows, None, None, w, dtype, eps)[1]
+        p = native.BlockNorm()
+        n = _norm_forward(p, None, None, rows, None, None, w, dtype, eps)[1]
+        _launch('mdmm_block_norm_fwd', 'rms_norm_fwd', p)
         return n.view(x.shape)
 
     @staticmethod
@@ -327,10 +369,14 @@ class _RmsNormFn(torch.autograd.Function):
             return None, None, None, None
         x, w = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
-        with _on(x.device):
-            d_x = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
-            sums = _norm_backward(None, None, x, None, None, w, ctx.branch, ctx.eps, None, _as_rows(g, x.shape[1]), None, None,
-                                  d_x, (False, False, need_w))
+        d_x = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
+        p = native.BlockNorm()
+        rows = _as_rows(g, x.shape[1])
+        sums, ws = _norm_backward(p, None, None, x, None, None, w, ctx.branch, ctx.eps, None, rows, None, None, d_x,
+                                  (False, False, need_w))
+        if x.shape[0]:
+            _launch('mdmm_block_norm_bwd', 'rms_norm_bwd', p)
+        del ws
         return None if d_x is None else d_x.view(g.shape), sums[2], None, None
 
 
@@ -351,8 +397,7 @@ def rms_norm(x, weight, eps=1e-6, dtype=None):
     if dtype not in _TYPES or (x.dtype == torch.bfloat16 and dtype != torch.bfloat16):
         raise ValueError('rms_norm: %s rows to %s' % (x.dtype, dtype))
     weight = _vector('rms_norm', 'weight', weight, H)
-    _check_device('rms_norm', x, weight)
-    return _RmsNormFn.apply(x, weight, float(eps), dtype)
+    return _apply(_check_device('rms_norm', x, weight), _RmsNormFn.apply, x, weight, float(eps), dtype)
 
 
 class _BlockNormFn(torch.autograd.Function):
@@ -363,8 +408,9 @@ class _BlockNormFn(torch.autograd.Function):
         rows = [None if t is None else _as_rows(t, H) for t in (y, gate, res)]
         ctx.save_for_backward(*rows, w, s, w_next)
         ctx.eps, ctx.shape = eps, res.shape
-        with _on(res.device):
-            out, n = _norm_forward(*rows, w, s, w_next, y.dtype, eps)
+        p = native.BlockNorm()
+        out, n = _norm_forward(p, *rows, w, s, w_next, y.dtype, eps)
+        _launch('mdmm_block_norm_fwd', 'block_norm_fwd', p)
         out = out.view(res.shape)
         return out if n is None else (out, n.view(res.shape))
 
@@ -376,17 +422,19 @@ class _BlockNormFn(torch.autograd.Function):
         y, gate, res, w, s, w_next = ctx.saved_tensors
         need = ctx.needs_input_grad                     # y, res, w, gate, s, w_next
         H, dev = res.shape[1], res.device
-        with _on(dev):
-            g_out = None if g_out is None else _as_rows(g_out, H)
-            g_n = None if g_n is None else _as_rows(g_n, H)
-            empty = lambda like: torch.empty(res.shape, device=dev, dtype=like.dtype)      # noqa: E731
-            d_y = empty(y) if need[0] else None
-            d_gate = empty(gate) if need[3] else None
-            d_res = empty(res) if need[1] and g_n is not None else None      # (without a next norm it is g_out itself)
-            sums = _norm_backward(y, gate, res, w, s, w_next, y.dtype, ctx.eps, g_out, g_n, d_y, d_gate, d_res,
+        g_out = None if g_out is None else _as_rows(g_out, H)
+        g_n = None if g_n is None else _as_rows(g_n, H)
+        d_y = torch.empty(res.shape, device=dev, dtype=y.dtype) if need[0] else None
+        d_gate = torch.empty(res.shape, device=dev, dtype=gate.dtype) if need[3] else None
+        d_res = torch.empty(res.shape, device=dev, dtype=res.dtype) if need[1] and g_n is not None else None
+        p = native.BlockNorm()
+        sums, ws = _norm_backward(p, y, gate, res, w, s, w_next, y.dtype, ctx.eps, g_out, g_n, d_y, d_gate, d_res,
                                   (need[2], need[4], need[5]))
-            if need[1] and d_res is None:
-                d_res = g_out
+        if res.shape[0]:
+            _launch('mdmm_block_norm_bwd', 'block_norm_bwd', p)
+        del ws
+        if need[1] and d_res is None:                    # (without a next norm it is g_out itself)
+            d_res = g_out
         view = lambda t: None if t is None else t.reshape(ctx.shape)                       # noqa: E731
         return view(d_y), view(d_res), sums[0], view(d_gate), sums[1], sums[2], None
 
@@ -410,8 +458,8 @@ def block_norm(y, residual, weight, gate=None, scale=None, next_weight=None, eps
         raise ValueError('%s: gate %s beside y %s' % (name, gate.dtype, y.dtype))
     _combo(name, y.dtype, y.dtype, residual.dtype)
     weight, scale, next_weight = _vectors(name, weight, scale, next_weight, H)
-    _check_device(name, y, residual, weight, gate, scale, next_weight)
-    return _BlockNormFn.apply(y, residual, weight, gate, scale, next_weight, float(eps))
+    dev = _check_device(name, y, residual, weight, gate, scale, next_weight)
+    return _apply(dev, _BlockNormFn.apply, y, residual, weight, gate, scale, next_weight, float(eps))
 
 
 # ---- the layer ---------------------------------------------------------------------------------------------------
@@ -424,11 +472,18 @@ class _GatedBlockFn(torch.autograd.Function):
     def forward(ctx, proj, res, h0, w, s, w_next, mask, reverse, eps):
         ctx.set_materialize_grads(False)
         T, B, H = res.shape
+        dev = proj.device
         keep = any(ctx.needs_input_grad)
-        with _on(proj.device):
-            h, last, states = _scan_forward(proj, H, h0, mask, reverse, torch.float32, keep)
-            rows, flat = _as_rows(res, H), _as_rows(proj, 3 * H)
-            out, n = _norm_forward(h.view(-1, H), flat[:, 2 * H:], rows, w, s, w_next, proj.dtype, eps)
+        h = torch.empty((T, B, H), device=dev, dtype=torch.float32)
+        rows, flat, states = _as_rows(res, H), _as_rows(proj, 3 * H), None
+        a, p = native.GatedScan(), native.BlockNorm()
+        out, n = _norm_forward(p, h.view(-1, H), flat[:, 2 * H:], rows, w, s, w_next, proj.dtype, eps)
+        if h.numel() == 0:
+            last = _no_steps_last(h0, B, H, dev)
+        else:
+            last, states, ws = _scan_forward(a, proj, H, h0, mask, reverse, h, keep)
+            _launch('mdmm_gated_block_fwd', 'gated_block_fwd', a, p)
+            del ws
         if keep:
             ctx.save_for_backward(proj, rows, h0, w, s, w_next, mask, states, h)
             ctx.reverse, ctx.eps = reverse, eps
@@ -446,23 +501,30 @@ class _GatedBlockFn(torch.autograd.Function):
         H, dev = H3 // 3, proj.device
         if g_out is None and g_n is None and g_last is None:
             return (None,) * 9
-        with _on(dev):
-            g_out = None if g_out is None else _as_rows(g_out, H)
-            g_n = None if g_n is None else _as_rows(g_n, H)
-            g_last = None if g_last is None else g_last.contiguous()
-            g_x = torch.empty(T, B, H3, device=dev, dtype=proj.dtype)
-            d_res = d_h = None
-            sums = [None, None, None]
-            if g_out is None and g_n is None:
-                g_x[..., 2 * H:].zero_()
-            else:
-                d_h = torch.empty(T * B, H, device=dev, dtype=torch.float32)
-                d_res = torch.empty(T * B, H, device=dev, dtype=res.dtype) if need[1] and g_n is not None else None
-                sums = _norm_backward(h.view(-1, H), _as_rows(proj, H3)[:, 2 * H:], res, w, s, w_next, proj.dtype, ctx.eps,
-                                      g_out, g_n, d_h, g_x.view(-1, H3)[:, 2 * H:], d_res, (need[3], need[4], need[5]))
-                if need[1] and d_res is None:
-                    d_res = g_out
-            g0 = _scan_backward(proj, H, h0, mask, ctx.reverse, torch.float32, states, d_h, g_last, g_x)
+        g_out = None if g_out is None else _as_rows(g_out, H)
+        g_n = None if g_n is None else _as_rows(g_n, H)
+        g_last = None if g_last is None else g_last.contiguous()
+        g_x = torch.empty((T, B, H3), device=dev, dtype=proj.dtype)
+        a, p = native.GatedScan(), native.BlockNorm()
+        d_res = d_h = ws = hold = None
+        sums = [None, None, None]
+        if g_out is None and g_n is None:
+            p.rows, p.H = T * B, H
+            g_x[..., 2 * H:].zero_()
+        else:
+            d_h = torch.empty((T * B, H), device=dev, dtype=torch.float32)
+            d_res = torch.empty((T * B, H), device=dev, dtype=res.dtype) if need[1] and g_n is not None else None
+            sums, ws = _norm_backward(p, h.view(-1, H), _as_rows(proj, H3)[:, 2 * H:], res, w, s, w_next, proj.dtype, ctx.eps,
+                                      g_out, g_n, d_h, g_x.view(-1, H3)[:, 2 * H:], d_res, need[3:6])
+            if need[1] and d_res is None:
+                d_res = g_out
+        if h.numel() == 0:
+            g0 = _no_steps_grad(h0, g_last if T == 0 else None)
+        else:
+            g0, hold = _scan_backward(a, proj, H, h0, mask, ctx.reverse, torch.float32, states, d_h, g_last, g_x,
+                                      h0 is not None and need[2])
+            _launch('mdmm_gated_block_bwd', 'gated_block_bwd', a, p)
+        del ws, hold
         return (g_x, None if d_res is None else d_res.reshape(T, B, H), g0, *sums, None, None, None)
 
 
@@ -491,8 +553,9 @@ def gated_block(proj, residual, h0, weight, scale=None, next_weight=None, mask=N
     T, B = proj.shape[:2]
     weight, scale, next_weight = _vectors(name, weight, scale, next_weight, H)
     h0, mask = _check_h0(name, h0, B, H), _mask_bytes(name, mask, (T, B))
-    _check_device(name, proj, residual, h0, weight, scale, next_weight, mask)
-    return _GatedBlockFn.apply(_unit_cols(proj), residual, h0, weight, scale, next_weight, mask, bool(reverse), float(eps))
+    dev = _check_device(name, proj, residual, h0, weight, scale, next_weight, mask)
+    return _apply(dev, _GatedBlockFn.apply, _unit_cols(proj), residual, h0, weight, scale, next_weight, mask, bool(reverse),
+                  float(eps))
 
 
 def gated_block_step(proj, residual, state, weight, scale=None, next_weight=None, mask=None, eps=1e-6, new_state=None):
@@ -505,19 +568,19 @@ def gated_block_step(proj, residual, state, weight, scale=None, next_weight=None
     mask = _mask_bytes(name, mask, (B,))
     _no_grad_only(name, proj, residual, state, w, s, w_next)
     _check_state(name, state, new_state, B, H)
-    _check_device(name, proj, residual, state, w, s, w_next, mask, new_state)
+    dev = _check_device(name, proj, residual, state, w, s, w_next, mask, new_state)
+    return _apply(dev, _block_step, _unit_cols(proj), _unit_cols(residual), state, w, s, w_next, mask, float(eps), new_state)
+
+
+def _block_step(proj, residual, state, w, s, w_next, mask, eps, new_state):
+    H = state.shape[1]
     new_state = torch.empty_like(state) if new_state is None else new_state
-    with _on(proj.device):
-        proj, residual = _unit_cols(proj), _unit_cols(residual)
-        out = torch.empty(B, H, device=proj.device, dtype=residual.dtype)
-        n = torch.empty(B, H, device=proj.device, dtype=proj.dtype) if w_next is not None else None
-        if B:
-            a, p = native.GatedScan(), native.BlockNorm()
-            _fill_scan(a, proj.unsqueeze(0), H, state, None if mask is None else mask.unsqueeze(0), False)
-            a.h_last = new_state.data_ptr()
-            _fill_norm(p, None, proj[:, 2 * H:], residual, w, s, w_next, proj.dtype, float(eps))
-            p.out, p.out_st = out.data_ptr(), H
-            if n is not None:
-                p.n, p.n_st = n.data_ptr(), H
-            ops._call('mdmm_gated_block_step', C.byref(a), C.byref(p), tag='gated_block_step[H=%d]' % H)
+    a, p = native.GatedScan(), native.BlockNorm()
+    out, n = _norm_forward(p, None, None, residual, w, s, w_next, proj.dtype, eps)
+    out = torch.empty(residual.shape, device=proj.device, dtype=residual.dtype)
+    p.out, p.out_st = out.data_ptr(), H
+    p.gate, p.gate_st = proj.data_ptr() + 2 * H * proj.element_size(), _row(proj)
+    if out.numel():
+        _fill_step(a, proj, H, state, mask, new_state)
+        _launch('mdmm_gated_block_step', 'gated_block_step', a, p)
     return (out, new_state) if n is None else (out, n, new_state)
