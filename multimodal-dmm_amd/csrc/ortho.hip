@@ -1,9 +1,18 @@
 // Orthogonalised matrix updates by Newton-Schulz products (mdmm_ortho_t): X = M / (|M|_F + eps), then
-// X <- ca X + (cb A + cc A A) X with A = X X^T.  X lies down (n rows <= m columns), so both Gram-side products are n x n.
-// The iteration multiplies a small singular value by up to ca per step (ca^5 = 485 over five), and a rounding of X with it:
-// everything stays in fp32, on the fp32 matrix instruction.
-// Workspace per matrix, n and m rounded up to whole tiles with zeros (which every product keeps): two X buffers, A and the
-// polynomial P = ca I + cb A + cc A A.  All matrices of a call share each launch.
+// X <- ca X + P X with P = cb A + cc A A, A = X X^T.  X lies down (n rows <= m columns).
+//
+// The iteration multiplies a small singular value by up to ca a step (ca^5 = 485 over five), and a rounding of X with it, so
+// bf16 operands are out; fp32 ones would run on the fp32 matrix instruction, a sixteenth of the fp16 one's rate.  Every
+// matrix is kept as two fp16 planes instead, SC x = h + l / LO with h = fp16(SC x), l = fp16(LO (SC x - h)): 22 to 23 bits
+// (entries are at most 1.3, so SC x stays normal down to 1e-6 and below a sixteenth of fp16's largest), and a product is
+// h h' + (h l' + l h') / LO, the last two summed apart -- three fp16 matrix instructions for one fp32 product, the dropped
+// l l' of 2^-23 of a term, and one rounding of the fp32 sum for every 16 terms where the fp32 instruction has one for every
+// two: the result is nearer to 64 bits than fp32 products (3.6e-7 against 2.2e-6 at 256 x 256).  ca X is added in fp32.
+//
+// X is stored both ways (n x m for A, m x n for P X) so that every product runs over two operands' rows: tiles of both come
+// straight into LDS (four buffers, the loads of three tiles ahead in flight), chunks of 16 bytes swapped within a row so that
+// the matrix instruction's reads meet all banks.  A and P are symmetric: tiles above the diagonal only, stored twice.  Sizes
+// are rounded up to whole tiles with zeros, which every product keeps.  All matrices of a call share each launch.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "../../include/mdmm_hip.h"
@@ -11,16 +20,34 @@
 namespace mdmm {
 namespace {
 
-constexpr int NT = 256, TILE = 64, KB = 16, SUMS = 64;
+constexpr int NT = 256, SUMS = 64;
+constexpr float SC = 64.0f, LO = 2048.0f;
+typedef _Float16 half_t;
+typedef half_t half4 __attribute__((ext_vector_type(4)));
+typedef half_t half8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-struct Item {               // one matrix's padded sizes and workspace
-  float *x0, *x1, *gram, *poly, *sums;
-  int32_t n, m, tall, reserved;
+// BM x BN tile of a product by 2 x 2 waves, BK deep, ST buffers
+template <int BM_, int BN_, int BK_, int ST_> struct Cfg {
+  static constexpr int BM = BM_, BN = BN_, BK = BK_, ST = ST_;
+  static constexpr int TI = BM / 64, TJ = BN / 64;              // 32 x 32 pieces of a wave
+  static constexpr int CPR = BK / 8;                            // chunks of a row
+  static constexpr int HALVES = (BM + BN) * BK * 2;             // of a buffer: A h, A l, B h, B l
+  static constexpr int LOADS = HALVES / 8 / NT;                 // chunks a thread loads for a buffer
+};
+typedef Cfg<64, 64, 64, 4> Small;
+typedef Cfg<128, 128, 32, 4> Large;
+
+struct Item {               // one matrix's padded sizes and workspace; a plane pair is h, then l
+  half_t *xn, *xt[2], *gram, *poly;
+  float* part;              // split sums of A
+  double* sums;
+  int32_t n, m, tall, splits;
 };
 struct Items {
   Item it[MDMM_ORTHO_MAX];
   int32_t first[MDMM_ORTHO_MAX + 1];       // first tile of each matrix in this launch
+  int32_t which[MDMM_ORTHO_MAX];           // its place in the call
   int32_t n;
 };
 
@@ -33,28 +60,23 @@ __device__ __forceinline__ int find(const int32_t* first, int n, int tile) {
   return lo;
 }
 
+__device__ __forceinline__ void split(float x, half_t& h, half_t& l) {       // x: already times SC
+  h = (half_t)x;
+  l = (half_t)((x - (float)h) * LO);
+}
+__device__ __forceinline__ float join(half_t h, half_t l) { return fmaf((float)l, 1.0f / LO, (float)h); }
+
 __device__ __forceinline__ float src_at(const mdmm_ortho_t& p, const mdmm_ortho_item_t& t, int64_t r, int64_t c) {
   const int64_t i = r * t.src_ld + c;
   return p.src_bf16 ? (float)((const __bf16*)t.src)[i] : ((const float*)t.src)[i];
 }
 
-// element (r, c) of the result: stored, or taken as one optimizer step
-__device__ __forceinline__ void put(const mdmm_ortho_t& p, const mdmm_ortho_item_t& t, int64_t r, int64_t c, float v) {
-  const int64_t o = r * t.dst_ld + c;
-  if (p.update) {
-    float* d = (float*)t.dst + o;
-    const float lr = p.lr_dev ? *p.lr_dev : p.lr;
-    *d = fmaf(-lr * t.gain, v, (1.0f - lr * p.decay) * *d);
-  } else if (p.dst_bf16) ((__bf16*)t.dst)[o] = (__bf16)v;
-  else ((float*)t.dst)[o] = v;
-}
-
-// momentum, and the sum of squares in SUMS pieces
+// momentum, and the sum of squares in SUMS pieces (in 64 bits: an error of the norm is a scale of X and grows like one)
 __global__ __launch_bounds__(NT) void ortho_sums_kernel(mdmm_ortho_t p, Items q) {
   const int k = blockIdx.y;
-  const mdmm_ortho_item_t& t = p.item[k];
+  const mdmm_ortho_item_t& t = p.item[q.which[k]];
   const int64_t total = (int64_t)t.rows * t.cols;
-  float s = 0.0f;
+  double s = 0.0;
   for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)SUMS * NT) {
     float v = src_at(p, t, i / t.cols, i % t.cols);
     if (t.mom) {
@@ -62,25 +84,33 @@ __global__ __launch_bounds__(NT) void ortho_sums_kernel(mdmm_ortho_t p, Items q)
       t.mom[i] = mv;
       v = p.nesterov ? fmaf(p.momentum, mv, v) : mv;
     }
-    s = fmaf(v, v, s);
+    s += (double)v * v;
   }
-  __shared__ float part[NT / 64];
+  __shared__ double part[NT / 64];
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) q.it[k].sums[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+  if (threadIdx.x == 0) q.it[k].sums[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
+// X both ways, 64 x 64 elements a workgroup
 __global__ __launch_bounds__(NT) void ortho_pack_kernel(mdmm_ortho_t p, Items q) {
-  const int k = blockIdx.y;
-  const mdmm_ortho_item_t& t = p.item[k];
+  __shared__ float tile[64][65];
+  const int k = find(q.first, q.n, blockIdx.x);
+  const mdmm_ortho_item_t& t = p.item[q.which[k]];
   const Item& w = q.it[k];
-  float s = 0.0f;
+  double s = 0.0;
   for (int i = 0; i < SUMS; ++i) s += w.sums[i];
-  const float inv = 1.0f / (sqrtf(s) + p.eps);
-  const int64_t total = (int64_t)w.n * w.m;
-  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)gridDim.x * NT) {
-    const int64_t a = i / w.m, b = i % w.m, r = w.tall ? b : a, c = w.tall ? a : b;
+  const float inv = (float)((double)SC / (sqrt(s) + (double)p.eps));
+  const int at = blockIdx.x - q.first[k], across = (w.tall ? w.n : w.m) / 64;       // tiles of the source's rows
+  const int64_t r0 = at / across * 64, c0 = at % across * 64;
+  const int64_t nm = (int64_t)w.n * w.m;
+  // the source's orientation: lying or standing plane pair
+  half_t* same = w.tall ? w.xt[0] : w.xn;
+  half_t* other = w.tall ? w.xn : w.xt[0];
+  const int64_t ld_same = w.tall ? w.n : w.m, ld_other = w.tall ? w.m : w.n;
+  for (int i = threadIdx.x; i < 4096; i += NT) {
+    const int64_t r = r0 + i / 64, c = c0 + i % 64;
     float v = 0.0f;
     if (r < t.rows && c < t.cols) {
       v = src_at(p, t, r, c);
@@ -90,72 +120,246 @@ __global__ __launch_bounds__(NT) void ortho_pack_kernel(mdmm_ortho_t p, Items q)
       }
       v *= inv;
     }
-    w.x0[i] = v;
+    tile[i / 64][i % 64] = v;
+    half_t h, l;
+    split(v, h, l);
+    same[r * ld_same + c] = h;
+    same[nm + r * ld_same + c] = l;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 4096; i += NT) {
+    half_t h, l;
+    split(tile[i % 64][i / 64], h, l);
+    const int64_t o = (c0 + i / 64) * ld_other + r0 + i % 64;
+    other[o] = h;
+    other[nm + o] = l;
   }
 }
 
-enum { GRAM, POLY, APPLY };
+enum { GRAM, POLY, APPLY, LAST };          // (LAST: an APPLY whose result goes to dst)
 
-// One 64 x 64 tile of a product, four waves of 32 x 32: GRAM A = X X^T, POLY P = ca I + cb A + cc A A (A symmetric: its
-// columns are read as rows), APPLY X' = P X (the last one into dst)
-template <int MODE>
-__global__ __launch_bounds__(NT) void ortho_product_kernel(mdmm_ortho_t p, Items q, int flip, int last) {
-  __shared__ float As[KB][TILE + 4], Bs[KB][TILE + 4];
-  const int k = find(q.first, q.n, blockIdx.x);
-  const Item& w = q.it[k];
-  const float* x = flip ? w.x1 : w.x0;
-  float* xn = flip ? w.x0 : w.x1;
-  const int K = MODE == GRAM ? w.m : w.n, J = MODE == APPLY ? w.m : w.n;
-  const int tile = blockIdx.x - q.first[k], tj = J / TILE;
-  const int i0 = tile / tj * TILE, j0 = tile % tj * TILE;
-  const float* a = MODE == GRAM ? x : MODE == POLY ? w.gram : w.poly;       // (n, K), rows
-  const float* b = MODE == POLY ? w.gram : x;                               // NT: (J, K) rows; APPLY: (K, J) rows
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-  f32x16 acc = {};
-  for (int k0 = 0; k0 < K; k0 += KB) {
-    const int r = tid >> 2, c = (tid & 3) * 4;
-    const float4 va = *(const float4*)(a + (int64_t)(i0 + r) * K + k0 + c);
-    float4 vb;
-    const int br = tid >> 4, bc = (tid & 15) * 4;
-    if (MODE == APPLY) vb = *(const float4*)(b + (int64_t)(k0 + br) * J + j0 + bc);
-    else vb = *(const float4*)(b + (int64_t)(j0 + r) * K + k0 + c);
-    __syncthreads();
-    As[c][r] = va.x; As[c + 1][r] = va.y; As[c + 2][r] = va.z; As[c + 3][r] = va.w;
-    if (MODE == APPLY) *(float4*)&Bs[br][bc] = vb;
-    else { Bs[c][r] = vb.x; Bs[c + 1][r] = vb.y; Bs[c + 2][r] = vb.z; Bs[c + 3][r] = vb.w; }
-    __syncthreads();
+// four consecutive rows i of one column j of a symmetric plane pair of n x n, both ways.  On the diagonal's tiles (i, j) and
+// (j, i) are both computed, and may round differently: there the upper one is stored in both places, the lower one nowhere
+__device__ __forceinline__ void put_sym(half_t* dst, int64_t n, int64_t i, int64_t j, const float* v, bool diagonal) {
+  half4 h4, l4;
 #pragma unroll
-    for (int kk = 0; kk < KB; kk += 2) {
-      const float fa = As[kk + (lane >> 5)][wi + (lane & 31)], fb = Bs[kk + (lane >> 5)][wj + (lane & 31)];
-      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(fa, fb, acc, 0, 0, 0);
-    }
-  }
-  const mdmm_ortho_item_t& t = p.item[k];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const int64_t i = i0 + wi + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), j = j0 + wj + (lane & 31);
-    float v = acc[e];
-    if (MODE == GRAM) w.gram[i * J + j] = v;
-    if (MODE == POLY) w.poly[i * J + j] = fmaf(p.cc, v, fmaf(p.cb, w.gram[i * J + j], i == j ? p.ca : 0.0f));
-    if (MODE == APPLY && !last) xn[i * J + j] = v;
-    if (MODE == APPLY && last) {
-      const int64_t r = w.tall ? j : i, c = w.tall ? i : j;
-      if (r < t.rows && c < t.cols) {
-        put(p, t, r, c, v);
+  for (int e = 0; e < 4; ++e) {
+    half_t h, l;
+    split(v[e], h, l);
+    h4[e] = h;
+    l4[e] = l;
+    if (!diagonal || i + e <= j) {
+      dst[(i + e) * n + j] = h;
+      dst[n * n + (i + e) * n + j] = l;
+      if (diagonal) {
+        dst[j * n + i + e] = h;
+        dst[n * n + j * n + i + e] = l;
       }
     }
+  }
+  if (!diagonal) {
+    *(half4*)(dst + j * n + i) = h4;
+    *(half4*)(dst + n * n + j * n + i) = l4;
+  }
+}
+
+// tile t of the triangle at and above the diagonal, row by row
+__device__ __forceinline__ void triangle(int t, int tiles, int& ti, int& tj) {
+  int r = (int)(((2 * tiles + 1) - sqrtf((float)(2 * tiles + 1) * (2 * tiles + 1) - 8.0f * t)) * 0.5f);
+  r = r < 0 ? 0 : r >= tiles ? tiles - 1 : r;
+  while (r > 0 && r * tiles - r * (r - 1) / 2 > t) --r;
+  while ((r + 1) * tiles - (r + 1) * r / 2 <= t) ++r;
+  ti = r;
+  tj = r + t - (r * tiles - r * (r - 1) / 2);
+}
+
+// all but the last N loads have landed, and this wave's reads of LDS are done
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+
+template <int MODE, class C>
+__global__ __launch_bounds__(NT) void ortho_product_kernel(mdmm_ortho_t p, Items q, int flip) {
+  __shared__ __align__(16) half_t lds[C::ST * C::HALVES];
+  constexpr bool PX = MODE == APPLY || MODE == LAST;
+  const int k = find(q.first, q.n, blockIdx.x);
+  const Item w = q.it[k];
+  const int n = w.n, J = PX ? w.m : n;
+  int tile = blockIdx.x - q.first[k], ti, tj, slice = 0;
+  if (PX) {
+    ti = tile / (J / C::BN);
+    tj = tile % (J / C::BN);
+  } else {
+    const int tiles = n / C::BM, all = tiles * (tiles + 1) / 2;
+    if (MODE == GRAM) { slice = tile / all; tile %= all; }
+    triangle(tile, tiles, ti, tj);
+  }
+  const int i0 = ti * C::BM, j0 = tj * C::BN;
+  const half_t* xt = w.xt[flip];
+  const half_t* a = MODE == GRAM ? w.xn : MODE == POLY ? w.gram : w.poly;
+  const half_t* b = MODE == GRAM ? w.xn : MODE == POLY ? w.gram : xt;
+  const int64_t K = MODE == GRAM ? w.m : n;               // columns of both
+  const int64_t la = (int64_t)n * K, lb = PX ? (int64_t)w.m * K : la;
+  const int steps_all = (int)(K / C::BK);
+  const int per = MODE == GRAM ? (steps_all + w.splits - 1) / w.splits : steps_all;
+  const int s0 = slice * per, nk = s0 + per < steps_all ? per : steps_all - s0;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // this thread's chunks of a buffer: where they come from
+  const half_t* from[C::LOADS];
+#pragma unroll
+  for (int c = 0; c < C::LOADS; ++c) {
+    constexpr int AC = C::BM * C::CPR, BC = C::BN * C::CPR;
+    const int first = c * NT;                              // (a multiple of NT: the whole workgroup is in one plane)
+    const bool in_b = first >= 2 * AC;
+    const int plane = in_b ? (first - 2 * AC) / BC : first / AC;
+    const int at = (in_b ? (first - 2 * AC) % BC : first % AC) + tid;
+    const int row = at / C::CPR, ch = (at % C::CPR) ^ (row / (16 / C::CPR) % C::CPR);
+    from[c] = (in_b ? b + plane * lb + (j0 + row) * K : a + plane * la + (i0 + row) * K) + (int64_t)s0 * C::BK + ch * 8;
+  }
+  auto load = [&](int buf) {
+#pragma unroll
+    for (int c = 0; c < C::LOADS; ++c) {
+      half_t* to = lds + buf * C::HALVES + (c * NT + wave * 64) * 8;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from[c],
+                                       (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+      from[c] += C::BK;
+    }
+  };
+  f32x16 main[C::TI][C::TJ] = {}, cross[C::TI][C::TJ] = {};
+  const int wi = (wave >> 1) * 32 * C::TI, wj = (wave & 1) * 32 * C::TJ;
+#pragma unroll
+  for (int s = 0; s < C::ST - 1; ++s)
+    if (s < nk) load(s);
+  for (int s = 0; s < nk; ++s) {
+    // buffer s has landed when no more than the loads of the buffers behind it are in flight
+    if (s + C::ST - 2 < nk) wait_loads<(C::ST - 2) * C::LOADS>();
+    else wait_loads<0>();
+    __builtin_amdgcn_s_barrier();             // (every wave's share; and all are done with the buffer that is filled next)
+    asm volatile("" ::: "memory");
+    if (s + C::ST - 1 < nk) load((s + C::ST - 1) % C::ST);
+    const half_t* A = lds + s % C::ST * C::HALVES;
+    const half_t* B = A + 2 * C::BM * C::BK;
+#pragma unroll
+    for (int kk = 0; kk < C::BK / 16; ++kk) {
+      half8 ah[C::TI], al[C::TI], bh[C::TJ], bl[C::TJ];
+      const int c = kk * 2 + (lane >> 5);
+#pragma unroll
+      for (int t = 0; t < C::TI; ++t) {
+        const int row = wi + t * 32 + (lane & 31), o = row * C::BK + ((c ^ (row / (16 / C::CPR) % C::CPR)) * 8);
+        ah[t] = *(const half8*)(A + o);
+        al[t] = *(const half8*)(A + C::BM * C::BK + o);
+      }
+#pragma unroll
+      for (int t = 0; t < C::TJ; ++t) {
+        const int row = wj + t * 32 + (lane & 31), o = row * C::BK + ((c ^ (row / (16 / C::CPR) % C::CPR)) * 8);
+        bh[t] = *(const half8*)(B + o);
+        bl[t] = *(const half8*)(B + C::BN * C::BK + o);
+      }
+#pragma unroll
+      for (int x = 0; x < C::TI; ++x)
+#pragma unroll
+        for (int y = 0; y < C::TJ; ++y) {
+          main[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bh[y], main[x][y], 0, 0, 0);
+          cross[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bl[y], cross[x][y], 0, 0, 0);
+          cross[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[x], bh[y], cross[x][y], 0, 0, 0);
+        }
+    }
+  }
+  // v: the product times SC (operands carry SC each)
+  const mdmm_ortho_item_t t = p.item[q.which[k]];
+  const int64_t nn = (int64_t)n * n, nm = (int64_t)n * w.m, m = w.m;
+  const float lr = MODE == LAST && p.update ? (p.lr_dev ? *p.lr_dev : p.lr) : 0.0f;
+#pragma unroll
+  for (int x = 0; x < C::TI; ++x)
+#pragma unroll
+    for (int y = 0; y < C::TJ; ++y)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        // four consecutive rows of one column
+        const int64_t i = i0 + wi + x * 32 + 8 * g + 4 * (lane >> 5), j = j0 + wj + y * 32 + (lane & 31);
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(cross[x][y][4 * g + e], 1.0f / LO, main[x][y][4 * g + e]) * (1.0f / SC);
+        if (MODE == GRAM) {
+          if (w.splits == 1) put_sym(w.gram, n, i, j, v, ti == tj);
+          else *(float4*)(w.part + slice * nn + j * n + i) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        if (MODE == POLY) {
+          const half4 h = *(const half4*)(w.gram + j * n + i), l = *(const half4*)(w.gram + nn + j * n + i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(p.cc, v[e], p.cb * join(h[e], l[e]));
+          put_sym(w.poly, n, i, j, v, ti == tj);
+        }
+        if (PX) {
+          const half4 h = *(const half4*)(xt + j * n + i), l = *(const half4*)(xt + nm + j * n + i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(p.ca, join(h[e], l[e]), v[e]);
+        }
+        if (MODE == APPLY) {
+          half4 h4, l4;
+          half_t* lie = w.xn + i * m + j;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            half_t hh, ll;
+            split(v[e], hh, ll);
+            h4[e] = hh;
+            l4[e] = ll;
+            lie[e * m] = hh;
+            lie[nm + e * m] = ll;
+          }
+          half_t* to = w.xt[flip ^ 1] + j * n + i;
+          *(half4*)to = h4;
+          *(half4*)(to + nm) = l4;
+        }
+        if (MODE == LAST) {
+          const int64_t r = w.tall ? j : i, c = w.tall ? i : j, step = w.tall ? 1 : t.dst_ld;
+          const int64_t end = w.tall ? (r < t.rows ? t.cols - c : 0) : (c < t.cols ? t.rows - r : 0);      // of the four
+          const int64_t o = r * t.dst_ld + c;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float u = v[e] * (1.0f / SC);
+            if (e >= end) continue;
+            if (p.update) {
+              float* d = (float*)t.dst + o + e * step;
+              *d = fmaf(-lr * t.gain, u, (1.0f - lr * p.decay) * *d);
+            } else if (p.dst_bf16) ((__bf16*)t.dst)[o + e * step] = (__bf16)u;
+            else ((float*)t.dst)[o + e * step] = u;
+          }
+        }
+      }
+}
+
+// the slices of A added up (each keeps the upper triangle of tiles, column by column)
+template <int BM> __global__ __launch_bounds__(NT) void ortho_fold_kernel(Items q) {
+  const Item w = q.it[blockIdx.y];
+  if (w.splits == 1) return;
+  const int64_t n = w.n, nn = n * n;
+  for (int64_t e = ((int64_t)blockIdx.x * NT + threadIdx.x) * 4; e < nn; e += (int64_t)gridDim.x * NT * 4) {
+    const int64_t j = e / n, i = e % n;
+    if (i / BM > j / BM) continue;
+    float4 v = *(const float4*)(w.part + e);
+    for (int s = 1; s < w.splits; ++s) {
+      const float4 x = *(const float4*)(w.part + s * nn + e);
+      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    }
+    const float f[4] = {v.x, v.y, v.z, v.w};
+    put_sym(w.gram, n, i, j, f, i / BM == j / BM);
   }
 }
 
 __global__ __launch_bounds__(NT) void ortho_copy_kernel(mdmm_ortho_t p, Items q) {       // steps = 0: X itself
-  const mdmm_ortho_item_t& t = p.item[blockIdx.y];
+  const mdmm_ortho_item_t& t = p.item[q.which[blockIdx.y]];
   const Item& w = q.it[blockIdx.y];
-  const int64_t total = (int64_t)t.rows * t.cols;
+  const int64_t total = (int64_t)t.rows * t.cols, nm = (int64_t)w.n * w.m;
   for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)gridDim.x * NT) {
-    const int64_t r = i / t.cols, c = i % t.cols;
-    const float v = w.tall ? w.x0[c * w.m + r] : w.x0[r * w.m + c];
-    put(p, t, r, c, v);
+    const int64_t r = i / t.cols, c = i % t.cols, o = w.tall ? c * w.m + r : r * w.m + c;
+    const float v = join(w.xn[o], w.xn[nm + o]) * (1.0f / SC);
+    const int64_t at = r * t.dst_ld + c;
+    if (p.update) {
+      float* d = (float*)t.dst + at;
+      const float lr = p.lr_dev ? *p.lr_dev : p.lr;
+      *d = fmaf(-lr * t.gain, v, (1.0f - lr * p.decay) * *d);
+    } else if (p.dst_bf16) ((__bf16*)t.dst)[at] = (__bf16)v;
+    else ((float*)t.dst)[at] = v;
   }
 }
 
@@ -173,35 +377,75 @@ int check(const mdmm_ortho_t* a) {
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// fills the workspace pointers (base may be NULL: sizes only) and returns the bytes used
-int64_t lay_out(const mdmm_ortho_t* a, Items* q) {
+// 128 x 128 tiles where the shorter side holds four of them, else 64 x 64: a small matrix is a matter of latency, and the
+// larger tile halves what a product loads
+bool large(const mdmm_ortho_item_t& t) { return (t.rows < t.cols ? t.rows : t.cols) > 384; }
+
+// the workspace: fills both size classes' lists (base NULL: sizes only), returns the bytes used
+int64_t lay_out(const mdmm_ortho_t* a, Items (&q)[2]) {
   char* base = (char*)a->ws;
   int64_t off = 0;
-  q->n = a->n;
+  auto take = [&](int64_t bytes) { char* p = base + off; off += up(bytes, 256); return p; };
+  q[0].n = q[1].n = 0;
   for (int i = 0; i < a->n; ++i) {
     const mdmm_ortho_item_t& t = a->item[i];
-    Item& w = q->it[i];
+    const bool big = large(t);
+    Items& l = q[big];
+    l.which[l.n] = i;
+    Item& w = l.it[l.n++];
+    const int pad = big ? Large::BM : Small::BM, bk = big ? Large::BK : Small::BK;
     w.tall = t.rows > t.cols;
-    w.n = (int32_t)up(w.tall ? t.cols : t.rows, TILE);
-    w.m = (int32_t)up(w.tall ? t.rows : t.cols, TILE);
+    w.n = (int32_t)up(w.tall ? t.cols : t.rows, pad);
+    w.m = (int32_t)up(w.tall ? t.rows : t.cols, pad);
+    // slices of A: while the tiles leave CUs idle and a slice keeps 256 columns
+    const int64_t tiles = (int64_t)(w.n / pad) * (w.n / pad + 1) / 2;
+    int64_t splits = 128 / tiles < w.m / 256 ? 128 / tiles : w.m / 256;
+    if (splits < 1) splits = 1;
+    const int64_t steps = w.m / bk, per = (steps + splits - 1) / splits;
+    w.splits = (int32_t)((steps + per - 1) / per);
     const int64_t x = (int64_t)w.n * w.m, g = (int64_t)w.n * w.n;
-    w.x0 = (float*)(base + off); off += 4 * x;
-    w.x1 = (float*)(base + off); off += 4 * x;
-    w.gram = (float*)(base + off); off += 4 * g;
-    w.poly = (float*)(base + off); off += 4 * g;
-    w.sums = (float*)(base + off); off += 4 * SUMS;
+    w.xn = (half_t*)take(4 * x);
+    w.xt[0] = (half_t*)take(4 * x);
+    w.xt[1] = (half_t*)take(4 * x);
+    w.gram = (half_t*)take(4 * g);
+    w.poly = (half_t*)take(4 * g);
+    w.part = (float*)take(w.splits > 1 ? 4 * g * w.splits : 0);
+    w.sums = (double*)take(8 * SUMS);
   }
   return off;
 }
 
-int tiles(Items* q, bool wide) {
+template <class F> int tiles(Items& q, F count) {
   int64_t total = 0;
-  for (int i = 0; i < q->n; ++i) {
-    q->first[i] = (int32_t)total;
-    total += (int64_t)(q->it[i].n / TILE) * ((wide ? q->it[i].m : q->it[i].n) / TILE);
+  for (int i = 0; i < q.n; ++i) {
+    q.first[i] = (int32_t)total;
+    total += count(q.it[i]);
   }
-  q->first[q->n] = (int32_t)total;
+  q.first[q.n] = (int32_t)total;
   return (int)total;
+}
+
+template <class C> void launch(const mdmm_ortho_t* a, Items& q, hipStream_t s) {
+  if (!q.n) return;
+  hipLaunchKernelGGL(ortho_sums_kernel, dim3(SUMS, q.n), dim3(NT), 0, s, *a, q);
+  const int packs = tiles(q, [](const Item& w) { return (int64_t)(w.n / 64) * (w.m / 64); });
+  hipLaunchKernelGGL(ortho_pack_kernel, dim3(packs), dim3(NT), 0, s, *a, q);
+  if (a->steps == 0) hipLaunchKernelGGL(ortho_copy_kernel, dim3(256, q.n), dim3(NT), 0, s, *a, q);
+  Items qg = q, qp = q, qa = q;
+  auto tri = [](const Item& w) { return (int64_t)(w.n / C::BM) * (w.n / C::BM + 1) / 2; };
+  const int gram = tiles(qg, [&](const Item& w) { return tri(w) * w.splits; });
+  const int poly = tiles(qp, tri);
+  const int apply = tiles(qa, [](const Item& w) { return (int64_t)(w.n / C::BM) * (w.m / C::BN); });
+  int64_t fold = 0;
+  for (int i = 0; i < q.n; ++i)
+    if (q.it[i].splits > 1 && (int64_t)q.it[i].n * q.it[i].n > fold) fold = (int64_t)q.it[i].n * q.it[i].n;
+  for (int k = 0; k < a->steps; ++k) {
+    hipLaunchKernelGGL((ortho_product_kernel<GRAM, C>), dim3(gram), dim3(NT), 0, s, *a, qg, k & 1);
+    if (fold) hipLaunchKernelGGL((ortho_fold_kernel<C::BM>), dim3((unsigned)(fold / (4 * NT)), q.n), dim3(NT), 0, s, q);
+    hipLaunchKernelGGL((ortho_product_kernel<POLY, C>), dim3(poly), dim3(NT), 0, s, *a, qp, k & 1);
+    if (k + 1 < a->steps) hipLaunchKernelGGL((ortho_product_kernel<APPLY, C>), dim3(apply), dim3(NT), 0, s, *a, qa, k & 1);
+    else hipLaunchKernelGGL((ortho_product_kernel<LAST, C>), dim3(apply), dim3(NT), 0, s, *a, qa, k & 1);
+  }
 }
 
 }  // namespace
@@ -211,8 +455,8 @@ using namespace mdmm;
 
 extern "C" int64_t mdmm_ortho_ws(const mdmm_ortho_t* a) {
   if (check(a)) return -1;
-  Items q;
-  return lay_out(a, &q);
+  Items q[2];
+  return lay_out(a, q);
 }
 
 extern "C" int mdmm_ortho(const mdmm_ortho_t* a, void* stream) {
@@ -222,19 +466,9 @@ extern "C" int mdmm_ortho(const mdmm_ortho_t* a, void* stream) {
   if (!a->ws || ((uintptr_t)a->ws & 255)) return a->ws ? MDMM_E_ALIGN : MDMM_E_ARG;
   for (int i = 0; i < a->n; ++i)
     if (!a->item[i].src || !a->item[i].dst) return MDMM_E_ARG;
-  hipStream_t s = (hipStream_t)stream;
-  Items q;
-  lay_out(a, &q);
-  hipLaunchKernelGGL(ortho_sums_kernel, dim3(SUMS, a->n), dim3(NT), 0, s, *a, q);
-  hipLaunchKernelGGL(ortho_pack_kernel, dim3(256, a->n), dim3(NT), 0, s, *a, q);
-  if (a->steps == 0) hipLaunchKernelGGL(ortho_copy_kernel, dim3(256, a->n), dim3(NT), 0, s, *a, q);
-  const int square = tiles(&q, false);
-  Items qw = q;
-  const int wide = tiles(&qw, true);
-  for (int k = 0; k < a->steps; ++k) {
-    hipLaunchKernelGGL(ortho_product_kernel<GRAM>, dim3(square), dim3(NT), 0, s, *a, q, k & 1, 0);
-    hipLaunchKernelGGL(ortho_product_kernel<POLY>, dim3(square), dim3(NT), 0, s, *a, q, k & 1, 0);
-    hipLaunchKernelGGL(ortho_product_kernel<APPLY>, dim3(wide), dim3(NT), 0, s, *a, qw, k & 1, k + 1 == a->steps);
-  }
+  Items q[2];
+  lay_out(a, q);
+  launch<Small>(a, q[0], (hipStream_t)stream);
+  launch<Large>(a, q[1], (hipStream_t)stream);
   return (int)hipGetLastError();
 }
