@@ -2,16 +2,18 @@
 // X <- ca X + P X with P = cb A + cc A A, A = X X^T.  X lies down (n rows <= m columns).
 //
 // The iteration multiplies a small singular value by up to ca a step (ca^5 = 485 over five), and a rounding of X with it, so
+// The iteration multiplies a small singular value by up to ca a step (ca^5 = 485 over five), and a rounding of X with it, so
 // bf16 operands are out; fp32 ones would run on the fp32 matrix instruction, a sixteenth of the fp16 one's rate.  Every
-// matrix is kept as two fp16 planes instead, SC x = h + l / LO with h = fp16(SC x), l = fp16(LO (SC x - h)): 22 to 23 bits
-// (entries are at most 1.3, so SC x stays normal down to 1e-6 and below a sixteenth of fp16's largest), and a product is
-// h h' + (h l' + l h') / LO, the last two summed apart -- three fp16 matrix instructions for one fp32 product, the dropped
-// l l' of 2^-23 of a term, and one rounding of the fp32 sum for every 16 terms where the fp32 instruction has one for every
-// two: the result is nearer to 64 bits than fp32 products (3.6e-7 against 2.2e-6 at 256 x 256).  ca X is added in fp32.
+// matrix is kept as two fp16 planes instead, s x = h + l with h = fp16(s x), l = fp16(s x - h): 22 to 23 bits.  s is as large
+// as the entries allow (X and A stay below 2: 2^14; P below 16: 2^12), so that l is a normal number down to entries of 1e-5
+// and below those wrong by 2e-12.  A product is h h' + h l' + l h': three fp16 matrix instructions, the dropped l l' 2^-23 of
+// a term, and three roundings of the fp32 sum for every 16 terms where the fp32 instruction has one for every two: the result
+// is nearer to 64 bits than fp32 products (1.1e-6 against 2.9e-6 at 2048 x 2048).  ca X is added in fp32.
 //
-// X is stored both ways (n x m for A, m x n for P X) so that every product runs over two operands' rows: tiles of both come
-// straight into LDS (four buffers, the loads of three tiles ahead in flight), chunks of 16 bytes swapped within a row so that
-// the matrix instruction's reads meet all banks.  A and P are symmetric: tiles above the diagonal only, stored twice.  Sizes
+// X is stored both ways (n x m for A, m x n for P X) so that every product runs over two operands' rows.  A row keeps 32
+// columns of h, then the same 32 of l: one cache line for a step of 32 (with the planes apart, each step took half lines and
+// two 2048 x 2048 products 142 us).  Tiles come straight into LDS, a step or more ahead, chunks of 16 bytes swapped within a
+// row so that the matrix instruction's reads meet all banks; neighbouring tiles go to one XCD, whose L2 then holds their rows.  A and P are symmetric: tiles above the diagonal only, stored twice.  Sizes
 // are rounded up to whole tiles with zeros, which every product keeps.  All matrices of a call share each launch.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -20,25 +22,29 @@
 namespace mdmm {
 namespace {
 
-constexpr int NT = 256, SUMS = 64;
-constexpr float SC = 64.0f, LO = 2048.0f;
+constexpr int NT = 256, SUMS = 256;
+constexpr float SX = 16384.0f, SP = 4096.0f;      // scales of X and A, and of P
 typedef _Float16 half_t;
 typedef half_t half4 __attribute__((ext_vector_type(4)));
 typedef half_t half8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// BM x BN tile of a product by 2 x 2 waves, BK deep, ST buffers
-template <int BM_, int BN_, int BK_, int ST_> struct Cfg {
-  static constexpr int BM = BM_, BN = BN_, BK = BK_, ST = ST_;
-  static constexpr int TI = BM / 64, TJ = BN / 64;              // 32 x 32 pieces of a wave
-  static constexpr int CPR = BK / 8;                            // chunks of a row
-  static constexpr int HALVES = (BM + BN) * BK * 2;             // of a buffer: A h, A l, B h, B l
-  static constexpr int LOADS = HALVES / 8 / NT;                 // chunks a thread loads for a buffer
+// BM x BN tile of a product by WI x WJ waves, BK deep, ST buffers, OCC waves a SIMD wanted
+template <int BM_, int BN_, int BK_, int ST_, int WI_, int WJ_, int OCC_> struct Cfg {
+  static constexpr int BM = BM_, BN = BN_, BK = BK_, ST = ST_, WI = WI_, WJ = WJ_, OCC = OCC_;
+  static constexpr int T = 64 * WI * WJ;                        // threads
+  static constexpr int TI = BM / 32 / WI, TJ = BN / 32 / WJ;    // 32 x 32 pieces of a wave
+  static constexpr int CPR = BK / 4;                            // chunks of a row: 8 halves each, h and l
+  static constexpr int HALVES = (BM + BN) * BK * 2;             // of a buffer: A's rows, then B's
+  static constexpr int LOADS = HALVES / 8 / T;                  // chunks a thread loads for a buffer
+  static_assert(BM * CPR % T == 0 && BN * CPR % T == 0, "a load instruction of the workgroup stays in one operand");
 };
-typedef Cfg<64, 64, 64, 4> Small;
-typedef Cfg<128, 128, 32, 4> Large;
+typedef Cfg<64, 64, 64, 4, 2, 2, 1> Small;
+// (two workgroups a CU, two buffers each.  Measured on P X of two 2048 x 2048: 112 us; one workgroup with four buffers 127, one
+// of 256 x 128 and 8 waves with three 126, steps of 64 columns 126)
+typedef Cfg<128, 128, 32, 2, 2, 2, 2> Large;
 
-struct Item {               // one matrix's padded sizes and workspace; a plane pair is h, then l
+struct Item {               // one matrix's padded sizes and workspace
   half_t *xn, *xt[2], *gram, *poly;
   float* part;              // split sums of A
   double* sums;
@@ -60,11 +66,14 @@ __device__ __forceinline__ int find(const int32_t* first, int n, int tile) {
   return lo;
 }
 
-__device__ __forceinline__ void split(float x, half_t& h, half_t& l) {       // x: already times SC
+__device__ __forceinline__ void split(float x, half_t& h, half_t& l) {       // x: already scaled
   h = (half_t)x;
-  l = (half_t)((x - (float)h) * LO);
+  l = (half_t)(x - (float)h);
 }
-__device__ __forceinline__ float join(half_t h, half_t l) { return fmaf((float)l, 1.0f / LO, (float)h); }
+__device__ __forceinline__ float join(half_t h, half_t l) { return (float)h + (float)l; }
+
+// column c of a row of `cols` columns as pairs: h there, l 32 further
+__device__ __forceinline__ int64_t at(int64_t row, int64_t cols, int64_t c) { return row * cols * 2 + (c >> 5) * 64 + (c & 31); }
 
 __device__ __forceinline__ float src_at(const mdmm_ortho_t& p, const mdmm_ortho_item_t& t, int64_t r, int64_t c) {
   const int64_t i = r * t.src_ld + c;
@@ -75,17 +84,20 @@ __device__ __forceinline__ float src_at(const mdmm_ortho_t& p, const mdmm_ortho_
 __global__ __launch_bounds__(NT) void ortho_sums_kernel(mdmm_ortho_t p, Items q) {
   const int k = blockIdx.y;
   const mdmm_ortho_item_t& t = p.item[q.which[k]];
-  const int64_t total = (int64_t)t.rows * t.cols;
   double s = 0.0;
-  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)SUMS * NT) {
-    float v = src_at(p, t, i / t.cols, i % t.cols);
-    if (t.mom) {
-      const float mv = fmaf(p.momentum, t.mom[i], v);
-      t.mom[i] = mv;
-      v = p.nesterov ? fmaf(p.momentum, mv, v) : mv;
+  // a workgroup's rows, its threads over the columns (rows shorter than a workgroup: several of them at once)
+  const int wide = t.cols < NT ? (t.cols < 16 ? 16 : t.cols < 64 ? 64 : NT) : NT, high = NT / wide;
+  for (int64_t r = (int64_t)blockIdx.x * high + threadIdx.x / wide; r < t.rows; r += (int64_t)SUMS * high)
+    for (int64_t c = threadIdx.x % wide; c < t.cols; c += wide) {
+      float v = src_at(p, t, r, c);
+      if (t.mom) {
+        float* mom = t.mom + r * t.cols + c;
+        const float mv = fmaf(p.momentum, *mom, v);
+        *mom = mv;
+        v = p.nesterov ? fmaf(p.momentum, mv, v) : mv;
+      }
+      s += (double)v * v;
     }
-    s += (double)v * v;
-  }
   __shared__ double part[NT / 64];
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
@@ -99,12 +111,15 @@ __global__ __launch_bounds__(NT) void ortho_pack_kernel(mdmm_ortho_t p, Items q)
   const int k = find(q.first, q.n, blockIdx.x);
   const mdmm_ortho_item_t& t = p.item[q.which[k]];
   const Item& w = q.it[k];
-  double s = 0.0;
-  for (int i = 0; i < SUMS; ++i) s += w.sums[i];
-  const float inv = (float)((double)SC / (sqrt(s) + (double)p.eps));
-  const int at = blockIdx.x - q.first[k], across = (w.tall ? w.n : w.m) / 64;       // tiles of the source's rows
-  const int64_t r0 = at / across * 64, c0 = at % across * 64;
-  const int64_t nm = (int64_t)w.n * w.m;
+  __shared__ double part[NT / 64];
+  double s = w.sums[threadIdx.x];
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = (part[0] + part[1]) + (part[2] + part[3]);
+  const float inv = (float)((double)SX / (sqrt(s) + (double)p.eps));
+  const int me = blockIdx.x - q.first[k], across = (w.tall ? w.n : w.m) / 64;       // tiles of the source's rows
+  const int64_t r0 = me / across * 64, c0 = me % across * 64;
   // the source's orientation: lying or standing plane pair
   half_t* same = w.tall ? w.xt[0] : w.xn;
   half_t* other = w.tall ? w.xn : w.xt[0];
@@ -123,16 +138,17 @@ __global__ __launch_bounds__(NT) void ortho_pack_kernel(mdmm_ortho_t p, Items q)
     tile[i / 64][i % 64] = v;
     half_t h, l;
     split(v, h, l);
-    same[r * ld_same + c] = h;
-    same[nm + r * ld_same + c] = l;
+    const int64_t o = at(r, ld_same, c);
+    same[o] = h;
+    same[o + 32] = l;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 4096; i += NT) {
     half_t h, l;
     split(tile[i % 64][i / 64], h, l);
-    const int64_t o = (c0 + i / 64) * ld_other + r0 + i % 64;
+    const int64_t o = at(c0 + i / 64, ld_other, r0 + i % 64);
     other[o] = h;
-    other[nm + o] = l;
+    other[o + 32] = l;
   }
 }
 
@@ -149,55 +165,70 @@ __device__ __forceinline__ void put_sym(half_t* dst, int64_t n, int64_t i, int64
     h4[e] = h;
     l4[e] = l;
     if (!diagonal || i + e <= j) {
-      dst[(i + e) * n + j] = h;
-      dst[n * n + (i + e) * n + j] = l;
+      half_t* d = dst + at(i + e, n, j);
+      d[0] = h;
+      d[32] = l;
       if (diagonal) {
-        dst[j * n + i + e] = h;
-        dst[n * n + j * n + i + e] = l;
+        d = dst + at(j, n, i + e);
+        d[0] = h;
+        d[32] = l;
       }
     }
   }
   if (!diagonal) {
-    *(half4*)(dst + j * n + i) = h4;
-    *(half4*)(dst + n * n + j * n + i) = l4;
+    half_t* d = dst + at(j, n, i);
+    *(half4*)d = h4;
+    *(half4*)(d + 32) = l4;
   }
 }
 
-// tile t of the triangle at and above the diagonal, row by row
-__device__ __forceinline__ void triangle(int t, int tiles, int& ti, int& tj) {
-  int r = (int)(((2 * tiles + 1) - sqrtf((float)(2 * tiles + 1) * (2 * tiles + 1) - 8.0f * t)) * 0.5f);
-  r = r < 0 ? 0 : r >= tiles ? tiles - 1 : r;
-  while (r > 0 && r * tiles - r * (r - 1) / 2 > t) --r;
-  while ((r + 1) * tiles - (r + 1) * r / 2 <= t) ++r;
+// tile t of those that reach the diagonal or lie above it, row by row; a row of tiles starts R tiles further right than the
+// one above (R = BM / BN)
+template <int R> __device__ __forceinline__ void triangle(int t, int across, int& ti, int& tj) {
+  // rows before r hold f(r) = r across - R r (r - 1) / 2 tiles
+  const float b = across + 0.5f * R;
+  int r = (int)((b - sqrtf(fmaxf(b * b - 2.0f * R * t, 0.0f))) / R);
+  const int rows = across / R;
+  r = r < 0 ? 0 : r >= rows ? rows - 1 : r;
+  while (r > 0 && r * across - R * r * (r - 1) / 2 > t) --r;
+  while ((r + 1) * across - R * (r + 1) * r / 2 <= t) ++r;
   ti = r;
-  tj = r + t - (r * tiles - r * (r - 1) / 2);
+  tj = R * r + t - (r * across - R * r * (r - 1) / 2);
 }
 
 // all but the last N loads have landed, and this wave's reads of LDS are done
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
 
+template <class C> __host__ __device__ int tri(int n) {          // tiles at and above the diagonal
+  constexpr int R = C::BM / C::BN;
+  const int rows = n / C::BM;
+  return rows * (n / C::BN) - R * rows * (rows - 1) / 2;
+}
+
 template <int MODE, class C>
-__global__ __launch_bounds__(NT) void ortho_product_kernel(mdmm_ortho_t p, Items q, int flip) {
+__global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(mdmm_ortho_t p, Items q, int flip) {
   __shared__ __align__(16) half_t lds[C::ST * C::HALVES];
   constexpr bool PX = MODE == APPLY || MODE == LAST;
-  const int k = find(q.first, q.n, blockIdx.x);
+  // consecutive workgroups go round the 8 XCDs: each XCD takes a run of consecutive tiles instead
+  const int total = gridDim.x, xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
+  const int me = xcd * each + (xcd < more ? xcd : more) + (blockIdx.x >> 3);
+  const int k = find(q.first, q.n, me);
   const Item w = q.it[k];
   const int n = w.n, J = PX ? w.m : n;
-  int tile = blockIdx.x - q.first[k], ti, tj, slice = 0;
+  int tile = me - q.first[k], ti, tj, slice = 0;
   if (PX) {
     ti = tile / (J / C::BN);
     tj = tile % (J / C::BN);
   } else {
-    const int tiles = n / C::BM, all = tiles * (tiles + 1) / 2;
+    const int all = tri<C>(n);
     if (MODE == GRAM) { slice = tile / all; tile %= all; }
-    triangle(tile, tiles, ti, tj);
+    triangle<C::BM / C::BN>(tile, n / C::BN, ti, tj);
   }
   const int i0 = ti * C::BM, j0 = tj * C::BN;
-  const half_t* xt = w.xt[flip];
+  const half_t* xt = flip ? w.xt[1] : w.xt[0];
   const half_t* a = MODE == GRAM ? w.xn : MODE == POLY ? w.gram : w.poly;
   const half_t* b = MODE == GRAM ? w.xn : MODE == POLY ? w.gram : xt;
   const int64_t K = MODE == GRAM ? w.m : n;               // columns of both
-  const int64_t la = (int64_t)n * K, lb = PX ? (int64_t)w.m * K : la;
   const int steps_all = (int)(K / C::BK);
   const int per = MODE == GRAM ? (steps_all + w.splits - 1) / w.splits : steps_all;
   const int s0 = slice * per, nk = s0 + per < steps_all ? per : steps_all - s0;
@@ -207,25 +238,22 @@ __global__ __launch_bounds__(NT) void ortho_product_kernel(mdmm_ortho_t p, Items
   const half_t* from[C::LOADS];
 #pragma unroll
   for (int c = 0; c < C::LOADS; ++c) {
-    constexpr int AC = C::BM * C::CPR, BC = C::BN * C::CPR;
-    const int first = c * NT;                              // (a multiple of NT: the whole workgroup is in one plane)
-    const bool in_b = first >= 2 * AC;
-    const int plane = in_b ? (first - 2 * AC) / BC : first / AC;
-    const int at = (in_b ? (first - 2 * AC) % BC : first % AC) + tid;
-    const int row = at / C::CPR, ch = (at % C::CPR) ^ (row / (16 / C::CPR) % C::CPR);
-    from[c] = (in_b ? b + plane * lb + (j0 + row) * K : a + plane * la + (i0 + row) * K) + (int64_t)s0 * C::BK + ch * 8;
+    const bool in_b = c * C::T >= C::BM * C::CPR;
+    const int ck = c * C::T - (in_b ? C::BM * C::CPR : 0) + tid;
+    const int row = ck / C::CPR, ch = (ck % C::CPR) ^ (row / (16 / C::CPR) % C::CPR);
+    from[c] = (in_b ? b + (j0 + row) * K * 2 : a + (i0 + row) * K * 2) + (int64_t)s0 * C::BK * 2 + ch * 8;
   }
   auto load = [&](int buf) {
 #pragma unroll
     for (int c = 0; c < C::LOADS; ++c) {
-      half_t* to = lds + buf * C::HALVES + (c * NT + wave * 64) * 8;
+      half_t* to = lds + buf * C::HALVES + (c * C::T + wave * 64) * 8;
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from[c],
                                        (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-      from[c] += C::BK;
+      from[c] += 2 * C::BK;
     }
   };
-  f32x16 main[C::TI][C::TJ] = {}, cross[C::TI][C::TJ] = {};
-  const int wi = (wave >> 1) * 32 * C::TI, wj = (wave & 1) * 32 * C::TJ;
+  f32x16 acc[C::TI][C::TJ] = {};
+  const int wi = wave / C::WJ * 32 * C::TI, wj = wave % C::WJ * 32 * C::TJ;
 #pragma unroll
   for (int s = 0; s < C::ST - 1; ++s)
     if (s < nk) load(s);
@@ -241,32 +269,38 @@ __global__ __launch_bounds__(NT) void ortho_product_kernel(mdmm_ortho_t p, Items
 #pragma unroll
     for (int kk = 0; kk < C::BK / 16; ++kk) {
       half8 ah[C::TI], al[C::TI], bh[C::TJ], bl[C::TJ];
-      const int c = kk * 2 + (lane >> 5);
+      // chunk of h; l's is 4 further (columns kk 16 + (lane / 32) 8 on, of each 32 columns' pair of half lines)
+      const int c = kk / 2 * 8 + kk % 2 * 2 + (lane >> 5);
 #pragma unroll
       for (int t = 0; t < C::TI; ++t) {
-        const int row = wi + t * 32 + (lane & 31), o = row * C::BK + ((c ^ (row / (16 / C::CPR) % C::CPR)) * 8);
-        ah[t] = *(const half8*)(A + o);
-        al[t] = *(const half8*)(A + C::BM * C::BK + o);
+        const int row = wi + t * 32 + (lane & 31), z = row / (16 / C::CPR) % C::CPR;
+        ah[t] = *(const half8*)(A + row * C::BK * 2 + (c ^ z) * 8);
+        al[t] = *(const half8*)(A + row * C::BK * 2 + ((c + 4) ^ z) * 8);
       }
 #pragma unroll
       for (int t = 0; t < C::TJ; ++t) {
-        const int row = wj + t * 32 + (lane & 31), o = row * C::BK + ((c ^ (row / (16 / C::CPR) % C::CPR)) * 8);
-        bh[t] = *(const half8*)(B + o);
-        bl[t] = *(const half8*)(B + C::BN * C::BK + o);
+        const int row = wj + t * 32 + (lane & 31), z = row / (16 / C::CPR) % C::CPR;
+        bh[t] = *(const half8*)(B + row * C::BK * 2 + (c ^ z) * 8);
+        bl[t] = *(const half8*)(B + row * C::BK * 2 + ((c + 4) ^ z) * 8);
       }
+      // (the three products of a piece apart from each other: none waits for the one before)
 #pragma unroll
       for (int x = 0; x < C::TI; ++x)
 #pragma unroll
-        for (int y = 0; y < C::TJ; ++y) {
-          main[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bh[y], main[x][y], 0, 0, 0);
-          cross[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bl[y], cross[x][y], 0, 0, 0);
-          cross[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[x], bh[y], cross[x][y], 0, 0, 0);
-        }
+        for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bl[y], acc[x][y], 0, 0, 0);
+#pragma unroll
+      for (int x = 0; x < C::TI; ++x)
+#pragma unroll
+        for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[x], bh[y], acc[x][y], 0, 0, 0);
+#pragma unroll
+      for (int x = 0; x < C::TI; ++x)
+#pragma unroll
+        for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bh[y], acc[x][y], 0, 0, 0);
     }
   }
-  // v: the product times SC (operands carry SC each)
+  // v: the result in its planes' scale
   const mdmm_ortho_item_t t = p.item[q.which[k]];
-  const int64_t nn = (int64_t)n * n, nm = (int64_t)n * w.m, m = w.m;
+  const int64_t nn = (int64_t)n * n, m = w.m;
   const float lr = MODE == LAST && p.update ? (p.lr_dev ? *p.lr_dev : p.lr) : 0.0f;
 #pragma unroll
   for (int x = 0; x < C::TI; ++x)
@@ -278,37 +312,41 @@ __global__ __launch_bounds__(NT) void ortho_product_kernel(mdmm_ortho_t p, Items
         const int64_t i = i0 + wi + x * 32 + 8 * g + 4 * (lane >> 5), j = j0 + wj + y * 32 + (lane & 31);
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = fmaf(cross[x][y][4 * g + e], 1.0f / LO, main[x][y][4 * g + e]) * (1.0f / SC);
+        for (int e = 0; e < 4; ++e) v[e] = acc[x][y][4 * g + e];
         if (MODE == GRAM) {
-          if (w.splits == 1) put_sym(w.gram, n, i, j, v, ti == tj);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= 1.0f / SX;
+          if (w.splits == 1) put_sym(w.gram, n, i, j, v, j0 < i0 + C::BM);
           else *(float4*)(w.part + slice * nn + j * n + i) = make_float4(v[0], v[1], v[2], v[3]);
         }
         if (MODE == POLY) {
-          const half4 h = *(const half4*)(w.gram + j * n + i), l = *(const half4*)(w.gram + nn + j * n + i);
+          const half_t* d = w.gram + at(j, n, i);
+          const half4 h = *(const half4*)d, l = *(const half4*)(d + 32);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(p.cc, v[e], p.cb * join(h[e], l[e]));
-          put_sym(w.poly, n, i, j, v, ti == tj);
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(p.cc * (SP / SX / SX), v[e], p.cb * (SP / SX) * join(h[e], l[e]));
+          put_sym(w.poly, n, i, j, v, j0 < i0 + C::BM);
         }
         if (PX) {
-          const half4 h = *(const half4*)(xt + j * n + i), l = *(const half4*)(xt + nm + j * n + i);
+          const half_t* d = xt + at(j, n, i);
+          const half4 h = *(const half4*)d, l = *(const half4*)(d + 32);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(p.ca, join(h[e], l[e]), v[e]);
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(p.ca, join(h[e], l[e]), v[e] * (1.0f / SP));
         }
         if (MODE == APPLY) {
           half4 h4, l4;
-          half_t* lie = w.xn + i * m + j;
+          half_t* lie = w.xn + at(i, m, j);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             half_t hh, ll;
             split(v[e], hh, ll);
             h4[e] = hh;
             l4[e] = ll;
-            lie[e * m] = hh;
-            lie[nm + e * m] = ll;
+            lie[2 * e * m] = hh;
+            lie[2 * e * m + 32] = ll;
           }
-          half_t* to = w.xt[flip ^ 1] + j * n + i;
+          half_t* to = (flip ? w.xt[0] : w.xt[1]) + at(j, n, i);
           *(half4*)to = h4;
-          *(half4*)(to + nm) = l4;
+          *(half4*)(to + 32) = l4;
         }
         if (MODE == LAST) {
           const int64_t r = w.tall ? j : i, c = w.tall ? i : j, step = w.tall ? 1 : t.dst_ld;
@@ -316,7 +354,7 @@ __global__ __launch_bounds__(NT) void ortho_product_kernel(mdmm_ortho_t p, Items
           const int64_t o = r * t.dst_ld + c;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float u = v[e] * (1.0f / SC);
+            const float u = v[e] * (1.0f / SX);
             if (e >= end) continue;
             if (p.update) {
               float* d = (float*)t.dst + o + e * step;
@@ -328,38 +366,39 @@ __global__ __launch_bounds__(NT) void ortho_product_kernel(mdmm_ortho_t p, Items
       }
 }
 
-// the slices of A added up (each keeps the upper triangle of tiles, column by column)
-template <int BM> __global__ __launch_bounds__(NT) void ortho_fold_kernel(Items q) {
+// the slices of A added up (each keeps the tiles at and above the diagonal, column by column)
+template <int BM, int BN> __global__ __launch_bounds__(NT) void ortho_fold_kernel(Items q) {
   const Item w = q.it[blockIdx.y];
   if (w.splits == 1) return;
   const int64_t n = w.n, nn = n * n;
   for (int64_t e = ((int64_t)blockIdx.x * NT + threadIdx.x) * 4; e < nn; e += (int64_t)gridDim.x * NT * 4) {
     const int64_t j = e / n, i = e % n;
-    if (i / BM > j / BM) continue;
+    const int64_t i0 = i / BM * BM, j0 = j / BN * BN;
+    if (j0 < i0) continue;
     float4 v = *(const float4*)(w.part + e);
     for (int s = 1; s < w.splits; ++s) {
       const float4 x = *(const float4*)(w.part + s * nn + e);
       v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
     }
     const float f[4] = {v.x, v.y, v.z, v.w};
-    put_sym(w.gram, n, i, j, f, i / BM == j / BM);
+    put_sym(w.gram, n, i, j, f, j0 < i0 + BM);
   }
 }
 
 __global__ __launch_bounds__(NT) void ortho_copy_kernel(mdmm_ortho_t p, Items q) {       // steps = 0: X itself
   const mdmm_ortho_item_t& t = p.item[q.which[blockIdx.y]];
   const Item& w = q.it[blockIdx.y];
-  const int64_t total = (int64_t)t.rows * t.cols, nm = (int64_t)w.n * w.m;
+  const int64_t total = (int64_t)t.rows * t.cols;
   for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)gridDim.x * NT) {
-    const int64_t r = i / t.cols, c = i % t.cols, o = w.tall ? c * w.m + r : r * w.m + c;
-    const float v = join(w.xn[o], w.xn[nm + o]) * (1.0f / SC);
-    const int64_t at = r * t.dst_ld + c;
+    const int64_t r = i / t.cols, c = i % t.cols, o = w.tall ? at(c, w.m, r) : at(r, w.m, c);
+    const float v = join(w.xn[o], w.xn[o + 32]) * (1.0f / SX);
+    const int64_t to = r * t.dst_ld + c;
     if (p.update) {
-      float* d = (float*)t.dst + at;
+      float* d = (float*)t.dst + to;
       const float lr = p.lr_dev ? *p.lr_dev : p.lr;
       *d = fmaf(-lr * t.gain, v, (1.0f - lr * p.decay) * *d);
-    } else if (p.dst_bf16) ((__bf16*)t.dst)[at] = (__bf16)v;
-    else ((float*)t.dst)[at] = v;
+    } else if (p.dst_bf16) ((__bf16*)t.dst)[to] = (__bf16)v;
+    else ((float*)t.dst)[to] = v;
   }
 }
 
@@ -397,9 +436,10 @@ int64_t lay_out(const mdmm_ortho_t* a, Items (&q)[2]) {
     w.tall = t.rows > t.cols;
     w.n = (int32_t)up(w.tall ? t.cols : t.rows, pad);
     w.m = (int32_t)up(w.tall ? t.rows : t.cols, pad);
-    // slices of A: while the tiles leave CUs idle and a slice keeps 256 columns
-    const int64_t tiles = (int64_t)(w.n / pad) * (w.n / pad + 1) / 2;
-    int64_t splits = 128 / tiles < w.m / 256 ? 128 / tiles : w.m / 256;
+    // slices of A: from 2048 columns on, while the tiles leave CUs idle, of 512 columns at least (joining them is a launch
+    // more, 4 us with its gap, which is what 768 columns take in one piece)
+    const int64_t tiles = big ? tri<Large>(w.n) : tri<Small>(w.n);
+    int64_t splits = w.m >= 2048 ? (128 / tiles < w.m / 512 ? 128 / tiles : w.m / 512) : 1;
     if (splits < 1) splits = 1;
     const int64_t steps = w.m / bk, per = (steps + splits - 1) / splits;
     w.splits = (int32_t)((steps + per - 1) / per);
@@ -432,19 +472,18 @@ template <class C> void launch(const mdmm_ortho_t* a, Items& q, hipStream_t s) {
   hipLaunchKernelGGL(ortho_pack_kernel, dim3(packs), dim3(NT), 0, s, *a, q);
   if (a->steps == 0) hipLaunchKernelGGL(ortho_copy_kernel, dim3(256, q.n), dim3(NT), 0, s, *a, q);
   Items qg = q, qp = q, qa = q;
-  auto tri = [](const Item& w) { return (int64_t)(w.n / C::BM) * (w.n / C::BM + 1) / 2; };
-  const int gram = tiles(qg, [&](const Item& w) { return tri(w) * w.splits; });
-  const int poly = tiles(qp, tri);
+  const int gram = tiles(qg, [](const Item& w) { return (int64_t)tri<C>(w.n) * w.splits; });
+  const int poly = tiles(qp, [](const Item& w) { return (int64_t)tri<C>(w.n); });
   const int apply = tiles(qa, [](const Item& w) { return (int64_t)(w.n / C::BM) * (w.m / C::BN); });
   int64_t fold = 0;
   for (int i = 0; i < q.n; ++i)
     if (q.it[i].splits > 1 && (int64_t)q.it[i].n * q.it[i].n > fold) fold = (int64_t)q.it[i].n * q.it[i].n;
   for (int k = 0; k < a->steps; ++k) {
-    hipLaunchKernelGGL((ortho_product_kernel<GRAM, C>), dim3(gram), dim3(NT), 0, s, *a, qg, k & 1);
-    if (fold) hipLaunchKernelGGL((ortho_fold_kernel<C::BM>), dim3((unsigned)(fold / (4 * NT)), q.n), dim3(NT), 0, s, q);
-    hipLaunchKernelGGL((ortho_product_kernel<POLY, C>), dim3(poly), dim3(NT), 0, s, *a, qp, k & 1);
-    if (k + 1 < a->steps) hipLaunchKernelGGL((ortho_product_kernel<APPLY, C>), dim3(apply), dim3(NT), 0, s, *a, qa, k & 1);
-    else hipLaunchKernelGGL((ortho_product_kernel<LAST, C>), dim3(apply), dim3(NT), 0, s, *a, qa, k & 1);
+    hipLaunchKernelGGL((ortho_product_kernel<GRAM, C>), dim3(gram), dim3(C::T), 0, s, *a, qg, k & 1);
+    if (fold) hipLaunchKernelGGL((ortho_fold_kernel<C::BM, C::BN>), dim3((unsigned)(fold / (4 * NT)), q.n), dim3(NT), 0, s, q);
+    hipLaunchKernelGGL((ortho_product_kernel<POLY, C>), dim3(poly), dim3(C::T), 0, s, *a, qp, k & 1);
+    if (k + 1 < a->steps) hipLaunchKernelGGL((ortho_product_kernel<APPLY, C>), dim3(apply), dim3(C::T), 0, s, *a, qa, k & 1);
+    else hipLaunchKernelGGL((ortho_product_kernel<LAST, C>), dim3(apply), dim3(C::T), 0, s, *a, qa, k & 1);
   }
 }
 

@@ -203,6 +203,172 @@ class FlatAdam(torch.optim.Optimizer):
                 self.param_groups[0][k] = val
 
 
+class FlatMuon(torch.optim.Optimizer):
+    """Weight matrices by orthogonalised momentum (the Muon optimizer), everything else by Adam, for the parameters of a
+    GradBucket.  A matrix W (rows, cols; a convolution's kernels as leading dimension x the rest) with gradient G:
+
+        M <- momentum M + G;   U = G + momentum M (nesterov) or M
+        O = ops.orthogonalise(U, ns_steps)
+        W <- (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) O
+
+    all matrices sharing the launches (csrc/ortho.hip: momentum in the first, the update in the last).  The other parameters
+    take mdmm_adam_flat's update with adam_lr, betas, eps, adam_weight_decay, one launch for all of them.
+
+    matrices: the parameters to treat as matrices; by default every one of two or more dimensions whose rows and columns both
+    exceed one.  (Embeddings and output layers are better left to Adam: pass the rest.)  lr and adam_lr are the 'lr' of the
+    two parameter groups (0: matrices, 1: the others); as a one-element CUDA tensor either may change between the replays of
+    a captured step, a float is a constant of the capture.  `step()` needs every gradient to be the bucket's view, as
+    FlatAdam's.  state_dict(): {'momentum_buffer'} per matrix, {'step', 'exp_avg', 'exp_avg_sq'} per other parameter."""
+
+    def __init__(self, bucket, lr=0.02, momentum=0.95, nesterov=True, ns_steps=5, weight_decay=0.0, matrices=None,
+                 adam_lr=1e-3, betas=(0.9, 0.999), eps=1e-8, adam_weight_decay=0.0):
+        if not bucket.flat.is_cuda:
+            raise RuntimeError('FlatMuon runs on the GPU (mdmm_ortho, mdmm_adam_flat)')
+        if not 0.0 <= momentum < 1.0 or int(ns_steps) != ns_steps or ns_steps < 0:
+            raise ValueError('FlatMuon: momentum %r in [0, 1), a number of steps, got %r' % (momentum, ns_steps))
+        for p in bucket.params:
+            if p.dtype != torch.float32 or not p.is_contiguous():
+                raise ValueError('FlatMuon: contiguous fp32 parameters')
+        shape = lambda p: (p.shape[0], p.numel() // p.shape[0]) if p.dim() > 1 and p.numel() else (0, 0)     # noqa: E731
+        if matrices is None:
+            chosen = [p for p in bucket.params if min(shape(p)) > 1]
+        else:
+            ids = {id(p) for p in matrices}
+            chosen = [p for p in bucket.params if id(p) in ids]
+            if len(chosen) != len(ids):
+                raise ValueError('FlatMuon: %d of the matrices are not in the bucket' % (len(ids) - len(chosen)))
+            for p in chosen:
+                if p.dim() < 2 or not p.numel():
+                    raise ValueError('FlatMuon: a matrix of shape %s' % (tuple(p.shape),))
+        own = {id(p) for p in chosen}
+        rest = [p for p in bucket.params if id(p) not in own]
+        groups = [dict(params=chosen, lr=lr, momentum=momentum, nesterov=bool(nesterov), ns_steps=int(ns_steps),
+                       weight_decay=weight_decay),
+                  dict(params=rest, lr=adam_lr, betas=betas, eps=eps, weight_decay=adam_weight_decay)]
+        super().__init__([g for g in groups if g['params']], {})
+        self._muon = self.param_groups[0] if chosen else None
+        self._adam = self.param_groups[-1] if rest else None
+        self.bucket, self._own = bucket, own
+        dev, n = bucket.flat.device, bucket.flat.numel()
+        self.exp_avg = torch.zeros(n, dtype=torch.float32, device=dev)          # (the matrices' part: their momentum)
+        self.exp_avg_sq = torch.zeros(n if rest else 0, dtype=torch.float32, device=dev)
+        self.step_dev = torch.zeros(1, dtype=torch.float32, device=dev)
+        self._lr_dev = torch.zeros(2, dtype=torch.float32, device=dev)
+        self._captured = [None, None]
+        offs = [0]
+        self._slices = {}
+        for p in bucket.params:
+            offs.append(offs[-1] + p.numel())
+            lo, hi = offs[-2:]
+            self._slices[id(p)] = (lo, hi)
+            if id(p) in own:
+                self.state[p] = {'momentum_buffer': self.exp_avg[lo:hi].view_as(p)}
+            else:
+                self.state[p] = {'step': self.step_dev.reshape(()), 'exp_avg': self.exp_avg[lo:hi].view_as(p),
+                                 'exp_avg_sq': self.exp_avg_sq[lo:hi].view_as(p)}
+        self._offs = torch.tensor(offs, dtype=torch.int64, device=dev)
+        self._ptrs, self._ptr_key = None, None
+
+    def add_param_group(self, param_group):
+        if hasattr(self, 'bucket'):
+            raise ValueError('FlatMuon: the parameters are the bucket\'s')
+        super().add_param_group(param_group)
+
+    def _lr(self, which, group):
+        """(device scalar or None, float) of a group's learning rate."""
+        lr = group['lr']
+        if isinstance(lr, torch.Tensor):
+            if not lr.is_cuda or lr.numel() != 1:
+                raise RuntimeError('FlatMuon: a tensor learning rate must be one element on the GPU (the kernel reads it there)')
+            self._lr_dev[which:which + 1].copy_(lr.detach().reshape(1))
+            return self._lr_dev[which:which + 1], 0.0
+        if torch.cuda.is_current_stream_capturing():
+            self._captured[which] = float(lr)
+        return None, float(lr)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        from . import ops, ortho
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        b = self.bucket
+        for p in b.params:                 # (host check, no launch: the kernels read the flat buffer)
+            if p.grad is None or p.grad.data_ptr() != b.flat.data_ptr() + 4 * self._slices[id(p)][0]:
+                raise RuntimeError('FlatMuon.step: gradients must be the bucket\'s views (GradBucket.check_views())')
+        with torch.cuda.device(b.flat.device):
+            if self._muon is not None:
+                g = self._muon
+                items = []
+                for p in g['params']:
+                    w = ortho.as_matrix(p.detach())
+                    items.append((p.grad.view(w.shape), self.state[p]['momentum_buffer'], w,
+                                  max(1.0, w.shape[0] / w.shape[1]) ** 0.5))
+                lr_dev, lr = self._lr(0, g)
+                ortho.launch(items, g['ns_steps'], 1e-7, ortho.COEFFICIENTS, False, False, momentum=float(g['momentum']),
+                             nesterov=g['nesterov'], update=True, lr=lr, lr_dev=lr_dev, decay=float(g['weight_decay']),
+                             device=b.flat.device)
+            if self._adam is not None:
+                g = self._adam
+                key = tuple(0 if id(p) in self._own else p.data_ptr() for p in b.params)
+                if key != self._ptr_key:
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError('FlatMuon: run one eager step before capturing (a parameter\'s storage changed)')
+                    self._ptrs = torch.tensor(key, dtype=torch.int64, device=b.flat.device)
+                    self._ptr_key = key
+                self.step_dev.add_(1.0)
+                lr_dev, lr = self._lr(1, g)
+                ops._call('mdmm_adam_flat', self._ptrs.data_ptr(), self._offs.data_ptr(), len(b.params), b.flat.data_ptr(),
+                          self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), b.flat.numel(), self.step_dev.data_ptr(),
+                          ops._ptr(lr_dev), lr, float(g['betas'][0]), float(g['betas'][1]), float(g['eps']),
+                          float(g['weight_decay']))
+        return loss
+
+    def check_replay(self):
+        """Called by GraphedElboStep before every replay: a float learning rate was frozen into the captured launches."""
+        for which, group in ((0, self._muon), (1, self._adam)):
+            was = self._captured[which]
+            if group is not None and was is not None and not isinstance(group['lr'], torch.Tensor) and float(group['lr']) != was:
+                raise RuntimeError('FlatMuon: lr changed from %g to %g after the step was captured -- a float lr is a constant '
+                                   'of the graph; pass a one-element CUDA tensor as lr to change it between replays'
+                                   % (was, float(group['lr'])))
+
+    def state_dict(self):
+        sd = super().state_dict()
+        # (copies: the packed entries are the live views)
+        sd['state'] = {i: {k: v.detach().clone() for k, v in st.items()} for i, st in sd['state'].items()}
+        return sd
+
+    def load_state_dict(self, state_dict):
+        """State of an optimizer over parameters of the same shapes and roles, copied INTO the flat buffers."""
+        have, given = self.param_groups, state_dict['param_groups']
+        if [len(g['params']) for g in given] != [len(g['params']) for g in have]:
+            raise ValueError('optimizer state for groups of %s parameters, FlatMuon has %s'
+                             % ([len(g['params']) for g in given], [len(g['params']) for g in have]))
+        steps = set()
+        with torch.no_grad():
+            for mine, theirs in zip(have, given):
+                for p, i in zip(mine['params'], theirs['params']):
+                    st = state_dict['state'].get(i)
+                    if st is None:
+                        continue
+                    if set(st) != set(self.state[p]):
+                        raise ValueError('FlatMuon: state %s for a parameter that keeps %s' % (sorted(st), sorted(self.state[p])))
+                    for k, v in st.items():
+                        if k == 'step':
+                            steps.add(float(v))
+                        else:
+                            self.state[p][k].copy_(v)
+                for k, v in theirs.items():
+                    if k != 'params' and k in mine:
+                        mine[k] = v
+            if len(steps) > 1:
+                raise ValueError('FlatMuon keeps one step count; the loaded state holds %s' % sorted(steps))
+            if steps:
+                self.step_dev.fill_(steps.pop())
+
+
 def shard_batch(inputs, mask, lengths, rank, world):
     """Contiguous split of the batch dimension (dim 1 of the time-first tensors)."""
     b_dim = len(lengths)

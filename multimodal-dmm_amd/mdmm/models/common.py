@@ -97,6 +97,65 @@ class GaussianGTF(nn.Module):
         return (1 - g) * self.z_lin(z) + g * nonlin, self.z_to_std(nonlin) + self.min_std
 
 
+class GatedLinearRNN(nn.Module):
+    """An inference RNN without a recurrent product (MultiDKS, rnn_cell='linear'): residual layers whose state follows the
+    gated linear recurrence, every product taken over all time steps at once.
+
+        x = inp(features);  n = rms_norm(x, norms[0])
+        per layer:  [f | c | g] = proj(n);  h_t = sigmoid(f_t) h_{t-1} + (1 - sigmoid(f_t)) c_t
+                    x = x + scale * silu(g) * rms_norm(h, post);  n = rms_norm(x, norms[next])
+
+    Runs on ops.rms_norm and ops.gated_block (GPU only).  forward(x (T,B,in_dim), h0 (num_layers, h_dim), mask (T,B) or None,
+    reverse, precision) -> (T,B,h_dim) in fp32; a step whose mask is 0 leaves every layer's state as it is.  `step` takes one
+    time step of streams whose states the caller keeps.  Forget biases start between 1 and 4: states that reach over 4 to 50
+    steps."""
+
+    def __init__(self, in_dim, h_dim, num_layers=1, bias=True):
+        super().__init__()
+        self.num_layers, self.bias = num_layers, bias
+        self.inp = nn.Linear(in_dim, h_dim, bias)
+        self.proj = nn.ModuleList([nn.Linear(h_dim, 3 * h_dim, bias) for _ in range(num_layers)])
+        self.norms = nn.ParameterList([nn.Parameter(torch.ones(h_dim)) for _ in range(num_layers)])
+        self.posts = nn.ParameterList([nn.Parameter(torch.ones(h_dim)) for _ in range(num_layers)])
+        self.scales = nn.ParameterList([nn.Parameter(torch.ones(h_dim)) for _ in range(num_layers)])
+        if bias:
+            for layer in self.proj:
+                nn.init.uniform_(layer.bias[:h_dim], 1.0, 4.0)
+
+    def _next(self, k):
+        return self.norms[k + 1] if k + 1 < self.num_layers else None
+
+    def forward(self, x, h0, mask=None, reverse=False, precision=None):
+        from .. import ops
+        t_max, b_dim = x.shape[:2]
+        res = ops.tall_projection(x.reshape(t_max * b_dim, -1), self.inp.weight, self.inp.bias, precision)
+        h_dim = res.shape[1]
+        # with bf16 operands the branch between norm, projection and block is stored as bf16 too, the residual stays fp32
+        low = ops.PRECISIONS[precision] == ops.native.PREC_BF16 and ops.linear_tiles_supported(res, self.proj[0].weight)
+        n = ops.rms_norm(res, self.norms[0], dtype=torch.bfloat16 if low else None)
+        res = res.view(t_max, b_dim, h_dim)
+        for k, layer in enumerate(self.proj):
+            n = n.view(-1, h_dim)
+            proj = (ops._LinearTilesFn.apply(n, layer.weight, layer.bias, torch.bfloat16) if low
+                    else ops.tall_projection(n, layer.weight, layer.bias, precision))
+            out = ops.gated_block(proj.view(t_max, b_dim, 3 * h_dim), res, h0[k], self.posts[k], scale=self.scales[k],
+                                  next_weight=self._next(k), mask=mask, reverse=reverse)
+            res, n = out[0], out[1]
+        return res
+
+    @torch.no_grad()
+    def step(self, x, states, mask=None):
+        """One time step: x (B,in_dim), states (num_layers,B,h_dim) fp32, updated in place, mask (B,) -> (B,h_dim)."""
+        from .. import ops
+        res = self.inp(x)
+        n = ops.rms_norm(res, self.norms[0])
+        for k, layer in enumerate(self.proj):
+            out = ops.gated_block_step(layer(n), res, states[k], self.posts[k], scale=self.scales[k],
+                                       next_weight=self._next(k), mask=mask, new_state=states[k])
+            res, n = out[0], out[1]
+        return res
+
+
 class _ConvBlock(nn.Module):
     """Shared shape of Conv / Deconv / AudioConv / AudioDeconv (common.py:70-112, 177-219).
 

@@ -41,9 +41,12 @@ class MultiDKS(MultiDGTS):
     def __init__(self, modalities, dims, dists=None, encoders=None, decoders=None,
                  h_dim=32, z_dim=32, z0_mean=0.0, z0_std=1.0, min_std=1e-3, feat_to_z=True,
                  rnn_dir='bwd', rnn_skip=True, rnn_layers=1, rnn_bias=True,
-                 device=torch.device('cuda:0')):
-        """Arguments as in the reference (dks.py:27-67)."""
+                 device=torch.device('cuda:0'), rnn_cell='gru'):
+        """Arguments as in the reference (dks.py:27-67), and rnn_cell: 'gru', or 'linear' for inference RNNs of gated
+        linear recurrences (common.GatedLinearRNN), parallel in time."""
         super().__init__()
+        if rnn_cell not in ('gru', 'linear'):
+            raise ValueError('MultiDKS: rnn_cell must be "gru" or "linear", got %r' % (rnn_cell,))
         self.modalities = modalities
         self.n_mods = len(modalities)
         self.dims = dict(zip(modalities, dims))
@@ -84,7 +87,7 @@ class MultiDKS(MultiDGTS):
         self.rnn = nn.ModuleDict()
         self.h0 = nn.ParameterDict()
         for m in self.modalities:
-            self.rnn[m] = nn.GRU(self.feat_dims[m], h_dim, rnn_layers, rnn_bias)
+            self.rnn[m] = (nn.GRU if rnn_cell == 'gru' else common.GatedLinearRNN)(self.feat_dims[m], h_dim, rnn_layers, rnn_bias)
             self.h0[m] = nn.Parameter(torch.zeros(rnn_layers, 1, h_dim))
         self.feat_to_z = feat_to_z
         comb_dim = z_dim + self.n_mods * h_dim
@@ -124,6 +127,8 @@ class MultiDKS(MultiDGTS):
         states in natural time order."""
         t_max, b_dim = feat.shape[:2]
         gru = self.rnn[m]
+        if isinstance(gru, common.GatedLinearRNN):
+            return gru(feat, self.h0[m][:, 0], mask if self.rnn_skip else None, self.rnn_dir == 'bwd', self.sweep_dtype)
         x = feat.reshape(t_max * b_dim, -1)
         h_seq = None
         for layer in range(gru.num_layers):
@@ -264,8 +269,10 @@ class MultiDKS(MultiDGTS):
                     feat = self._plug(self.enc[m], self._zero_input(m, t_max, b_dim, dev).flatten(0, 1))
                     feat = feat.reshape(t_max, b_dim, -1)
                     gone = torch.zeros(t_max, b_dim, device=dev, dtype=torch.bool)
-                    if self.rnn_skip:       # never updated: stays at the initial state of the top layer
+                    if self.rnn_skip and isinstance(self.rnn[m], nn.GRU):   # never updated: the top layer's initial state
                         h = self.h0[m][-1].reshape(1, 1, -1).expand(t_max, b_dim, -1)
+                    elif self.rnn_skip:     # (states never updated, one row of features: one row for every step)
+                        h = self._rnn(m, feat[:1, :1].contiguous(), gone[:1, :1]).expand(t_max, b_dim, -1)
                     else:                   # zero-masked inputs: every sequence sees the same features
                         h = self._rnn(m, feat[:, :1].contiguous(), gone[:, :1]).expand(-1, b_dim, -1)
                     left[m] = (feat, h, gone)
