@@ -15,25 +15,24 @@
 namespace mdmm {
 namespace {
 
-// steps of a wave; most waves; steps between two states kept for the backward pass (its tiles, above KEEP2 steps)
-constexpr int S = 8, WMAX = 8, KEEP = 32, KEEP2 = 64;
+// steps of a wave; most waves; up to ONE steps are one tile; beyond, steps of a tile, whose first state is kept for the
+// backward pass
+constexpr int S = 8, WMAX = 8, ONE = S * WMAX, KEEP = 32;
 
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T, int VEC> struct Raw;           // VEC elements as loaded
 template <> struct Raw<float, 1> { unsigned x; };
 template <> struct Raw<float, 2> { u32x2 x; };
-template <> struct Raw<float, 4> { u32x4 x; };
 template <> struct Raw<__bf16, 1> { unsigned short x; };
 template <> struct Raw<__bf16, 2> { unsigned x; };
-template <> struct Raw<__bf16, 4> { u32x2 x; };
 
 template <int VEC> __device__ __forceinline__ void widen(const Raw<float, VEC>& r, float* v) { __builtin_memcpy(v, &r, sizeof r); }
-__device__ __forceinline__ void widen2(unsigned x, float* v) { v[0] = __uint_as_float(x << 16); v[1] = __uint_as_float(x & 0xffff0000u); }
 __device__ __forceinline__ void widen(const Raw<__bf16, 1>& r, float* v) { v[0] = __uint_as_float((unsigned)r.x << 16); }
-__device__ __forceinline__ void widen(const Raw<__bf16, 2>& r, float* v) { widen2(r.x, v); }
-__device__ __forceinline__ void widen(const Raw<__bf16, 4>& r, float* v) { widen2(r.x[0], v); widen2(r.x[1], v + 2); }
+__device__ __forceinline__ void widen(const Raw<__bf16, 2>& r, float* v) {
+  v[0] = __uint_as_float(r.x << 16);
+  v[1] = __uint_as_float(r.x & 0xffff0000u);
+}
 
 template <typename T, int VEC> __device__ __forceinline__ Raw<T, VEC> narrow(const float* v) {
   T t[VEC];
@@ -55,16 +54,14 @@ template <typename T, int VEC> struct Step<T, VEC, true> {
       : r(__builtin_amdgcn_make_buffer_rsrc((void*)((T*)base + at), 0, live && base ? 0x7fffffff : 0, 0x00020000)) {}
   __device__ __forceinline__ Raw<T, VEC> get(unsigned o) const {
     Raw<T, VEC> v;
-    if constexpr (sizeof(v) == 16) v.x = __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0);
-    else if constexpr (sizeof(v) == 8) v.x = __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0);
+    if constexpr (sizeof(v) == 8) v.x = __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0);
     else if constexpr (sizeof(v) == 4) v.x = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
     else v.x = __builtin_amdgcn_raw_buffer_load_b16(r, o, 0, 0);
     return v;
   }
   __device__ __forceinline__ void put(unsigned o, const float* f) const {
     const Raw<T, VEC> v = narrow<T, VEC>(f);
-    if constexpr (sizeof(v) == 16) __builtin_amdgcn_raw_buffer_store_b128(v.x, r, o, 0, 0);
-    else if constexpr (sizeof(v) == 8) __builtin_amdgcn_raw_buffer_store_b64(v.x, r, o, 0, 0);
+    if constexpr (sizeof(v) == 8) __builtin_amdgcn_raw_buffer_store_b64(v.x, r, o, 0, 0);
     else if constexpr (sizeof(v) == 4) __builtin_amdgcn_raw_buffer_store_b32(v.x, r, o, 0, 0);
     else __builtin_amdgcn_raw_buffer_store_b16(v.x, r, o, 0, 0);
   }
@@ -111,22 +108,24 @@ template <typename IO, typename HO, bool BUF> struct Lane {
 };
 
 __device__ __forceinline__ int64_t time_of(const mdmm_gated_scan_t& p, int64_t i) { return p.reverse ? p.T - 1 - i : i; }
+__device__ __forceinline__ int64_t onward(const mdmm_gated_scan_t& p) { return p.reverse ? -1 : 1; }
 
 // f, c and the mask of a wave's S steps from step i0 on as loaded (a step past the end: zeros)
 template <typename IO, typename HO, int VEC, bool BUF> struct Steps {
   Raw<IO, VEC> f[S], c[S];
   unsigned char m[S];
   template <bool C> __device__ __forceinline__ void fetch(const mdmm_gated_scan_t& p, const Lane<IO, HO, BUF>& l, int64_t i0, bool any) {
+    const int64_t step = onward(p) * p.gates_st, mstep = onward(p) * p.mask_st;
+    int64_t at = time_of(p, i0) * p.gates_st, mat = time_of(p, i0) * p.mask_st;
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int64_t t = time_of(p, i0 + s);
+    for (int s = 0; s < S; ++s, at += step, mat += mstep) {
       const bool in = any && i0 + s < p.T;
-      f[s] = Step<IO, VEC, BUF>(p.gates, t * p.gates_st, in).get(l.gates);
-      if (C) c[s] = Step<IO, VEC, BUF>(p.gates, t * p.gates_st + p.H, in).get(l.gates);
+      f[s] = Step<IO, VEC, BUF>(p.gates, at, in).get(l.gates);
+      if (C) c[s] = Step<IO, VEC, BUF>(p.gates, at + p.H, in).get(l.gates);
       if constexpr (BUF) {
-        __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(p.mask + t * p.mask_st), 0, in && p.mask ? 0x7fffffff : 0, 0x00020000);
+        __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(p.mask + mat), 0, in && p.mask ? 0x7fffffff : 0, 0x00020000);
         m[s] = __builtin_amdgcn_raw_buffer_load_b8(r, l.mask, 0, 0);
-      } else m[s] = in && p.mask && l.live ? p.mask[t * p.mask_st + l.mask] : 0;
+      } else m[s] = in && p.mask && l.live ? p.mask[mat + l.mask] : 0;
     }
   }
   // bit s: step s is there and its mask lets it through
@@ -192,9 +191,10 @@ __global__ __launch_bounds__(64 * WMAX) void scan_split_kernel(mdmm_gated_scan_t
     const int64_t i0 = first + (BWD ? n - 1 - i : i) * S;
     x.template fetch<!BWD>(p, l, i0, i < n);
     if (BWD) {
+      int64_t at = time_of(p, i0) * stride;
 #pragma unroll
-      for (int s = 0; s < S; ++s)
-        g[s] = Step<HO, VEC, BUF>(p.g_h, time_of(p, i0 + s) * stride, i < n && i0 + s < p.T).get(l.h);
+      for (int s = 0; s < S; ++s, at += onward(p) * stride)
+        g[s] = Step<HO, VEC, BUF>(p.g_h, at, i < n && i0 + s < p.T).get(l.h);
     }
   };
   fetch(0);
@@ -293,12 +293,13 @@ __global__ __launch_bounds__(64 * WMAX, 4) void scan_fwd_kernel(mdmm_gated_scan_
         }
       }
     }
-    if (wave * S % KEEP == 0 && i0 < p.T) Step<float, VEC, BUF>(p.states, i0 / KEEP * stride, true).put(l.f32, h);
+    if (wave == 0) Step<float, VEC, BUF>(p.states, tile * stride, true).put(l.f32, h);
+    int64_t at = time_of(p, i0) * stride;
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
+    for (int s = 0; s < S; ++s, at += onward(p) * stride) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) h[e] = fmaf(a[s][e], h[e], b[s][e]);
-      Step<HO, VEC, BUF>(p.h, time_of(p, i0 + s) * stride, i0 + s < p.T).put(l.h, h);
+      Step<HO, VEC, BUF>(p.h, at, i0 + s < p.T).put(l.h, h);
     }
     if (W == 1) {
 #pragma unroll
@@ -322,8 +323,9 @@ __global__ __launch_bounds__(64 * WMAX) void scan_bwd_kernel(mdmm_gated_scan_t p
     const bool any = tile >= t0;
     const int64_t i0 = tile * pl.tile + wave * S;
     x.template fetch<true>(p, l, i0, any);
+    int64_t at = time_of(p, i0) * stride;
 #pragma unroll
-    for (int s = 0; s < S; ++s) g[s] = Step<HO, VEC, BUF>(p.g_h, time_of(p, i0 + s) * stride, any && i0 + s < p.T).get(l.h);
+    for (int s = 0; s < S; ++s, at += onward(p) * stride) g[s] = Step<HO, VEC, BUF>(p.g_h, at, any && i0 + s < p.T).get(l.h);
     start = Step<float, VEC, BUF>(p.states, tile * stride, any).get(l.f32);
   };
   fetch(t1 - 1);
@@ -395,8 +397,9 @@ __global__ __launch_bounds__(64 * WMAX) void scan_bwd_kernel(mdmm_gated_scan_t p
         h[e] = fmaf(a[s][e], h[e], k[s][e] * cv[s][e]);
         cv[s][e] = (on >> s & 1) ? before - cv[s][e] : 0.0f;
       }
+    int64_t at = time_of(p, i0 + S - 1) * p.g_gates_st;
 #pragma unroll
-    for (int s = S - 1; s >= 0; --s) {
+    for (int s = S - 1; s >= 0; --s, at -= onward(p) * p.g_gates_st) {
       float df[VEC], dc[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
@@ -405,7 +408,6 @@ __global__ __launch_bounds__(64 * WMAX) void scan_bwd_kernel(mdmm_gated_scan_t p
         df[e] = dc[e] * a[s][e] * cv[s][e];
         d[e] = a[s][e] * G;
       }
-      const int64_t at = time_of(p, i0 + s) * p.g_gates_st;
       Step<IO, VEC, BUF>(p.g_gates, at, i0 + s < p.T).put(l.g_gates, df);
       Step<IO, VEC, BUF>(p.g_gates, at + p.H, i0 + s < p.T).put(l.g_gates, dc);
     }
@@ -441,7 +443,7 @@ int check(const mdmm_gated_scan_t* a) {
 
 bool none(const mdmm_gated_scan_t* a) { return a->T == 0 || a->B == 0 || a->H == 0; }
 
-Plan plan(const mdmm_gated_scan_t* a, bool bwd) {
+Plan plan(const mdmm_gated_scan_t* a) {
   Plan p;
   const uintptr_t es = a->gates_bf16 ? 2 : 4, hs = a->h_bf16 ? 2 : 4;
   auto fits = [&](int v) {
@@ -451,16 +453,16 @@ Plan plan(const mdmm_gated_scan_t* a, bool bwd) {
            a->g_gates_st % v == 0 && a->g_gates_sb % v == 0 && ((uintptr_t)a->states & m4) == 0 &&
            ((uintptr_t)a->h_last & m4) == 0 && ((uintptr_t)a->g_h0 & m4) == 0;
   };
+  // (four channels a thread spill in the forward pass: 123 us at 512 x 256 x 512 in bf16, with two 94)
   p.vec = fits(2) ? 2 : 1;
-  if (!bwd && fits(4) && (int64_t)a->B * a->H >= 64 * 4 * 512) p.vec = 4;
   auto reach = [&](int64_t sb) { return (sb < 0 ? 0x80000000ll : (a->B - 1) * sb + 2 * (int64_t)a->H) * 4 < 0x7fffffffll; };
   p.buf = reach(a->gates_sb) && reach(a->g_gates_sb) && reach(a->H) && reach(a->mask_sb);
   p.chunks = a->H / p.vec;
   p.wgs = (p.chunks * a->B + 63) / 64;
-  // up to KEEP2 steps one tile; beyond, forward tiles of 8 waves (at 512 x 256 x 512 in bf16 106 us, of 4 waves 122) and
-  // backward ones of 4 (159 us, of 8 waves 179: three of them, twelve waves, fit a CU's registers, but one of 8)
+  // up to ONE steps one tile; beyond, tiles of 4 waves (at 512 x 256 x 512 in bf16 94 us forward and 155 backward, of 8
+  // waves 98 and 179: of the backward pass three workgroups of 4 waves fit a CU's registers, but one of 8)
   const int64_t waves = (a->T + S - 1) / S;
-  p.waves = (int)(a->T <= KEEP2 ? waves : bwd ? KEEP / S : WMAX);
+  p.waves = (int)(a->T <= ONE ? waves : KEEP / S);
   p.tile = p.waves * S;
   p.tiles = (a->T + p.tile - 1) / p.tile;
   // fewer than two workgroups a CU: time over workgroups too, two a CU (20011 x 3 x 200 in fp32: 133 us for the four launches
@@ -480,31 +482,24 @@ template <typename IO, typename HO, int VEC, bool BUF>
 int launch(const mdmm_gated_scan_t* a, const Plan& pl, bool bwd, hipStream_t s) {
   const dim3 grid((unsigned)pl.wgs, (unsigned)pl.splits), block(64 * pl.waves);
 #define RUN(K) hipLaunchKernelGGL(K, grid, block, 0, s, *a, pl)
-  if (bwd) {
-    if constexpr (VEC < 4) {
-      if (pl.splits > 1) RUN((scan_split_kernel<IO, HO, VEC, BUF, true>));
-      RUN((scan_bwd_kernel<IO, HO, VEC, BUF>));
-    }
-  } else {
-    if constexpr (VEC < 4) {
-      if (pl.splits > 1) RUN((scan_split_kernel<IO, HO, VEC, BUF, false>));
-    }
-    RUN((scan_fwd_kernel<IO, HO, VEC, BUF>));
+  if (pl.splits > 1) {
+    if (bwd) RUN((scan_split_kernel<IO, HO, VEC, BUF, true>));
+    else RUN((scan_split_kernel<IO, HO, VEC, BUF, false>));
   }
+  if (bwd) RUN((scan_bwd_kernel<IO, HO, VEC, BUF>));
+  else RUN((scan_fwd_kernel<IO, HO, VEC, BUF>));
 #undef RUN
   return (int)hipGetLastError();
 }
 
 template <typename IO, typename HO>
 int launch(const mdmm_gated_scan_t* a, const Plan& pl, bool bwd, hipStream_t s) {
-  if (!pl.buf) return pl.vec == 1 ? launch<IO, HO, 1, false>(a, pl, bwd, s) : pl.vec == 2 ? launch<IO, HO, 2, false>(a, pl, bwd, s)
-                                                                             : launch<IO, HO, 4, false>(a, pl, bwd, s);
-  return pl.vec == 1 ? launch<IO, HO, 1, true>(a, pl, bwd, s) : pl.vec == 2 ? launch<IO, HO, 2, true>(a, pl, bwd, s)
-                                                                            : launch<IO, HO, 4, true>(a, pl, bwd, s);
+  if (!pl.buf) return pl.vec == 1 ? launch<IO, HO, 1, false>(a, pl, bwd, s) : launch<IO, HO, 2, false>(a, pl, bwd, s);
+  return pl.vec == 1 ? launch<IO, HO, 1, true>(a, pl, bwd, s) : launch<IO, HO, 2, true>(a, pl, bwd, s);
 }
 
 int run(const mdmm_gated_scan_t* a, bool bwd, hipStream_t s) {
-  const Plan pl = plan(a, bwd);
+  const Plan pl = plan(a);
   if (pl.wgs > 0x7fffffff) return MDMM_E_LIMIT;
   if (pl.splits > 1 && !a->ws) return MDMM_E_ARG;
   if (!a->gates_bf16) return launch<float, float>(a, pl, bwd, s);
@@ -518,13 +513,13 @@ using namespace mdmm;
 
 extern "C" int64_t mdmm_gated_scan_states(const mdmm_gated_scan_t* a) {
   if (check(a)) return -1;
-  return a->T > KEEP2 ? ((int64_t)a->T + KEEP - 1) / KEEP * a->B * a->H : 0;         // (a single tile starts at h0)
+  return a->T > ONE ? ((int64_t)a->T + KEEP - 1) / KEEP * a->B * a->H : 0;         // (a single tile starts at h0)
 }
 
-extern "C" int64_t mdmm_gated_scan_ws(const mdmm_gated_scan_t* a, int bwd) {
+extern "C" int64_t mdmm_gated_scan_ws(const mdmm_gated_scan_t* a, int) {
   if (check(a)) return -1;
   if (none(a)) return 0;
-  const Plan pl = plan(a, bwd);
+  const Plan pl = plan(a);
   return pl.splits > 1 ? 2 * (int64_t)pl.splits * a->B * a->H : 0;
 }
 
@@ -540,7 +535,7 @@ extern "C" int mdmm_gated_scan_bwd(const mdmm_gated_scan_t* a, void* stream) {
   const int rc = check(a);
   if (rc) return rc;
   if (none(a)) return 0;
-  if (!a->g_gates || (a->T > KEEP2 && !a->states)) return MDMM_E_ARG;
+  if (!a->g_gates || (a->T > ONE && !a->states)) return MDMM_E_ARG;
   if (a->g_h0_sum && !a->g_h0) return MDMM_E_ARG;
   const int e = run(a, true, (hipStream_t)stream);
   if (e || !a->g_h0_sum) return e;
