@@ -50,20 +50,27 @@ struct Item {               // one matrix's padded sizes and workspace
   double* sums;
   int32_t n, m, tall, splits;
 };
+enum { PACKS, GRAMS, POLYS, APPLIES, LISTS };
 struct Items {
   Item it[MDMM_ORTHO_MAX];
-  int32_t first[MDMM_ORTHO_MAX + 1];       // first tile of each matrix in this launch
-  int32_t which[MDMM_ORTHO_MAX];           // its place in the call
-  int32_t n;
+  int32_t first[LISTS][MDMM_ORTHO_MAX + 1];       // first tile of each matrix in a launch
+  int32_t which[MDMM_ORTHO_MAX];                  // its place in the call
+  int32_t n, reserved;
 };
+// What the launches of one size class share.  The first launch takes it as its argument and leaves it in the workspace; the
+// others read it there: arguments live in host memory, where each of the dependent loads that find a tile's matrix would
+// wait for the bus
+struct Call {
+  mdmm_ortho_t p;
+  Items q;
+};
+static_assert(sizeof(Call) <= 3968, "a launch's arguments");
 
+// the matrix a tile belongs to: every lane looks at one matrix's end (one load where a search has four in a row)
+static_assert(MDMM_ORTHO_MAX <= 64, "a wave's lanes");
 __device__ __forceinline__ int find(const int32_t* first, int n, int tile) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (first[mid] <= tile) lo = mid; else hi = mid - 1;
-  }
-  return lo;
+  const int lane = threadIdx.x & 63;
+  return (int)__popcll(__ballot(lane < n && first[lane < n ? lane + 1 : 0] <= tile));
 }
 
 __device__ __forceinline__ void split(float x, half_t& h, half_t& l) {       // x: already scaled
@@ -81,9 +88,14 @@ __device__ __forceinline__ float src_at(const mdmm_ortho_t& p, const mdmm_ortho_
 }
 
 // momentum, and the sum of squares in SUMS pieces (in 64 bits: an error of the norm is a scale of X and grows like one)
-__global__ __launch_bounds__(NT) void ortho_sums_kernel(mdmm_ortho_t p, Items q) {
+__global__ __launch_bounds__(NT) void ortho_sums_kernel(Call call, Call* keep) {
+  const mdmm_ortho_t& p = call.p;
   const int k = blockIdx.y;
-  const mdmm_ortho_item_t& t = p.item[q.which[k]];
+  const mdmm_ortho_item_t& t = p.item[call.q.which[k]];
+  if (blockIdx.x == 0 && k == 0) {
+    const __attribute__((address_space(4))) unsigned* args = (const __attribute__((address_space(4))) unsigned*)__builtin_amdgcn_kernarg_segment_ptr();
+    for (int i = threadIdx.x; i < (int)(sizeof(Call) / 4); i += NT) ((unsigned*)keep)[i] = args[i];
+  }
   double s = 0.0;
   // a workgroup's rows, its threads over the columns (rows shorter than a workgroup: several of them at once)
   const int wide = t.cols < NT ? (t.cols < 16 ? 16 : t.cols < 64 ? 64 : NT) : NT, high = NT / wide;
@@ -102,13 +114,15 @@ __global__ __launch_bounds__(NT) void ortho_sums_kernel(mdmm_ortho_t p, Items q)
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) q.it[k].sums[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+  if (threadIdx.x == 0) call.q.it[k].sums[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
 // X both ways, 64 x 64 elements a workgroup
-__global__ __launch_bounds__(NT) void ortho_pack_kernel(mdmm_ortho_t p, Items q) {
+__global__ __launch_bounds__(NT) void ortho_pack_kernel(const Call* __restrict__ call) {
   __shared__ float tile[64][65];
-  const int k = find(q.first, q.n, blockIdx.x);
+  const mdmm_ortho_t& p = call->p;
+  const Items& q = call->q;
+  const int k = find(q.first[PACKS], q.n, blockIdx.x);
   const mdmm_ortho_item_t& t = p.item[q.which[k]];
   const Item& w = q.it[k];
   __shared__ double part[NT / 64];
@@ -118,7 +132,7 @@ __global__ __launch_bounds__(NT) void ortho_pack_kernel(mdmm_ortho_t p, Items q)
   __syncthreads();
   s = (part[0] + part[1]) + (part[2] + part[3]);
   const float inv = (float)((double)SX / (sqrt(s) + (double)p.eps));
-  const int me = blockIdx.x - q.first[k], across = (w.tall ? w.n : w.m) / 64;       // tiles of the source's rows
+  const int me = blockIdx.x - q.first[PACKS][k], across = (w.tall ? w.n : w.m) / 64;       // tiles of the source's rows
   const int64_t r0 = me / across * 64, c0 = me % across * 64;
   // the source's orientation: lying or standing plane pair
   half_t* same = w.tall ? w.xt[0] : w.xn;
@@ -206,16 +220,18 @@ template <class C> __host__ __device__ int tri(int n) {          // tiles at and
 }
 
 template <int MODE, class C>
-__global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(mdmm_ortho_t p, Items q, int flip) {
+__global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call* __restrict__ call, int flip) {
   __shared__ __align__(16) half_t lds[C::ST * C::HALVES];
   constexpr bool PX = MODE == APPLY || MODE == LAST;
+  constexpr int LIST = MODE == GRAM ? GRAMS : MODE == POLY ? POLYS : APPLIES;
+  const Items& q = call->q;
   // consecutive workgroups go round the 8 XCDs: each XCD takes a run of consecutive tiles instead
   const int total = gridDim.x, xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
   const int me = xcd * each + (xcd < more ? xcd : more) + (blockIdx.x >> 3);
-  const int k = find(q.first, q.n, me);
+  const int k = find(q.first[LIST], q.n, me);
   const Item w = q.it[k];
   const int n = w.n, J = PX ? w.m : n;
-  int tile = me - q.first[k], ti, tj, slice = 0;
+  int tile = me - q.first[LIST][k], ti, tj, slice = 0;
   if (PX) {
     ti = tile / (J / C::BN);
     tj = tile % (J / C::BN);
@@ -252,8 +268,20 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(mdmm_ortho_
       from[c] += 2 * C::BK;
     }
   };
-  f32x16 acc[C::TI][C::TJ] = {};
+  // what the result is joined with, on its way while the product runs (the small tile has the registers)
+  constexpr bool EARLY = MODE != GRAM && C::TI * C::TJ == 1;
   const int wi = wave / C::WJ * 32 * C::TI, wj = wave % C::WJ * 32 * C::TJ;
+  const half_t* beside = MODE == POLY ? w.gram : xt;
+  half4 eh[EARLY ? 4 : 1], el[EARLY ? 4 : 1];
+  if constexpr (EARLY) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const half_t* d = beside + at(j0 + wj + (lane & 31), n, i0 + wi + 8 * g + 4 * (lane >> 5));
+      eh[g] = *(const half4*)d;
+      el[g] = *(const half4*)(d + 32);
+    }
+  }
+  f32x16 acc[C::TI][C::TJ] = {};
 #pragma unroll
   for (int s = 0; s < C::ST - 1; ++s)
     if (s < nk) load(s);
@@ -299,9 +327,12 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(mdmm_ortho_
     }
   }
   // v: the result in its planes' scale
+  const mdmm_ortho_t& p = call->p;
   const mdmm_ortho_item_t t = p.item[q.which[k]];
+  const float ca = p.ca, cb = p.cb, cc = p.cc, decay = p.decay;
+  const bool update = p.update, low = p.dst_bf16;
   const int64_t nn = (int64_t)n * n, m = w.m;
-  const float lr = MODE == LAST && p.update ? (p.lr_dev ? *p.lr_dev : p.lr) : 0.0f;
+  const float lr = MODE == LAST && update ? (p.lr_dev ? *p.lr_dev : p.lr) : 0.0f;
 #pragma unroll
   for (int x = 0; x < C::TI; ++x)
 #pragma unroll
@@ -313,6 +344,15 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(mdmm_ortho_
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[x][y][4 * g + e];
+        half4 h, l;
+        if constexpr (EARLY) {
+          h = eh[g];
+          l = el[g];
+        } else if constexpr (MODE != GRAM) {
+          const half_t* d = beside + at(j, n, i);
+          h = *(const half4*)d;
+          l = *(const half4*)(d + 32);
+        }
         if (MODE == GRAM) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] *= 1.0f / SX;
@@ -320,17 +360,13 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(mdmm_ortho_
           else *(float4*)(w.part + slice * nn + j * n + i) = make_float4(v[0], v[1], v[2], v[3]);
         }
         if (MODE == POLY) {
-          const half_t* d = w.gram + at(j, n, i);
-          const half4 h = *(const half4*)d, l = *(const half4*)(d + 32);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(p.cc * (SP / SX / SX), v[e], p.cb * (SP / SX) * join(h[e], l[e]));
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(cc * (SP / SX / SX), v[e], cb * (SP / SX) * join(h[e], l[e]));
           put_sym(w.poly, n, i, j, v, j0 < i0 + C::BM);
         }
         if (PX) {
-          const half_t* d = xt + at(j, n, i);
-          const half4 h = *(const half4*)d, l = *(const half4*)(d + 32);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(p.ca, join(h[e], l[e]), v[e] * (1.0f / SP));
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(ca, join(h[e], l[e]), v[e] * (1.0f / SP));
         }
         if (MODE == APPLY) {
           half4 h4, l4;
@@ -356,10 +392,10 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(mdmm_ortho_
           for (int e = 0; e < 4; ++e) {
             const float u = v[e] * (1.0f / SX);
             if (e >= end) continue;
-            if (p.update) {
+            if (update) {
               float* d = (float*)t.dst + o + e * step;
-              *d = fmaf(-lr * t.gain, u, (1.0f - lr * p.decay) * *d);
-            } else if (p.dst_bf16) ((__bf16*)t.dst)[o + e * step] = (__bf16)u;
+              *d = fmaf(-lr * t.gain, u, (1.0f - lr * decay) * *d);
+            } else if (low) ((__bf16*)t.dst)[o + e * step] = (__bf16)u;
             else ((float*)t.dst)[o + e * step] = u;
           }
         }
@@ -367,8 +403,8 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(mdmm_ortho_
 }
 
 // the slices of A added up (each keeps the tiles at and above the diagonal, column by column)
-template <int BM, int BN> __global__ __launch_bounds__(NT) void ortho_fold_kernel(Items q) {
-  const Item w = q.it[blockIdx.y];
+template <int BM, int BN> __global__ __launch_bounds__(NT) void ortho_fold_kernel(const Call* __restrict__ call) {
+  const Item w = call->q.it[blockIdx.y];
   if (w.splits == 1) return;
   const int64_t n = w.n, nn = n * n;
   for (int64_t e = ((int64_t)blockIdx.x * NT + threadIdx.x) * 4; e < nn; e += (int64_t)gridDim.x * NT * 4) {
@@ -385,7 +421,9 @@ template <int BM, int BN> __global__ __launch_bounds__(NT) void ortho_fold_kerne
   }
 }
 
-__global__ __launch_bounds__(NT) void ortho_copy_kernel(mdmm_ortho_t p, Items q) {       // steps = 0: X itself
+__global__ __launch_bounds__(NT) void ortho_copy_kernel(const Call* __restrict__ call) {       // steps = 0: X itself
+  const mdmm_ortho_t& p = call->p;
+  const Items& q = call->q;
   const mdmm_ortho_item_t& t = p.item[q.which[blockIdx.y]];
   const Item& w = q.it[blockIdx.y];
   const int64_t total = (int64_t)t.rows * t.cols;
@@ -423,7 +461,7 @@ bool large(const mdmm_ortho_item_t& t) { return (t.rows < t.cols ? t.rows : t.co
 // the workspace: fills both size classes' lists (base NULL: sizes only), returns the bytes used
 int64_t lay_out(const mdmm_ortho_t* a, Items (&q)[2]) {
   char* base = (char*)a->ws;
-  int64_t off = 0;
+  int64_t off = 2 * up(sizeof(Call), 256);
   auto take = [&](int64_t bytes) { char* p = base + off; off += up(bytes, 256); return p; };
   q[0].n = q[1].n = 0;
   for (int i = 0; i < a->n; ++i) {
@@ -455,35 +493,38 @@ int64_t lay_out(const mdmm_ortho_t* a, Items (&q)[2]) {
   return off;
 }
 
-template <class F> int tiles(Items& q, F count) {
+template <class F> int tiles(Items& q, int list, F count) {
   int64_t total = 0;
   for (int i = 0; i < q.n; ++i) {
-    q.first[i] = (int32_t)total;
+    q.first[list][i] = (int32_t)total;
     total += count(q.it[i]);
   }
-  q.first[q.n] = (int32_t)total;
+  q.first[list][q.n] = (int32_t)total;
   return (int)total;
 }
 
-template <class C> void launch(const mdmm_ortho_t* a, Items& q, hipStream_t s) {
-  if (!q.n) return;
-  hipLaunchKernelGGL(ortho_sums_kernel, dim3(SUMS, q.n), dim3(NT), 0, s, *a, q);
-  const int packs = tiles(q, [](const Item& w) { return (int64_t)(w.n / 64) * (w.m / 64); });
-  hipLaunchKernelGGL(ortho_pack_kernel, dim3(packs), dim3(NT), 0, s, *a, q);
-  if (a->steps == 0) hipLaunchKernelGGL(ortho_copy_kernel, dim3(256, q.n), dim3(NT), 0, s, *a, q);
-  Items qg = q, qp = q, qa = q;
-  const int gram = tiles(qg, [](const Item& w) { return (int64_t)tri<C>(w.n) * w.splits; });
-  const int poly = tiles(qp, [](const Item& w) { return (int64_t)tri<C>(w.n); });
-  const int apply = tiles(qa, [](const Item& w) { return (int64_t)(w.n / C::BM) * (w.m / C::BN); });
+template <class C> void launch(const mdmm_ortho_t* a, const Items& items, Call* keep, hipStream_t s) {
+  if (!items.n) return;
+  Call c;
+  c.p = *a;
+  c.q = items;
+  Items& q = c.q;
+  const int packs = tiles(q, PACKS, [](const Item& w) { return (int64_t)(w.n / 64) * (w.m / 64); });
+  const int gram = tiles(q, GRAMS, [](const Item& w) { return (int64_t)tri<C>(w.n) * w.splits; });
+  const int poly = tiles(q, POLYS, [](const Item& w) { return (int64_t)tri<C>(w.n); });
+  const int apply = tiles(q, APPLIES, [](const Item& w) { return (int64_t)(w.n / C::BM) * (w.m / C::BN); });
   int64_t fold = 0;
   for (int i = 0; i < q.n; ++i)
     if (q.it[i].splits > 1 && (int64_t)q.it[i].n * q.it[i].n > fold) fold = (int64_t)q.it[i].n * q.it[i].n;
+  hipLaunchKernelGGL(ortho_sums_kernel, dim3(SUMS, q.n), dim3(NT), 0, s, c, keep);
+  hipLaunchKernelGGL(ortho_pack_kernel, dim3(packs), dim3(NT), 0, s, keep);
+  if (a->steps == 0) hipLaunchKernelGGL(ortho_copy_kernel, dim3(256, q.n), dim3(NT), 0, s, keep);
   for (int k = 0; k < a->steps; ++k) {
-    hipLaunchKernelGGL((ortho_product_kernel<GRAM, C>), dim3(gram), dim3(C::T), 0, s, *a, qg, k & 1);
-    if (fold) hipLaunchKernelGGL((ortho_fold_kernel<C::BM, C::BN>), dim3((unsigned)(fold / (4 * NT)), q.n), dim3(NT), 0, s, q);
-    hipLaunchKernelGGL((ortho_product_kernel<POLY, C>), dim3(poly), dim3(C::T), 0, s, *a, qp, k & 1);
-    if (k + 1 < a->steps) hipLaunchKernelGGL((ortho_product_kernel<APPLY, C>), dim3(apply), dim3(C::T), 0, s, *a, qa, k & 1);
-    else hipLaunchKernelGGL((ortho_product_kernel<LAST, C>), dim3(apply), dim3(C::T), 0, s, *a, qa, k & 1);
+    hipLaunchKernelGGL((ortho_product_kernel<GRAM, C>), dim3(gram), dim3(C::T), 0, s, keep, k & 1);
+    if (fold) hipLaunchKernelGGL((ortho_fold_kernel<C::BM, C::BN>), dim3((unsigned)(fold / (4 * NT)), q.n), dim3(NT), 0, s, keep);
+    hipLaunchKernelGGL((ortho_product_kernel<POLY, C>), dim3(poly), dim3(C::T), 0, s, keep, k & 1);
+    if (k + 1 < a->steps) hipLaunchKernelGGL((ortho_product_kernel<APPLY, C>), dim3(apply), dim3(C::T), 0, s, keep, k & 1);
+    else hipLaunchKernelGGL((ortho_product_kernel<LAST, C>), dim3(apply), dim3(C::T), 0, s, keep, k & 1);
   }
 }
 
@@ -507,7 +548,7 @@ extern "C" int mdmm_ortho(const mdmm_ortho_t* a, void* stream) {
     if (!a->item[i].src || !a->item[i].dst) return MDMM_E_ARG;
   Items q[2];
   lay_out(a, q);
-  launch<Small>(a, q[0], (hipStream_t)stream);
-  launch<Large>(a, q[1], (hipStream_t)stream);
+  launch<Small>(a, q[0], (Call*)a->ws, (hipStream_t)stream);
+  launch<Large>(a, q[1], (Call*)((char*)a->ws + up(sizeof(Call), 256)), (hipStream_t)stream);
   return (int)hipGetLastError();
 }
