@@ -46,6 +46,10 @@ def _apply(device, fn, *args):
         return fn(*args)
 
 
+def _grad_wanted(*tensors):
+    return torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors])
+
+
 _FN = {}
 
 
@@ -178,26 +182,27 @@ def _no_steps_grad(h0, g_last):
     return g_last if h0.dim() == 2 else ops.colsum(g_last)
 
 
+def _run_scan(gates, h0, mask, reverse, keep=False):
+    """-> (h, h_last, states kept for the backward pass)."""
+    T, B, H2 = gates.shape
+    H = H2 // 2
+    h = torch.empty((T, B, H), device=gates.device, dtype=gates.dtype)
+    if h.numel() == 0:
+        return h, _no_steps_last(h0, B, H, gates.device), None
+    a = native.GatedScan()
+    last, states, ws = _scan_forward(a, gates, H, h0, mask, reverse, h, keep)
+    _launch('mdmm_gated_scan_fwd', 'gated_scan_fwd', a)
+    del ws
+    return h, last, states
+
+
 class _GatedScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gates, h0, mask, reverse):
         ctx.set_materialize_grads(False)
-        T, B, H2 = gates.shape
-        H = H2 // 2
-        need = ctx.needs_input_grad
-        keep = need[0] or need[1]
-        h = torch.empty((T, B, H), device=gates.device, dtype=gates.dtype)
-        states = None
-        if h.numel() == 0:
-            last = _no_steps_last(h0, B, H, gates.device)
-        else:
-            a = native.GatedScan()
-            last, states, ws = _scan_forward(a, gates, H, h0, mask, reverse, h, keep)
-            _launch('mdmm_gated_scan_fwd', 'gated_scan_fwd', a)
-            del ws
-        if keep:
-            ctx.save_for_backward(gates, h0, mask, states)
-            ctx.reverse = reverse
+        h, last, states = _run_scan(gates, h0, mask, reverse, True)
+        ctx.save_for_backward(gates, h0, mask, states)
+        ctx.reverse = reverse
         return h, last
 
     @staticmethod
@@ -232,7 +237,10 @@ def gated_scan(gates, h0=None, mask=None, reverse=False):
     T, B, H2 = gates.shape
     h0, mask = _check_h0('gated_scan', h0, B, H2 // 2), _mask_bytes('gated_scan', mask, (T, B))
     dev = _check_device('gated_scan', gates, h0, mask)
-    return _apply(dev, _GatedScanFn.apply, _unit_cols(gates), h0, mask, bool(reverse))
+    gates, reverse = _unit_cols(gates), bool(reverse)
+    if _grad_wanted(gates, h0):
+        return _apply(dev, _GatedScanFn.apply, gates, h0, mask, reverse)
+    return _apply(dev, _run_scan, gates, h0, mask, reverse)[:2]
 
 
 def _no_grad_only(name, *tensors):
@@ -313,15 +321,15 @@ def _fill_norm(p, y, gate, res, w, s, w_next, branch, eps):
     p.w, p.scale, p.w_next = ops._ptr(w), ops._ptr(s), ops._ptr(w_next)
 
 
-def _norm_forward(p, y, gate, res, w, s, w_next, branch, eps):
-    """Fills the struct of a forward call on row-major (rows, H) operands -> (out or None, n or None)."""
+def _norm_forward(p, y, gate, res, w, s, w_next, branch, eps, shape):
+    """Fills the struct of a forward call on row-major (rows, H) operands -> (out or None, n or None) in `shape`."""
     out = n = None
     _fill_norm(p, y, gate, res, w, s, w_next, branch, eps)
     if y is not None:
-        out = torch.empty(res.shape, device=res.device, dtype=res.dtype)
+        out = torch.empty(shape, device=res.device, dtype=res.dtype)
         p.out, p.out_st = out.data_ptr(), p.H
     if w_next is not None:
-        n = torch.empty(res.shape, device=res.device, dtype=branch)
+        n = torch.empty(shape, device=res.device, dtype=branch)
         p.n, p.n_st = n.data_ptr(), p.H
     return out, n
 
@@ -350,6 +358,14 @@ def _norm_backward(p, y, gate, res, w, s, w_next, branch, eps, g_out, g_n, d_y, 
     return sums, ws
 
 
+def _run_norm(y, gate, res, w, s, w_next, branch, eps, shape):
+    """Row-major operands -> (out or None, n or None) in `shape`."""
+    p = native.BlockNorm()
+    out, n = _norm_forward(p, y, gate, res, w, s, w_next, branch, eps, shape)
+    _launch('mdmm_block_norm_fwd', 'block_norm_fwd', p)
+    return out, n
+
+
 class _RmsNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, eps, dtype):
@@ -357,10 +373,7 @@ class _RmsNormFn(torch.autograd.Function):
         rows = _as_rows(x, x.shape[-1])
         ctx.save_for_backward(rows, w)
         ctx.eps, ctx.branch = eps, dtype
-        p = native.BlockNorm()
-        n = _norm_forward(p, None, None, rows, None, None, w, dtype, eps)[1]
-        _launch('mdmm_block_norm_fwd', 'rms_norm_fwd', p)
-        return n.view(x.shape)
+        return _run_norm(None, None, rows, None, None, w, dtype, eps, x.shape)[1]
 
     @staticmethod
     @once_differentiable
@@ -397,7 +410,10 @@ def rms_norm(x, weight, eps=1e-6, dtype=None):
     if dtype not in _TYPES or (x.dtype == torch.bfloat16 and dtype != torch.bfloat16):
         raise ValueError('rms_norm: %s rows to %s' % (x.dtype, dtype))
     weight = _vector('rms_norm', 'weight', weight, H)
-    return _apply(_check_device('rms_norm', x, weight), _RmsNormFn.apply, x, weight, float(eps), dtype)
+    dev = _check_device('rms_norm', x, weight)
+    if _grad_wanted(x, weight):
+        return _apply(dev, _RmsNormFn.apply, x, weight, float(eps), dtype)
+    return _apply(dev, _run_norm, None, None, _as_rows(x, H), None, None, weight, dtype, float(eps), x.shape)[1]
 
 
 class _BlockNormFn(torch.autograd.Function):
@@ -408,11 +424,8 @@ class _BlockNormFn(torch.autograd.Function):
         rows = [None if t is None else _as_rows(t, H) for t in (y, gate, res)]
         ctx.save_for_backward(*rows, w, s, w_next)
         ctx.eps, ctx.shape = eps, res.shape
-        p = native.BlockNorm()
-        out, n = _norm_forward(p, *rows, w, s, w_next, y.dtype, eps)
-        _launch('mdmm_block_norm_fwd', 'block_norm_fwd', p)
-        out = out.view(res.shape)
-        return out if n is None else (out, n.view(res.shape))
+        out, n = _run_norm(*rows, w, s, w_next, y.dtype, eps, res.shape)
+        return out if n is None else (out, n)
 
     @staticmethod
     @once_differentiable
@@ -459,10 +472,30 @@ def block_norm(y, residual, weight, gate=None, scale=None, next_weight=None, eps
     _combo(name, y.dtype, y.dtype, residual.dtype)
     weight, scale, next_weight = _vectors(name, weight, scale, next_weight, H)
     dev = _check_device(name, y, residual, weight, gate, scale, next_weight)
-    return _apply(dev, _BlockNormFn.apply, y, residual, weight, gate, scale, next_weight, float(eps))
+    if _grad_wanted(y, residual, weight, gate, scale, next_weight):
+        return _apply(dev, _BlockNormFn.apply, y, residual, weight, gate, scale, next_weight, float(eps))
+    rows = [None if t is None else _as_rows(t, H) for t in (y, gate, residual)]
+    out, n = _apply(dev, _run_norm, *rows, weight, scale, next_weight, y.dtype, float(eps), residual.shape)
+    return out if n is None else (out, n)
 
 
 # ---- the layer ---------------------------------------------------------------------------------------------------
+
+def _run_block(proj, rows, h0, w, s, w_next, mask, reverse, eps, shape, keep=False):
+    """-> (out, n or None, h_last, states kept for the backward pass, h)."""
+    T, B, H = shape
+    dev = proj.device
+    h = torch.empty((T, B, H), device=dev, dtype=torch.float32)
+    a, p = native.GatedScan(), native.BlockNorm()
+    gate = _as_rows(proj, 3 * H)[:, 2 * H:]              # (a copy where proj's rows have no one stride: held until the launch)
+    out, n = _norm_forward(p, h.view(-1, H), gate, rows, w, s, w_next, proj.dtype, eps, shape)
+    if h.numel() == 0:
+        return out, n, _no_steps_last(h0, B, H, dev), None, h
+    last, states, ws = _scan_forward(a, proj, H, h0, mask, reverse, h, keep)
+    _launch('mdmm_gated_block_fwd', 'gated_block_fwd', a, p)
+    del ws
+    return out, n, last, states, h
+
 
 class _GatedBlockFn(torch.autograd.Function):
     """gated_scan and block_norm on one projection: the state stays fp32 between them, and their gradients land in one
@@ -471,24 +504,11 @@ class _GatedBlockFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, proj, res, h0, w, s, w_next, mask, reverse, eps):
         ctx.set_materialize_grads(False)
-        T, B, H = res.shape
-        dev = proj.device
-        keep = any(ctx.needs_input_grad)
-        h = torch.empty((T, B, H), device=dev, dtype=torch.float32)
-        rows, flat, states = _as_rows(res, H), _as_rows(proj, 3 * H), None
-        a, p = native.GatedScan(), native.BlockNorm()
-        out, n = _norm_forward(p, h.view(-1, H), flat[:, 2 * H:], rows, w, s, w_next, proj.dtype, eps)
-        if h.numel() == 0:
-            last = _no_steps_last(h0, B, H, dev)
-        else:
-            last, states, ws = _scan_forward(a, proj, H, h0, mask, reverse, h, keep)
-            _launch('mdmm_gated_block_fwd', 'gated_block_fwd', a, p)
-            del ws
-        if keep:
-            ctx.save_for_backward(proj, rows, h0, w, s, w_next, mask, states, h)
-            ctx.reverse, ctx.eps = reverse, eps
-        out = out.view(T, B, H)
-        return (out, last) if n is None else (out, n.view(T, B, H), last)
+        rows = _as_rows(res, res.shape[-1])
+        out, n, last, states, h = _run_block(proj, rows, h0, w, s, w_next, mask, reverse, eps, res.shape, True)
+        ctx.save_for_backward(proj, rows, h0, w, s, w_next, mask, states, h)
+        ctx.reverse, ctx.eps = reverse, eps
+        return (out, last) if n is None else (out, n, last)
 
     @staticmethod
     @once_differentiable
@@ -514,8 +534,9 @@ class _GatedBlockFn(torch.autograd.Function):
         else:
             d_h = torch.empty((T * B, H), device=dev, dtype=torch.float32)
             d_res = torch.empty((T * B, H), device=dev, dtype=res.dtype) if need[1] and g_n is not None else None
-            sums, ws = _norm_backward(p, h.view(-1, H), _as_rows(proj, H3)[:, 2 * H:], res, w, s, w_next, proj.dtype, ctx.eps,
-                                      g_out, g_n, d_h, g_x.view(-1, H3)[:, 2 * H:], d_res, need[3:6])
+            gate = _as_rows(proj, H3)[:, 2 * H:]         # (held until the launch, as in the forward pass)
+            sums, ws = _norm_backward(p, h.view(-1, H), gate, res, w, s, w_next, proj.dtype, ctx.eps, g_out, g_n, d_h,
+                                      g_x.view(-1, H3)[:, 2 * H:], d_res, need[3:6])
             if need[1] and d_res is None:
                 d_res = g_out
         if h.numel() == 0:
@@ -554,8 +575,12 @@ def gated_block(proj, residual, h0, weight, scale=None, next_weight=None, mask=N
     weight, scale, next_weight = _vectors(name, weight, scale, next_weight, H)
     h0, mask = _check_h0(name, h0, B, H), _mask_bytes(name, mask, (T, B))
     dev = _check_device(name, proj, residual, h0, weight, scale, next_weight, mask)
-    return _apply(dev, _GatedBlockFn.apply, _unit_cols(proj), residual, h0, weight, scale, next_weight, mask, bool(reverse),
-                  float(eps))
+    proj, reverse = _unit_cols(proj), bool(reverse)
+    if _grad_wanted(proj, residual, h0, weight, scale, next_weight):
+        return _apply(dev, _GatedBlockFn.apply, proj, residual, h0, weight, scale, next_weight, mask, reverse, float(eps))
+    out, n, last = _apply(dev, _run_block, proj, _as_rows(residual, H), h0, weight, scale, next_weight, mask, reverse, float(eps),
+                          residual.shape)[:3]
+    return (out, last) if n is None else (out, n, last)
 
 
 def gated_block_step(proj, residual, state, weight, scale=None, next_weight=None, mask=None, eps=1e-6, new_state=None):
@@ -576,7 +601,7 @@ def _block_step(proj, residual, state, w, s, w_next, mask, eps, new_state):
     H = state.shape[1]
     new_state = torch.empty_like(state) if new_state is None else new_state
     a, p = native.GatedScan(), native.BlockNorm()
-    out, n = _norm_forward(p, None, None, residual, w, s, w_next, proj.dtype, eps)
+    out, n = _norm_forward(p, None, None, residual, w, s, w_next, proj.dtype, eps, residual.shape)
     out = torch.empty(residual.shape, device=proj.device, dtype=residual.dtype)
     p.out, p.out_st = out.data_ptr(), H
     p.gate, p.gate_st = proj.data_ptr() + 2 * H * proj.element_size(), _row(proj)

@@ -463,6 +463,33 @@ def test_block_partial_gradients():
 
 
 @gpu
+def test_block_on_any_strides():
+    """Batch-first projections and residuals (whose rows have no one stride), column slices and expanded tensors: bit for bit
+    what contiguous copies give, with gradients and without."""
+    gen = torch.Generator().manual_seed(13)
+    T, B, H = 45, 6, 20
+    wide = make(gen, B, T, 3 * H + 8).cuda()
+    res_b = make(gen, B, T, 2 * H).cuda()
+    mask = (torch.rand(B, T, generator=gen) > 0.3).cuda().t()
+    w, w2 = make(gen, H).cuda(), make(gen, 2 * H).cuda()[::2]
+    h0 = make(gen, H, B).cuda().t()
+    g = [make(gen, H).cuda().expand(T, B, H), make(gen, B, T, H).cuda().transpose(0, 1), make(gen, H, B).cuda().t()]
+    for proj in (wide[..., 4:4 + 3 * H].transpose(0, 1), make(gen, 3 * H).cuda().expand(T, B, 3 * H)):
+        res = res_b[..., ::2].transpose(0, 1)
+        outs = []
+        for fix in (lambda t: t, lambda t: t.contiguous()):
+            args = [fix(t).detach() for t in (proj, res, h0, w, w2)]
+            with torch.no_grad():
+                found = list(ops.gated_block(*args[:4], next_weight=args[4], mask=fix(mask)))
+            args = [a.requires_grad_(True) for a in args]
+            got = ops.gated_block(*args[:4], next_weight=args[4], mask=fix(mask))
+            found += list(got) + list(torch.autograd.grad(got, args, [fix(t) for t in g]))
+            outs.append(found)
+        for a, b in zip(*outs):
+            assert torch.equal(a, b)
+
+
+@gpu
 def test_replayed_from_a_graph():
     """Forward and backward of a layer captured once and replayed on new inputs, with eager work between the replays:
     bit for bit the eager results."""
