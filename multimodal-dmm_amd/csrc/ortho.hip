@@ -39,7 +39,8 @@ template <int BM_, int BN_, int BK_, int ST_, int WI_, int WJ_, int OCC_> struct
   static constexpr int LOADS = HALVES / 8 / T;                  // chunks a thread loads for a buffer
   static_assert(BM * CPR % T == 0 && BN * CPR % T == 0, "a load instruction of the workgroup stays in one operand");
 };
-typedef Cfg<64, 64, 64, 4, 2, 2, 1> Small;
+// (two workgroups a CU, four buffers each.  P X of two 256 x 4096: 13.6 us, with one of 128 KB 17)
+typedef Cfg<64, 64, 32, 4, 2, 2, 2> Small;
 // (two workgroups a CU, two buffers each.  Measured on P X of two 2048 x 2048: 112 us; one workgroup with four buffers 127, one
 // of 256 x 128 and 8 waves with three 126, steps of 64 columns 126)
 typedef Cfg<128, 128, 32, 2, 2, 2, 2> Large;
@@ -125,6 +126,26 @@ __global__ __launch_bounds__(NT) void ortho_pack_kernel(const Call* __restrict__
   const int k = find(q.first[PACKS], q.n, blockIdx.x);
   const mdmm_ortho_item_t& t = p.item[q.which[k]];
   const Item& w = q.it[k];
+  const int me = blockIdx.x - q.first[PACKS][k], across = (w.tall ? w.n : w.m) / 64;       // tiles of the source's rows
+  const int64_t r0 = me / across * 64, c0 = me % across * 64;
+  // the source's orientation: lying or standing plane pair
+  half_t* same = w.tall ? w.xt[0] : w.xn;
+  half_t* other = w.tall ? w.xn : w.xt[0];
+  const int64_t ld_same = w.tall ? w.n : w.m, ld_other = w.tall ? w.m : w.n;
+  float x[4096 / NT];                  // every load on its way before the first is used
+#pragma unroll
+  for (int u = 0; u < 4096 / NT; ++u) {
+    const int i = threadIdx.x + u * NT;
+    const int64_t r = r0 + i / 64, c = c0 + i % 64;
+    x[u] = 0.0f;
+    if (r < t.rows && c < t.cols) {
+      x[u] = src_at(p, t, r, c);
+      if (t.mom) {
+        const float mv = t.mom[r * t.cols + c];
+        x[u] = p.nesterov ? fmaf(p.momentum, mv, x[u]) : mv;
+      }
+    }
+  }
   __shared__ double part[NT / 64];
   double s = w.sums[threadIdx.x];
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
@@ -132,23 +153,11 @@ __global__ __launch_bounds__(NT) void ortho_pack_kernel(const Call* __restrict__
   __syncthreads();
   s = (part[0] + part[1]) + (part[2] + part[3]);
   const float inv = (float)((double)SX / (sqrt(s) + (double)p.eps));
-  const int me = blockIdx.x - q.first[PACKS][k], across = (w.tall ? w.n : w.m) / 64;       // tiles of the source's rows
-  const int64_t r0 = me / across * 64, c0 = me % across * 64;
-  // the source's orientation: lying or standing plane pair
-  half_t* same = w.tall ? w.xt[0] : w.xn;
-  half_t* other = w.tall ? w.xn : w.xt[0];
-  const int64_t ld_same = w.tall ? w.n : w.m, ld_other = w.tall ? w.m : w.n;
-  for (int i = threadIdx.x; i < 4096; i += NT) {
+#pragma unroll
+  for (int u = 0; u < 4096 / NT; ++u) {
+    const int i = threadIdx.x + u * NT;
     const int64_t r = r0 + i / 64, c = c0 + i % 64;
-    float v = 0.0f;
-    if (r < t.rows && c < t.cols) {
-      v = src_at(p, t, r, c);
-      if (t.mom) {
-        const float mv = t.mom[r * t.cols + c];
-        v = p.nesterov ? fmaf(p.momentum, mv, v) : mv;
-      }
-      v *= inv;
-    }
+    const float v = x[u] * inv;
     tile[i / 64][i % 64] = v;
     half_t h, l;
     split(v, h, l);
