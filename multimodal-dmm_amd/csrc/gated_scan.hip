@@ -500,7 +500,7 @@ int launch(const mdmm_gated_scan_t* a, const Plan& pl, bool bwd, hipStream_t s) 
 
 int run(const mdmm_gated_scan_t* a, bool bwd, hipStream_t s) {
   const Plan pl = plan(a);
-  if (pl.wgs > 0x7fffffff) return MDMM_E_LIMIT;
+  if (pl.wgs > (1 << 22)) return MDMM_E_LIMIT;         // (a grid's threads fit 32 bits)
   if (pl.splits > 1 && !a->ws) return MDMM_E_ARG;
   if (!a->gates_bf16) return launch<float, float>(a, pl, bwd, s);
   return a->h_bf16 ? launch<__bf16, __bf16>(a, pl, bwd, s) : launch<__bf16, float>(a, pl, bwd, s);

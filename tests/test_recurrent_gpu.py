@@ -170,6 +170,56 @@ def test_scan_strided_inputs_and_float_mask():
 
 
 @gpu
+def test_scan_over_sequences_2_gib_apart():
+    """Gates whose sequences lie 2 GiB apart (a step's offsets do not fit 31 bits) against a compact copy."""
+    gen = torch.Generator().manual_seed(14)
+    T, B, H = 70, 3, 6
+    far = 2 ** 29
+    room = torch.empty((B - 1) * far + T * 2 * H, device='cuda')
+    wide = room.as_strided((T, B, 2 * H), (2 * H, far, 1))
+    wide.copy_(make(gen, T, B, 2 * H))
+    g = make(gen, T, B, H).cuda()
+    for reverse in (False, True):
+        outs = []
+        for x in (wide.detach(), wide.contiguous()):
+            x.requires_grad_(True)
+            h, last = ops.gated_scan(x, reverse=reverse)
+            outs.append((h, last, torch.autograd.grad(h, x, g)[0]))
+        for a, b in zip(*outs):
+            assert torch.equal(a, b)
+
+
+@gpu
+def test_scan_past_32_bits():
+    """4.8e9 gates: the last steps of the whole scan against a scan of them alone from the state in front of them.  The two
+    group their steps differently: 1e-5 covers fp32 sums of values of order one, the bf16 outputs a rounding each."""
+    T, B, H, k = 9200, 512, 512, 37
+    gates = torch.empty(T, B, 2 * H, device='cuda', dtype=BF16)
+    for i in range(0, T, 400):
+        gates[i:i + 400].normal_()
+    assert gates.numel() > 2 ** 32
+    with torch.no_grad():
+        h, last = ops.gated_scan(gates)
+        _, state = ops.gated_scan(gates[:T - k])
+        tail, end = ops.gated_scan(gates[T - k:], state)
+    assert (last - end).abs().max() <= 1e-5
+    assert ((h[T - k:].float() - tail.float()).abs() <= 1e-5 + 2 * HALF[BF16] * tail.float().abs()).all()
+
+
+@gpu
+def test_norm_past_32_bits():
+    rows, H = 3600000, 1200
+    x = torch.empty(rows, H, device='cuda', dtype=BF16)
+    for i in range(0, rows, 200000):
+        x[i:i + 200000].normal_()
+    assert x.numel() > 2 ** 32
+    w = torch.linspace(0.5, 1.5, H, device='cuda')
+    with torch.no_grad():
+        n = ops.rms_norm(x, w)
+        assert torch.equal(n[-1000:], ops.rms_norm(x[-1000:], w)) and torch.equal(n[:1000], ops.rms_norm(x[:1000], w))
+
+
+@gpu
 @pytest.mark.parametrize('shape', [(0, 3, 8), (4, 0, 8), (4, 3, 0)])
 def test_scan_empty(shape):
     T, B, H = shape
