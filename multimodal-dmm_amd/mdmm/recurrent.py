@@ -481,20 +481,46 @@ def block_norm(y, residual, weight, gate=None, scale=None, next_weight=None, eps
 
 # ---- the layer ---------------------------------------------------------------------------------------------------
 
+def _up4(n):
+    return (n + 3) & ~3
+
+
+def _fill_block(p, proj, rows, h, w, s, w_next, eps):
+    """The norm's struct on the states at address h and the gate's columns of proj -> a copy to hold until the launch, where
+    proj's rows have no one stride."""
+    H = rows.shape[1]
+    _fill_norm(p, None, None, rows, w, s, w_next, proj.dtype, eps)
+    flat = proj if proj.is_contiguous() else _as_rows(proj, 3 * H)
+    p.y, p.y_st = h, H
+    p.gate, p.gate_st = flat.data_ptr() + 2 * H * flat.element_size(), 3 * H if flat is proj else _row(flat)
+    return flat
+
+
 def _run_block(proj, rows, h0, w, s, w_next, mask, reverse, eps, shape, keep=False):
-    """-> (out, n or None, h_last, states kept for the backward pass, h)."""
+    """-> (out, n or None, h_last, one buffer: the states of every step, then those kept for the backward pass)."""
     T, B, H = shape
     dev = proj.device
-    h = torch.empty((T, B, H), device=dev, dtype=torch.float32)
+    out = torch.empty(shape, device=dev, dtype=rows.dtype)
+    n = torch.empty(shape, device=dev, dtype=proj.dtype) if w_next is not None else None
+    if out.numel() == 0:
+        return out, n, _no_steps_last(h0, B, H, dev), None
+    last = torch.empty((B, H), device=dev, dtype=torch.float32)
     a, p = native.GatedScan(), native.BlockNorm()
-    gate = _as_rows(proj, 3 * H)[:, 2 * H:]              # (a copy where proj's rows have no one stride: held until the launch)
-    out, n = _norm_forward(p, h.view(-1, H), gate, rows, w, s, w_next, proj.dtype, eps, shape)
-    if h.numel() == 0:
-        return out, n, _no_steps_last(h0, B, H, dev), None, h
-    last, states, ws = _scan_forward(a, proj, H, h0, mask, reverse, h, keep)
+    _fill_scan(a, proj, H, h0, mask, reverse)
+    kept = _size('mdmm_gated_scan_states', a) if keep else 0
+    size = _up4(T * B * H)
+    states = torch.empty(size + kept, device=dev, dtype=torch.float32)
+    a.h, a.h_last = states.data_ptr(), last.data_ptr()
+    if kept:
+        a.states = a.h + 4 * size
+    flat = _fill_block(p, proj, rows, a.h, w, s, w_next, eps)
+    p.out, p.out_st = out.data_ptr(), H
+    if n is not None:
+        p.n, p.n_st = n.data_ptr(), H
+    ws = _scan_ws(a, 0, dev)
     _launch('mdmm_gated_block_fwd', 'gated_block_fwd', a, p)
-    del ws
-    return out, n, last, states, h
+    del ws, flat
+    return out, n, last, states
 
 
 class _GatedBlockFn(torch.autograd.Function):
@@ -505,15 +531,15 @@ class _GatedBlockFn(torch.autograd.Function):
     def forward(ctx, proj, res, h0, w, s, w_next, mask, reverse, eps):
         ctx.set_materialize_grads(False)
         rows = _as_rows(res, res.shape[-1])
-        out, n, last, states, h = _run_block(proj, rows, h0, w, s, w_next, mask, reverse, eps, res.shape, True)
-        ctx.save_for_backward(proj, rows, h0, w, s, w_next, mask, states, h)
+        out, n, last, states = _run_block(proj, rows, h0, w, s, w_next, mask, reverse, eps, res.shape, True)
+        ctx.save_for_backward(proj, rows, h0, w, s, w_next, mask, states)
         ctx.reverse, ctx.eps = reverse, eps
         return (out, last) if n is None else (out, n, last)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        proj, res, h0, w, s, w_next, mask, states, h = ctx.saved_tensors
+        proj, res, h0, w, s, w_next, mask, states = ctx.saved_tensors
         g_out, g_last = grads[0], grads[-1]
         g_n = grads[1] if len(grads) == 3 else None
         need = ctx.needs_input_grad                    # proj, res, h0, w, s, w_next
@@ -525,28 +551,58 @@ class _GatedBlockFn(torch.autograd.Function):
         g_n = None if g_n is None else _as_rows(g_n, H)
         g_last = None if g_last is None else g_last.contiguous()
         g_x = torch.empty((T, B, H3), device=dev, dtype=proj.dtype)
+        through = g_out is not None or g_n is not None
+        sums = [torch.empty(H, device=dev, dtype=torch.float32) if k and through else None for k in need[3:6]]
+        d_res = None
+        if need[1]:                                    # (without a next norm it is g_out itself)
+            d_res = torch.empty((T, B, H), device=dev, dtype=res.dtype) if g_n is not None else \
+                None if g_out is None else g_out.reshape(T, B, H)
+        if g_x.numel() == 0:
+            return (g_x, d_res, _no_steps_grad(h0, g_last if T == 0 else None),
+                    *(None if t is None else t.zero_() for t in sums), None, None, None)
         a, p = native.GatedScan(), native.BlockNorm()
-        d_res = d_h = ws = hold = None
-        sums = [None, None, None]
-        if g_out is None and g_n is None:
-            p.rows, p.H = T * B, H
+        p.rows, p.H = T * B, H
+        _fill_scan(a, proj, H, h0, mask, ctx.reverse)
+        size = _up4(T * B * H)
+        base = states.data_ptr()
+        if states.numel() > size:
+            a.states = base + 4 * size
+        a.g_last = ops._ptr(g_last)
+        a.g_gates, a.g_gates_st, a.g_gates_sb = g_x.data_ptr(), B * H3, H3
+        flat = _fill_block(p, proj, res, base, w, s, w_next, ctx.eps) if through else None
+        # one scratch: the states' gradient | the norms' slabs | each sequence's gradient of h0 | the scan's splits
+        slabs = _size('mdmm_block_norm_ws', p) if through else 0
+        per = _up4(B * H) if h0 is not None and need[2] else 0
+        splits = _size('mdmm_gated_scan_ws', a, 1)
+        lead = size if through else 0
+        scratch = torch.empty(lead + _up4(slabs) + per + splits, device=dev, dtype=torch.float32)
+        at = scratch.data_ptr()
+        g0 = None
+        if through:
+            if g_out is not None:
+                p.g_out, p.g_out_st = g_out.data_ptr(), _row(g_out)
+            if g_n is not None:
+                p.g_n, p.g_n_st = g_n.data_ptr(), _row(g_n)
+                if d_res is not None:
+                    p.d_res, p.d_res_st = d_res.data_ptr(), H
+            p.d_y, p.d_y_st, p.ws = at, H, at + 4 * lead
+            p.d_gate, p.d_gate_st = g_x.data_ptr() + 2 * H * g_x.element_size(), H3
+            p.d_w, p.d_scale, p.d_w_next = [ops._ptr(t) for t in sums]
+            a.g_h = at
+        else:
             g_x[..., 2 * H:].zero_()
-        else:
-            d_h = torch.empty((T * B, H), device=dev, dtype=torch.float32)
-            d_res = torch.empty((T * B, H), device=dev, dtype=res.dtype) if need[1] and g_n is not None else None
-            gate = _as_rows(proj, H3)[:, 2 * H:]         # (held until the launch, as in the forward pass)
-            sums, ws = _norm_backward(p, h.view(-1, H), gate, res, w, s, w_next, proj.dtype, ctx.eps, g_out, g_n, d_h,
-                                      g_x.view(-1, H3)[:, 2 * H:], d_res, need[3:6])
-            if need[1] and d_res is None:
-                d_res = g_out
-        if h.numel() == 0:
-            g0 = _no_steps_grad(h0, g_last if T == 0 else None)
-        else:
-            g0, hold = _scan_backward(a, proj, H, h0, mask, ctx.reverse, torch.float32, states, d_h, g_last, g_x,
-                                      h0 is not None and need[2])
-            _launch('mdmm_gated_block_bwd', 'gated_block_bwd', a, p)
-        del ws, hold
-        return (g_x, None if d_res is None else d_res.reshape(T, B, H), g0, *sums, None, None, None)
+        at += 4 * (lead + _up4(slabs))
+        if per:
+            g0 = torch.empty(h0.shape, device=dev, dtype=torch.float32)
+            if h0.dim() == 1:
+                a.g_h0, a.g_h0_sum = at, g0.data_ptr()
+            else:
+                a.g_h0 = g0.data_ptr()
+        if splits:
+            a.ws = at + 4 * per
+        _launch('mdmm_gated_block_bwd', 'gated_block_bwd', a, p)
+        del scratch, flat
+        return (g_x, d_res, g0, *sums, None, None, None)
 
 
 def _check_block(name, proj, residual, lead):
