@@ -1161,8 +1161,9 @@ int mdmm_gated_block_step(const mdmm_gated_scan_t* scan, const mdmm_block_norm_t
  *   dst = (1 - lr decay) dst - lr gain X     (update 1: one optimizer step on the fp32 parameter dst; lr = *lr_dev, or
  *                                             the argument where lr_dev is NULL)
  * M = src (rows, cols) with row stride src_ld, fp32 or bf16 (src_bf16); with mom (contiguous fp32 rows x cols): first
- * mom = momentum mom + src, then M = mom, or src + momentum mom with nesterov.  No two matrices' mom or dst overlap.  dst has src's shape, its own row stride,
- * and type (dst_bf16, update 0 only).  ws: mdmm_ortho_ws() bytes, 256-byte aligned.
+ * mom = momentum mom + src, then M = mom, or src + momentum mom with nesterov.  No two matrices' mom or dst overlap.  dst has
+ * src's shape, its own row stride, and type (dst_bf16, update 0 only).  ws: mdmm_ortho_ws() bytes, 256-byte aligned.
+ * ca, cb, cc must keep the singular values of X below 2 and those of P below 16, where the kernels' number format ends.
  * --------------------------------------------------------------------------------- */
 #define MDMM_ORTHO_MAX 24
 typedef struct mdmm_ortho_item {

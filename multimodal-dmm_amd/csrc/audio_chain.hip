@@ -124,8 +124,8 @@ __device__ __forceinline__ float lazy_apply(const LazyTab* t, int q, float g, fl
   const float gm = (relu && fmaf(y, a.x, a.y) <= 0.f) ? 0.f : g;
   return a.x * (gm - m.x - xh * m.y);
 }
-// the layer's weights into LDS in the order the two products' PACKED multiply-adds take them (v_pk_fma_f32: two
-// neighbouring output channels per instruction, their weights one aligned 8-byte operand):
+// the layer's weights into LDS in the order the two products take them (two neighbouring output channels at a time, their
+// weights one aligned 8-byte read):
 //   wu[cs][cb / 2][slot][cb % 2], slot 0 = tap 1 (even outputs), 1 = tap 0, 2 = tap 2 (odd outputs)      (up_core)
 //   wd[cb][cs / 2][tap][cs % 2]                                                                        (down_core)
 template <typename SH>

@@ -2,9 +2,13 @@
 //   u = y r w, r = rsqrt(mean(y^2) + eps);  out = res + s silu(g) u;  n = out r' w'
 // Backward, with d = g_out + r' (q - out r'^2 mean(q out)), q = g_n w' :  d_res = d, d_s = sum d silu(g) u,
 // d_g = d s u silu'(g), p = d s silu(g):  d_w = sum p y r,  d_y = r (p w - y r mean(p w y r)),  d_w' = sum g_n out r'.
-// A row is held in registers by TPR threads (NV pieces of VEC columns each) from its loads to its stores, so every tensor
-// passes once; the three column sums are kept per thread over all rows of a workgroup and leave as one slab a workgroup,
-// which fold_kernel adds up in a fixed order.
+// Bound by HBM: a row is held in registers from its loads to its stores, so every tensor passes once, and the next row's
+// loads are in flight behind the present row's sums.  Up to 256 columns a row is one wave's (4 a workgroup, no barrier in a
+// sum); a longer one a workgroup's, 4 columns a thread (8 from 2049 on), whose waves meet in LDS once a sum.  Rows that are
+// not aligned to 4 elements take columns one by one.  The three column sums of the backward pass stay in a thread over all
+// of its rows and leave as one slab a workgroup; norm_fold_kernel adds the slabs up in a fixed order, without atomics.
+// 65536 x 1280 in bf16: forward 159 us (840 MB, 5.3 TB/s, a copy's rate), backward 312 (1.34 GB, 4.3 TB/s: three sums a
+// row between its loads and its last store), fold 7.  A row or two: the launch, 4 to 5 us.
 #include "gated.h"
 
 namespace mdmm {

@@ -10,6 +10,8 @@
 // tile's are used up.  Where the channels alone do not fill the chip, time is also split over workgroups: a first launch
 // composes each split (reading f, c once more; backward f, g), the second starts each split from the splits in front of it.
 // Nothing waits for another workgroup, and no sum is formed by atomics: results do not depend on the schedule.
+// 512 x 256 x 512 in bf16: forward 96 us (403 MB, 4.2 TB/s), backward 153 (672 MB, 4.4 TB/s).  20011 x 3 x 200 in fp32, split:
+// 22 + 32 forward, 22 + 52 backward.
 #include "gated.h"
 
 namespace mdmm {
@@ -437,6 +439,7 @@ __global__ __launch_bounds__(1024) void scan_rows_kernel(const float* __restrict
 int check(const mdmm_gated_scan_t* a) {
   if (!a || a->T < 0 || a->B < 0 || a->H < 0) return MDMM_E_ARG;
   if (!a->gates_bf16 && a->h_bf16) return MDMM_E_ARG;
+  if (a->gates_sb < 0 || a->g_gates_sb < 0 || a->mask_sb < 0) return MDMM_E_ARG;         // (a negative offset: no channels)
   if (a->T > 0 && a->B > 0 && a->H > 0 && !a->gates) return MDMM_E_ARG;
   return 0;
 }

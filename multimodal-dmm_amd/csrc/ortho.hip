@@ -2,19 +2,23 @@
 // X <- ca X + P X with P = cb A + cc A A, A = X X^T.  X lies down (n rows <= m columns).
 //
 // The iteration multiplies a small singular value by up to ca a step (ca^5 = 485 over five), and a rounding of X with it, so
-// The iteration multiplies a small singular value by up to ca a step (ca^5 = 485 over five), and a rounding of X with it, so
 // bf16 operands are out; fp32 ones would run on the fp32 matrix instruction, a sixteenth of the fp16 one's rate.  Every
 // matrix is kept as two fp16 planes instead, s x = h + l with h = fp16(s x), l = fp16(s x - h): 22 to 23 bits.  s is as large
 // as the entries allow (X and A stay below 2: 2^14; P below 16: 2^12), so that l is a normal number down to entries of 1e-5
 // and below those wrong by 2e-12.  A product is h h' + h l' + l h': three fp16 matrix instructions, the dropped l l' 2^-23 of
-// a term, and three roundings of the fp32 sum for every 16 terms where the fp32 instruction has one for every two: the result
-// is nearer to 64 bits than fp32 products (1.1e-6 against 2.9e-6 at 2048 x 2048).  ca X is added in fp32.
+// a term: the result is nearer to 64 bits than fp32 products by the library (6e-7 against 2.9e-6 at 2048 x 2048).  ca X is
+// added in fp32.
 //
 // X is stored both ways (n x m for A, m x n for P X) so that every product runs over two operands' rows.  A row keeps 32
 // columns of h, then the same 32 of l: one cache line for a step of 32 (with the planes apart, each step took half lines and
 // two 2048 x 2048 products 142 us).  Tiles come straight into LDS, a step or more ahead, chunks of 16 bytes swapped within a
-// row so that the matrix instruction's reads meet all banks; neighbouring tiles go to one XCD, whose L2 then holds their rows.  A and P are symmetric: tiles above the diagonal only, stored twice.  Sizes
-// are rounded up to whole tiles with zeros, which every product keeps.  All matrices of a call share each launch.
+// row so that the matrix instruction's reads meet all banks; neighbouring tiles go to one XCD, whose L2 then holds their
+// rows.  A and P are symmetric: tiles at and above the diagonal only, stored twice.  Sizes are rounded up to whole tiles with
+// zeros, which every product keeps.  All matrices of a call share each launch.
+//
+// Large matrices are bound by feeding the matrix instruction: P X of two 2048 x 2048 takes 112 us (920 TFLOP/s of fp16, the
+// library's own fp16 product of that size 640), without its loads 78, without its matrix instructions 76.  Small ones are
+// bound by the seventeen launches of five steps, 8 to 12 us each.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "../../include/mdmm_hip.h"
@@ -23,6 +27,7 @@ namespace mdmm {
 namespace {
 
 constexpr int NT = 256, SUMS = 256;
+constexpr int FLUSH = 128;                        // columns of one sum inside the matrix instruction
 constexpr float SX = 16384.0f, SP = 4096.0f;      // scales of X and A, and of P
 typedef _Float16 half_t;
 typedef half_t half4 __attribute__((ext_vector_type(4)));
@@ -290,50 +295,60 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
       el[g] = *(const half4*)(d + 32);
     }
   }
-  f32x16 acc[C::TI][C::TJ] = {};
+  f32x16 sum[C::TI][C::TJ] = {};
 #pragma unroll
   for (int s = 0; s < C::ST - 1; ++s)
     if (s < nk) load(s);
-  for (int s = 0; s < nk; ++s) {
-    // buffer s has landed when no more than the loads of the buffers behind it are in flight
-    if (s + C::ST - 2 < nk) wait_loads<(C::ST - 2) * C::LOADS>();
-    else wait_loads<0>();
-    __builtin_amdgcn_s_barrier();             // (every wave's share; and all are done with the buffer that is filled next)
-    asm volatile("" ::: "memory");
-    if (s + C::ST - 1 < nk) load((s + C::ST - 1) % C::ST);
-    const half_t* A = lds + s % C::ST * C::HALVES;
-    const half_t* B = A + 2 * C::BM * C::BK;
+  // FLUSH columns at a time, the pieces added by the vector unit: the matrix instruction does not round its sum to nearest,
+  // and over a diagonal of A (1662 positive terms) that came to 4e-6 (6e-7 with pieces)
+  for (int from_s = 0; from_s < nk; from_s += FLUSH / C::BK) {
+    const int to_s = from_s + FLUSH / C::BK < nk ? from_s + FLUSH / C::BK : nk;
+    f32x16 acc[C::TI][C::TJ] = {};
+    for (int s = from_s; s < to_s; ++s) {
+      // buffer s has landed when no more than the loads of the buffers behind it are in flight
+      if (s + C::ST - 2 < nk) wait_loads<(C::ST - 2) * C::LOADS>();
+      else wait_loads<0>();
+      __builtin_amdgcn_s_barrier();             // (every wave's share; and all are done with the buffer that is filled next)
+      asm volatile("" ::: "memory");
+      if (s + C::ST - 1 < nk) load((s + C::ST - 1) % C::ST);
+      const half_t* A = lds + s % C::ST * C::HALVES;
+      const half_t* B = A + 2 * C::BM * C::BK;
 #pragma unroll
-    for (int kk = 0; kk < C::BK / 16; ++kk) {
-      half8 ah[C::TI], al[C::TI], bh[C::TJ], bl[C::TJ];
-      // chunk of h; l's is 4 further (columns kk 16 + (lane / 32) 8 on, of each 32 columns' pair of half lines)
-      const int c = kk / 2 * 8 + kk % 2 * 2 + (lane >> 5);
+      for (int kk = 0; kk < C::BK / 16; ++kk) {
+        half8 ah[C::TI], al[C::TI], bh[C::TJ], bl[C::TJ];
+        // chunk of h; l's is 4 further (columns kk 16 + (lane / 32) 8 on, of each 32 columns' pair of half lines)
+        const int c = kk / 2 * 8 + kk % 2 * 2 + (lane >> 5);
 #pragma unroll
-      for (int t = 0; t < C::TI; ++t) {
-        const int row = wi + t * 32 + (lane & 31), z = row / (16 / C::CPR) % C::CPR;
-        ah[t] = *(const half8*)(A + row * C::BK * 2 + (c ^ z) * 8);
-        al[t] = *(const half8*)(A + row * C::BK * 2 + ((c + 4) ^ z) * 8);
+        for (int t = 0; t < C::TI; ++t) {
+          const int row = wi + t * 32 + (lane & 31), z = row / (16 / C::CPR) % C::CPR;
+          ah[t] = *(const half8*)(A + row * C::BK * 2 + (c ^ z) * 8);
+          al[t] = *(const half8*)(A + row * C::BK * 2 + ((c + 4) ^ z) * 8);
+        }
+#pragma unroll
+        for (int t = 0; t < C::TJ; ++t) {
+          const int row = wj + t * 32 + (lane & 31), z = row / (16 / C::CPR) % C::CPR;
+          bh[t] = *(const half8*)(B + row * C::BK * 2 + (c ^ z) * 8);
+          bl[t] = *(const half8*)(B + row * C::BK * 2 + ((c + 4) ^ z) * 8);
+        }
+        // (the three products of a piece apart from each other: none waits for the one before)
+#pragma unroll
+        for (int x = 0; x < C::TI; ++x)
+#pragma unroll
+          for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bl[y], acc[x][y], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < C::TI; ++x)
+#pragma unroll
+          for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[x], bh[y], acc[x][y], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < C::TI; ++x)
+#pragma unroll
+          for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bh[y], acc[x][y], 0, 0, 0);
       }
-#pragma unroll
-      for (int t = 0; t < C::TJ; ++t) {
-        const int row = wj + t * 32 + (lane & 31), z = row / (16 / C::CPR) % C::CPR;
-        bh[t] = *(const half8*)(B + row * C::BK * 2 + (c ^ z) * 8);
-        bl[t] = *(const half8*)(B + row * C::BK * 2 + ((c + 4) ^ z) * 8);
-      }
-      // (the three products of a piece apart from each other: none waits for the one before)
-#pragma unroll
-      for (int x = 0; x < C::TI; ++x)
-#pragma unroll
-        for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bl[y], acc[x][y], 0, 0, 0);
-#pragma unroll
-      for (int x = 0; x < C::TI; ++x)
-#pragma unroll
-        for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[x], bh[y], acc[x][y], 0, 0, 0);
-#pragma unroll
-      for (int x = 0; x < C::TI; ++x)
-#pragma unroll
-        for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bh[y], acc[x][y], 0, 0, 0);
     }
+#pragma unroll
+    for (int x = 0; x < C::TI; ++x)
+#pragma unroll
+      for (int y = 0; y < C::TJ; ++y) sum[x][y] += acc[x][y];
   }
   // v: the result in its planes' scale
   const mdmm_ortho_t& p = call->p;
@@ -352,7 +367,7 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
         const int64_t i = i0 + wi + x * 32 + 8 * g + 4 * (lane >> 5), j = j0 + wj + y * 32 + (lane & 31);
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[x][y][4 * g + e];
+        for (int e = 0; e < 4; ++e) v[e] = sum[x][y][4 * g + e];
         half4 h, l;
         if constexpr (EARLY) {
           h = eh[g];

@@ -224,8 +224,8 @@ class FlatMuon(torch.optim.Optimizer):
                  adam_lr=1e-3, betas=(0.9, 0.999), eps=1e-8, adam_weight_decay=0.0):
         if not bucket.flat.is_cuda:
             raise RuntimeError('FlatMuon runs on the GPU (mdmm_ortho, mdmm_adam_flat)')
-        if not 0.0 <= momentum < 1.0 or int(ns_steps) != ns_steps or ns_steps < 0:
-            raise ValueError('FlatMuon: momentum %r in [0, 1), a number of steps, got %r' % (momentum, ns_steps))
+        if not 0.0 <= momentum < 1.0 or int(ns_steps) != ns_steps or not 0 <= ns_steps <= 1000:
+            raise ValueError('FlatMuon: momentum %r in [0, 1), a number of steps up to 1000, got %r' % (momentum, ns_steps))
         for p in bucket.params:
             if p.dtype != torch.float32 or not p.is_contiguous():
                 raise ValueError('FlatMuon: contiguous fp32 parameters')

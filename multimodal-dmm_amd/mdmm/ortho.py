@@ -4,11 +4,37 @@ import ctypes as C
 
 import torch
 
-from . import native, ops
+from . import native
 
 # X <- a X + (b A + c A^2) X, A = X X^T: these take every singular value in (0, 1] to about 1 (between 0.7 and 1.2) in five
 # steps, the slope a at 0 as steep as that allows -- the values of the Muon optimizer's published description
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+# the kernels' fp16 plane pairs hold X and A up to 4, P = b A + c A^2 up to 16; a step count that no iteration needs
+MAX_X, MAX_P, MAX_STEPS = 1.95, 15.5, 1000
+
+
+def _bounded(steps, a, b, c):
+    """Whether the singular values and P's, from (0, 1] on, stay within what the kernels hold."""
+    top = 1.0
+    for _ in range(steps):
+        ends = [top * top]                          # u = s^2: the end, p's slope and P's slope at zero
+        if c:
+            ends.append(-b / (2.0 * c))
+            root = 9.0 * b * b - 20.0 * a * c
+            if root >= 0.0:
+                ends += [(-3.0 * b + sign * root ** 0.5) / (10.0 * c) for sign in (1.0, -1.0)]
+        elif b:
+            ends.append(-a / (3.0 * b))
+        ends = [u for u in ends if 0.0 <= u <= top * top]
+        new = max([u ** 0.5 * abs(a + b * u + c * u * u) for u in ends])
+        if not (top <= MAX_X and max([abs(b * u + c * u * u) for u in ends]) <= MAX_P):
+            return False
+        if not new > top:
+            return new == new
+        top = new
+    return True
 
 
 def as_matrix(t):
@@ -43,12 +69,17 @@ def orthogonalise(mats, steps=5, eps=1e-7, coefficients=COEFFICIENTS):
     Newton-Schulz steps in fp32 on M / (|M|_F + eps); every matrix of the list shares the launches.
 
     mats: fp32 or bf16 tensors of two or more dimensions (more than two: leading dimension x the rest), either side the
-    longer.  -> a list of contiguous tensors of their shapes and types.  No gradient."""
+    longer, at most 65536.  coefficients: (a, b, c) of X <- a X + (b A + c A^2) X, A = X X^T, such that singular values in
+    (0, 1] stay below 1.95 (refused otherwise).  -> a list of contiguous tensors of their shapes and types.  No gradient."""
     mats = [mats] if torch.is_tensor(mats) else list(mats)
-    if int(steps) != steps or steps < 0:
-        raise ValueError('orthogonalise: a number of steps, got %r' % (steps,))
+    if int(steps) != steps or not 0 <= steps <= MAX_STEPS:
+        raise ValueError('orthogonalise: a number of steps, 0 to %d, got %r' % (MAX_STEPS, steps))
     if len(coefficients) != 3:
         raise ValueError('orthogonalise: three coefficients, got %r' % (coefficients,))
+    coefficients = tuple(float(c) for c in coefficients)
+    if coefficients != COEFFICIENTS and not _bounded(int(steps), *coefficients):
+        raise ValueError('orthogonalise: singular values must stay below %g and those of b A + c A^2 below %g, with %r they do not'
+                         % (MAX_X, MAX_P, coefficients))
     if not mats:
         return []
     for m in mats:
@@ -74,5 +105,8 @@ def orthogonalise(mats, steps=5, eps=1e-7, coefficients=COEFFICIENTS):
                     items.append((src, None, as_matrix(o), 1.0))
             if items:
                 bf = dtype == torch.bfloat16
-                launch(items, int(steps), float(eps), tuple(float(c) for c in coefficients), bf, bf, device=dev)
+                launch(items, int(steps), float(eps), coefficients, bf, bf, device=dev)
     return outs
+
+
+from . import ops  # noqa: E402  (last: ops re-exports this module's functions, whichever of the two is imported first)

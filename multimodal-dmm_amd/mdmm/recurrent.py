@@ -15,7 +15,7 @@ import ctypes as C
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import native, ops
+from . import native
 
 _TYPES = (torch.float32, torch.bfloat16)
 
@@ -93,6 +93,11 @@ def _mask_bytes(name, mask, lead):
     if tuple(mask.shape) != tuple(lead):
         raise ValueError('%s: mask must be %s, got %s' % (name, tuple(lead), tuple(mask.shape)))
     return mask if mask.dtype in (torch.bool, torch.uint8) else mask.detach() != 0
+
+
+def _check_sizes(name, *sizes):
+    if max(sizes) > 2 ** 31 - 1:
+        raise ValueError('%s: dimensions below 2^31, got %s' % (name, sizes))
 
 
 def _unit_cols(t):
@@ -235,6 +240,7 @@ def gated_scan(gates, h0=None, mask=None, reverse=False):
         raise ValueError('gated_scan: gates must be (T, B, 2H), got %s' % (tuple(gates.shape),))
     _check_type('gated_scan', gates)
     T, B, H2 = gates.shape
+    _check_sizes('gated_scan', T, B, H2)
     h0, mask = _check_h0('gated_scan', h0, B, H2 // 2), _mask_bytes('gated_scan', mask, (T, B))
     dev = _check_device('gated_scan', gates, h0, mask)
     gates, reverse = _unit_cols(gates), bool(reverse)
@@ -266,6 +272,7 @@ def gated_scan_step(gates, state, mask=None, new_state=None):
         raise ValueError('gated_scan_step: gates must be (B, 2H), got %s' % (tuple(gates.shape),))
     _check_type('gated_scan_step', gates)
     B, H = gates.shape[0], gates.shape[1] // 2
+    _check_sizes('gated_scan_step', B, 2 * H)
     mask = _mask_bytes('gated_scan_step', mask, (B,))
     _no_grad_only('gated_scan_step', gates, state)
     _check_state('gated_scan_step', state, new_state, B, H)
@@ -612,6 +619,7 @@ def _check_block(name, proj, residual, lead):
                          % (name, tuple(proj.shape), '(T, B, 3H)' if lead == 2 else '(B, 3H)', tuple(residual.shape)))
     _check_type(name, proj, residual)
     _check_width(name, H)
+    _check_sizes(name, *residual.shape)
     _combo(name, torch.float32, proj.dtype, residual.dtype)
     return H
 
@@ -665,3 +673,6 @@ def _block_step(proj, residual, state, w, s, w_next, mask, eps, new_state):
         _fill_step(a, proj, H, state, mask, new_state)
         _launch('mdmm_gated_block_step', 'gated_block_step', a, p)
     return (out, new_state) if n is None else (out, n, new_state)
+
+
+from . import ops  # noqa: E402  (last: ops re-exports this module's functions, whichever of the two is imported first)

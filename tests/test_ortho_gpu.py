@@ -166,3 +166,39 @@ def test_no_cpu_fallback():
     assert ops.orthogonalise([]) == []
     with pytest.raises(native.MdmmError):
         ops.orthogonalise([torch.zeros(4, 4)])
+
+
+@gpu
+@pytest.mark.parametrize('coefficients', [(1.5, -0.5, 0.0), (2.0, -1.5, 0.5)])
+def test_other_coefficients(coefficients):
+    """Polynomials that map [0, 1] to itself with slopes up to a there: the module's first bound with their own G."""
+    a, b, c = coefficients
+    gen = torch.Generator().manual_seed(7)
+    m = torch.randn(70, 130, generator=gen)
+    x = m.double() / (m.double().norm() + 1e-7)
+    bound = 0.0
+    for k in range(6):
+        bound = a * bound + 2 * (a + 2 * abs(b) + 3 * abs(c)) * U * math.sqrt(130) * float(x.norm())
+        if k < 5:
+            g = x @ x.t()
+            x = a * x + (b * g + c * (g @ g)) @ x
+    got = ops.orthogonalise([m.cuda()], coefficients=coefficients)[0].cpu().double()
+    assert float((got - x).norm()) <= bound
+
+
+@pytest.mark.parametrize('call', [
+    lambda: ops.orthogonalise([torch.zeros(5, 5)], steps=1001),
+    lambda: ops.orthogonalise([torch.zeros(5, 5)], coefficients=(float('nan'), 0.0, 0.0)),
+    lambda: ops.orthogonalise([torch.zeros(5, 5)], coefficients=(4.0, 0.0, 0.0)),           # 4 after a step
+    lambda: ops.orthogonalise([torch.zeros(5, 5)], coefficients=(3.4445, -4.775, 2.6)),     # 1.27, then 3.2
+    lambda: ops.orthogonalise([torch.zeros(5, 5)], coefficients=(1.0, 0.0, 16.0)),          # P = 16 in the first step
+])
+def test_diverging_iterations_are_refused(call):
+    with pytest.raises(ValueError):
+        call()
+
+
+def test_bounded_iterations_are_not_refused():
+    for c in (ortho.COEFFICIENTS, (1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (1.875, -1.25, 0.375), (1.0, 0.0, 0.0), (0.0, 0.0, 0.0)):
+        with pytest.raises(native.MdmmError):         # (the device's refusal, which comes last)
+            ops.orthogonalise([torch.zeros(4, 4)], coefficients=c)

@@ -5,6 +5,10 @@ every step adds at most 8 u of the terms' absolute sum (a and k are formed to 4 
 for the products of a's that a scan over pieces forms), so e_t = a_t e_{t-1} + 8 u S_t with S_t = a_t S_{t-1} + k_t |c_t|;
 the adjoint the same way.  A stored tensor adds half a step of its type.
 """
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -632,3 +636,27 @@ def test_refusals(call):
 def test_no_cpu_fallback(call):
     with pytest.raises(native.MdmmError):
         call()
+
+
+@pytest.mark.parametrize('call', [
+    lambda: ops.gated_scan(Z(1, 1, 2).expand(2 ** 31, 1, 2)), lambda: ops.gated_scan_step(Z(1, 2).expand(2 ** 31, 2), Z(1, 1)),
+    lambda: ops.gated_block(Z(1, 1, 3).expand(2 ** 31, 1, 3), Z(1, 1, 1).expand(2 ** 31, 1, 1), None, Z(1))])
+def test_dimensions_past_32_bits_are_refused(call):
+    with pytest.raises(ValueError, match='2\\^31'):
+        call()
+
+
+def test_negative_batch_strides_are_refused_by_the_library():
+    for field in ('gates_sb', 'g_gates_sb', 'mask_sb'):
+        a = native.GatedScan()
+        a.T, a.B, a.H, a.gates = 3, 2, 4, 64
+        assert native.lib().mdmm_gated_scan_ws(a, 0) >= 0
+        setattr(a, field, -8)
+        assert native.lib().mdmm_gated_scan_ws(a, 0) < 0 and native.lib().mdmm_gated_scan_fwd(a, None) < 0
+
+
+@pytest.mark.parametrize('module', ['recurrent', 'ortho', 'ops'])
+def test_modules_import_in_any_order(module):
+    """Each as the first module of a process."""
+    subprocess.run([sys.executable, '-c', 'import mdmm.%s, mdmm.ops; mdmm.ops.gated_scan, mdmm.ops.orthogonalise' % module],
+                   check=True, env=dict(os.environ, PYTHONPATH=os.path.dirname(os.path.dirname(native.__file__))), timeout=300)
