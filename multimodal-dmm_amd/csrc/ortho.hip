@@ -296,59 +296,108 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
     }
   }
   f32x16 sum[C::TI][C::TJ] = {};
+  // a piece's operands in registers: chunk of h, l's is 4 further (columns kk 16 + (lane / 32) 8 on, of each 32 columns' pair
+  // of half lines)
+  struct Part { half8 ah[C::TI], al[C::TI], bh[C::TJ], bl[C::TJ]; };
+  auto read = [&](Part& f, int buf, int kk) {
+    const half_t* A = lds + buf * C::HALVES;
+    const half_t* B = A + 2 * C::BM * C::BK;
+    const int c = kk / 2 * 8 + kk % 2 * 2 + (lane >> 5);
 #pragma unroll
-  for (int s = 0; s < C::ST - 1; ++s)
-    if (s < nk) load(s);
-  // FLUSH columns at a time, the pieces added by the vector unit: the matrix instruction does not round its sum to nearest,
-  // and over a diagonal of A (1662 positive terms) that came to 4e-6 (6e-7 with pieces)
-  for (int from_s = 0; from_s < nk; from_s += FLUSH / C::BK) {
-    const int to_s = from_s + FLUSH / C::BK < nk ? from_s + FLUSH / C::BK : nk;
-    f32x16 acc[C::TI][C::TJ] = {};
-    for (int s = from_s; s < to_s; ++s) {
-      // buffer s has landed when no more than the loads of the buffers behind it are in flight
-      if (s + C::ST - 2 < nk) wait_loads<(C::ST - 2) * C::LOADS>();
-      else wait_loads<0>();
-      __builtin_amdgcn_s_barrier();             // (every wave's share; and all are done with the buffer that is filled next)
-      asm volatile("" ::: "memory");
-      if (s + C::ST - 1 < nk) load((s + C::ST - 1) % C::ST);
-      const half_t* A = lds + s % C::ST * C::HALVES;
-      const half_t* B = A + 2 * C::BM * C::BK;
-#pragma unroll
-      for (int kk = 0; kk < C::BK / 16; ++kk) {
-        half8 ah[C::TI], al[C::TI], bh[C::TJ], bl[C::TJ];
-        // chunk of h; l's is 4 further (columns kk 16 + (lane / 32) 8 on, of each 32 columns' pair of half lines)
-        const int c = kk / 2 * 8 + kk % 2 * 2 + (lane >> 5);
-#pragma unroll
-        for (int t = 0; t < C::TI; ++t) {
-          const int row = wi + t * 32 + (lane & 31), z = row / (16 / C::CPR) % C::CPR;
-          ah[t] = *(const half8*)(A + row * C::BK * 2 + (c ^ z) * 8);
-          al[t] = *(const half8*)(A + row * C::BK * 2 + ((c + 4) ^ z) * 8);
-        }
-#pragma unroll
-        for (int t = 0; t < C::TJ; ++t) {
-          const int row = wj + t * 32 + (lane & 31), z = row / (16 / C::CPR) % C::CPR;
-          bh[t] = *(const half8*)(B + row * C::BK * 2 + (c ^ z) * 8);
-          bl[t] = *(const half8*)(B + row * C::BK * 2 + ((c + 4) ^ z) * 8);
-        }
-        // (the three products of a piece apart from each other: none waits for the one before)
-#pragma unroll
-        for (int x = 0; x < C::TI; ++x)
-#pragma unroll
-          for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bl[y], acc[x][y], 0, 0, 0);
-#pragma unroll
-        for (int x = 0; x < C::TI; ++x)
-#pragma unroll
-          for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[x], bh[y], acc[x][y], 0, 0, 0);
-#pragma unroll
-        for (int x = 0; x < C::TI; ++x)
-#pragma unroll
-          for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[x], bh[y], acc[x][y], 0, 0, 0);
-      }
+    for (int t = 0; t < C::TI; ++t) {
+      const int row = wi + t * 32 + (lane & 31), z = row / (16 / C::CPR) % C::CPR;
+      f.ah[t] = *(const half8*)(A + row * C::BK * 2 + (c ^ z) * 8);
+      f.al[t] = *(const half8*)(A + row * C::BK * 2 + ((c + 4) ^ z) * 8);
     }
+#pragma unroll
+    for (int t = 0; t < C::TJ; ++t) {
+      const int row = wj + t * 32 + (lane & 31), z = row / (16 / C::CPR) % C::CPR;
+      f.bh[t] = *(const half8*)(B + row * C::BK * 2 + (c ^ z) * 8);
+      f.bl[t] = *(const half8*)(B + row * C::BK * 2 + ((c + 4) ^ z) * 8);
+    }
+  };
+  f32x16 acc[C::TI][C::TJ];
+  auto multiply = [&](const Part& f) {           // (the three products of a piece apart: none waits for the one before)
 #pragma unroll
     for (int x = 0; x < C::TI; ++x)
 #pragma unroll
-      for (int y = 0; y < C::TJ; ++y) sum[x][y] += acc[x][y];
+      for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[x], f.bl[y], acc[x][y], 0, 0, 0);
+#pragma unroll
+    for (int x = 0; x < C::TI; ++x)
+#pragma unroll
+      for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[x], f.bh[y], acc[x][y], 0, 0, 0);
+#pragma unroll
+    for (int x = 0; x < C::TI; ++x)
+#pragma unroll
+      for (int y = 0; y < C::TJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[x], f.bh[y], acc[x][y], 0, 0, 0);
+  };
+  // FLUSH columns at a time, the pieces added by the vector unit: the matrix instruction does not round its sum to nearest,
+  // and over a diagonal of A (1662 positive terms) that came to 4e-6 (6e-7 with pieces)
+  constexpr int RUN = FLUSH / C::BK;
+  if constexpr (C::TI * C::TJ == 1) {
+    // a wave alone on its SIMD, so a step's operands are read from LDS under the products of the step before.  At the barrier
+    // of step s every wave holds step s in registers: its buffer takes step s + ST
+    static_assert(C::BK == 32 && RUN % 2 == 0, "two pieces a step, two steps' registers in turn");
+    Part f[2][2];
+#pragma unroll
+    for (int s = 0; s < C::ST; ++s)
+      if (s < nk) load(s);
+    if (C::ST <= nk) wait_loads<(C::ST - 1) * C::LOADS>();
+    else wait_loads<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(f[0][0], 0, 0);
+    read(f[0][1], 0, 1);
+    for (int from_s = 0; from_s < nk; from_s += RUN) {
+      acc[0][0] = f32x16{};
+#pragma unroll
+      for (int u = 0; u < RUN; ++u) {
+        const int s = from_s + u;
+        if (s >= nk) break;
+        if (s + 1 < nk) {
+          // buffer s + 1 has landed when no more than the loads of the buffers behind it are in flight
+          if (s + C::ST - 1 < nk) wait_loads<(C::ST - 2) * C::LOADS>();
+          else wait_loads<0>();
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          if (s + C::ST < nk) load(s % C::ST);
+          read(f[(u + 1) & 1][0], (s + 1) % C::ST, 0);
+          read(f[(u + 1) & 1][1], (s + 1) % C::ST, 1);
+        }
+        multiply(f[u & 1][0]);
+        multiply(f[u & 1][1]);
+      }
+      sum[0][0] += acc[0][0];
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < C::ST - 1; ++s)
+      if (s < nk) load(s);
+    for (int from_s = 0; from_s < nk; from_s += RUN) {
+      const int to_s = from_s + RUN < nk ? from_s + RUN : nk;
+#pragma unroll
+      for (int x = 0; x < C::TI; ++x)
+#pragma unroll
+        for (int y = 0; y < C::TJ; ++y) acc[x][y] = f32x16{};
+      for (int s = from_s; s < to_s; ++s) {
+        // buffer s has landed when no more than the loads of the buffers behind it are in flight
+        if (s + C::ST - 2 < nk) wait_loads<(C::ST - 2) * C::LOADS>();
+        else wait_loads<0>();
+        __builtin_amdgcn_s_barrier();             // (every wave's share; and all are done with the buffer that is filled next)
+        asm volatile("" ::: "memory");
+        if (s + C::ST - 1 < nk) load((s + C::ST - 1) % C::ST);
+#pragma unroll
+        for (int kk = 0; kk < C::BK / 16; ++kk) {
+          Part f;
+          read(f, s % C::ST, kk);
+          multiply(f);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < C::TI; ++x)
+#pragma unroll
+        for (int y = 0; y < C::TJ; ++y) sum[x][y] += acc[x][y];
+    }
   }
   // v: the result in its planes' scale
   const mdmm_ortho_t& p = call->p;
