@@ -59,11 +59,10 @@ struct Item {               // one matrix's padded sizes and workspace
 enum { PACKS, GRAMS, POLYS, APPLIES, LISTS };
 struct Items {
   Item it[MDMM_ORTHO_MAX];
-  int32_t first[LISTS][MDMM_ORTHO_MAX + 1];       // first tile of each matrix in a launch
-  int32_t which[MDMM_ORTHO_MAX];                  // its place in the call
+  int32_t first[LISTS][MDMM_ORTHO_MAX + 1];       // first tile of each matrix in a launch (past the last one: INT32_MAX)
   int32_t n, reserved;
 };
-// What the launches of one size class share.  The first launch takes it as its argument and leaves it in the workspace; the
+// What the launches of one size class share (p.item: that class's matrices alone, in q.it's order).  The first launch takes it as its argument and leaves it in the workspace; the
 // others read it there: arguments live in host memory, where each of the dependent loads that find a tile's matrix would
 // wait for the bus
 struct Call {
@@ -72,11 +71,31 @@ struct Call {
 };
 static_assert(sizeof(Call) <= 3968, "a launch's arguments");
 
-// the matrix a tile belongs to: every lane looks at one matrix's end (one load where a search has four in a row)
+// A launch finds a tile's matrix in one round trip to memory: each lane loads one matrix's entries, at the same time as the
+// table of first tiles that tells which lane's are wanted (one after the other, 3 us more over the seventeen launches of eleven
+// small matrices)
 static_assert(MDMM_ORTHO_MAX <= 64, "a wave's lanes");
-__device__ __forceinline__ int find(const int32_t* first, int n, int tile) {
-  const int lane = threadIdx.x & 63;
-  return (int)__popcll(__ballot(lane < n && first[lane < n ? lane + 1 : 0] <= tile));
+template <class T> struct Entries {
+  unsigned v[sizeof(T) / 4];
+  __device__ __forceinline__ Entries(const T* table) {
+    const int lane = threadIdx.x & 63;
+    __builtin_memcpy(v, table + (lane < MDMM_ORTHO_MAX ? lane : 0), sizeof(T));
+  }
+  __device__ __forceinline__ T of(int k) const {
+    unsigned u[sizeof(T) / 4];
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 4); ++i) u[i] = __builtin_amdgcn_readlane(v[i], k);
+    T t;
+    __builtin_memcpy(&t, u, sizeof(T));
+    return t;
+  }
+};
+struct Found { int k, first; };          // the matrix that tile belongs to, its first tile
+__device__ __forceinline__ Found find(const int32_t* first, int tile) {
+  const int lane = threadIdx.x & 63, l = lane < MDMM_ORTHO_MAX ? lane : 0;
+  const int begin = first[l], end = first[l + 1];
+  const int k = (int)__popcll(__ballot(lane < MDMM_ORTHO_MAX && end <= tile));
+  return {k, __builtin_amdgcn_readlane(begin, k)};
 }
 
 __device__ __forceinline__ void split(float x, half_t& h, half_t& l) {       // x: already scaled
@@ -97,7 +116,7 @@ __device__ __forceinline__ float src_at(const mdmm_ortho_t& p, const mdmm_ortho_
 __global__ __launch_bounds__(NT) void ortho_sums_kernel(Call call, Call* keep) {
   const mdmm_ortho_t& p = call.p;
   const int k = blockIdx.y;
-  const mdmm_ortho_item_t& t = p.item[call.q.which[k]];
+  const mdmm_ortho_item_t& t = p.item[k];
   if (blockIdx.x == 0 && k == 0) {
     const __attribute__((address_space(4))) unsigned* args = (const __attribute__((address_space(4))) unsigned*)__builtin_amdgcn_kernarg_segment_ptr();
     for (int i = threadIdx.x; i < (int)(sizeof(Call) / 4); i += NT) ((unsigned*)keep)[i] = args[i];
@@ -128,10 +147,12 @@ __global__ __launch_bounds__(NT) void ortho_pack_kernel(const Call* __restrict__
   __shared__ float tile[64][65];
   const mdmm_ortho_t& p = call->p;
   const Items& q = call->q;
-  const int k = find(q.first[PACKS], q.n, blockIdx.x);
-  const mdmm_ortho_item_t& t = p.item[q.which[k]];
-  const Item& w = q.it[k];
-  const int me = blockIdx.x - q.first[PACKS][k], across = (w.tall ? w.n : w.m) / 64;       // tiles of the source's rows
+  const Entries<mdmm_ortho_item_t> ts(p.item);
+  const Entries<Item> ws(q.it);
+  const Found f = find(q.first[PACKS], blockIdx.x);
+  const mdmm_ortho_item_t t = ts.of(f.k);
+  const Item w = ws.of(f.k);
+  const int me = blockIdx.x - f.first, across = (w.tall ? w.n : w.m) / 64;       // tiles of the source's rows
   const int64_t r0 = me / across * 64, c0 = me % across * 64;
   // the source's orientation: lying or standing plane pair
   half_t* same = w.tall ? w.xt[0] : w.xn;
@@ -242,10 +263,18 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
   // consecutive workgroups go round the 8 XCDs: each XCD takes a run of consecutive tiles instead
   const int total = gridDim.x, xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
   const int me = xcd * each + (xcd < more ? xcd : more) + (blockIdx.x >> 3);
-  const int k = find(q.first[LIST], q.n, me);
-  const Item w = q.it[k];
+  const Entries<mdmm_ortho_item_t> ts(call->p.item);
+  const Entries<Item> ws(q.it);
+  const Found f = find(q.first[LIST], me);
+  const Item w = ws.of(f.k);
+  mdmm_ortho_item_t t = {};
+  if (MODE == LAST) t = ts.of(f.k);
+  const mdmm_ortho_t& p = call->p;
+  const float ca = p.ca, cb = p.cb, cc = p.cc, decay = p.decay;
+  const bool update = p.update, low = p.dst_bf16;
+  const float lr = MODE == LAST && update ? (p.lr_dev ? *p.lr_dev : p.lr) : 0.0f;
   const int n = w.n, J = PX ? w.m : n;
-  int tile = me - q.first[LIST][k], ti, tj, slice = 0;
+  int tile = me - f.first, ti, tj, slice = 0;
   if (PX) {
     ti = tile / (J / C::BN);
     tj = tile % (J / C::BN);
@@ -338,7 +367,7 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
     // a wave alone on its SIMD, so a step's operands are read from LDS under the products of the step before.  At the barrier
     // of step s every wave holds step s in registers: its buffer takes step s + ST
     static_assert(C::BK == 32 && RUN % 2 == 0, "two pieces a step, two steps' registers in turn");
-    Part f[2][2];
+    Part r[2][2];
 #pragma unroll
     for (int s = 0; s < C::ST; ++s)
       if (s < nk) load(s);
@@ -346,8 +375,8 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
     else wait_loads<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    read(f[0][0], 0, 0);
-    read(f[0][1], 0, 1);
+    read(r[0][0], 0, 0);
+    read(r[0][1], 0, 1);
     for (int from_s = 0; from_s < nk; from_s += RUN) {
       acc[0][0] = f32x16{};
 #pragma unroll
@@ -361,11 +390,11 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
           if (s + C::ST < nk) load(s % C::ST);
-          read(f[(u + 1) & 1][0], (s + 1) % C::ST, 0);
-          read(f[(u + 1) & 1][1], (s + 1) % C::ST, 1);
+          read(r[(u + 1) & 1][0], (s + 1) % C::ST, 0);
+          read(r[(u + 1) & 1][1], (s + 1) % C::ST, 1);
         }
-        multiply(f[u & 1][0]);
-        multiply(f[u & 1][1]);
+        multiply(r[u & 1][0]);
+        multiply(r[u & 1][1]);
       }
       sum[0][0] += acc[0][0];
     }
@@ -400,12 +429,7 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
     }
   }
   // v: the result in its planes' scale
-  const mdmm_ortho_t& p = call->p;
-  const mdmm_ortho_item_t t = p.item[q.which[k]];
-  const float ca = p.ca, cb = p.cb, cc = p.cc, decay = p.decay;
-  const bool update = p.update, low = p.dst_bf16;
   const int64_t nn = (int64_t)n * n, m = w.m;
-  const float lr = MODE == LAST && update ? (p.lr_dev ? *p.lr_dev : p.lr) : 0.0f;
 #pragma unroll
   for (int x = 0; x < C::TI; ++x)
 #pragma unroll
@@ -497,7 +521,7 @@ template <int BM, int BN> __global__ __launch_bounds__(NT) void ortho_fold_kerne
 __global__ __launch_bounds__(NT) void ortho_copy_kernel(const Call* __restrict__ call) {       // steps = 0: X itself
   const mdmm_ortho_t& p = call->p;
   const Items& q = call->q;
-  const mdmm_ortho_item_t& t = p.item[q.which[blockIdx.y]];
+  const mdmm_ortho_item_t& t = p.item[blockIdx.y];
   const Item& w = q.it[blockIdx.y];
   const int64_t total = (int64_t)t.rows * t.cols;
   for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)gridDim.x * NT) {
@@ -532,7 +556,7 @@ int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 bool large(const mdmm_ortho_item_t& t) { return (t.rows < t.cols ? t.rows : t.cols) > 384; }
 
 // the workspace: fills both size classes' lists (base NULL: sizes only), returns the bytes used
-int64_t lay_out(const mdmm_ortho_t* a, Items (&q)[2]) {
+int64_t lay_out(const mdmm_ortho_t* a, Items (&q)[2], mdmm_ortho_item_t (*items)[MDMM_ORTHO_MAX] = nullptr) {
   char* base = (char*)a->ws;
   int64_t off = 2 * up(sizeof(Call), 256);
   auto take = [&](int64_t bytes) { char* p = base + off; off += up(bytes, 256); return p; };
@@ -541,7 +565,7 @@ int64_t lay_out(const mdmm_ortho_t* a, Items (&q)[2]) {
     const mdmm_ortho_item_t& t = a->item[i];
     const bool big = large(t);
     Items& l = q[big];
-    l.which[l.n] = i;
+    if (items) items[big][l.n] = t;
     Item& w = l.it[l.n++];
     const int pad = big ? Large::BM : Small::BM, bk = big ? Large::BK : Small::BK;
     w.tall = t.rows > t.cols;
@@ -572,14 +596,15 @@ template <class F> int tiles(Items& q, int list, F count) {
     q.first[list][i] = (int32_t)total;
     total += count(q.it[i]);
   }
-  q.first[list][q.n] = (int32_t)total;
+  for (int i = q.n; i <= MDMM_ORTHO_MAX; ++i) q.first[list][i] = i == q.n ? (int32_t)total : INT32_MAX;
   return (int)total;
 }
 
-template <class C> void launch(const mdmm_ortho_t* a, const Items& items, Call* keep, hipStream_t s) {
+template <class C> void launch(const mdmm_ortho_t* a, const Items& items, const mdmm_ortho_item_t* mats, Call* keep, hipStream_t s) {
   if (!items.n) return;
   Call c;
   c.p = *a;
+  for (int i = 0; i < MDMM_ORTHO_MAX; ++i) c.p.item[i] = mats[i];
   c.q = items;
   Items& q = c.q;
   const int packs = tiles(q, PACKS, [](const Item& w) { return (int64_t)(w.n / 64) * (w.m / 64); });
@@ -619,9 +644,10 @@ extern "C" int mdmm_ortho(const mdmm_ortho_t* a, void* stream) {
   if (!a->ws || ((uintptr_t)a->ws & 255)) return a->ws ? MDMM_E_ALIGN : MDMM_E_ARG;
   for (int i = 0; i < a->n; ++i)
     if (!a->item[i].src || !a->item[i].dst) return MDMM_E_ARG;
-  Items q[2];
-  lay_out(a, q);
-  launch<Small>(a, q[0], (Call*)a->ws, (hipStream_t)stream);
-  launch<Large>(a, q[1], (Call*)((char*)a->ws + up(sizeof(Call), 256)), (hipStream_t)stream);
+  Items q[2] = {};
+  mdmm_ortho_item_t mats[2][MDMM_ORTHO_MAX] = {};
+  lay_out(a, q, mats);
+  launch<Small>(a, q[0], mats[0], (Call*)a->ws, (hipStream_t)stream);
+  launch<Large>(a, q[1], mats[1], (Call*)((char*)a->ws + up(sizeof(Call), 256)), (hipStream_t)stream);
   return (int)hipGetLastError();
 }
