@@ -218,7 +218,7 @@ class _GatedScanFn(torch.autograd.Function):
         gates, h0, mask, states = ctx.saved_tensors
         g_h = None if g_h is None else g_h.contiguous()
         g_last = None if g_last is None else g_last.contiguous()
-        g_x = torch.empty(gates.shape, device=gates.device, dtype=gates.dtype)
+        g_x = _new(gates, gates.dtype)
         if g_x.numel() == 0:
             return g_x, _no_steps_grad(h0, g_last if gates.shape[0] == 0 else None), None, None
         a = native.GatedScan()
@@ -306,6 +306,25 @@ def _as_rows(t, H):
     return _unit_cols(t.reshape(-1, H))
 
 
+def _row(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _flat(t, H):
+    """(t, or a view or copy of it, whose rows of H have one stride; that stride), None for None."""
+    if t is None or t.is_contiguous():          # (no view: one costs as much as a launch)
+        return None if t is None else (t, H)
+    t = _as_rows(t, H)
+    return t, _row(t)
+
+
+def _new(like, dtype):
+    """A new contiguous tensor of like's shape."""
+    if like.dtype is dtype and like.is_contiguous():
+        return torch.empty_like(like)
+    return torch.empty(like.shape, device=like.device, dtype=dtype)
+
+
 def _combo(name, y, branch, res):
     key = tuple(d == torch.bfloat16 for d in (y, branch, res))
     if key not in ((False, False, False), (True, True, True), (True, True, False), (False, True, False), (False, True, True)):
@@ -313,62 +332,61 @@ def _combo(name, y, branch, res):
     return key
 
 
-def _row(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _fill_norm(p, y, gate, res, w, s, w_next, branch, eps):
-    p.rows, p.H, p.eps = res.shape[0], res.shape[1], eps
-    p.branch_bf16, p.res_bf16 = int(branch == torch.bfloat16), int(res.dtype == torch.bfloat16)
-    p.res, p.res_st = res.data_ptr(), _row(res)
+def _fill_norm(p, rows, H, y, gate, res, w, s, w_next, branch, eps):
+    """y, gate, res: _flat()'s pairs."""
+    p.rows, p.H, p.eps = rows, H, eps
+    t, p.res_st = res
+    p.res, p.branch_bf16, p.res_bf16 = t.data_ptr(), branch is torch.bfloat16, t.dtype is torch.bfloat16
     if y is not None:
-        p.y, p.y_st, p.y_bf16 = y.data_ptr(), _row(y), int(y.dtype == torch.bfloat16)
+        t, p.y_st = y
+        p.y, p.y_bf16 = t.data_ptr(), t.dtype is torch.bfloat16
     if gate is not None:
-        p.gate, p.gate_st = gate.data_ptr(), _row(gate)
-    p.w, p.scale, p.w_next = ops._ptr(w), ops._ptr(s), ops._ptr(w_next)
-
-
-def _norm_forward(p, y, gate, res, w, s, w_next, branch, eps, shape):
-    """Fills the struct of a forward call on row-major (rows, H) operands -> (out or None, n or None) in `shape`."""
-    out = n = None
-    _fill_norm(p, y, gate, res, w, s, w_next, branch, eps)
-    if y is not None:
-        out = torch.empty(shape, device=res.device, dtype=res.dtype)
-        p.out, p.out_st = out.data_ptr(), p.H
+        t, p.gate_st = gate
+        p.gate = t.data_ptr()
+    if w is not None:
+        p.w = w.data_ptr()
+    if s is not None:
+        p.scale = s.data_ptr()
     if w_next is not None:
-        n = torch.empty(shape, device=res.device, dtype=branch)
-        p.n, p.n_st = n.data_ptr(), p.H
-    return out, n
+        p.w_next = w_next.data_ptr()
 
 
-def _norm_backward(p, y, gate, res, w, s, w_next, branch, eps, g_out, g_n, d_y, d_gate, d_res, want):
-    """Fills the struct of a backward call: d_y, d_gate, d_res row-major views (None: not wanted), want = (d_w, d_scale,
-    d_w_next) flags -> (the three column sums, None where not wanted; scratch to hold until the launch)."""
-    H, dev = res.shape[1], res.device
-    _fill_norm(p, y, gate, res, w, s, w_next, branch, eps)
+def _norm_backward(p, like, g_out, g_n, d_y, d_gate, d_res, want):
+    """Fills in the gradients of a backward call: g_out, g_n _flat()'s pairs, d_y, d_gate, d_res contiguous tensors (None: not
+    wanted), want = (d_w, d_scale, d_w_next) flags, like: a vector of H -> (the three column sums, None where not wanted;
+    scratch to hold until the launch)."""
+    H = p.H
     if g_out is not None:
-        p.g_out, p.g_out_st = g_out.data_ptr(), _row(g_out)
+        p.g_out, p.g_out_st = g_out[0].data_ptr(), g_out[1]
     if g_n is not None:
-        p.g_n, p.g_n_st = g_n.data_ptr(), _row(g_n)
+        p.g_n, p.g_n_st = g_n[0].data_ptr(), g_n[1]
     if d_y is not None:
-        p.d_y, p.d_y_st = d_y.data_ptr(), _row(d_y)
+        p.d_y, p.d_y_st = d_y.data_ptr(), H
     if d_gate is not None:
-        p.d_gate, p.d_gate_st = d_gate.data_ptr(), _row(d_gate)
+        p.d_gate, p.d_gate_st = d_gate.data_ptr(), H
     if d_res is not None:
-        p.d_res, p.d_res_st = d_res.data_ptr(), _row(d_res)
-    sums = [torch.empty(H, device=dev, dtype=torch.float32) if k else None for k in want]
-    if res.shape[0] == 0:
+        p.d_res, p.d_res_st = d_res.data_ptr(), H
+    sums = [torch.empty_like(like) if k else None for k in want]
+    if p.rows == 0:
         return [None if t is None else t.zero_() for t in sums], None
-    p.d_w, p.d_scale, p.d_w_next = (ops._ptr(t) for t in sums)
-    ws = torch.empty(_size('mdmm_block_norm_ws', p), device=dev, dtype=torch.float32)
+    p.d_w, p.d_scale, p.d_w_next = [ops._ptr(t) for t in sums]
+    ws = like.new_empty(_size('mdmm_block_norm_ws', p))
     p.ws = ws.data_ptr()
     return sums, ws
 
 
-def _run_norm(y, gate, res, w, s, w_next, branch, eps, shape):
-    """Row-major operands -> (out or None, n or None) in `shape`."""
+def _run_norm(y, gate, res, w, s, w_next, branch, eps, H):
+    """y, gate, res: tensors of one shape, or None for the first two -> (out or None, n or None)."""
     p = native.BlockNorm()
-    out, n = _norm_forward(p, y, gate, res, w, s, w_next, branch, eps, shape)
+    flat = _flat(y, H), _flat(gate, H), _flat(res, H)             # (held until the launch)
+    _fill_norm(p, res.numel() // H, H, *flat, w, s, w_next, branch, eps)
+    out = n = None
+    if y is not None:
+        out = _new(res, res.dtype)
+        p.out, p.out_st = out.data_ptr(), H
+    if w_next is not None:
+        n = _new(res, branch)
+        p.n, p.n_st = n.data_ptr(), H
     _launch('mdmm_block_norm_fwd', 'block_norm_fwd', p)
     return out, n
 
@@ -377,10 +395,9 @@ class _RmsNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, eps, dtype):
         ctx.set_materialize_grads(False)
-        rows = _as_rows(x, x.shape[-1])
-        ctx.save_for_backward(rows, w)
+        ctx.save_for_backward(x, w)
         ctx.eps, ctx.branch = eps, dtype
-        return _run_norm(None, None, rows, None, None, w, dtype, eps, x.shape)[1]
+        return _run_norm(None, None, x, None, None, w, dtype, eps, w.shape[0])[1]
 
     @staticmethod
     @once_differentiable
@@ -389,15 +406,16 @@ class _RmsNormFn(torch.autograd.Function):
             return None, None, None, None
         x, w = ctx.saved_tensors
         need_x, need_w = ctx.needs_input_grad[:2]
-        d_x = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
+        H = w.shape[0]
+        d_x = _new(g, x.dtype) if need_x else None
         p = native.BlockNorm()
-        rows = _as_rows(g, x.shape[1])
-        sums, ws = _norm_backward(p, None, None, x, None, None, w, ctx.branch, ctx.eps, None, rows, None, None, d_x,
-                                  (False, False, need_w))
-        if x.shape[0]:
+        res, g_n = _flat(x, H), _flat(g, H)
+        _fill_norm(p, x.numel() // H, H, None, None, res, None, None, w, ctx.branch, ctx.eps)
+        sums, ws = _norm_backward(p, w, None, g_n, None, None, d_x, (False, False, need_w))
+        if ws is not None:
             _launch('mdmm_block_norm_bwd', 'rms_norm_bwd', p)
-        del ws
-        return None if d_x is None else d_x.view(g.shape), sums[2], None, None
+        del ws, res, g_n
+        return d_x, sums[2], None, None
 
 
 def _check_width(name, H):
@@ -420,18 +438,16 @@ def rms_norm(x, weight, eps=1e-6, dtype=None):
     dev = _check_device('rms_norm', x, weight)
     if _grad_wanted(x, weight):
         return _apply(dev, _RmsNormFn.apply, x, weight, float(eps), dtype)
-    return _apply(dev, _run_norm, None, None, _as_rows(x, H), None, None, weight, dtype, float(eps), x.shape)[1]
+    return _apply(dev, _run_norm, None, None, x, None, None, weight, dtype, float(eps), H)[1]
 
 
 class _BlockNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, res, w, gate, s, w_next, eps):
         ctx.set_materialize_grads(False)
-        H = res.shape[-1]
-        rows = [None if t is None else _as_rows(t, H) for t in (y, gate, res)]
-        ctx.save_for_backward(*rows, w, s, w_next)
-        ctx.eps, ctx.shape = eps, res.shape
-        out, n = _run_norm(*rows, w, s, w_next, y.dtype, eps, res.shape)
+        ctx.save_for_backward(y, gate, res, w, s, w_next)
+        ctx.eps = eps
+        out, n = _run_norm(y, gate, res, w, s, w_next, y.dtype, eps, w.shape[0])
         return out if n is None else (out, n)
 
     @staticmethod
@@ -441,22 +457,20 @@ class _BlockNormFn(torch.autograd.Function):
             return (None,) * 7
         y, gate, res, w, s, w_next = ctx.saved_tensors
         need = ctx.needs_input_grad                     # y, res, w, gate, s, w_next
-        H, dev = res.shape[1], res.device
-        g_out = None if g_out is None else _as_rows(g_out, H)
-        g_n = None if g_n is None else _as_rows(g_n, H)
-        d_y = torch.empty(res.shape, device=dev, dtype=y.dtype) if need[0] else None
-        d_gate = torch.empty(res.shape, device=dev, dtype=gate.dtype) if need[3] else None
-        d_res = torch.empty(res.shape, device=dev, dtype=res.dtype) if need[1] and g_n is not None else None
+        H, like = w.shape[0], g_n if g_out is None else g_out
+        d_y = _new(like, y.dtype) if need[0] else None
+        d_gate = _new(like, gate.dtype) if need[3] else None
+        d_res = _new(like, res.dtype) if need[1] and g_n is not None else None
         p = native.BlockNorm()
-        sums, ws = _norm_backward(p, y, gate, res, w, s, w_next, y.dtype, ctx.eps, g_out, g_n, d_y, d_gate, d_res,
-                                  (need[2], need[4], need[5]))
-        if res.shape[0]:
+        flat = _flat(y, H), _flat(gate, H), _flat(res, H), _flat(g_out, H), _flat(g_n, H)
+        _fill_norm(p, res.numel() // H, H, *flat[:3], w, s, w_next, y.dtype, ctx.eps)
+        sums, ws = _norm_backward(p, w, *flat[3:], d_y, d_gate, d_res, (need[2], need[4], need[5]))
+        if ws is not None:
             _launch('mdmm_block_norm_bwd', 'block_norm_bwd', p)
-        del ws
+        del ws, flat
         if need[1] and d_res is None:                    # (without a next norm it is g_out itself)
             d_res = g_out
-        view = lambda t: None if t is None else t.reshape(ctx.shape)                       # noqa: E731
-        return view(d_y), view(d_res), sums[0], view(d_gate), sums[1], sums[2], None
+        return d_y, d_res, sums[0], d_gate, sums[1], sums[2], None
 
 
 def block_norm(y, residual, weight, gate=None, scale=None, next_weight=None, eps=1e-6):
@@ -481,8 +495,7 @@ def block_norm(y, residual, weight, gate=None, scale=None, next_weight=None, eps
     dev = _check_device(name, y, residual, weight, gate, scale, next_weight)
     if _grad_wanted(y, residual, weight, gate, scale, next_weight):
         return _apply(dev, _BlockNormFn.apply, y, residual, weight, gate, scale, next_weight, float(eps))
-    rows = [None if t is None else _as_rows(t, H) for t in (y, gate, residual)]
-    out, n = _apply(dev, _run_norm, *rows, weight, scale, next_weight, y.dtype, float(eps), residual.shape)
+    out, n = _apply(dev, _run_norm, y, gate, residual, weight, scale, next_weight, y.dtype, float(eps), H)
     return out if n is None else (out, n)
 
 
@@ -492,23 +505,22 @@ def _up4(n):
     return (n + 3) & ~3
 
 
-def _fill_block(p, proj, rows, h, w, s, w_next, eps):
-    """The norm's struct on the states at address h and the gate's columns of proj -> a copy to hold until the launch, where
-    proj's rows have no one stride."""
-    H = rows.shape[1]
-    _fill_norm(p, None, None, rows, w, s, w_next, proj.dtype, eps)
-    flat = proj if proj.is_contiguous() else _as_rows(proj, 3 * H)
+def _fill_block(p, proj, res, rows, H, h, w, s, w_next, eps):
+    """The norm's struct on the states at address h and the gate's columns of proj -> tensors to hold until the launch (proj's
+    and the residual's copies, where their rows have no one stride)."""
+    res, (flat, st) = _flat(res, H), _flat(proj, 3 * H)
+    _fill_norm(p, rows, H, None, None, res, w, s, w_next, proj.dtype, eps)
     p.y, p.y_st = h, H
-    p.gate, p.gate_st = flat.data_ptr() + 2 * H * flat.element_size(), 3 * H if flat is proj else _row(flat)
-    return flat
+    p.gate, p.gate_st = flat.data_ptr() + 2 * H * flat.element_size(), st
+    return res, flat
 
 
-def _run_block(proj, rows, h0, w, s, w_next, mask, reverse, eps, shape, keep=False):
+def _run_block(proj, res, h0, w, s, w_next, mask, reverse, eps, keep=False):
     """-> (out, n or None, h_last, one buffer: the states of every step, then those kept for the backward pass)."""
-    T, B, H = shape
+    T, B, H = res.shape
     dev = proj.device
-    out = torch.empty(shape, device=dev, dtype=rows.dtype)
-    n = torch.empty(shape, device=dev, dtype=proj.dtype) if w_next is not None else None
+    out = _new(res, res.dtype)
+    n = _new(res, proj.dtype) if w_next is not None else None
     if out.numel() == 0:
         return out, n, _no_steps_last(h0, B, H, dev), None
     last = torch.empty((B, H), device=dev, dtype=torch.float32)
@@ -520,7 +532,7 @@ def _run_block(proj, rows, h0, w, s, w_next, mask, reverse, eps, shape, keep=Fal
     a.h, a.h_last = states.data_ptr(), last.data_ptr()
     if kept:
         a.states = a.h + 4 * size
-    flat = _fill_block(p, proj, rows, a.h, w, s, w_next, eps)
+    flat = _fill_block(p, proj, res, T * B, H, a.h, w, s, w_next, eps)
     p.out, p.out_st = out.data_ptr(), H
     if n is not None:
         p.n, p.n_st = n.data_ptr(), H
@@ -537,9 +549,8 @@ class _GatedBlockFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, proj, res, h0, w, s, w_next, mask, reverse, eps):
         ctx.set_materialize_grads(False)
-        rows = _as_rows(res, res.shape[-1])
-        out, n, last, states = _run_block(proj, rows, h0, w, s, w_next, mask, reverse, eps, res.shape, True)
-        ctx.save_for_backward(proj, rows, h0, w, s, w_next, mask, states)
+        out, n, last, states = _run_block(proj, res, h0, w, s, w_next, mask, reverse, eps, True)
+        ctx.save_for_backward(proj, res, h0, w, s, w_next, mask, states)
         ctx.reverse, ctx.eps = reverse, eps
         return (out, last) if n is None else (out, n, last)
 
@@ -554,21 +565,18 @@ class _GatedBlockFn(torch.autograd.Function):
         H, dev = H3 // 3, proj.device
         if g_out is None and g_n is None and g_last is None:
             return (None,) * 9
-        g_out = None if g_out is None else _as_rows(g_out, H)
-        g_n = None if g_n is None else _as_rows(g_n, H)
-        g_last = None if g_last is None else g_last.contiguous()
-        g_x = torch.empty((T, B, H3), device=dev, dtype=proj.dtype)
-        through = g_out is not None or g_n is not None
-        sums = [torch.empty(H, device=dev, dtype=torch.float32) if k and through else None for k in need[3:6]]
         d_res = None
         if need[1]:                                    # (without a next norm it is g_out itself)
-            d_res = torch.empty((T, B, H), device=dev, dtype=res.dtype) if g_n is not None else \
-                None if g_out is None else g_out.reshape(T, B, H)
+            d_res = g_out if g_n is None else _new(g_n, res.dtype)
+        g_out, g_n = _flat(g_out, H), _flat(g_n, H)
+        g_last = None if g_last is None else g_last.contiguous()
+        g_x = _new(proj, proj.dtype)
+        through = g_out is not None or g_n is not None
+        sums = [torch.empty_like(w) if k and through else None for k in need[3:6]]
         if g_x.numel() == 0:
             return (g_x, d_res, _no_steps_grad(h0, g_last if T == 0 else None),
                     *(None if t is None else t.zero_() for t in sums), None, None, None)
         a, p = native.GatedScan(), native.BlockNorm()
-        p.rows, p.H = T * B, H
         _fill_scan(a, proj, H, h0, mask, ctx.reverse)
         size = _up4(T * B * H)
         base = states.data_ptr()
@@ -576,20 +584,21 @@ class _GatedBlockFn(torch.autograd.Function):
             a.states = base + 4 * size
         a.g_last = ops._ptr(g_last)
         a.g_gates, a.g_gates_st, a.g_gates_sb = g_x.data_ptr(), B * H3, H3
-        flat = _fill_block(p, proj, res, base, w, s, w_next, ctx.eps) if through else None
+        p.rows, p.H = T * B, H
+        flat = _fill_block(p, proj, res, T * B, H, base, w, s, w_next, ctx.eps) if through else None
         # one scratch: the states' gradient | the norms' slabs | each sequence's gradient of h0 | the scan's splits
         slabs = _size('mdmm_block_norm_ws', p) if through else 0
         per = _up4(B * H) if h0 is not None and need[2] else 0
         splits = _size('mdmm_gated_scan_ws', a, 1)
         lead = size if through else 0
-        scratch = torch.empty(lead + _up4(slabs) + per + splits, device=dev, dtype=torch.float32)
+        scratch = w.new_empty(lead + _up4(slabs) + per + splits)
         at = scratch.data_ptr()
         g0 = None
         if through:
             if g_out is not None:
-                p.g_out, p.g_out_st = g_out.data_ptr(), _row(g_out)
+                p.g_out, p.g_out_st = g_out[0].data_ptr(), g_out[1]
             if g_n is not None:
-                p.g_n, p.g_n_st = g_n.data_ptr(), _row(g_n)
+                p.g_n, p.g_n_st = g_n[0].data_ptr(), g_n[1]
                 if d_res is not None:
                     p.d_res, p.d_res_st = d_res.data_ptr(), H
             p.d_y, p.d_y_st, p.ws = at, H, at + 4 * lead
@@ -642,8 +651,7 @@ def gated_block(proj, residual, h0, weight, scale=None, next_weight=None, mask=N
     proj, reverse = _unit_cols(proj), bool(reverse)
     if _grad_wanted(proj, residual, h0, weight, scale, next_weight):
         return _apply(dev, _GatedBlockFn.apply, proj, residual, h0, weight, scale, next_weight, mask, reverse, float(eps))
-    out, n, last = _apply(dev, _run_block, proj, _as_rows(residual, H), h0, weight, scale, next_weight, mask, reverse, float(eps),
-                          residual.shape)[:3]
+    out, n, last = _apply(dev, _run_block, proj, residual, h0, weight, scale, next_weight, mask, reverse, float(eps))[:3]
     return (out, last) if n is None else (out, n, last)
 
 
@@ -665,9 +673,12 @@ def _block_step(proj, residual, state, w, s, w_next, mask, eps, new_state):
     H = state.shape[1]
     new_state = torch.empty_like(state) if new_state is None else new_state
     a, p = native.GatedScan(), native.BlockNorm()
-    out, n = _norm_forward(p, None, None, residual, w, s, w_next, proj.dtype, eps, residual.shape)
-    out = torch.empty(residual.shape, device=proj.device, dtype=residual.dtype)
+    _fill_norm(p, proj.shape[0], H, None, None, (residual, _row(residual)), w, s, w_next, proj.dtype, eps)
+    out, n = _new(residual, residual.dtype), None
     p.out, p.out_st = out.data_ptr(), H
+    if w_next is not None:
+        n = _new(residual, proj.dtype)
+        p.n, p.n_st = n.data_ptr(), H
     p.gate, p.gate_st = proj.data_ptr() + 2 * H * proj.element_size(), _row(proj)
     if out.numel():
         _fill_step(a, proj, H, state, mask, new_state)
