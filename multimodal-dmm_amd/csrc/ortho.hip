@@ -2,16 +2,16 @@
 // X <- ca X + P X with P = cb A + cc A A, A = X X^T.  X lies down (n rows <= m columns).
 //
 // The iteration multiplies a small singular value by up to ca a step (ca^5 = 485 over five), and a rounding of X with it, so
-// bf16 operands are out; fp32 ones would run on the fp32 matrix instruction, a sixteenth of the fp16 one's rate.  Every
-// matrix is kept as two fp16 planes instead, s x = h + l with h = fp16(s x), l = fp16(s x - h): 22 to 23 bits.  s is as large
-// as the entries allow (X and A stay below 2: 2^14; P below 16: 2^12), so that l is a normal number down to entries of 1e-5
-// and below those wrong by 2e-12.  A product is h h' + h l' + l h': three fp16 matrix instructions, the dropped l l' 2^-23 of
-// a term: the result is nearer to 64 bits than fp32 products by the library (6e-7 against 2.9e-6 at 2048 x 2048).  ca X is
-// added in fp32.
+// bf16 operands are out; fp32 ones would run on the fp32 matrix instruction, a sixteenth of the fp16 one's rate.  Matrices
+// with more than 64 rows are kept as two fp16 planes instead, s x = h + l with h = fp16(s x), l = fp16(s x - h): 22 to 23
+// bits.  s is as large as the entries allow (X and A stay below 2: 2^14; P below 16: 2^12), so that l is a normal number down
+// to entries of 1e-5 and below those wrong by 2e-12.  A product is h h' + h l' + l h': three fp16 matrix instructions, the
+// dropped l l' 2^-23 of a term: the result is nearer to 64 bits than fp32 products by the library (6e-7 against 2.9e-6 at
+// 2048 x 2048).  ca X is added in fp32.  (Up to 64 rows: fp32, see WHOLE.)
 //
 // X is stored both ways (n x m for A, m x n for P X) so that every product runs over two operands' rows.  A row keeps 32
 // columns of h, then the same 32 of l: one cache line for a step of 32 (with the planes apart, each step took half lines and
-// two 2048 x 2048 products 142 us).  Tiles come straight into LDS, a step or more ahead, chunks of 16 bytes swapped within a
+// two 2048 x 2048 products 142 us); fp32 rows take the same bytes.  Tiles come straight into LDS, a step or more ahead, chunks of 16 bytes swapped within a
 // row so that the matrix instruction's reads meet all banks; neighbouring tiles go to one XCD, whose L2 then holds their
 // rows.  A and P are symmetric: tiles at and above the diagonal only, stored twice.  Sizes are rounded up to whole tiles with
 // zeros, which every product keeps.  All matrices of a call share each launch.
@@ -21,6 +21,7 @@
 // bound by the seventeen launches of five steps, 8 to 12 us each.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 #include "../../include/mdmm_hip.h"
 
 namespace mdmm {
@@ -33,6 +34,8 @@ typedef _Float16 half_t;
 typedef half_t half4 __attribute__((ext_vector_type(4)));
 typedef half_t half8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 // BM x BN tile of a product by WI x WJ waves, BK deep, ST buffers, OCC waves a SIMD wanted
 template <int BM_, int BN_, int BK_, int ST_, int WI_, int WJ_, int OCC_> struct Cfg {
@@ -44,8 +47,14 @@ template <int BM_, int BN_, int BK_, int ST_, int WI_, int WJ_, int OCC_> struct
   static constexpr int LOADS = HALVES / 8 / T;                  // chunks a thread loads for a buffer
   static_assert(BM * CPR % T == 0 && BN * CPR % T == 0, "a load instruction of the workgroup stays in one operand");
 };
+// A matrix whose shorter side fits one small tile is kept in fp32 and multiplied by the fp32 matrix instruction.  The fp16 one
+// aligns the products of eight columns to the largest of them and drops what falls below its last bit: no matter beside the
+// rounding of fp32 sums over hundreds of rows, but over a few of them the larger error (7 x 146: 1.8e-6 off against 0.7e-6
+// in fp32 by the library).  A wave's step takes 1024 cycles instead of 192, which such a matrix's few steps have room for.
+constexpr int WHOLE = 64;
 // (two workgroups a CU, four buffers each.  P X of two 256 x 4096: 13.6 us, with one of 128 KB 17)
 typedef Cfg<64, 64, 32, 4, 2, 2, 2> Small;
+static_assert(Small::BM == WHOLE && Small::BN == WHOLE && Small::TI * Small::TJ == 1, "one tile, one piece a wave");
 // (two workgroups a CU, two buffers each.  Measured on P X of two 2048 x 2048: 112 us; one workgroup with four buffers 127, one
 // of 256 x 128 and 8 waves with three 126, steps of 64 columns 126)
 typedef Cfg<128, 128, 32, 2, 2, 2, 2> Large;
@@ -102,10 +111,52 @@ __device__ __forceinline__ void split(float x, half_t& h, half_t& l) {       // 
   h = (half_t)x;
   l = (half_t)(x - (float)h);
 }
-__device__ __forceinline__ float join(half_t h, half_t l) { return (float)h + (float)l; }
 
 // column c of a row of `cols` columns as pairs: h there, l 32 further
 __device__ __forceinline__ int64_t at(int64_t row, int64_t cols, int64_t c) { return row * cols * 2 + (c >> 5) * 64 + (c & 31); }
+
+// Elements of a matrix in either format: pairs, or (whole) fp32 in the same bytes of a row.  A row is 2 cols halves in both
+__device__ __forceinline__ half_t* place(half_t* m, int64_t row, int64_t cols, int64_t c, bool whole) {
+  return whole ? m + (row * cols + c) * 2 : m + at(row, cols, c);
+}
+__device__ __forceinline__ void put(half_t* d, float v, bool whole) {
+  if (whole) {
+    *(float*)d = v;
+    return;
+  }
+  half_t h, l;
+  split(v, h, l);
+  d[0] = h;
+  d[32] = l;
+}
+// four neighbours of a row (c a multiple of four)
+__device__ __forceinline__ void put4(half_t* m, int64_t row, int64_t cols, int64_t c, const float* v, bool whole) {
+  if (whole) {
+    *(float4*)place(m, row, cols, c, true) = make_float4(v[0], v[1], v[2], v[3]);
+    return;
+  }
+  half4 h4, l4;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    half_t h, l;
+    split(v[e], h, l);
+    h4[e] = h;
+    l4[e] = l;
+  }
+  half_t* d = place(m, row, cols, c, false);
+  *(half4*)d = h4;
+  *(half4*)(d + 32) = l4;
+}
+struct Four { u32x2 a, b; };         // as loaded: two fp32 each, or four h and four l
+__device__ __forceinline__ Four get4(const half_t* m, int64_t row, int64_t cols, int64_t c, bool whole) {
+  const half_t* d = place((half_t*)m, row, cols, c, whole);
+  return {*(const u32x2*)d, *(const u32x2*)(d + (whole ? 4 : 32))};
+}
+__device__ __forceinline__ float of4(const Four& f, int e, bool whole) {
+  const half4 h = __builtin_bit_cast(half4, f.a), l = __builtin_bit_cast(half4, f.b);
+  const unsigned x = e == 0 ? f.a[0] : e == 1 ? f.a[1] : e == 2 ? f.b[0] : f.b[1];
+  return whole ? __builtin_bit_cast(float, x) : (float)h[e] + (float)l[e];
+}
 
 __device__ __forceinline__ float src_at(const mdmm_ortho_t& p, const mdmm_ortho_item_t& t, int64_t r, int64_t c) {
   const int64_t i = r * t.src_ld + c;
@@ -179,56 +230,35 @@ __global__ __launch_bounds__(NT) void ortho_pack_kernel(const Call* __restrict__
   __syncthreads();
   s = (part[0] + part[1]) + (part[2] + part[3]);
   const float inv = (float)((double)SX / (sqrt(s) + (double)p.eps));
+  auto store = [&](auto as) {
+    constexpr bool whole = decltype(as)::value;
 #pragma unroll
-  for (int u = 0; u < 4096 / NT; ++u) {
-    const int i = threadIdx.x + u * NT;
-    const int64_t r = r0 + i / 64, c = c0 + i % 64;
-    const float v = x[u] * inv;
-    tile[i / 64][i % 64] = v;
-    half_t h, l;
-    split(v, h, l);
-    const int64_t o = at(r, ld_same, c);
-    same[o] = h;
-    same[o + 32] = l;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 4096; i += NT) {
-    half_t h, l;
-    split(tile[i % 64][i / 64], h, l);
-    const int64_t o = at(c0 + i / 64, ld_other, r0 + i % 64);
-    other[o] = h;
-    other[o + 32] = l;
-  }
+    for (int u = 0; u < 4096 / NT; ++u) {
+      const int i = threadIdx.x + u * NT;
+      const float v = x[u] * inv;
+      tile[i / 64][i % 64] = v;
+      put(place(same, r0 + i / 64, ld_same, c0 + i % 64, whole), v, whole);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 4096; i += NT) put(place(other, c0 + i / 64, ld_other, r0 + i % 64, whole), tile[i % 64][i / 64], whole);
+  };
+  if (w.n == WHOLE) store(std::true_type{});
+  else store(std::false_type{});
 }
 
 enum { GRAM, POLY, APPLY, LAST };          // (LAST: an APPLY whose result goes to dst)
 
-// four consecutive rows i of one column j of a symmetric plane pair of n x n, both ways.  On the diagonal's tiles (i, j) and
+// four consecutive rows i of one column j of a symmetric matrix of n x n, both ways.  On the diagonal's tiles (i, j) and
 // (j, i) are both computed, and may round differently: there the upper one is stored in both places, the lower one nowhere
-__device__ __forceinline__ void put_sym(half_t* dst, int64_t n, int64_t i, int64_t j, const float* v, bool diagonal) {
-  half4 h4, l4;
+__device__ __forceinline__ void put_sym(half_t* dst, int64_t n, int64_t i, int64_t j, const float* v, bool diagonal, bool whole) {
+  half_t* down = place(dst, i, n, j, whole);
+  if (!diagonal) put4(dst, j, n, i, v, whole);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    half_t h, l;
-    split(v[e], h, l);
-    h4[e] = h;
-    l4[e] = l;
+  for (int e = 0; e < 4; ++e)
     if (!diagonal || i + e <= j) {
-      half_t* d = dst + at(i + e, n, j);
-      d[0] = h;
-      d[32] = l;
-      if (diagonal) {
-        d = dst + at(j, n, i + e);
-        d[0] = h;
-        d[32] = l;
-      }
+      put(down + 2 * e * n, v[e], whole);
+      if (diagonal) put(place(dst, j, n, i + e, whole), v[e], whole);
     }
-  }
-  if (!diagonal) {
-    half_t* d = dst + at(j, n, i);
-    *(half4*)d = h4;
-    *(half4*)(d + 32) = l4;
-  }
 }
 
 // tile t of those that reach the diagonal or lie above it, row by row; a row of tiles starts R tiles further right than the
@@ -254,27 +284,17 @@ template <class C> __host__ __device__ int tri(int n) {          // tiles at and
   return rows * (n / C::BN) - R * rows * (rows - 1) / 2;
 }
 
-template <int MODE, class C>
-__global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call* __restrict__ call, int flip) {
-  __shared__ __align__(16) half_t lds[C::ST * C::HALVES];
+// tile `tile` of one matrix's product, in one of the formats
+template <int MODE, class C, bool whole>
+__device__ __forceinline__ void product(half_t (&lds)[C::ST * C::HALVES], const Call* __restrict__ call, const Item& w,
+                                        const mdmm_ortho_item_t& t, int tile, int flip) {
   constexpr bool PX = MODE == APPLY || MODE == LAST;
-  constexpr int LIST = MODE == GRAM ? GRAMS : MODE == POLY ? POLYS : APPLIES;
-  const Items& q = call->q;
-  // consecutive workgroups go round the 8 XCDs: each XCD takes a run of consecutive tiles instead
-  const int total = gridDim.x, xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
-  const int me = xcd * each + (xcd < more ? xcd : more) + (blockIdx.x >> 3);
-  const Entries<mdmm_ortho_item_t> ts(call->p.item);
-  const Entries<Item> ws(q.it);
-  const Found f = find(q.first[LIST], me);
-  const Item w = ws.of(f.k);
-  mdmm_ortho_item_t t = {};
-  if (MODE == LAST) t = ts.of(f.k);
   const mdmm_ortho_t& p = call->p;
   const float ca = p.ca, cb = p.cb, cc = p.cc, decay = p.decay;
   const bool update = p.update, low = p.dst_bf16;
   const float lr = MODE == LAST && update ? (p.lr_dev ? *p.lr_dev : p.lr) : 0.0f;
   const int n = w.n, J = PX ? w.m : n;
-  int tile = me - f.first, ti, tj, slice = 0;
+  int ti, tj, slice = 0;
   if (PX) {
     ti = tile / (J / C::BN);
     tj = tile % (J / C::BN);
@@ -308,21 +328,20 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
       half_t* to = lds + buf * C::HALVES + (c * C::T + wave * 64) * 8;
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from[c],
                                        (__attribute__((address_space(3))) void*)to, 16, 0, 0);
-      from[c] += 2 * C::BK;
     }
+  };
+  auto advance = [&] {
+#pragma unroll
+    for (int c = 0; c < C::LOADS; ++c) from[c] += 2 * C::BK;
   };
   // what the result is joined with, on its way while the product runs (the small tile has the registers)
   constexpr bool EARLY = MODE != GRAM && C::TI * C::TJ == 1;
   const int wi = wave / C::WJ * 32 * C::TI, wj = wave % C::WJ * 32 * C::TJ;
   const half_t* beside = MODE == POLY ? w.gram : xt;
-  half4 eh[EARLY ? 4 : 1], el[EARLY ? 4 : 1];
+  Four early[EARLY ? 4 : 1];
   if constexpr (EARLY) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const half_t* d = beside + at(j0 + wj + (lane & 31), n, i0 + wi + 8 * g + 4 * (lane >> 5));
-      eh[g] = *(const half4*)d;
-      el[g] = *(const half4*)(d + 32);
-    }
+    for (int g = 0; g < 4; ++g) early[g] = get4(beside, j0 + wj + (lane & 31), n, i0 + wi + 8 * g + 4 * (lane >> 5), whole);
   }
   f32x16 sum[C::TI][C::TJ] = {};
   // a piece's operands in registers: chunk of h, l's is 4 further (columns kk 16 + (lane / 32) 8 on, of each 32 columns' pair
@@ -346,7 +365,18 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
     }
   };
   f32x16 acc[C::TI][C::TJ];
-  auto multiply = [&](const Part& f) {           // (the three products of a piece apart: none waits for the one before)
+  auto multiply = [&](const Part& f) {
+    if constexpr (whole) {
+      // the reads hold columns 4 c .. 4 c + 3 of both operands; an instruction takes one from each half of the wave
+      const f32x4 a0 = __builtin_bit_cast(f32x4, f.ah[0]), a1 = __builtin_bit_cast(f32x4, f.al[0]);
+      const f32x4 b0 = __builtin_bit_cast(f32x4, f.bh[0]), b1 = __builtin_bit_cast(f32x4, f.bl[0]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a0[e], b0[e], acc[0][0], 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a1[e], b1[e], acc[0][0], 0, 0, 0);
+      return;
+    }
+    // (the three products of a piece apart: none waits for the one before)
 #pragma unroll
     for (int x = 0; x < C::TI; ++x)
 #pragma unroll
@@ -370,7 +400,7 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
     Part r[2][2];
 #pragma unroll
     for (int s = 0; s < C::ST; ++s)
-      if (s < nk) load(s);
+      if (s < nk) load(s), advance();
     if (C::ST <= nk) wait_loads<(C::ST - 1) * C::LOADS>();
     else wait_loads<0>();
     __builtin_amdgcn_s_barrier();
@@ -390,18 +420,23 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
           if (s + C::ST < nk) load(s % C::ST);
+          advance();
           read(r[(u + 1) & 1][0], (s + 1) % C::ST, 0);
           read(r[(u + 1) & 1][1], (s + 1) % C::ST, 1);
         }
         multiply(r[u & 1][0]);
         multiply(r[u & 1][1]);
+        if (whole && u + 1 < RUN) {              // (a sum of 32 columns)
+          sum[0][0] += acc[0][0];
+          acc[0][0] = f32x16{};
+        }
       }
       sum[0][0] += acc[0][0];
     }
   } else {
 #pragma unroll
     for (int s = 0; s < C::ST - 1; ++s)
-      if (s < nk) load(s);
+      if (s < nk) load(s), advance();
     for (int from_s = 0; from_s < nk; from_s += RUN) {
       const int to_s = from_s + RUN < nk ? from_s + RUN : nk;
 #pragma unroll
@@ -415,6 +450,7 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
         __builtin_amdgcn_s_barrier();             // (every wave's share; and all are done with the buffer that is filled next)
         asm volatile("" ::: "memory");
         if (s + C::ST - 1 < nk) load((s + C::ST - 1) % C::ST);
+        advance();
 #pragma unroll
         for (int kk = 0; kk < C::BK / 16; ++kk) {
           Part f;
@@ -441,45 +477,29 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = sum[x][y][4 * g + e];
-        half4 h, l;
-        if constexpr (EARLY) {
-          h = eh[g];
-          l = el[g];
-        } else if constexpr (MODE != GRAM) {
-          const half_t* d = beside + at(j, n, i);
-          h = *(const half4*)d;
-          l = *(const half4*)(d + 32);
-        }
+        Four with;
+        if constexpr (EARLY) with = early[g];
+        else if constexpr (MODE != GRAM) with = get4(beside, j, n, i, whole);
         if (MODE == GRAM) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] *= 1.0f / SX;
-          if (w.splits == 1) put_sym(w.gram, n, i, j, v, j0 < i0 + C::BM);
+          if (w.splits == 1) put_sym(w.gram, n, i, j, v, j0 < i0 + C::BM, whole);
           else *(float4*)(w.part + slice * nn + j * n + i) = make_float4(v[0], v[1], v[2], v[3]);
         }
         if (MODE == POLY) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(cc * (SP / SX / SX), v[e], cb * (SP / SX) * join(h[e], l[e]));
-          put_sym(w.poly, n, i, j, v, j0 < i0 + C::BM);
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(cc * (SP / SX / SX), v[e], cb * (SP / SX) * of4(with, e, whole));
+          put_sym(w.poly, n, i, j, v, j0 < i0 + C::BM, whole);
         }
         if (PX) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(ca, join(h[e], l[e]), v[e] * (1.0f / SP));
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(ca, of4(with, e, whole), v[e] * (1.0f / SP));
         }
         if (MODE == APPLY) {
-          half4 h4, l4;
-          half_t* lie = w.xn + at(i, m, j);
+          half_t* down = place(w.xn, i, m, j, whole);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            half_t hh, ll;
-            split(v[e], hh, ll);
-            h4[e] = hh;
-            l4[e] = ll;
-            lie[2 * e * m] = hh;
-            lie[2 * e * m + 32] = ll;
-          }
-          half_t* to = (flip ? w.xt[0] : w.xt[1]) + at(j, n, i);
-          *(half4*)to = h4;
-          *(half4*)(to + 32) = l4;
+          for (int e = 0; e < 4; ++e) put(down + 2 * e * m, v[e], whole);
+          put4(flip ? w.xt[0] : w.xt[1], j, n, i, v, whole);
         }
         if (MODE == LAST) {
           const int64_t r = w.tall ? j : i, c = w.tall ? i : j, step = w.tall ? 1 : t.dst_ld;
@@ -499,23 +519,50 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
       }
 }
 
+template <int MODE, class C>
+__global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call* __restrict__ call, int flip) {
+  __shared__ __align__(16) half_t lds[C::ST * C::HALVES];
+  constexpr int LIST = MODE == GRAM ? GRAMS : MODE == POLY ? POLYS : APPLIES;
+  const Items& q = call->q;
+  // consecutive workgroups go round the 8 XCDs: each XCD takes a run of consecutive tiles instead
+  const int total = gridDim.x, xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
+  const int me = xcd * each + (xcd < more ? xcd : more) + (blockIdx.x >> 3);
+  const Entries<mdmm_ortho_item_t> ts(call->p.item);
+  const Entries<Item> ws(q.it);
+  const Found f = find(q.first[LIST], me);
+  const Item w = ws.of(f.k);
+  mdmm_ortho_item_t t = {};
+  if (MODE == LAST) t = ts.of(f.k);
+  if constexpr (C::BM == WHOLE)
+    if (w.n == WHOLE) {
+      product<MODE, C, true>(lds, call, w, t, me - f.first, flip);
+      return;
+    }
+  product<MODE, C, false>(lds, call, w, t, me - f.first, flip);
+}
+
 // the slices of A added up (each keeps the tiles at and above the diagonal, column by column)
 template <int BM, int BN> __global__ __launch_bounds__(NT) void ortho_fold_kernel(const Call* __restrict__ call) {
   const Item w = call->q.it[blockIdx.y];
   if (w.splits == 1) return;
   const int64_t n = w.n, nn = n * n;
-  for (int64_t e = ((int64_t)blockIdx.x * NT + threadIdx.x) * 4; e < nn; e += (int64_t)gridDim.x * NT * 4) {
-    const int64_t j = e / n, i = e % n;
-    const int64_t i0 = i / BM * BM, j0 = j / BN * BN;
-    if (j0 < i0) continue;
-    float4 v = *(const float4*)(w.part + e);
-    for (int s = 1; s < w.splits; ++s) {
-      const float4 x = *(const float4*)(w.part + s * nn + e);
-      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+  auto join = [&](auto as) {
+    constexpr bool whole = decltype(as)::value;
+    for (int64_t e = ((int64_t)blockIdx.x * NT + threadIdx.x) * 4; e < nn; e += (int64_t)gridDim.x * NT * 4) {
+      const int64_t j = e / n, i = e % n;
+      const int64_t i0 = i / BM * BM, j0 = j / BN * BN;
+      if (j0 < i0) continue;
+      float4 v = *(const float4*)(w.part + e);
+      for (int s = 1; s < w.splits; ++s) {
+        const float4 x = *(const float4*)(w.part + s * nn + e);
+        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+      }
+      const float f[4] = {v.x, v.y, v.z, v.w};
+      put_sym(w.gram, n, i, j, f, j0 < i0 + BM, whole);
     }
-    const float f[4] = {v.x, v.y, v.z, v.w};
-    put_sym(w.gram, n, i, j, f, j0 < i0 + BM);
-  }
+  };
+  if (BM == WHOLE && n == WHOLE) join(std::true_type{});
+  else join(std::false_type{});
 }
 
 __global__ __launch_bounds__(NT) void ortho_copy_kernel(const Call* __restrict__ call) {       // steps = 0: X itself
@@ -525,8 +572,10 @@ __global__ __launch_bounds__(NT) void ortho_copy_kernel(const Call* __restrict__
   const Item& w = q.it[blockIdx.y];
   const int64_t total = (int64_t)t.rows * t.cols;
   for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)gridDim.x * NT) {
-    const int64_t r = i / t.cols, c = i % t.cols, o = w.tall ? at(c, w.m, r) : at(r, w.m, c);
-    const float v = join(w.xn[o], w.xn[o + 32]) * (1.0f / SX);
+    const int64_t r = i / t.cols, c = i % t.cols;
+    const bool whole = w.n == WHOLE;
+    const half_t* x = place(w.xn, w.tall ? c : r, w.m, w.tall ? r : c, whole);
+    const float v = (whole ? *(const float*)x : (float)x[0] + (float)x[32]) * (1.0f / SX);
     const int64_t to = r * t.dst_ld + c;
     if (p.update) {
       float* d = (float*)t.dst + to;

@@ -202,3 +202,15 @@ def test_bounded_iterations_are_not_refused():
     for c in (ortho.COEFFICIENTS, (1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (1.875, -1.25, 0.375), (1.0, 0.0, 0.0), (0.0, 0.0, 0.0)):
         with pytest.raises(native.MdmmError):         # (the device's refusal, which comes last)
             ops.orthogonalise([torch.zeros(4, 4)], coefficients=c)
+
+
+@gpu
+@pytest.mark.parametrize('shape', [(7, 146), (146, 7), (5, 300), (27, 2), (40, 256), (64, 4096), (4096, 33), (64, 65), (65, 64)])
+def test_short_sides(shape):
+    """Shorter sides about one tile of 64, with the longer side in one piece and in several; the iterate after 0 steps too."""
+    gen = torch.Generator().manual_seed(8 + sum(shape))
+    m = (0.02 * torch.randn(shape, generator=gen)).cuda()
+    keep = m.clone()
+    for steps in (0, 1, 5):
+        check(m, ops.orthogonalise([m], steps=steps)[0], steps)
+    assert torch.equal(m, keep)
