@@ -9,6 +9,7 @@
 // of its rows and leave as one slab a workgroup; norm_fold_kernel adds the slabs up in a fixed order, without atomics.
 // 65536 x 1280 in bf16: forward 159 us (840 MB, 5.3 TB/s, a copy's rate), backward 312 (1.34 GB, 4.3 TB/s: three sums a
 // row between its loads and its last store), fold 7.  A row or two: the launch, 4 to 5 us.
+#include <type_traits>
 #include "gated.h"
 
 namespace mdmm {
@@ -44,11 +45,11 @@ template <typename T, int VEC> struct Row {
     else if constexpr (sizeof(v) == 4) v.x = __builtin_amdgcn_raw_buffer_load_b32(r, c * (int)sizeof(T), 0, 0);
     else v.x = __builtin_amdgcn_raw_buffer_load_b16(r, c * (int)sizeof(T), 0, 0);
   }
-  __device__ __forceinline__ void put(const float* f, int c) const {
+  template <typename F> __device__ __forceinline__ void put(const F* f, int c) const {
     Raw<T, VEC> v;
     T t[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) t[e] = (T)f[e];          // (bf16: to nearest, ties to even)
+    for (int e = 0; e < VEC; ++e) t[e] = (T)(float)f[e];          // (bf16: to nearest, ties to even)
     __builtin_memcpy(&v, t, sizeof v);
     if constexpr (sizeof(v) == 16) __builtin_amdgcn_raw_buffer_store_b128(v.x, r, c * (int)sizeof(T), 0, 0);
     else if constexpr (sizeof(v) == 8) __builtin_amdgcn_raw_buffer_store_b64(v.x, r, c * (int)sizeof(T), 0, 0);
@@ -96,9 +97,20 @@ __device__ __forceinline__ float wave_total(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+__device__ __forceinline__ double wave_total(double v) {
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+__device__ __forceinline__ float rsqrt_(float v) { return rsqrtf(v); }
+__device__ __forceinline__ double rsqrt_(double v) { return 1.0 / sqrt(v); }
+__device__ __forceinline__ float gate_(float g) { return sigmoid_(g); }
+__device__ __forceinline__ double gate_(double g) { return 1.0 / (1.0 + exp(-g)); }
+__device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ double fma_(double a, double b, double c) { return fma(a, b, c); }
+
 // N sums over a row's threads (a wave, or WIDE the workgroup of up to 16 waves), in every one of them.  lds: 2 sets of
 // 2 x 16 words, the words past the last wave zero (a wave that runs ahead writes the other set)
-template <bool WIDE, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float* lds, int& slot) {
+template <bool WIDE, int N, typename A> __device__ __forceinline__ void row_sums(A (&v)[N], float* lds, int& slot) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = wave_total(v[i]);
   if constexpr (WIDE) {
@@ -111,8 +123,8 @@ template <bool WIDE, int N> __device__ __forceinline__ void row_sums(float (&v)[
     for (int i = 0; i < N; ++i) v[i] = row16_total(s[i * 16 + (threadIdx.x & 15)]);
   }
 }
-template <bool WIDE> __device__ __forceinline__ float row_sum(float v, float* lds, int& slot) {
-  float a[1] = {v};
+template <bool WIDE, typename A> __device__ __forceinline__ A row_sum(A v, float* lds, int& slot) {
+  A a[1] = {v};
   row_sums<WIDE, 1>(a, lds, slot);
   return a[0];
 }
@@ -199,6 +211,9 @@ template <typename Y, typename Br, typename R, int VEC, int NV, int MAXT, bool A
 __global__ __launch_bounds__(MAXT, MAXT == 512 && NV * VEC == 4 ? (sizeof(Y) + sizeof(R) == 4 ? 5 : 4) : 1)
 void norm_bwd_kernel(mdmm_block_norm_t p) {
   constexpr bool WIDE = MAXT > 256;
+  // Rows of up to four columns in 64 bits: a norm's gradient is what q w' keeps beside the direction of out, eps alone for one
+  // column and little for two (300 x 1, the residual's gradient: 3e-8 off, in fp32 7e-6 and by fp32 tensor operations the same)
+  typedef typename std::conditional<VEC == 1 && NV == 1, double, float>::type A;
   __shared__ float lds[64];
   __shared__ float fold[WIDE ? 1 : 256 * VEC];
   clear_sums<WIDE>(lds);
@@ -206,11 +221,11 @@ void norm_bwd_kernel(mdmm_block_norm_t p) {
   const int lane = WIDE ? (int)threadIdx.x : (int)(threadIdx.x & 63), tpr = WIDE ? (int)blockDim.x : 64;
 #pragma unroll
   for (int k = 0; k < NV; ++k) c[k] = (k * tpr + lane) * VEC;
-  const float inv = 1.0f / (float)p.H;
+  const A inv = (A)1.0 / (A)p.H;
   const int wave = WIDE ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t step = (int64_t)gridDim.x * (WIDE ? 1 : 4);
   int64_t row = (int64_t)blockIdx.x * (WIDE ? 1 : 4) + wave;
-  float aw[NV][VEC] = {}, as[NV][VEC] = {}, an[NV][VEC] = {};
+  A aw[NV][VEC] = {}, as[NV][VEC] = {}, an[NV][VEC] = {};
   float w[NV][VEC], s[NV][VEC], wn[NV][VEC];
   keep<VEC, NV>(w, p.w, 0.0f, c, p.H);
   keep<VEC, NV>(s, p.scale, 1.0f, c, p.H);
@@ -228,47 +243,53 @@ void norm_bwd_kernel(mdmm_block_norm_t p) {
   };
   fetch_row(row);
   for (; row < p.rows; row += step) {
-    float x[NV][VEC], g[NV][VEC], sg[NV][VEC], o[NV][VEC], q[NV][VEC], d[NV][VEC];
-    float ss = 0.0f;
+    A x[NV][VEC], g[NV][VEC], sg[NV][VEC], o[NV][VEC], q[NV][VEC], d[NV][VEC];
+    A ss = 0.0f;
+    auto taken = [](const auto& raw, A* v) {
+      float f[VEC];
+      widen(raw, f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = f[e];
+    };
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if (ALL || p.y) widen(ry[k], x[k]);
-      if (ALL || p.gate) widen(rg[k], g[k]);
-      if (ALL || p.g_n) widen(res[k], o[k]);
-      if (ALL || p.g_n) widen(rq[k], q[k]);
-      widen(rd[k], d[k]);
+      if (ALL || p.y) taken(ry[k], x[k]);
+      if (ALL || p.gate) taken(rg[k], g[k]);
+      if (ALL || p.g_n) taken(res[k], o[k]);
+      if (ALL || p.g_n) taken(rq[k], q[k]);
+      taken(rd[k], d[k]);
       if (ALL || p.y)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) ss += x[k][e] * x[k][e];
     }
     fetch_row(row + step);                   // in flight behind this row's arithmetic
-    float r = 0.0f;
+    A r = 0.0f;
     if (ALL || p.y) {
-      r = rsqrtf(row_sum<WIDE>(ss, lds, slot) * inv + p.eps);
+      r = rsqrt_(row_sum<WIDE>(ss, lds, slot) * inv + p.eps);
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           x[k][e] *= r;
-          sg[k][e] = (ALL || p.gate) ? sigmoid_(g[k][e]) : 1.0f;
+          sg[k][e] = (ALL || p.gate) ? gate_(g[k][e]) : (A)1.0;
         }
     }
     if (ALL || p.g_n) {
-      float sums[2] = {0.0f, 0.0f};
+      A sums[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           if (ALL || p.y) {
-            float u = x[k][e] * w[k][e];
+            A u = x[k][e] * w[k][e];
             if (ALL || p.gate) u *= g[k][e] * sg[k][e];
-            o[k][e] = fmaf(s[k][e], u, o[k][e]);
+            o[k][e] = fma_((A)s[k][e], u, o[k][e]);
           }
           sums[0] += o[k][e] * o[k][e];
           sums[1] += q[k][e] * wn[k][e] * o[k][e];
         }
       row_sums<WIDE, 2>(sums, lds, slot);
-      const float r2 = rsqrtf(sums[0] * inv + p.eps), m = sums[1] * inv * r2 * r2;
+      const A r2 = rsqrt_(sums[0] * inv + p.eps), m = sums[1] * inv * r2 * r2;
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -283,19 +304,19 @@ void norm_bwd_kernel(mdmm_block_norm_t p) {
       for (int k = 0; k < NV; ++k) out.put(d[k], c[k]);
     }
     if (ALL || p.y) {
-      float sm = 0.0f;
+      A sm = 0.0f;
       const Row<Br, VEC> out(p.d_gate, row * p.d_gate_st, p.H);
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        float dg[VEC];
+        A dg[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           // act = silu(g) = g sg, slope = silu'(g) = sg + act (1 - sg)
-          const float act = (ALL || p.gate) ? g[k][e] * sg[k][e] : 1.0f;
-          const float u = x[k][e] * w[k][e], ds = d[k][e] * s[k][e];
+          const A act = (ALL || p.gate) ? g[k][e] * sg[k][e] : (A)1.0;
+          const A u = x[k][e] * w[k][e], ds = d[k][e] * s[k][e];
           as[k][e] += d[k][e] * act * u;
-          dg[e] = ds * u * fmaf(-act, sg[k][e], sg[k][e] + act);
-          const float t = ds * act;
+          dg[e] = ds * u * fma_(-act, sg[k][e], sg[k][e] + act);
+          const A t = ds * act;
           aw[k][e] += t * x[k][e];
           d[k][e] = t * w[k][e];
           sm += d[k][e] * x[k][e];
@@ -307,7 +328,7 @@ void norm_bwd_kernel(mdmm_block_norm_t p) {
         const Row<Y, VEC> dst(p.d_y, row * p.d_y_st, p.H);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-          float dy[VEC];
+          A dy[VEC];
 #pragma unroll
           for (int e = 0; e < VEC; ++e) dy[e] = r * (d[k][e] - x[k][e] * sm);
           dst.put(dy, c[k]);
@@ -321,11 +342,11 @@ void norm_bwd_kernel(mdmm_block_norm_t p) {
   for (int which = 0; which < 3; ++which)
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      float (&acc)[VEC] = which == 0 ? aw[k] : which == 1 ? as[k] : an[k];
+      auto& acc = which == 0 ? aw[k] : which == 1 ? as[k] : an[k];
       if constexpr (!WIDE) {
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) fold[threadIdx.x * VEC + e] = acc[e];
+        for (int e = 0; e < VEC; ++e) fold[threadIdx.x * VEC + e] = (float)acc[e];
         __syncthreads();
         if (threadIdx.x < 64 * VEC) {
           const int i = threadIdx.x, col = k * 64 * VEC + i;
@@ -334,7 +355,7 @@ void norm_bwd_kernel(mdmm_block_norm_t p) {
       } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
-          if (c[k] + e < p.H) slab[which * p.H + c[k] + e] = acc[e];
+          if (c[k] + e < p.H) slab[which * p.H + c[k] + e] = (float)acc[e];
       }
     }
 }
@@ -440,6 +461,7 @@ Plan plan(const mdmm_block_norm_t* a) {
                   aligned(a->g_n, a->g_n_st, a->branch_bf16) && aligned(a->d_y, a->d_y_st, a->y_bf16) &&
                   aligned(a->d_gate, a->d_gate_st, a->branch_bf16) && aligned(a->d_res, a->d_res_st, a->res_bf16) &&
                   aligned(a->w, 0, 0) && aligned(a->scale, 0, 0) && aligned(a->w_next, 0, 0);
+  if (a->H <= 4) return {1, 1, 256, 256};          // (64-bit arithmetic: norm_bwd_kernel)
   const int h = a->H, w4 = (h + 255) / 256 * 64, w8 = (h + 511) / 512 * 64;
   if (v4) {
     if (h <= 256) return {4, 1, 256, 256};
@@ -501,7 +523,7 @@ int dispatch(const mdmm_block_norm_t* a, bool bwd, hipStream_t s) {
   const int64_t g = grid_of(a, q, bwd);
 #define CASE(v, n, t) if (q.vec == v && q.nv == n && q.maxt == t) return launch<Y, Br, R, v, n, t>(a, g, q.threads, bwd, s)
   CASE(4, 1, 256); CASE(4, 1, 512); CASE(4, 2, 512); CASE(4, 2, 1024);
-  CASE(1, 4, 256); CASE(1, 4, 512); CASE(1, 4, 1024); CASE(1, 8, 1024);
+  CASE(1, 1, 256); CASE(1, 4, 256); CASE(1, 4, 512); CASE(1, 4, 1024); CASE(1, 8, 1024);
 #undef CASE
   return MDMM_E_ARG;
 }

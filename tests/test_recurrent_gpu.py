@@ -660,3 +660,29 @@ def test_modules_import_in_any_order(module):
     """Each as the first module of a process."""
     subprocess.run([sys.executable, '-c', 'import mdmm.%s, mdmm.ops; mdmm.ops.gated_scan, mdmm.ops.orthogonalise' % module],
                    check=True, env=dict(os.environ, PYTHONPATH=os.path.dirname(os.path.dirname(native.__file__))), timeout=300)
+
+
+@gpu
+@pytest.mark.parametrize('H', [1, 2, 3, 4])
+def test_narrow_rows_keep_their_gradients(H):
+    """A row of one column is normalised to its sign: its gradient is eps r^3, what two nearly equal terms leave.  The inputs
+    are exact, the arithmetic is 64-bit and only the stored gradients (and the fp32 slabs of the sums, 4 u of their terms'
+    absolute sum) are rounded."""
+    gen = torch.Generator().manual_seed(11)
+    t = [make(gen, 300, H) for _ in range(5)] + [make(gen, H, mean=1.0, std=0.2) for _ in range(3)]
+    y, res, gate, g_out, g_n, w, s, w2 = t
+    cpu = [v.double().requires_grad_() for v in (y, res, w, gate, s, w2)]
+    out = cpu[1] + cpu[4] * torch.nn.functional.silu(cpu[3]) * cpu[0] * (cpu[0].square().mean(-1, keepdim=True) + 1e-6).rsqrt() * cpu[2]
+    n = out * (out.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * cpu[5]
+    want = torch.autograd.grad([out, n], cpu, [g_out.double(), g_n.double()])
+    dev = [v.cuda().requires_grad_() for v in (y, res, w, gate, s, w2)]
+    got = torch.autograd.grad(ops.block_norm(dev[0], dev[1], dev[2], gate=dev[3], scale=dev[4], next_weight=dev[5]), dev,
+                              [g_out.cuda(), g_n.cuda()])
+    # terms of the sums: d_w = sum d_y-like terms p y r, bounded by |d_res s silu(g) y r| etc.
+    r = (y.double().square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    act = torch.nn.functional.silu(gate.double())
+    terms = {2: want[1] * s.double() * act * y.double() * r, 4: want[1] * act * y.double() * r * w.double(),
+             5: g_n.double() * out.detach() * (out.detach().square().mean(-1, keepdim=True) + 1e-6).rsqrt()}
+    for i, (a, b) in enumerate(zip(got, want)):
+        bound = 8 * U * terms[i].abs().sum(0) if i in terms else 2 * U * b.abs()
+        assert ((a.cpu().double() - b).abs() <= bound + 1e-38).all(), (i, (a.cpu().double() - b).abs().max())
