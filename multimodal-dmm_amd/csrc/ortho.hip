@@ -3,17 +3,17 @@
 //
 // The iteration multiplies a small singular value by up to ca a step (ca^5 = 485 over five), and a rounding of X with it, so
 // bf16 operands are out; fp32 ones would run on the fp32 matrix instruction, a sixteenth of the fp16 one's rate.  Matrices
-// with more than 64 rows are kept as two fp16 planes instead, s x = h + l with h = fp16(s x), l = fp16(s x - h): 22 to 23
+// with more than 128 rows are kept as two fp16 planes instead, s x = h + l with h = fp16(s x), l = fp16(s x - h): 22 to 23
 // bits.  s is as large as the entries allow (X and A stay below 2: 2^14; P below 16: 2^12), so that l is a normal number down
 // to entries of 1e-5 and below those wrong by 2e-12.  A product is h h' + h l' + l h': three fp16 matrix instructions, the
 // dropped l l' 2^-23 of a term: the result is nearer to 64 bits than fp32 products by the library (6e-7 against 2.9e-6 at
-// 2048 x 2048).  ca X is added in fp32.  (Up to 64 rows: fp32, see WHOLE.)
+// 2048 x 2048).  ca X is added in fp32.  (Up to 128 rows: fp32, see WHOLE.)
 //
 // X is stored both ways (n x m for A, m x n for P X) so that every product runs over two operands' rows.  A row keeps 32
 // columns of h, then the same 32 of l: one cache line for a step of 32 (with the planes apart, each step took half lines and
-// two 2048 x 2048 products 142 us); fp32 rows take the same bytes.  Tiles come straight into LDS, a step or more ahead, chunks of 16 bytes swapped within a
-// row so that the matrix instruction's reads meet all banks; neighbouring tiles go to one XCD, whose L2 then holds their
-// rows.  A and P are symmetric: tiles at and above the diagonal only, stored twice.  Sizes are rounded up to whole tiles with
+// two 2048 x 2048 products 142 us); fp32 rows take the same bytes.  Tiles come straight into LDS, a step or more ahead, chunks
+// of 16 bytes swapped within a row so that the matrix instruction's reads meet all banks; neighbouring tiles go to one XCD,
+// whose L2 then holds their rows.  A and P are symmetric: tiles at and above the diagonal only, stored twice.  Sizes are rounded up to whole tiles with
 // zeros, which every product keeps.  All matrices of a call share each launch.
 //
 // Large matrices are bound by feeding the matrix instruction: P X of two 2048 x 2048 takes 112 us (920 TFLOP/s of fp16, the
@@ -47,14 +47,15 @@ template <int BM_, int BN_, int BK_, int ST_, int WI_, int WJ_, int OCC_> struct
   static constexpr int LOADS = HALVES / 8 / T;                  // chunks a thread loads for a buffer
   static_assert(BM * CPR % T == 0 && BN * CPR % T == 0, "a load instruction of the workgroup stays in one operand");
 };
-// A matrix whose shorter side fits one small tile is kept in fp32 and multiplied by the fp32 matrix instruction.  The fp16 one
+// A matrix whose shorter side fits two small tiles is kept in fp32 and multiplied by the fp32 matrix instruction.  The fp16 one
 // aligns the products of eight columns to the largest of them and drops what falls below its last bit: no matter beside the
-// rounding of fp32 sums over hundreds of rows, but over a few of them the larger error (7 x 146: 1.8e-6 off against 0.7e-6
-// in fp32 by the library).  A wave's step takes 1024 cycles instead of 192, which such a matrix's few steps have room for.
-constexpr int WHOLE = 64;
+// rounding of fp32 sums over hundreds of rows, but over a few of them the larger error (7 x 146: 2.1e-6 off against 0.7e-6
+// in fp32 by the library, 65 x 1500: 1.6e-6 against 1.1e-6; here 0.9e-6 and 0.8e-6).  A wave's step takes 1024 cycles instead of
+// 192, which such a matrix's few steps have room for.
+constexpr int WHOLE = 128;
 // (two workgroups a CU, four buffers each.  P X of two 256 x 4096: 13.6 us, with one of 128 KB 17)
 typedef Cfg<64, 64, 32, 4, 2, 2, 2> Small;
-static_assert(Small::BM == WHOLE && Small::BN == WHOLE && Small::TI * Small::TJ == 1, "one tile, one piece a wave");
+static_assert(Small::TI * Small::TJ == 1, "fp32 rows: one piece a wave");
 // (two workgroups a CU, two buffers each.  Measured on P X of two 2048 x 2048: 112 us; one workgroup with four buffers 127, one
 // of 256 x 128 and 8 waves with three 126, steps of 64 columns 126)
 typedef Cfg<128, 128, 32, 2, 2, 2, 2> Large;
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(NT) void ortho_pack_kernel(const Call* __restrict__
     __syncthreads();
     for (int i = threadIdx.x; i < 4096; i += NT) put(place(other, c0 + i / 64, ld_other, r0 + i % 64, whole), tile[i % 64][i / 64], whole);
   };
-  if (w.n == WHOLE) store(std::true_type{});
+  if (w.n <= WHOLE) store(std::true_type{});
   else store(std::false_type{});
 }
 
@@ -533,8 +534,8 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
   const Item w = ws.of(f.k);
   mdmm_ortho_item_t t = {};
   if (MODE == LAST) t = ts.of(f.k);
-  if constexpr (C::BM == WHOLE)
-    if (w.n == WHOLE) {
+  if constexpr (C::TI * C::TJ == 1)
+    if (w.n <= WHOLE) {
       product<MODE, C, true>(lds, call, w, t, me - f.first, flip);
       return;
     }
@@ -561,7 +562,7 @@ template <int BM, int BN> __global__ __launch_bounds__(NT) void ortho_fold_kerne
       put_sym(w.gram, n, i, j, f, j0 < i0 + BM, whole);
     }
   };
-  if (BM == WHOLE && n == WHOLE) join(std::true_type{});
+  if (BM < 128 && n <= WHOLE) join(std::true_type{});
   else join(std::false_type{});
 }
 
@@ -573,7 +574,7 @@ __global__ __launch_bounds__(NT) void ortho_copy_kernel(const Call* __restrict__
   const int64_t total = (int64_t)t.rows * t.cols;
   for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)gridDim.x * NT) {
     const int64_t r = i / t.cols, c = i % t.cols;
-    const bool whole = w.n == WHOLE;
+    const bool whole = w.n <= WHOLE;
     const half_t* x = place(w.xn, w.tall ? c : r, w.m, w.tall ? r : c, whole);
     const float v = (whole ? *(const float*)x : (float)x[0] + (float)x[32]) * (1.0f / SX);
     const int64_t to = r * t.dst_ld + c;
