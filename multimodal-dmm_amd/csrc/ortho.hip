@@ -16,9 +16,9 @@
 // whose L2 then holds their rows.  A and P are symmetric: tiles at and above the diagonal only, stored twice.  Sizes are rounded up to whole tiles with
 // zeros, which every product keeps.  All matrices of a call share each launch.
 //
-// Large matrices are bound by feeding the matrix instruction: P X of two 2048 x 2048 takes 112 us (920 TFLOP/s of fp16, the
+// Large matrices are bound by feeding the matrix instruction: P X of two 2048 x 2048 takes 115 us (900 TFLOP/s of fp16, the
 // library's own fp16 product of that size 640), without its loads 78, without its matrix instructions 76.  Small ones are
-// bound by the seventeen launches of five steps, 8 to 12 us each.
+// bound by the seventeen launches of five steps, 6 to 11 us each.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <type_traits>
