@@ -1068,9 +1068,9 @@ int mdmm_cat_head_nll_bwd(const float* hid, const float* w, const float* label, 
  * Gated linear recurrence over time (ABI 34), the recurrence of an inference RNN without a recurrent product: per channel
  *   h_t = a_t h_{t-1} + (1 - a_t) c_t,   a_t = sigmoid(f_t);   mask[t][b] = 0: h_t = h_{t-1} (f, c of that step not used)
  * as the skip updates of the GRU above (dks.py:224-227).  gates (T, B, >= 2H): f in columns [0, H), c in [H, 2H), unit
- * stride along the columns, any strides over t and b (elements); fp32, or bf16 with gates_bf16.  h (T, B, H) contiguous,
- * time-indexed, fp32 or (with gates_bf16 only) bf16 with h_bf16.  The state is fp32 throughout.  reverse: from the last
- * step to the first.  h0: row b at b * h0_sb (0: one row for all; NULL: zeros).  h_last (B, H): the state behind the last
+ * stride along the columns, any strides over t and b (elements, none over b negative); fp32, or bf16 with gates_bf16.
+ * h (T, B, H) contiguous, time-indexed, fp32 or (with gates_bf16 only) bf16 with h_bf16.  The state is fp32 throughout.
+ * reverse: from the last step to the first.  h0: row b at b * h0_sb (0: one row for all; NULL: zeros).  h_last (B, H): the state behind the last
  * step taken (NULL: not wanted).
  * states: mdmm_gated_scan_states() floats the forward pass leaves for the backward one (NULL in a forward-only call).
  * ws: mdmm_gated_scan_ws(a, bwd) floats of scratch per call (0: NULL is fine).
