@@ -56,8 +56,8 @@ constexpr int WHOLE = 128;
 // (two workgroups a CU, four buffers each.  P X of two 256 x 4096: 13.6 us, with one of 128 KB 17)
 typedef Cfg<64, 64, 32, 4, 2, 2, 2> Small;
 static_assert(Small::TI * Small::TJ == 1, "fp32 rows: one piece a wave");
-// (two workgroups a CU, two buffers each.  Measured on P X of two 2048 x 2048: 112 us; one workgroup with four buffers 127, one
-// of 256 x 128 and 8 waves with three 126, steps of 64 columns 126)
+// (two workgroups a CU, two buffers each.  Measured on P X of two 2048 x 2048: 115 us; one workgroup with four buffers 127, one
+// of 256 x 128 and 8 waves with three 126, 8 waves 125, tiles of 128 x 64 139, steps of 64 columns 126)
 typedef Cfg<128, 128, 32, 2, 2, 2, 2> Large;
 
 struct Item {               // one matrix's padded sizes and workspace
@@ -601,9 +601,15 @@ int check(const mdmm_ortho_t* a) {
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// 128 x 128 tiles where the shorter side holds four of them, else 64 x 64: a small matrix is a matter of latency, and the
-// larger tile halves what a product loads
-bool large(const mdmm_ortho_item_t& t) { return (t.rows < t.cols ? t.rows : t.cols) > 384; }
+// A call's larger matrices (more than 384 rows) take 128 x 128 tiles in P X, where those are 256 or more, one for each CU: the
+// larger tile halves what a product loads.  Fewer leave CUs idle and the others alone with one workgroup, whose loads and
+// products then hardly overlap.  Five steps with it and with the small tile: 1000 x 4096 (256 tiles) 482 us and 513, one
+// 2048 x 2048 (256) 892 and 945, two (512) 1470 and 1676; with A and P on large tiles too, two of 2048 x 2048 1553, one 971, one
+// 400 x 400 373 where small ones take 141
+int64_t large_tiles(const mdmm_ortho_item_t& t) {
+  const int64_t n = t.rows < t.cols ? t.rows : t.cols, m = t.rows < t.cols ? t.cols : t.rows;
+  return n > 384 ? up(n, Large::BM) / Large::BM * (up(m, Large::BN) / Large::BN) : 0;
+}
 
 // the workspace: fills both size classes' lists (base NULL: sizes only), returns the bytes used
 int64_t lay_out(const mdmm_ortho_t* a, Items (&q)[2], mdmm_ortho_item_t (*items)[MDMM_ORTHO_MAX] = nullptr) {
@@ -611,22 +617,24 @@ int64_t lay_out(const mdmm_ortho_t* a, Items (&q)[2], mdmm_ortho_item_t (*items)
   int64_t off = 2 * up(sizeof(Call), 256);
   auto take = [&](int64_t bytes) { char* p = base + off; off += up(bytes, 256); return p; };
   q[0].n = q[1].n = 0;
+  int64_t total = 0;
+  for (int i = 0; i < a->n; ++i) total += large_tiles(a->item[i]);
   for (int i = 0; i < a->n; ++i) {
     const mdmm_ortho_item_t& t = a->item[i];
-    const bool big = large(t);
+    const bool big = total >= 256 && large_tiles(t) > 0;
     Items& l = q[big];
     if (items) items[big][l.n] = t;
     Item& w = l.it[l.n++];
-    const int pad = big ? Large::BM : Small::BM, bk = big ? Large::BK : Small::BK;
+    const int pad = big ? Large::BM : Small::BM;
     w.tall = t.rows > t.cols;
     w.n = (int32_t)up(w.tall ? t.cols : t.rows, pad);
     w.m = (int32_t)up(w.tall ? t.rows : t.cols, pad);
     // slices of A: from 2048 columns on, while the tiles leave CUs idle, of 512 columns at least (joining them is a launch
     // more, 4 us with its gap, which is what 768 columns take in one piece)
-    const int64_t tiles = big ? tri<Large>(w.n) : tri<Small>(w.n);
+    const int64_t tiles = tri<Small>(w.n);
     int64_t splits = w.m >= 2048 ? (128 / tiles < w.m / 512 ? 128 / tiles : w.m / 512) : 1;
     if (splits < 1) splits = 1;
-    const int64_t steps = w.m / bk, per = (steps + splits - 1) / splits;
+    const int64_t steps = w.m / Small::BK, per = (steps + splits - 1) / splits;
     w.splits = (int32_t)((steps + per - 1) / per);
     const int64_t x = (int64_t)w.n * w.m, g = (int64_t)w.n * w.n;
     w.xn = (half_t*)take(4 * x);
@@ -650,7 +658,8 @@ template <class F> int tiles(Items& q, int list, F count) {
   return (int)total;
 }
 
-template <class C> void launch(const mdmm_ortho_t* a, const Items& items, const mdmm_ortho_item_t* mats, Call* keep, hipStream_t s) {
+// C: the tile of A and P, D: that of P X
+template <class C, class D> void launch(const mdmm_ortho_t* a, const Items& items, const mdmm_ortho_item_t* mats, Call* keep, hipStream_t s) {
   if (!items.n) return;
   Call c;
   c.p = *a;
@@ -660,7 +669,7 @@ template <class C> void launch(const mdmm_ortho_t* a, const Items& items, const 
   const int packs = tiles(q, PACKS, [](const Item& w) { return (int64_t)(w.n / 64) * (w.m / 64); });
   const int gram = tiles(q, GRAMS, [](const Item& w) { return (int64_t)tri<C>(w.n) * w.splits; });
   const int poly = tiles(q, POLYS, [](const Item& w) { return (int64_t)tri<C>(w.n); });
-  const int apply = tiles(q, APPLIES, [](const Item& w) { return (int64_t)(w.n / C::BM) * (w.m / C::BN); });
+  const int apply = tiles(q, APPLIES, [](const Item& w) { return (int64_t)(w.n / D::BM) * (w.m / D::BN); });
   int64_t fold = 0;
   for (int i = 0; i < q.n; ++i)
     if (q.it[i].splits > 1 && (int64_t)q.it[i].n * q.it[i].n > fold) fold = (int64_t)q.it[i].n * q.it[i].n;
@@ -671,8 +680,8 @@ template <class C> void launch(const mdmm_ortho_t* a, const Items& items, const 
     hipLaunchKernelGGL((ortho_product_kernel<GRAM, C>), dim3(gram), dim3(C::T), 0, s, keep, k & 1);
     if (fold) hipLaunchKernelGGL((ortho_fold_kernel<C::BM, C::BN>), dim3((unsigned)(fold / (4 * NT)), q.n), dim3(NT), 0, s, keep);
     hipLaunchKernelGGL((ortho_product_kernel<POLY, C>), dim3(poly), dim3(C::T), 0, s, keep, k & 1);
-    if (k + 1 < a->steps) hipLaunchKernelGGL((ortho_product_kernel<APPLY, C>), dim3(apply), dim3(C::T), 0, s, keep, k & 1);
-    else hipLaunchKernelGGL((ortho_product_kernel<LAST, C>), dim3(apply), dim3(C::T), 0, s, keep, k & 1);
+    if (k + 1 < a->steps) hipLaunchKernelGGL((ortho_product_kernel<APPLY, D>), dim3(apply), dim3(D::T), 0, s, keep, k & 1);
+    else hipLaunchKernelGGL((ortho_product_kernel<LAST, D>), dim3(apply), dim3(D::T), 0, s, keep, k & 1);
   }
 }
 
@@ -697,7 +706,7 @@ extern "C" int mdmm_ortho(const mdmm_ortho_t* a, void* stream) {
   Items q[2] = {};
   mdmm_ortho_item_t mats[2][MDMM_ORTHO_MAX] = {};
   lay_out(a, q, mats);
-  launch<Small>(a, q[0], mats[0], (Call*)a->ws, (hipStream_t)stream);
-  launch<Large>(a, q[1], mats[1], (Call*)((char*)a->ws + up(sizeof(Call), 256)), (hipStream_t)stream);
+  launch<Small, Small>(a, q[0], mats[0], (Call*)a->ws, (hipStream_t)stream);
+  launch<Small, Large>(a, q[1], mats[1], (Call*)((char*)a->ws + up(sizeof(Call), 256)), (hipStream_t)stream);
   return (int)hipGetLastError();
 }

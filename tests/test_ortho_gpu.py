@@ -214,3 +214,12 @@ def test_short_sides(shape):
     for steps in (0, 1, 5):
         check(m, ops.orthogonalise([m], steps=steps)[0], steps)
     assert torch.equal(m, keep)
+
+
+@gpu
+def test_large_and_small_together():
+    """Enough large matrices for the large tile, of odd sizes and both orientations, beside small ones."""
+    gen = torch.Generator().manual_seed(12)
+    mats = [(0.01 * torch.randn(s, generator=gen)).cuda() for s in ((1100, 1500), (20, 30), (1500, 1101), (900, 2001), (200, 70))]
+    for m, o in zip(mats, ops.orthogonalise(mats)):
+        check(m, o)
