@@ -164,8 +164,9 @@ __device__ __forceinline__ float src_at(const mdmm_ortho_t& p, const mdmm_ortho_
   return p.src_bf16 ? (float)((const __bf16*)t.src)[i] : ((const float*)t.src)[i];
 }
 
-// momentum, and the sum of squares in SUMS pieces (in 64 bits: an error of the norm is a scale of X and grows like one)
-__global__ __launch_bounds__(NT) void ortho_sums_kernel(Call call, Call* keep) {
+// momentum, and the sum of squares in SUMS pieces (in 64 bits: an error of the norm is a scale of X and grows like one).
+// LONG: eight loads of a thread on their way at once (two of 2048 x 2048 25 -> 12 us; eleven small matrices 6.4 -> 10)
+template <bool LONG> __global__ __launch_bounds__(NT) void ortho_sums_kernel(Call call, Call* keep) {
   const mdmm_ortho_t& p = call.p;
   const int k = blockIdx.y;
   const mdmm_ortho_item_t& t = p.item[k];
@@ -176,17 +177,29 @@ __global__ __launch_bounds__(NT) void ortho_sums_kernel(Call call, Call* keep) {
   double s = 0.0;
   // a workgroup's rows, its threads over the columns (rows shorter than a workgroup: several of them at once)
   const int wide = t.cols < NT ? (t.cols < 16 ? 16 : t.cols < 64 ? 64 : NT) : NT, high = NT / wide;
-  for (int64_t r = (int64_t)blockIdx.x * high + threadIdx.x / wide; r < t.rows; r += (int64_t)SUMS * high)
-    for (int64_t c = threadIdx.x % wide; c < t.cols; c += wide) {
-      float v = src_at(p, t, r, c);
+  for (int64_t r = (int64_t)blockIdx.x * high + threadIdx.x / wide; r < t.rows; r += (int64_t)SUMS * high) {
+    int64_t c = threadIdx.x % wide;
+    auto take = [&](float v, float before, int64_t at) {
       if (t.mom) {
-        float* mom = t.mom + r * t.cols + c;
-        const float mv = fmaf(p.momentum, *mom, v);
-        *mom = mv;
+        const float mv = fmaf(p.momentum, before, v);
+        t.mom[at] = mv;
         v = p.nesterov ? fmaf(p.momentum, mv, v) : mv;
       }
       s += (double)v * v;
-    }
+    };
+    if constexpr (LONG)
+      for (; c + 7 * wide < t.cols; c += 8 * wide) {
+        float v[8], before[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = src_at(p, t, r, c + e * wide);
+          before[e] = t.mom ? t.mom[r * t.cols + c + e * wide] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) take(v[e], before[e], r * t.cols + c + e * wide);
+      }
+    for (; c < t.cols; c += wide) take(src_at(p, t, r, c), t.mom ? t.mom[r * t.cols + c] : 0.0f, r * t.cols + c);
+  }
   __shared__ double part[NT / 64];
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
@@ -562,7 +575,7 @@ template <int BM, int BN> __global__ __launch_bounds__(NT) void ortho_fold_kerne
       put_sym(w.gram, n, i, j, f, j0 < i0 + BM, whole);
     }
   };
-  if (BM < 128 && n <= WHOLE) join(std::true_type{});
+  if (n <= WHOLE) join(std::true_type{});
   else join(std::false_type{});
 }
 
@@ -673,7 +686,7 @@ template <class C, class D> void launch(const mdmm_ortho_t* a, const Items& item
   int64_t fold = 0;
   for (int i = 0; i < q.n; ++i)
     if (q.it[i].splits > 1 && (int64_t)q.it[i].n * q.it[i].n > fold) fold = (int64_t)q.it[i].n * q.it[i].n;
-  hipLaunchKernelGGL(ortho_sums_kernel, dim3(SUMS, q.n), dim3(NT), 0, s, c, keep);
+  hipLaunchKernelGGL((ortho_sums_kernel<D::BM == Large::BM>), dim3(SUMS, q.n), dim3(NT), 0, s, c, keep);
   hipLaunchKernelGGL(ortho_pack_kernel, dim3(packs), dim3(NT), 0, s, keep);
   if (a->steps == 0) hipLaunchKernelGGL(ortho_copy_kernel, dim3(256, q.n), dim3(NT), 0, s, keep);
   for (int k = 0; k < a->steps; ++k) {
