@@ -162,6 +162,7 @@ class FlatAdam(torch.optim.Optimizer):
                       self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), b.flat.numel(), self.step_dev.data_ptr(),
                       None if lr_dev is None else lr_dev.data_ptr(), 0.0 if lr_dev is not None else float(lr),
                       float(grp['betas'][0]), float(grp['betas'][1]), float(grp['eps']), float(grp['weight_decay']))
+        torch.autograd.graph.increment_version(b.params)        # (written by address: what is cached by version is stale)
         return loss
 
     def check_replay(self):
@@ -323,6 +324,7 @@ class FlatMuon(torch.optim.Optimizer):
                           self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), b.flat.numel(), self.step_dev.data_ptr(),
                           ops._ptr(lr_dev), lr, float(g['betas'][0]), float(g['betas'][1]), float(g['eps']),
                           float(g['weight_decay']))
+        torch.autograd.graph.increment_version(b.params)        # (written by address: what is cached by version is stale)
         return loss
 
     def check_replay(self):

@@ -127,6 +127,12 @@ class GatedLinearRNN(nn.Module):
 
     def forward(self, x, h0, mask=None, reverse=False, precision=None):
         from .. import ops
+        ops.drop_packs(self.parameters())      # (a graph captured here has to build its own at every replay)
+        return self.run(x, h0, mask, reverse, precision)
+
+    def run(self, x, h0, mask=None, reverse=False, precision=None):
+        """forward for a caller that has dropped the parameters' operand packs at its own entry (MultiDKS)."""
+        from .. import ops
         t_max, b_dim = x.shape[:2]
         res = ops.tall_projection(x.reshape(t_max * b_dim, -1), self.inp.weight, self.inp.bias, precision)
         h_dim = res.shape[1]

@@ -128,7 +128,7 @@ class MultiDKS(MultiDGTS):
         t_max, b_dim = feat.shape[:2]
         gru = self.rnn[m]
         if isinstance(gru, common.GatedLinearRNN):
-            return gru(feat, self.h0[m][:, 0], mask if self.rnn_skip else None, self.rnn_dir == 'bwd', self.sweep_dtype)
+            return gru.run(feat, self.h0[m][:, 0], mask if self.rnn_skip else None, self.rnn_dir == 'bwd', self.sweep_dtype)
         x = feat.reshape(t_max * b_dim, -1)
         h_seq = None
         for layer in range(gru.num_layers):

@@ -406,6 +406,11 @@ def clear_caches(params=()):
         _GRAD_SCALE.clear()
         raise native.MdmmError('a Bernoulli-loss gradient left without its upstream scalar was never taken by the layer that '
                                'produced the logits (ops._GRAD_SCALE): the last backward pass used an unscaled gradient')
+    drop_packs(params)
+
+
+def drop_packs(params):
+    """Drop the operand packs cached on parameters: the next use of each builds its own from the parameter's present values."""
     for p in params:
         if hasattr(p, '_mdmm_pack'):
             del p._mdmm_pack
@@ -1777,7 +1782,9 @@ class _LinearTilesFn(torch.autograd.Function):
         heads = (_heads_shape(k, n) and os.environ.get('MDMM_GEMM_GENERIC') != '1'
                  and (k == 256 or x.dtype == torch.bfloat16) and (n == 256 or out_dtype == torch.bfloat16 or k == 256))
         if heads:
-            wf = _lin_pack(weight)[0]
+            # (the transpose is the backward pass's, kept for it: by then another call may have built packs of its own on the
+            # weight, inside a graph that is not replayed yet)
+            wf, ctx.pack_t = _lin_pack(weight)
             if x.dtype != torch.bfloat16:
                 x = x.to(torch.bfloat16)            # (the saved copy too: half the bytes)
         else:
@@ -1816,7 +1823,7 @@ class _LinearTilesFn(torch.autograd.Function):
             if g.dtype != torch.bfloat16:
                 g = g.to(torch.bfloat16)
             if ctx.needs_input_grad[0]:
-                gx = _gemm_bf16(g, False, _lin_pack(weight)[1], False, m, k, n, tag='linear_dgrad[%dx%d]' % (k, n),
+                gx = _gemm_bf16(g, False, ctx.pack_t, False, m, k, n, tag='linear_dgrad[%dx%d]' % (k, n),
                                 out_dtype=gx_dtype)
         elif ctx.needs_input_grad[0]:
             gx = _gemm_bf16(g, False, w, True, m, k, n, tag='linear_dgrad[%dx%d]' % (k, n), out_dtype=gx_dtype)

@@ -355,3 +355,77 @@ def test_replayed_training_step():
     # replayed): a relative 2^-24 of each gradient, which Adam's first steps (a sign) do not amplify beyond lr 1e-3 x 1e-4
     for k in ends[0]:
         assert (ends[0][k] - ends[1][k]).abs().max() <= 1e-5, k
+
+
+@gpu
+@pytest.mark.parametrize('opt_kind', ['muon', 'adam'])
+def test_weights_that_an_optimizer_wrote_are_the_ones_used(opt_kind):
+    """The module on its own with bf16 operands at a width whose products keep the weight's bf16 copy: after updates through
+    the optimizer's launches, outputs and gradients are bit for bit those of a new module of the same weights."""
+    torch.manual_seed(4)
+    T, B, H = 16, 32, 256
+    rnn = common.GatedLinearRNN(H, H, 2).cuda()
+    x, h0, g = torch.randn(T, B, H).cuda(), torch.zeros(2, H).cuda(), torch.randn(T, B, H).cuda()
+    bucket = GradBucket(rnn.parameters())
+    opt = FlatMuon(bucket, lr=0.05) if opt_kind == 'muon' else FlatAdam(bucket, lr=0.05)
+
+    def run(m):
+        xd = x.clone().requires_grad_(True)
+        y = m(xd, h0, None, False, torch.bfloat16)
+        y.backward(g)
+        return y.detach(), xd.grad
+    for _ in range(3):
+        bucket.release()
+        got = run(rnn)
+        new = common.GatedLinearRNN(H, H, 2).cuda()
+        new.load_state_dict(rnn.state_dict())
+        for a, b in zip(got, run(new)):
+            assert torch.equal(a, b)
+        for p, q in zip(rnn.parameters(), new.parameters()):
+            assert torch.equal(p.grad, q.grad)
+        bucket.check_views()
+        versions = [p._version for p in rnn.parameters()]
+        opt.step()
+        assert all(p._version > v for p, v in zip(rnn.parameters(), versions))
+
+
+@gpu
+def test_replayed_module_uses_the_present_weights():
+    """A forward pass captured after eager ones, replayed after updates of the weights: what the eager module gives."""
+    torch.manual_seed(5)
+    T, B, H = 16, 32, 256
+    rnn = common.GatedLinearRNN(H, H, 1).cuda()
+    x, h0 = torch.randn(T, B, H).cuda(), torch.zeros(1, H).cuda()
+    bucket = GradBucket(rnn.parameters())
+    opt = FlatMuon(bucket, lr=0.05)
+    with torch.no_grad():
+        rnn(x, h0, None, False, torch.bfloat16)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = rnn(x, h0, None, False, torch.bfloat16)
+    for k in range(3):
+        bucket.flat.normal_()
+        opt.step()
+        graph.replay()
+        new = common.GatedLinearRNN(H, H, 1).cuda()
+        new.load_state_dict(rnn.state_dict())
+        with torch.no_grad():
+            want = new(x, h0, None, False, torch.bfloat16)
+        torch.cuda.synchronize()
+        assert torch.equal(held, want)
+
+
+@gpu
+def test_eager_backward_behind_a_capture():
+    """A backward pass of an eager call after another call of the module was captured and not replayed."""
+    torch.manual_seed(7)
+    T, B, H = 16, 32, 256
+    rnn = common.GatedLinearRNN(H, H, 1).cuda()
+    x, h0, g = torch.randn(T, B, H).cuda(), torch.zeros(1, H).cuda(), torch.randn(T, B, H).cuda()
+    xd = x.clone().requires_grad_(True)
+    want = torch.autograd.grad(rnn(xd, h0, None, False, torch.bfloat16), xd, g)[0]
+    y = rnn(xd, h0, None, False, torch.bfloat16)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        rnn(x, h0, None, False, torch.bfloat16)
+    assert torch.equal(torch.autograd.grad(y, xd, g)[0], want)
