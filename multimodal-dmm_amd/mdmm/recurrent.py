@@ -13,6 +13,7 @@ States, row statistics and sums are fp32 whatever the tensors' type; every store
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import native
@@ -46,8 +47,14 @@ def _apply(device, fn, *args):
         return fn(*args)
 
 
+def _tangent(tensors):
+    """Whether one of them carries a forward-mode tangent (which the kernels, reading addresses, would drop)."""
+    return forward_ad._current_level >= 0 and any([t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors])
+
+
 def _grad_wanted(*tensors):
-    return torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors])
+    """Whether the call goes through its autograd node (which refuses tangents)."""
+    return torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors]) or _tangent(tensors)
 
 
 _FN = {}
@@ -250,7 +257,7 @@ def gated_scan(gates, h0=None, mask=None, reverse=False):
 
 
 def _no_grad_only(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if _grad_wanted(*tensors):
         raise ValueError('%s has no gradient: call it under torch.no_grad(), or %s for training'
                          % (name, name.replace('_step', '')))
 

@@ -686,3 +686,31 @@ def test_narrow_rows_keep_their_gradients(H):
     for i, (a, b) in enumerate(zip(got, want)):
         bound = 8 * U * terms[i].abs().sum(0) if i in terms else 2 * U * b.abs()
         assert ((a.cpu().double() - b).abs() <= bound + 1e-38).all(), (i, (a.cpu().double() - b).abs().max())
+
+
+def dual(*shape, **kw):
+    return torch.autograd.forward_ad.make_dual(Z(*shape, **kw), torch.ones(*shape, **kw))
+
+
+@gpu
+@pytest.mark.parametrize('grad', [True, False])
+def test_forward_mode_is_refused(grad):
+    """A tangent that went in and did not come out would be a wrong derivative: every operator raises."""
+    w = torch.ones(3, device='cuda')
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        for call in (lambda: ops.gated_scan(dual(4, 2, 6, device='cuda')),
+                     lambda: ops.gated_scan(Z(4, 2, 6, device='cuda'), dual(3, device='cuda')),
+                     lambda: ops.rms_norm(dual(2, 3, device='cuda'), w), lambda: ops.rms_norm(Z(2, 3, device='cuda'), dual(3, device='cuda')),
+                     lambda: ops.block_norm(Z(2, 3, device='cuda'), dual(2, 3, device='cuda'), w),
+                     lambda: ops.gated_block(dual(4, 2, 9, device='cuda'), Z(4, 2, 3, device='cuda'), None, w)):
+            with pytest.raises(NotImplementedError):
+                call()
+        ops.gated_scan(Z(4, 2, 6, device='cuda'))              # (no tangent: as ever)
+
+
+def test_forward_mode_is_refused_by_the_steps():
+    with torch.autograd.forward_ad.dual_level():
+        for call in (lambda: ops.gated_scan_step(dual(2, 6), Z(2, 3)), lambda: ops.gated_scan_step(Z(2, 6), dual(2, 3)),
+                     lambda: ops.gated_block_step(Z(2, 9), dual(2, 3), Z(2, 3), Z(3))):
+            with pytest.raises(ValueError):
+                call()
