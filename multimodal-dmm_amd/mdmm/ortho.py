@@ -70,7 +70,8 @@ def orthogonalise(mats, steps=5, eps=1e-7, coefficients=COEFFICIENTS):
 
     mats: fp32 or bf16 tensors of two or more dimensions (more than two: leading dimension x the rest), either side the
     longer, at most 65536.  coefficients: (a, b, c) of X <- a X + (b A + c A^2) X, A = X X^T, such that singular values in
-    (0, 1] stay below 1.95 (refused otherwise).  -> a list of contiguous tensors of their shapes and types.  No gradient."""
+    (0, 1] stay below 1.95 (refused otherwise).  -> a list of contiguous tensors of their shapes and types.  No gradient: a
+    matrix that wants one is refused."""
     mats = [mats] if torch.is_tensor(mats) else list(mats)
     if int(steps) != steps or not 0 <= steps <= MAX_STEPS:
         raise ValueError('orthogonalise: a number of steps, 0 to %d, got %r' % (MAX_STEPS, steps))
@@ -85,10 +86,13 @@ def orthogonalise(mats, steps=5, eps=1e-7, coefficients=COEFFICIENTS):
     for m in mats:
         if m.dim() < 2:
             raise ValueError('orthogonalise: matrices, got shape %s' % (tuple(m.shape),))
+        if recurrent._grad_wanted(m):
+            raise ValueError('orthogonalise has no gradient: call it under torch.no_grad(), or on detached matrices')
         if m.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError('orthogonalise: fp32 or bf16 matrices, got %s' % m.dtype)
         if m.shape[0] > 65536 or m.numel() > 65536 * max(m.shape[0], 1):
             raise ValueError('orthogonalise: at most 65536 rows and columns, got %s' % (tuple(m.shape),))
+    for m in mats:
         ops._need_gpu(m)
         if m.device != mats[0].device:
             raise ValueError('orthogonalise: matrices on %s and %s' % (mats[0].device, m.device))
@@ -109,4 +113,4 @@ def orthogonalise(mats, steps=5, eps=1e-7, coefficients=COEFFICIENTS):
     return outs
 
 
-from . import ops  # noqa: E402  (last: ops re-exports this module's functions, whichever of the two is imported first)
+from . import ops, recurrent  # noqa: E402  (last: ops re-exports this module's functions, whichever of the two is imported first)
