@@ -9,6 +9,10 @@
 // dropped l l' 2^-23 of a term: the result is nearer to 64 bits than fp32 products by the library (6e-7 against 2.9e-6 at
 // 2048 x 2048).  ca X is added in fp32.  (Up to 128 rows: fp32, see WHOLE.)
 //
+// A fixed s would lose X where eps makes it small (|M|_F of 1e-12 at eps 1e-7: 3e-5 off, in fp32 6e-8).  So what is kept is
+// 2^k X with k from a bound t of X's singular values, |M|_F / (|M|_F + eps) at first and the polynomial's largest value on
+// [0, t] after a step (Range); k = 0 from t = 1/2 on.  Then A is kept as 4^k A, P as 4^k P 2^-q.
+//
 // X is stored both ways (n x m for A, m x n for P X) so that every product runs over two operands' rows.  A row keeps 32
 // columns of h, then the same 32 of l: one cache line for a step of 32 (with the planes apart, each step took half lines and
 // two 2048 x 2048 products 142 us); fp32 rows take the same bytes.  Tiles come straight into LDS, a step or more ahead, chunks
@@ -20,6 +24,7 @@
 // library's own fp16 product of that size 640), without its loads 78, without its matrix instructions 76.  Small ones are
 // bound by the seventeen launches of five steps, 6 to 11 us each.
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 #include <type_traits>
 #include "../../include/mdmm_hip.h"
@@ -75,9 +80,16 @@ struct Items {
 // What the launches of one size class share (p.item: that class's matrices alone, in q.it's order).  The first launch takes it as its argument and leaves it in the workspace; the
 // others read it there: arguments live in host memory, where each of the dependent loads that find a tile's matrix would
 // wait for the bus
+// |x (ca + cb x^2 + cc x^4)| at its extrema, value[i] at x^2 = at[i] (none: infinity), and q, with which |cb| + |cc| / 4 stays
+// below P's 15.5: what a step needs to bound its result and to scale P
+struct Range {
+  float at[2], value[2];
+  int32_t q;
+};
 struct Call {
   mdmm_ortho_t p;
   Items q;
+  Range r;
 };
 static_assert(sizeof(Call) <= 3968, "a launch's arguments");
 
@@ -106,6 +118,24 @@ __device__ __forceinline__ Found find(const int32_t* first, int tile) {
   const int begin = first[l], end = first[l + 1];
   const int k = (int)__popcll(__ballot(lane < MDMM_ORTHO_MAX && end <= tile));
   return {k, __builtin_amdgcn_readlane(begin, k)};
+}
+
+// the bound of every matrix's X, of even and odd steps: behind the call in the workspace
+struct Bounds { float t[2][MDMM_ORTHO_MAX]; };
+__device__ __forceinline__ Bounds* bounds(const Call* call) { return (Bounds*)(call + 1); }
+// k of a bound t: 2^k t in [1/2, 1) below 1/2, up to 2^120 (X below 2^-120: as fp32 runs out)
+__device__ __forceinline__ int shift_of(float t) {
+  if (!(t > 0.0f && t < 0.5f)) return 0;
+  const int k = -__builtin_amdgcn_frexp_expf(t);
+  return k < 120 ? k : 120;
+}
+__device__ __forceinline__ float next_bound(const mdmm_ortho_t& p, const Range& r, float t) {
+  const float u = t * t;
+  float v = fabsf(t * (p.ca + u * (p.cb + u * p.cc)));
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (u > r.at[i] && r.value[i] > v) v = r.value[i];
+  return v;
 }
 
 __device__ __forceinline__ void split(float x, half_t& h, half_t& l) {       // x: already scaled
@@ -243,13 +273,19 @@ __global__ __launch_bounds__(NT) void ortho_pack_kernel(const Call* __restrict__
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
   s = (part[0] + part[1]) + (part[2] + part[3]);
-  const float inv = (float)((double)SX / (sqrt(s) + (double)p.eps));
+  const double norm = sqrt(s), bound = norm / (norm + (double)p.eps);
+  // 2^k SX / (|M| + eps) as inv 2^e: with eps 0 it need not fit fp32
+  const double scale = (double)SX / (norm + (double)p.eps);
+  const int e = __builtin_amdgcn_frexp_exp(scale);
+  const float inv = (float)__builtin_amdgcn_frexp_mant(scale);
+  const int exponent = e + shift_of((float)bound);
+  if (me == 0 && threadIdx.x == 0) bounds(call)->t[0][f.k] = (float)bound;
   auto store = [&](auto as) {
     constexpr bool whole = decltype(as)::value;
 #pragma unroll
     for (int u = 0; u < 4096 / NT; ++u) {
       const int i = threadIdx.x + u * NT;
-      const float v = x[u] * inv;
+      const float v = ldexpf(x[u], exponent) * inv;
       tile[i / 64][i % 64] = v;
       put(place(same, r0 + i / 64, ld_same, c0 + i % 64, whole), v, whole);
     }
@@ -301,7 +337,7 @@ template <class C> __host__ __device__ int tri(int n) {          // tiles at and
 // tile `tile` of one matrix's product, in one of the formats
 template <int MODE, class C, bool whole>
 __device__ __forceinline__ void product(half_t (&lds)[C::ST * C::HALVES], const Call* __restrict__ call, const Item& w,
-                                        const mdmm_ortho_item_t& t, int tile, int flip) {
+                                        const mdmm_ortho_item_t& t, int tile, int flip, float bound, float next) {
   constexpr bool PX = MODE == APPLY || MODE == LAST;
   const mdmm_ortho_t& p = call->p;
   const float ca = p.ca, cb = p.cb, cc = p.cc, decay = p.decay;
@@ -480,6 +516,9 @@ __device__ __forceinline__ void product(half_t (&lds)[C::ST * C::HALVES], const 
   }
   // v: the result in its planes' scale
   const int64_t nn = (int64_t)n * n, m = w.m;
+  const int k = shift_of(bound), up = MODE == APPLY ? shift_of(next) - k : 0, q = k ? call->r.q : 0;
+  const float pa = ldexpf(cc * (SP / SX / SX), -2 * k - q), pb = ldexpf(cb * (SP / SX), -q);          // of POLY
+  const float xa = ldexpf(ca, up), xb = ldexpf(1.0f / SP, up - 2 * k + q), out = ldexpf(1.0f / SX, -k);      // of P X
 #pragma unroll
   for (int x = 0; x < C::TI; ++x)
 #pragma unroll
@@ -502,12 +541,12 @@ __device__ __forceinline__ void product(half_t (&lds)[C::ST * C::HALVES], const 
         }
         if (MODE == POLY) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(cc * (SP / SX / SX), v[e], cb * (SP / SX) * of4(with, e, whole));
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(pa, v[e], pb * of4(with, e, whole));
           put_sym(w.poly, n, i, j, v, j0 < i0 + C::BM, whole);
         }
         if (PX) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaf(ca, of4(with, e, whole), v[e] * (1.0f / SP));
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(xa, of4(with, e, whole), v[e] * xb);
         }
         if (MODE == APPLY) {
           half_t* down = place(w.xn, i, m, j, whole);
@@ -521,7 +560,7 @@ __device__ __forceinline__ void product(half_t (&lds)[C::ST * C::HALVES], const 
           const int64_t o = r * t.dst_ld + c;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float u = v[e] * (1.0f / SX);
+            const float u = v[e] * out;
             if (e >= end) continue;
             if (update) {
               float* d = (float*)t.dst + o + e * step;
@@ -543,16 +582,22 @@ __global__ __launch_bounds__(C::T, C::OCC) void ortho_product_kernel(const Call*
   const int me = xcd * each + (xcd < more ? xcd : more) + (blockIdx.x >> 3);
   const Entries<mdmm_ortho_item_t> ts(call->p.item);
   const Entries<Item> ws(q.it);
+  const int lane = threadIdx.x & 63, l = lane < MDMM_ORTHO_MAX ? lane : 0;
+  const Bounds* t_of = bounds(call);
+  const float t_now = MODE == GRAM ? 0.0f : t_of->t[flip][l], t_next = MODE == APPLY ? t_of->t[flip ^ 1][l] : 0.0f;
   const Found f = find(q.first[LIST], me);
   const Item w = ws.of(f.k);
+  auto of_k = [&](float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), f.k)); };
+  const float bound = of_k(t_now), next = of_k(t_next);
+  if (MODE == POLY && me == f.first && threadIdx.x == 0) bounds(call)->t[flip ^ 1][f.k] = next_bound(call->p, call->r, bound);
   mdmm_ortho_item_t t = {};
   if (MODE == LAST) t = ts.of(f.k);
   if constexpr (C::TI * C::TJ == 1)
     if (w.n <= WHOLE) {
-      product<MODE, C, true>(lds, call, w, t, me - f.first, flip);
+      product<MODE, C, true>(lds, call, w, t, me - f.first, flip, bound, next);
       return;
     }
-  product<MODE, C, false>(lds, call, w, t, me - f.first, flip);
+  product<MODE, C, false>(lds, call, w, t, me - f.first, flip, bound, next);
 }
 
 // the slices of A added up (each keeps the tiles at and above the diagonal, column by column)
@@ -589,7 +634,7 @@ __global__ __launch_bounds__(NT) void ortho_copy_kernel(const Call* __restrict__
     const int64_t r = i / t.cols, c = i % t.cols;
     const bool whole = w.n <= WHOLE;
     const half_t* x = place(w.xn, w.tall ? c : r, w.m, w.tall ? r : c, whole);
-    const float v = (whole ? *(const float*)x : (float)x[0] + (float)x[32]) * (1.0f / SX);
+    const float v = (whole ? *(const float*)x : (float)x[0] + (float)x[32]) * ldexpf(1.0f / SX, -shift_of(bounds(call)->t[0][blockIdx.y]));
     const int64_t to = r * t.dst_ld + c;
     if (p.update) {
       float* d = (float*)t.dst + to;
@@ -612,7 +657,8 @@ int check(const mdmm_ortho_t* a) {
   return 0;
 }
 
-int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+constexpr int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+constexpr int64_t KEPT = up(sizeof(Call) + sizeof(Bounds), 256);         // of a size class in the workspace
 
 // A call's larger matrices (more than 384 rows) take 128 x 128 tiles in P X, where those are 256 or more, one for each CU: the
 // larger tile halves what a product loads.  Fewer leave CUs idle and the others alone with one workgroup, whose loads and
@@ -627,7 +673,7 @@ int64_t large_tiles(const mdmm_ortho_item_t& t) {
 // the workspace: fills both size classes' lists (base NULL: sizes only), returns the bytes used
 int64_t lay_out(const mdmm_ortho_t* a, Items (&q)[2], mdmm_ortho_item_t (*items)[MDMM_ORTHO_MAX] = nullptr) {
   char* base = (char*)a->ws;
-  int64_t off = 2 * up(sizeof(Call), 256);
+  int64_t off = up(2 * KEPT, 4096);         // (two 256 x 4096: 185 us, at 2 KEPT 188)
   auto take = [&](int64_t bytes) { char* p = base + off; off += up(bytes, 256); return p; };
   q[0].n = q[1].n = 0;
   int64_t total = 0;
@@ -671,6 +717,25 @@ template <class F> int tiles(Items& q, int list, F count) {
   return (int)total;
 }
 
+Range range_of(const mdmm_ortho_t* a) {
+  Range r = {{INFINITY, INFINITY}, {0.0f, 0.0f}, 0};
+  const double ca = a->ca, cb = a->cb, cc = a->cc;
+  double at[2] = {INFINITY, INFINITY};
+  if (cc != 0.0) {
+    const double root = 9.0 * cb * cb - 20.0 * ca * cc;
+    if (root >= 0.0)
+      for (int i = 0; i < 2; ++i) at[i] = (-3.0 * cb + (i ? 1.0 : -1.0) * sqrt(root)) / (10.0 * cc);
+  } else if (cb != 0.0) at[0] = -ca / (3.0 * cb);
+  for (int i = 0; i < 2; ++i)
+    if (at[i] > 0.0 && at[i] < 16.0) {
+      r.at[i] = (float)at[i];
+      r.value[i] = (float)(sqrt(at[i]) * fabs(ca + at[i] * (cb + at[i] * cc)));
+    }
+  const double top = (fabs(cb) + fabs(cc) / 4.0) / 15.5;
+  if (top > 1.0 && top < 1e30) r.q = ilogb(top) + 1;
+  return r;
+}
+
 // C: the tile of A and P, D: that of P X
 template <class C, class D> void launch(const mdmm_ortho_t* a, const Items& items, const mdmm_ortho_item_t* mats, Call* keep, hipStream_t s) {
   if (!items.n) return;
@@ -678,6 +743,7 @@ template <class C, class D> void launch(const mdmm_ortho_t* a, const Items& item
   c.p = *a;
   for (int i = 0; i < MDMM_ORTHO_MAX; ++i) c.p.item[i] = mats[i];
   c.q = items;
+  c.r = range_of(a);
   Items& q = c.q;
   const int packs = tiles(q, PACKS, [](const Item& w) { return (int64_t)(w.n / 64) * (w.m / 64); });
   const int gram = tiles(q, GRAMS, [](const Item& w) { return (int64_t)tri<C>(w.n) * w.splits; });
@@ -720,6 +786,6 @@ extern "C" int mdmm_ortho(const mdmm_ortho_t* a, void* stream) {
   mdmm_ortho_item_t mats[2][MDMM_ORTHO_MAX] = {};
   lay_out(a, q, mats);
   launch<Small, Small>(a, q[0], mats[0], (Call*)a->ws, (hipStream_t)stream);
-  launch<Small, Large>(a, q[1], mats[1], (Call*)((char*)a->ws + up(sizeof(Call), 256)), (hipStream_t)stream);
+  launch<Small, Large>(a, q[1], mats[1], (Call*)((char*)a->ws + KEPT), (hipStream_t)stream);
   return (int)hipGetLastError();
 }

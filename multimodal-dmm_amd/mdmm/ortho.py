@@ -66,7 +66,9 @@ def launch(items, steps, eps, coefficients, src_bf16, dst_bf16, momentum=0.0, ne
 
 def orthogonalise(mats, steps=5, eps=1e-7, coefficients=COEFFICIENTS):
     """The nearest-orthogonal direction of every matrix of a list, U V^T of M = U S V^T approximately, by `steps`
-    Newton-Schulz steps in fp32 on M / (|M|_F + eps); every matrix of the list shares the launches.
+    Newton-Schulz steps on M / (|M|_F + eps), accurate to a few roundings of fp32: with shorter sides of up to 128 the matrices
+    are fp32, beyond kept to 22 to 23 bits instead of 24 with better sums (the error of fp32 products by the library: 0.3 to 0.8
+    of it, up to 1.3 for shorter sides below ten).  Matrices of one type and size class share the launches, 24 to a call.
 
     mats: fp32 or bf16 tensors of two or more dimensions (more than two: leading dimension x the rest), either side the
     longer, at most 65536.  coefficients: (a, b, c) of X <- a X + (b A + c A^2) X, A = X X^T, such that singular values in

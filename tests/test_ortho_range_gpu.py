@@ -19,3 +19,75 @@ def test_gradients_are_refused():
     for call in (lambda: ops.orthogonalise([w.detach()]), torch.no_grad()(lambda: ops.orthogonalise([w]))):
         with pytest.raises(native.MdmmError):          # (the device's refusal, which comes last)
             call()
+
+
+def check_scaled(m, got, steps, eps, coefficients=ortho.COEFFICIENTS):
+    """check()'s second bound with any eps and coefficients: no more than 8 times the error of the same products in fp32 by
+    torch, or than 8 times what one rounding of each iterate's elements costs, and the stored result's own rounding."""
+    a, b, c = coefficients
+
+    def iterate(dtype):
+        x = m.cpu().to(dtype)
+        tall = x.shape[0] > x.shape[1]
+        x = x.t() if tall else x
+        norm = float(m.double().norm())            # (in 64 bits on both sides: fp32's sum of squares has no range for it)
+        x = (x.double() / (norm + eps)).to(dtype)
+        kept, flat = [x.double().norm()], [None]
+        for _ in range(steps):
+            g = x @ x.t()
+            p = b * g + c * (g @ g)
+            flat.append(float(abs(a) * x.double().norm() + p.double().norm() * x.double().norm()))
+            x = a * x + p @ x
+            kept.append(float(x.double().norm()))
+        return (x.t() if tall else x), flat
+    want, flat = iterate(torch.float64)
+    plain = iterate(torch.float32)[0].double()
+    slope = max(abs(a), 1.0)
+    floor = sum(slope ** (steps - k) * U * n for k, n in enumerate(flat) if k)
+    near = 8 * max(float((plain - want).norm()), floor) + 64 * U * float(want.norm())
+    err = float((got.cpu().double() - want).norm())
+    assert err <= near, (err / float(want.norm()), near / float(want.norm()))
+
+
+@gpu
+@pytest.mark.parametrize('norm', [1e-9, 1e-11, 1e-12, 1e-14, 1e-18])
+@pytest.mark.parametrize('shape', [(256, 256), (300, 140), (256, 4096), (30, 40)])
+def test_norms_far_below_eps(shape, norm):
+    """|M| / (|M| + eps) down to 1e-11: the result is as accurate relative to its own size as at any other norm."""
+    gen = torch.Generator().manual_seed(21)
+    m = torch.randn(shape, generator=gen)
+    m = (m * (norm / float(m.double().norm()))).cuda()
+    for steps in (0, 1, 5, 9):
+        check_scaled(m, ops.orthogonalise([m], steps=steps)[0], steps, 1e-7)
+
+
+@gpu
+@pytest.mark.parametrize('eps,norm', [(0.0, 1e-36), (0.0, 1e37), (1e3, 1e-6), (1e10, 1.0), (1e-30, 1e-34), (1e-7, 1e30)])
+def test_any_eps_and_norm(eps, norm):
+    gen = torch.Generator().manual_seed(22)
+    for shape in ((200, 150), (20, 50), (1100, 1500)):
+        m = torch.randn(shape, generator=gen)
+        m = (m * (norm / float(m.double().norm()))).cuda()
+        n = 2 if shape[0] > 1000 else 1                # (two of them: enough large tiles)
+        for o in ops.orthogonalise([m] * n, eps=eps):
+            check_scaled(m, o, 5, eps)
+
+
+@gpu
+@pytest.mark.parametrize('coefficients,steps', [((0.0, 1.0, 0.0), 2), ((0.5, 0.0, 0.0), 30), ((0.0, -20.0, 10.0), 1), ((1.5, -0.5, 0.0), 12)])
+def test_small_norms_under_other_coefficients(coefficients, steps):
+    """Iterations without a linear term, shrinking ones and slow ones, from norms of 1 and far below."""
+    gen = torch.Generator().manual_seed(23)
+    for norm in (1.0, 1e-9):
+        m = torch.randn(170, 140, generator=gen)
+        m = (m * (norm / float(m.double().norm()))).cuda()
+        check_scaled(m, ops.orthogonalise([m], steps=steps, coefficients=coefficients)[0], steps, 1e-7, coefficients)
+
+
+@gpu
+def test_matrices_of_different_norms_in_one_call():
+    gen = torch.Generator().manual_seed(24)
+    mats = [(torch.randn(s, generator=gen) * k).cuda() for s, k in (((150, 200), 1.0), ((200, 150), 1e-14), ((20, 30), 1e-13),
+                                                                   ((140, 2100), 1e-15), ((150, 200), 1e-3))]
+    for m, o in zip(mats, ops.orthogonalise(mats)):
+        check_scaled(m, o, 5, 1e-7)
