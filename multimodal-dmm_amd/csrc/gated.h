@@ -29,9 +29,7 @@ struct Gate {
   }
 };
 
-// sigmoid alone: 1 / (1 + exp(-x)), relative error 6e-8 (1 + |x|); exp may overflow to infinity (then 0)
-__device__ __forceinline__ float sigmoid_(float x) {
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f));
-}
+// sigmoid alone, to the same accuracy wherever x lies (1 / (1 + 2^(-x log2(e))) is off by 6e-8 (1 + |x|) of itself)
+__device__ __forceinline__ float sigmoid_(float x) { return Gate(x).a; }
 
 }  // namespace mdmm

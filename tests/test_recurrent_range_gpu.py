@@ -1,0 +1,38 @@
+"""The recurrent operators over the whole range of values and sizes: gates of any size, scans over several tiles."""
+import pytest
+import torch
+
+from mdmm import ops
+from test_recurrent_gpu import BF16, F32, U, close, make, scan_ref
+
+gpu = pytest.mark.gpu
+Z = torch.zeros
+GATES = torch.tensor([-80.0, -60.0, -40.0, -20.0, -10.0, -5.0, -3.0, 0.5, 3.0, 10.0, 17.0, 30.0, 88.0, 1e2, 1e4, 3e7, 1e8, 1e12])
+
+
+def gated_rows(H):
+    gen = torch.Generator().manual_seed(31 + H)
+    rows = 64
+    gate = GATES[torch.randint(0, len(GATES), (rows, H), generator=gen)] * (1 + 0.01 * torch.rand(rows, H, generator=gen))
+    y, w = make(gen, rows, H), make(gen, H, std=0.1, mean=1.0)
+    g_out = torch.where(torch.rand(rows, H, generator=gen) > 0.5, 1.0, -1.0)
+    return rows, gate, y, w, g_out, y.double() * torch.rsqrt(y.double().square().mean(-1, keepdim=True) + 1e-6) * w.double()
+
+
+# The gate's factor 6 u (its exponential, the sum, the reciprocal, two products), r 14 u (a sum of H squares in pieces, at most
+# 20 u of the mean, half of it in its root, and the root's own 4), four products; twice that is allowed
+TOL = 2 * (6 + 14 + 4) * U
+
+
+@gpu
+@pytest.mark.parametrize('H', [3, 100, 256, 700])
+def test_gates_of_any_size(H):
+    """silu(g) to a few units of its own size wherever g lies: an output without a residual is a product."""
+    rows, gate, y, w, _, u = gated_rows(H)
+    want = gate.double() * torch.sigmoid(gate.double()) * u
+    out = ops.block_norm(y.cuda(), Z(rows, H).cuda(), w.cuda(), gate=gate.cuda())
+    assert ((out.cpu().double() - want).abs() <= TOL * want.abs() + 1e-37).all()
+    # the step form: a state that the masked step leaves as it is
+    proj = torch.cat([Z(rows, 2 * H), gate], -1).cuda()
+    out, _ = ops.gated_block_step(proj, Z(rows, H).cuda(), y.cuda(), w.cuda(), mask=Z(rows, dtype=torch.bool).cuda())
+    assert ((out.cpu().double() - want).abs() <= TOL * want.abs() + 1e-37).all()
