@@ -103,8 +103,18 @@ __device__ __forceinline__ double wave_total(double v) {
 }
 __device__ __forceinline__ float rsqrt_(float v) { return rsqrtf(v); }
 __device__ __forceinline__ double rsqrt_(double v) { return 1.0 / sqrt(v); }
-__device__ __forceinline__ float gate_(float g) { return sigmoid_(g); }
-__device__ __forceinline__ double gate_(double g) { return 1.0 / (1.0 + exp(-g)); }
+// act = silu(g) = g a and slope = silu'(g) = a (1 + g k), a = sigmoid(g), k = 1 - a formed apart: as a difference from 1 it
+// would leave the slope of large gates, which is 1, off by 6e-8 |g|
+__device__ __forceinline__ void gate_(float g, float& act, float& slope) {
+  const Gate y(g);
+  act = g * y.a;
+  slope = fmaf(act, y.k, y.a);
+}
+__device__ __forceinline__ void gate_(double g, double& act, double& slope) {
+  const double a = 1.0 / (1.0 + exp(-g));
+  act = g * a;
+  slope = fma(act, 1.0 / (1.0 + exp(g)), a);
+}
 __device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fma_(double a, double b, double c) { return fma(a, b, c); }
 
@@ -243,7 +253,7 @@ void norm_bwd_kernel(mdmm_block_norm_t p) {
   };
   fetch_row(row);
   for (; row < p.rows; row += step) {
-    A x[NV][VEC], g[NV][VEC], sg[NV][VEC], o[NV][VEC], q[NV][VEC], d[NV][VEC];
+    A x[NV][VEC], g[NV][VEC], slope[NV][VEC], o[NV][VEC], q[NV][VEC], d[NV][VEC];        // (g: silu(gate) once taken)
     A ss = 0.0f;
     auto taken = [](const auto& raw, A* v) {
       float f[VEC];
@@ -271,7 +281,8 @@ void norm_bwd_kernel(mdmm_block_norm_t p) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           x[k][e] *= r;
-          sg[k][e] = (ALL || p.gate) ? gate_(g[k][e]) : (A)1.0;
+          if (ALL || p.gate) gate_(g[k][e], g[k][e], slope[k][e]);
+          else g[k][e] = (A)1.0, slope[k][e] = (A)0.0;
         }
     }
     if (ALL || p.g_n) {
@@ -281,8 +292,7 @@ void norm_bwd_kernel(mdmm_block_norm_t p) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           if (ALL || p.y) {
-            A u = x[k][e] * w[k][e];
-            if (ALL || p.gate) u *= g[k][e] * sg[k][e];
+            const A u = x[k][e] * w[k][e] * g[k][e];
             o[k][e] = fma_((A)s[k][e], u, o[k][e]);
           }
           sums[0] += o[k][e] * o[k][e];
@@ -311,12 +321,10 @@ void norm_bwd_kernel(mdmm_block_norm_t p) {
         A dg[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          // act = silu(g) = g sg, slope = silu'(g) = sg + act (1 - sg)
-          const A act = (ALL || p.gate) ? g[k][e] * sg[k][e] : (A)1.0;
           const A u = x[k][e] * w[k][e], ds = d[k][e] * s[k][e];
-          as[k][e] += d[k][e] * act * u;
-          dg[e] = ds * u * fma_(-act, sg[k][e], sg[k][e] + act);
-          const A t = ds * act;
+          as[k][e] += d[k][e] * g[k][e] * u;
+          dg[e] = ds * u * slope[k][e];
+          const A t = ds * g[k][e];
           aw[k][e] += t * x[k][e];
           d[k][e] = t * w[k][e];
           sm += d[k][e] * x[k][e];

@@ -36,3 +36,18 @@ def test_gates_of_any_size(H):
     proj = torch.cat([Z(rows, 2 * H), gate], -1).cuda()
     out, _ = ops.gated_block_step(proj, Z(rows, H).cuda(), y.cuda(), w.cuda(), mask=Z(rows, dtype=torch.bool).cuda())
     assert ((out.cpu().double() - want).abs() <= TOL * want.abs() + 1e-37).all()
+
+
+@gpu
+@pytest.mark.parametrize('H', [3, 100, 256, 700])
+def test_slopes_of_any_gate(H):
+    """The gate's gradient g_out u silu'(g) to a few units of its own size.  silu'(g) = a (1 + g k) adds u (1 + |g k|) /
+    |1 + g k| on the way to its zero at g = -1.28, from which these gates keep away."""
+    rows, gate, y, w, g_out, u = gated_rows(H)
+    g64 = gate.double()
+    k = torch.sigmoid(-g64)
+    want = g_out.double() * u * torch.sigmoid(g64) * (1 + g64 * k)
+    lost = (1 + (g64 * k).abs()) / (1 + g64 * k).abs()
+    gd = gate.cuda().requires_grad_(True)
+    got = torch.autograd.grad(ops.block_norm(y.cuda(), Z(rows, H).cuda(), w.cuda(), gate=gd), gd, g_out.cuda())[0]
+    assert ((got.cpu().double() - want).abs() <= TOL * (1 + lost) * want.abs() + 1e-37).all()
