@@ -1162,7 +1162,8 @@ int mdmm_gated_block_step(const mdmm_gated_scan_t* scan, const mdmm_block_norm_t
  *                                             the argument where lr_dev is NULL)
  * M = src (rows, cols) with row stride src_ld, fp32 or bf16 (src_bf16); with mom (contiguous fp32 rows x cols): first
  * mom = momentum mom + src, then M = mom, or src + momentum mom with nesterov.  No two matrices' mom or dst overlap.  dst has
- * src's shape, its own row stride, and type (dst_bf16, update 0 only).  ws: mdmm_ortho_ws() bytes, 256-byte aligned.
+ * src's shape, its own row stride, and type (dst_bf16, update 0 only).  ws: mdmm_ortho_ws() bytes (< 0: the refusal's code), 256-byte
+ * aligned.
  * X, A and P = cb A + cc A^2 of a matrix whose shorter side exceeds 128 are kept as pairs of fp16 numbers, 22 to 23 bits where
  * fp32 has 24, at a power-of-two scale that follows the size of X; all others, and every sum, in fp32.
  * ca, cb, cc must keep the singular values of X below 2 and those of P below 16, where the pairs end.

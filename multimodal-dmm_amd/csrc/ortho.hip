@@ -770,7 +770,7 @@ template <class C, class D> void launch(const mdmm_ortho_t* a, const Items& item
 using namespace mdmm;
 
 extern "C" int64_t mdmm_ortho_ws(const mdmm_ortho_t* a) {
-  if (check(a)) return -1;
+  if (const int rc = check(a)) return rc;
   Items q[2];
   return lay_out(a, q);
 }

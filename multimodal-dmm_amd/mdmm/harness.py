@@ -216,13 +216,14 @@ class FlatMuon(torch.optim.Optimizer):
     take mdmm_adam_flat's update with adam_lr, betas, eps, adam_weight_decay, one launch for all of them.
 
     matrices: the parameters to treat as matrices; by default every one of two or more dimensions whose rows and columns both
-    exceed one.  (Embeddings and output layers are better left to Adam: pass the rest.)  lr and adam_lr are the 'lr' of the
-    two parameter groups (0: matrices, 1: the others); as a one-element CUDA tensor either may change between the replays of
+    exceed one and do not exceed 65536.  (Embeddings and output layers are better left to Adam: pass the rest.)  lr and
+    adam_lr are the 'lr' of the two parameter groups (0: matrices, 1: the others); as a one-element CUDA tensor either may change between the replays of
     a captured step, a float is a constant of the capture.  `step()` needs every gradient to be the bucket's view, as
     FlatAdam's.  state_dict(): {'momentum_buffer'} per matrix, {'step', 'exp_avg', 'exp_avg_sq'} per other parameter."""
 
     def __init__(self, bucket, lr=0.02, momentum=0.95, nesterov=True, ns_steps=5, weight_decay=0.0, matrices=None,
                  adam_lr=1e-3, betas=(0.9, 0.999), eps=1e-8, adam_weight_decay=0.0):
+        from . import ortho
         if not bucket.flat.is_cuda:
             raise RuntimeError('FlatMuon runs on the GPU (mdmm_ortho, mdmm_adam_flat)')
         if not 0.0 <= momentum < 1.0 or int(ns_steps) != ns_steps or not 0 <= ns_steps <= 1000:
@@ -232,7 +233,7 @@ class FlatMuon(torch.optim.Optimizer):
                 raise ValueError('FlatMuon: contiguous fp32 parameters')
         shape = lambda p: (p.shape[0], p.numel() // p.shape[0]) if p.dim() > 1 and p.numel() else (0, 0)     # noqa: E731
         if matrices is None:
-            chosen = [p for p in bucket.params if min(shape(p)) > 1]
+            chosen = [p for p in bucket.params if min(shape(p)) > 1 and max(shape(p)) <= ortho.MAX_SIDE]
         else:
             ids = {id(p) for p in matrices}
             chosen = [p for p in bucket.params if id(p) in ids]
@@ -241,6 +242,8 @@ class FlatMuon(torch.optim.Optimizer):
             for p in chosen:
                 if p.dim() < 2 or not p.numel():
                     raise ValueError('FlatMuon: a matrix of shape %s' % (tuple(p.shape),))
+                if max(shape(p)) > ortho.MAX_SIDE:
+                    raise ValueError('FlatMuon: matrices of at most %d rows and columns, got %s' % (ortho.MAX_SIDE, tuple(p.shape)))
         own = {id(p) for p in chosen}
         rest = [p for p in bucket.params if id(p) not in own]
         groups = [dict(params=chosen, lr=lr, momentum=momentum, nesterov=bool(nesterov), ns_steps=int(ns_steps),

@@ -13,6 +13,7 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 # the kernels' fp16 plane pairs hold X and A up to 4, P = b A + c A^2 up to 16; a step count that no iteration needs
 MAX_X, MAX_P, MAX_STEPS = 1.95, 15.5, 1000
+MAX_SIDE = 65536
 
 
 def _bounded(steps, a, b, c):
@@ -92,8 +93,8 @@ def orthogonalise(mats, steps=5, eps=1e-7, coefficients=COEFFICIENTS):
             raise ValueError('orthogonalise has no gradient: call it under torch.no_grad(), or on detached matrices')
         if m.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError('orthogonalise: fp32 or bf16 matrices, got %s' % m.dtype)
-        if m.shape[0] > 65536 or m.numel() > 65536 * max(m.shape[0], 1):
-            raise ValueError('orthogonalise: at most 65536 rows and columns, got %s' % (tuple(m.shape),))
+        if m.shape[0] > MAX_SIDE or m.numel() > MAX_SIDE * max(m.shape[0], 1):
+            raise ValueError('orthogonalise: at most %d rows and columns, got %s' % (MAX_SIDE, tuple(m.shape)))
     for m in mats:
         ops._need_gpu(m)
         if m.device != mats[0].device:

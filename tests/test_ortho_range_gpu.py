@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from mdmm import native, ops, ortho
+from mdmm.harness import FlatMuon, GradBucket
 from test_ortho_gpu import U, check
 
 gpu = pytest.mark.gpu
@@ -91,3 +92,29 @@ def test_matrices_of_different_norms_in_one_call():
                                                                    ((140, 2100), 1e-15), ((150, 200), 1e-3))]
     for m, o in zip(mats, ops.orthogonalise(mats)):
         check_scaled(m, o, 5, 1e-7)
+
+
+@gpu
+def test_muon_leaves_sides_past_the_limit_to_adam():
+    """65537 rows: refused as a matrix, Adam's by default (which updates it), before any step."""
+    long = torch.nn.Parameter(torch.zeros(65537, 2, device='cuda'))
+    short = torch.nn.Parameter(torch.zeros(65536, 2, device='cuda'))
+    bucket = GradBucket([short, long])
+    with pytest.raises(ValueError, match='65536'):
+        FlatMuon(bucket, matrices=[short, long])
+    opt = FlatMuon(bucket, adam_lr=0.5)
+    assert [g['params'] for g in opt.param_groups] == [[short], [long]]
+    bucket.flat.fill_(1.0)
+    opt.step()
+    assert torch.allclose(long.detach(), torch.full_like(long, -0.5)) and float(short.detach().abs().min()) > 0
+
+
+def test_the_library_says_why_it_refuses_a_matrix():
+    a = native.Ortho()
+    a.n = 1
+    a.item[0].rows, a.item[0].cols, a.item[0].src_ld, a.item[0].dst_ld = 70000, 5, 5, 5
+    codes = [native.lib().mdmm_ortho_ws(a)]
+    a.item[0].rows = 0
+    codes.append(native.lib().mdmm_ortho_ws(a))
+    a.item[0].rows = 7
+    assert codes == [-2, -1] and native.lib().mdmm_ortho_ws(a) > 0
