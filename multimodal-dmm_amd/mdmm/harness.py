@@ -216,7 +216,8 @@ class FlatMuon(torch.optim.Optimizer):
     take mdmm_adam_flat's update with adam_lr, betas, eps, adam_weight_decay, one launch for all of them.
 
     matrices: the parameters to treat as matrices; by default every one of two or more dimensions whose rows and columns both
-    exceed one and do not exceed 65536.  (Embeddings and output layers are better left to Adam: pass the rest.)  lr and
+    exceed one and do not exceed 65536, but for (layers, 1, width) tensors: those are the models' initial RNN states (and
+    the kernels of 1-D convolutions with a single channel on one side), rows that no product mixes.  (Embeddings and output layers are better left to Adam: pass the rest.)  lr and
     adam_lr are the 'lr' of the two parameter groups (0: matrices, 1: the others); as a one-element CUDA tensor either may change between the replays of
     a captured step, a float is a constant of the capture.  `step()` needs every gradient to be the bucket's view, as
     FlatAdam's.  state_dict(): {'momentum_buffer'} per matrix, {'step', 'exp_avg', 'exp_avg_sq'} per other parameter."""
@@ -233,7 +234,8 @@ class FlatMuon(torch.optim.Optimizer):
                 raise ValueError('FlatMuon: contiguous fp32 parameters')
         shape = lambda p: (p.shape[0], p.numel() // p.shape[0]) if p.dim() > 1 and p.numel() else (0, 0)     # noqa: E731
         if matrices is None:
-            chosen = [p for p in bucket.params if min(shape(p)) > 1 and max(shape(p)) <= ortho.MAX_SIDE]
+            chosen = [p for p in bucket.params if min(shape(p)) > 1 and max(shape(p)) <= ortho.MAX_SIDE
+                      and not (p.dim() == 3 and p.shape[1] == 1)]
         else:
             ids = {id(p) for p in matrices}
             chosen = [p for p in bucket.params if id(p) in ids]

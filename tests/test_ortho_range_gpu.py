@@ -3,7 +3,7 @@ other tests do not reach, and refusals."""
 import pytest
 import torch
 
-from mdmm import native, ops, ortho
+from mdmm import models, native, ops, ortho
 from mdmm.harness import FlatMuon, GradBucket
 from test_ortho_gpu import U, check
 
@@ -118,3 +118,14 @@ def test_the_library_says_why_it_refuses_a_matrix():
     codes.append(native.lib().mdmm_ortho_ws(a))
     a.item[0].rows = 7
     assert codes == [-2, -1] and native.lib().mdmm_ortho_ws(a) > 0
+
+
+@gpu
+@pytest.mark.parametrize('cell', ['gru', 'linear'])
+def test_muon_leaves_initial_states_to_adam(cell):
+    """The default choice on a model with two-layer RNNs: its initial states (2, 1, H) are no matrices."""
+    m = models.MultiDKS(['a', 'b'], [3, 4], h_dim=12, z_dim=6, rnn_layers=2, device=torch.device('cuda:0'), rnn_cell=cell)
+    opt = FlatMuon(GradBucket(m.parameters()))
+    chosen = {id(p) for p in opt.param_groups[0]['params']}
+    named = {k: id(p) in chosen for k, p in m.named_parameters()}
+    assert all(not named['h0.' + k] for k in 'ab') and {named[k] for k in named if k.endswith('weight')} == {True}
