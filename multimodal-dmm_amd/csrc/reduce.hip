@@ -628,7 +628,8 @@ __global__ __launch_bounds__(NT) void adam_flat_kernel(float* const* __restrict_
     const int64_t i = base + r * NT + threadIdx.x;
     if (i >= n) break;
     while (i >= k_end) { ++k; k_end = offs[k + 1]; pk = p_ptrs[k] - offs[k]; }
-    if (!p_ptrs[k]) continue;               // (left to another optimizer)
+    // NULL: left to another optimizer.  (6.8e6 elements: 34.3 us; without this test 35.8, with a flag kept beside pk 36.4)
+    if (!p_ptrs[k]) continue;
     const float pv = pk[i];
     const float gr = fmaf(wd, pv, g[i]);
     const float mm = fmaf(w1, gr - m[i], m[i]);
