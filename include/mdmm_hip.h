@@ -1072,7 +1072,8 @@ int mdmm_cat_head_nll_bwd(const float* hid, const float* w, const float* label, 
  * h (T, B, H) contiguous, time-indexed, fp32 or (with gates_bf16 only) bf16 with h_bf16.  The state is fp32 throughout.
  * reverse: from the last step to the first.  h0: row b at b * h0_sb (0: one row for all; NULL: zeros).  h_last (B, H): the state behind the last
  * step taken (NULL: not wanted).
- * states: mdmm_gated_scan_states() floats the forward pass leaves for the backward one (NULL in a forward-only call).
+ * states: mdmm_gated_scan_states() floats the forward pass leaves for the backward one (NULL in a forward-only call; not
+ * touched where that is 0).
  * ws: mdmm_gated_scan_ws(a, bwd) floats of scratch per call (0: NULL is fine).
  * backward: g_h (T, B, H) in h's type (NULL: none), g_last (B, H) fp32 (NULL: none); g_gates in the gates' type and
  * column order with its own strides (every element of its 2H columns is written, 0 where the mask is 0); g_h0 (B, H) fp32

@@ -501,7 +501,9 @@ int launch(const mdmm_gated_scan_t* a, const Plan& pl, bool bwd, hipStream_t s) 
   return pl.vec == 1 ? launch<IO, HO, 1, true>(a, pl, bwd, s) : launch<IO, HO, 2, true>(a, pl, bwd, s);
 }
 
-int run(const mdmm_gated_scan_t* a, bool bwd, hipStream_t s) {
+int run(const mdmm_gated_scan_t* args, bool bwd, hipStream_t s) {
+  mdmm_gated_scan_t keep = *args, *a = &keep;
+  if (a->T <= ONE) a->states = nullptr;                // (room for none of them: mdmm_gated_scan_states)
   const Plan pl = plan(a);
   if (pl.wgs > (1 << 22)) return MDMM_E_LIMIT;         // (a grid's threads fit 32 bits)
   if (pl.splits > 1 && !a->ws) return MDMM_E_ARG;

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from mdmm import ops
+from mdmm import native, ops
 from test_recurrent_gpu import BF16, F32, U, close, make, scan_ref
 
 gpu = pytest.mark.gpu
@@ -51,3 +51,26 @@ def test_slopes_of_any_gate(H):
     gd = gate.cuda().requires_grad_(True)
     got = torch.autograd.grad(ops.block_norm(y.cuda(), Z(rows, H).cuda(), w.cuda(), gate=gd), gd, g_out.cuda())[0]
     assert ((got.cpu().double() - want).abs() <= TOL * (1 + lost) * want.abs() + 1e-37).all()
+
+
+@gpu
+@pytest.mark.parametrize('T,B,H', [(1, 3, 20), (64, 2, 12), (40, 3, 33)])
+def test_no_states_are_written_where_none_are_asked_for(T, B, H):
+    """A C caller with one buffer for everything: up to 64 steps mdmm_gated_scan_states is 0, and what lies at `states` is
+    neither written nor read."""
+    gen = torch.Generator().manual_seed(T)
+    x, g = make(gen, T, B, 2 * H).cuda(), make(gen, T, B, H).cuda()
+    xd = x.clone().requires_grad_(True)
+    want = ops.gated_scan(xd)[0]
+    want_g = torch.autograd.grad(want, xd, g)[0]
+    room = torch.full((4 * B * H,), 7.0, device='cuda')
+    h, g_x = torch.empty(T, B, H, device='cuda'), torch.empty_like(x)
+    a = native.GatedScan()
+    a.T, a.B, a.H = T, B, H
+    a.gates, a.gates_st, a.gates_sb, a.h, a.states = x.data_ptr(), 2 * B * H, 2 * H, h.data_ptr(), room.data_ptr()
+    assert native.lib().mdmm_gated_scan_states(a) == 0 and native.lib().mdmm_gated_scan_ws(a, 0) == 0
+    stream = torch.cuda.current_stream().cuda_stream
+    native.check(native.lib().mdmm_gated_scan_fwd(a, stream), 'mdmm_gated_scan_fwd')
+    a.g_h, a.g_gates, a.g_gates_st, a.g_gates_sb = g.data_ptr(), g_x.data_ptr(), 2 * B * H, 2 * H
+    native.check(native.lib().mdmm_gated_scan_bwd(a, stream), 'mdmm_gated_scan_bwd')
+    assert torch.equal(room, torch.full_like(room, 7.0)) and torch.equal(h, want) and torch.equal(g_x, want_g)
