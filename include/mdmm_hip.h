@@ -32,6 +32,7 @@ extern "C" {
 #define MDMM_E_ARG (-1)    /* bad size / NULL pointer                          */
 #define MDMM_E_LIMIT (-2)  /* exceeds MDMM_MAX_* or the LDS budget of one CU    */
 #define MDMM_E_ALIGN (-3)  /* packed weight buffers must be 16-byte aligned    */
+#define MDMM_E_ALIAS (-4)  /* an output shares memory with an input            */
 
 int mdmm_version(void);
 const char* mdmm_strerror(int code);
@@ -1071,7 +1072,7 @@ int mdmm_cat_head_nll_bwd(const float* hid, const float* w, const float* label, 
  * stride along the columns, any strides over t and b (elements, none over b negative); fp32, or bf16 with gates_bf16.
  * h (T, B, H) contiguous, time-indexed, fp32 or (with gates_bf16 only) bf16 with h_bf16.  The state is fp32 throughout.
  * reverse: from the last step to the first.  h0: row b at b * h0_sb (0: one row for all; NULL: zeros).  h_last (B, H): the state behind the last
- * step taken (NULL: not wanted).
+ * step taken (NULL: not wanted); with T = 1 it may be h0 itself (h0_sb = H), else it shares memory with no input.
  * states: mdmm_gated_scan_states() floats the forward pass leaves for the backward one (NULL in a forward-only call; not
  * touched where that is 0).
  * ws: mdmm_gated_scan_ws(a, bwd) floats of scratch per call (0: NULL is fine).

@@ -580,6 +580,11 @@ extern "C" int mdmm_gated_block_step(const mdmm_gated_scan_t* q, const mdmm_bloc
   if (q->B == 0) return 0;
   if (q->T != 1 || !q->gates || !q->h_last || !p->res || !p->out || !p->w || (p->w_next && !p->n)) return MDMM_E_ARG;
   if (!!q->gates_bf16 != !!p->branch_bf16 || (!p->branch_bf16 && p->res_bf16)) return MDMM_E_ARG;
+  const Region last = region(q->h_last, q->B, q->H, q->H, 4);
+  if (last_state_on_input(q) || meet(last, region(p->res, q->B, p->res_st, q->H, p->res_bf16 ? 2 : 4)) ||
+      meet(last, region(p->gate, q->B, p->gate_st, q->H, p->branch_bf16 ? 2 : 4)) || meet(last, region(p->w, 1, 0, q->H, 4)) ||
+      meet(last, region(p->scale, 1, 0, q->H, 4)) || meet(last, region(p->w_next, 1, 0, q->H, 4)))
+    return MDMM_E_ALIAS;
   hipStream_t s = (hipStream_t)stream;
   if (!p->branch_bf16) return launch_step<float, float>(q, p, s);
   return p->res_bf16 ? launch_step<__bf16, __bf16>(q, p, s) : launch_step<__bf16, float>(q, p, s);

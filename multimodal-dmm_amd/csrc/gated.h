@@ -32,4 +32,27 @@ struct Gate {
 // sigmoid alone, to the same accuracy wherever x lies (1 / (1 + 2^(-x log2(e))) is off by 6e-8 (1 + |x|) of itself)
 __device__ __forceinline__ float sigmoid_(float x) { return Gate(x).a; }
 
+// Host side.  The bytes that `rows` rows of n elements of `size` bytes take, `step` elements apart; whether two regions meet
+struct Region { const char* at; int64_t bytes; };
+inline Region region(const void* p, int64_t rows, int64_t step, int64_t n, int64_t size) {
+  return {(const char*)p, p ? ((rows - 1) * step + n) * size : 0};
+}
+inline bool meet(const Region& a, const Region& b) { return a.at && b.at && a.at < b.at + b.bytes && b.at < a.at + a.bytes; }
+
+// h_last, written while other workgroups still read, shares memory with an input (one that is h0 itself, a time step in place,
+// does not: a thread writes what it alone has read)
+inline bool last_state_on_input(const mdmm_gated_scan_t* a) {
+  if (!a->h_last) return false;
+  const Region last = region(a->h_last, a->B, a->H, a->H, 4);
+  const bool in_place = a->T == 1 && a->h_last == a->h0 && a->h0_sb == a->H;
+  if (!in_place && meet(last, region(a->h0, a->B, a->h0_sb, a->H, 4))) return true;
+  const int64_t es = a->gates_bf16 ? 2 : 4, past = (a->T - 1) * a->gates_st, mpast = (a->T - 1) * a->mask_st;
+  Region gates = region(a->gates, a->B, a->gates_sb, 2 * (int64_t)a->H, es), mask = region(a->mask, a->B, a->mask_sb, 1, 1);
+  gates.at += (past < 0 ? past : 0) * es;
+  gates.bytes += (past < 0 ? -past : past) * es;
+  mask.at += mask.at && mpast < 0 ? mpast : 0;
+  mask.bytes += mpast < 0 ? -mpast : mpast;
+  return meet(last, gates) || meet(last, mask);
+}
+
 }  // namespace mdmm

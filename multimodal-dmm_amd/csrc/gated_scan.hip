@@ -533,6 +533,7 @@ extern "C" int mdmm_gated_scan_fwd(const mdmm_gated_scan_t* a, void* stream) {
   if (rc) return rc;
   if (none(a)) return 0;
   if (!a->h) return MDMM_E_ARG;
+  if (last_state_on_input(a)) return MDMM_E_ALIAS;
   return run(a, false, (hipStream_t)stream);
 }
 

@@ -1026,6 +1026,7 @@ extern "C" const char* mdmm_strerror(int code) {
   if (code == MDMM_E_ARG) return "mdmm: bad argument (size or NULL pointer)";
   if (code == MDMM_E_LIMIT) return "mdmm: exceeds MDMM_MAX_* or the 160 KiB LDS budget";
   if (code == MDMM_E_ALIGN) return "mdmm: packed weight buffers must be 16-byte aligned";
+  if (code == MDMM_E_ALIAS) return "mdmm: the new state shares memory with an input (in place: the state as a whole)";
   if (code > 0) return hipGetErrorString((hipError_t)code);
   return "mdmm: unknown error";
 }

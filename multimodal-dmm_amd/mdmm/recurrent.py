@@ -274,7 +274,7 @@ def _check_state(name, state, new_state, B, H):
 def gated_scan_step(gates, state, mask=None, new_state=None):
     """One time step of gated_scan for streams whose state the caller keeps: gates (B,2H), state (B,H) fp32, mask (B,).
     -> (h (B,H) in the gates' type, new state (B,H) fp32).  new_state: where the state goes; `state` itself updates it in
-    place, None allocates.  No gradient."""
+    place, None allocates; it shares memory with no other input.  No gradient."""
     if gates.dim() != 2 or gates.shape[1] % 2:
         raise ValueError('gated_scan_step: gates must be (B, 2H), got %s' % (tuple(gates.shape),))
     _check_type('gated_scan_step', gates)

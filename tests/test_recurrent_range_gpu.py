@@ -74,3 +74,80 @@ def test_no_states_are_written_where_none_are_asked_for(T, B, H):
     a.g_h, a.g_gates, a.g_gates_st, a.g_gates_sb = g.data_ptr(), g_x.data_ptr(), 2 * B * H, 2 * H
     native.check(native.lib().mdmm_gated_scan_bwd(a, stream), 'mdmm_gated_scan_bwd')
     assert torch.equal(room, torch.full_like(room, 7.0)) and torch.equal(h, want) and torch.equal(g_x, want_g)
+
+
+def shared(H=3):
+    flat = Z(64)
+    return flat[:2 * H].view(2, H), flat[H:3 * H].view(2, H), flat[:6 * H].view(2, 3 * H), flat[20:20 + 2 * H].view(2, H)
+
+
+@pytest.mark.parametrize('call', [
+    lambda a, b, p, c: ops.gated_block_step(Z(2, 9), a, c, Z(3), new_state=a),             # the residual
+    lambda a, b, p, c: ops.gated_block_step(Z(2, 9), a, a, Z(3), new_state=a),             # the residual and the state
+    lambda a, b, p, c: ops.gated_block_step(Z(2, 9), c, a, Z(3), new_state=b),             # the state, a row further
+    lambda a, b, p, c: ops.gated_block_step(p, Z(2, 3), c, Z(3), new_state=b),             # the projection
+    lambda a, b, p, c: ops.gated_block_step(Z(2, 9), Z(2, 3), c, a[0], new_state=a),       # the weight
+    lambda a, b, p, c: ops.gated_scan_step(p[:, :6], c, new_state=a),
+    lambda a, b, p, c: ops.gated_scan_step(Z(2, 6), a, new_state=b)])
+def test_new_states_on_top_of_inputs_are_refused(call):
+    with pytest.raises(ValueError, match='shares memory'):
+        call(*shared())
+
+
+def test_new_states_beside_inputs_are_not():
+    a, b, p, c = shared()
+    for call in (lambda: ops.gated_block_step(Z(2, 9), Z(2, 3), a, Z(3), new_state=a), lambda: ops.gated_scan_step(Z(2, 6), a, new_state=c),
+                 lambda: ops.gated_scan_step(p[:, :6], c, new_state=c)):
+        with pytest.raises(native.MdmmError):          # (the device's refusal, which comes last)
+            call()
+
+
+def step_structs(B=2, H=4):
+    """A time step on made-up addresses, for refusals that come before any launch."""
+    a, p = native.GatedScan(), native.BlockNorm()
+    a.T, a.B, a.H = 1, B, H
+    a.gates, a.gates_sb, a.h0, a.h0_sb, a.h_last, a.mask, a.mask_sb = 0x10000, 3 * H, 0x20000, H, 0x30000, 0x40000, 1
+    p.rows, p.H, p.eps = B, H, 1e-6
+    p.res, p.res_st, p.out, p.out_st, p.w, p.scale, p.w_next = 0x50000, H, 0x60000, H, 0x70000, 0x80000, 0x90000
+    p.n, p.n_st, p.gate, p.gate_st = 0xa0000, H, 0x10000 + 8 * H, 3 * H
+    return a, p
+
+
+@pytest.mark.parametrize('at', ['gates', 'gates + 72', 'h0 + 16', 'h0 - 16', 'mask', 'mask - 31', 'res', 'res + 31', 'w', 'scale + 8',
+                                'w_next - 28'])
+def test_new_states_on_top_of_inputs_are_refused(at):
+    name, _, off = at.partition(' ')
+    off = int(off.replace(' ', '') or 0)
+    a, p = step_structs()
+    a.h_last = (getattr(a, name) if hasattr(a, name) else getattr(p, name)) + off
+    assert native.lib().mdmm_gated_block_step(a, p, None) == -4
+    if hasattr(a, name):
+        a.h = 0xb0000
+        assert native.lib().mdmm_gated_scan_fwd(a, None) == -4
+
+
+def test_longer_scans_in_place_are_refused():
+    a, _ = step_structs()
+    a.T, a.h, a.h_last = 2, 0xb0000, a.h0
+    assert native.lib().mdmm_gated_scan_fwd(a, None) == -4
+
+
+@gpu
+def test_steps_in_place_and_beside():
+    """In place, into another tensor and into a neighbour within one buffer: the same; on top of an input: an error."""
+    gen = torch.Generator().manual_seed(3)
+    H = 4
+    proj, res, w = make(gen, 2, 3 * H).cuda(), make(gen, 2, H).cuda(), torch.ones(H, device='cuda')
+    start = make(gen, 2, H).cuda()
+    want_out, want = ops.gated_block_step(proj, res, start, w)
+    both = torch.zeros(4, H, device='cuda')
+    for state, new in ((start.clone(), None), (both[:2].copy_(start), both[2:])):
+        out, got = ops.gated_block_step(proj, res, state, w, new_state=state if new is None else new)
+        assert torch.equal(out, want_out) and torch.equal(got, want)
+    both[:2].copy_(start)
+    for args, new in (((res, start), res), ((both[:2], both[:2]), both[:2]), ((res, both[:2]), both[1:3])):
+        with pytest.raises(native.MdmmError, match='shares memory'):
+            ops.gated_block_step(proj, args[0], args[1], w, new_state=new)
+    gates = make(gen, 2, 2 * H).cuda()
+    with pytest.raises(native.MdmmError, match='shares memory'):
+        ops.gated_scan_step(gates, start, new_state=gates.view(4, H)[1:3])
