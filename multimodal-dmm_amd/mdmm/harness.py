@@ -348,30 +348,36 @@ class FlatMuon(torch.optim.Optimizer):
         return sd
 
     def load_state_dict(self, state_dict):
-        """State of an optimizer over parameters of the same shapes and roles, copied INTO the flat buffers."""
+        """State of an optimizer over parameters of the same shapes and roles, copied INTO the flat buffers -- all of it or, where
+        it does not fit, nothing.  A learning rate that is a tensor here stays that tensor and takes the loaded value."""
         have, given = self.param_groups, state_dict['param_groups']
         if [len(g['params']) for g in given] != [len(g['params']) for g in have]:
             raise ValueError('optimizer state for groups of %s parameters, FlatMuon has %s'
                              % ([len(g['params']) for g in given], [len(g['params']) for g in have]))
-        steps = set()
+        steps, copies = set(), []
+        for mine, theirs in zip(have, given):
+            for p, i in zip(mine['params'], theirs['params']):
+                st = state_dict['state'].get(i)
+                if st is None:
+                    continue
+                if set(st) != set(self.state[p]):
+                    raise ValueError('FlatMuon: state %s for a parameter that keeps %s' % (sorted(st), sorted(self.state[p])))
+                for k, v in st.items():
+                    if k == 'step':
+                        steps.add(float(v))
+                    elif v.shape != p.shape:
+                        raise ValueError('FlatMuon: %s of shape %s for a parameter of shape %s' % (k, tuple(v.shape), tuple(p.shape)))
+                    else:
+                        copies.append((self.state[p][k], v))
+        if len(steps) > 1:
+            raise ValueError('FlatMuon keeps one step count; the loaded state holds %s' % sorted(steps))
         with torch.no_grad():
+            for to, v in copies:
+                to.copy_(v)
             for mine, theirs in zip(have, given):
-                for p, i in zip(mine['params'], theirs['params']):
-                    st = state_dict['state'].get(i)
-                    if st is None:
-                        continue
-                    if set(st) != set(self.state[p]):
-                        raise ValueError('FlatMuon: state %s for a parameter that keeps %s' % (sorted(st), sorted(self.state[p])))
-                    for k, v in st.items():
-                        if k == 'step':
-                            steps.add(float(v))
-                        else:
-                            self.state[p][k].copy_(v)
                 for k, v in theirs.items():
                     if k != 'params' and k in mine:
                         mine[k] = v
-            if len(steps) > 1:
-                raise ValueError('FlatMuon keeps one step count; the loaded state holds %s' % sorted(steps))
             if steps:
                 self.step_dev.fill_(steps.pop())
 

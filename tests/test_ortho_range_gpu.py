@@ -129,3 +129,25 @@ def test_muon_leaves_initial_states_to_adam(cell):
     chosen = {id(p) for p in opt.param_groups[0]['params']}
     named = {k: id(p) in chosen for k, p in m.named_parameters()}
     assert all(not named['h0.' + k] for k in 'ab') and {named[k] for k in named if k.endswith('weight')} == {True}
+
+
+def two_params(cols=3):
+    return GradBucket([torch.nn.Parameter(torch.ones(s, device='cuda')) for s in ((5, cols), (7,))])
+
+
+@gpu
+def test_muon_loads_all_of_a_state_or_nothing():
+    """A momentum of another shape (one that would broadcast) is refused, and nothing of that state is taken."""
+    a, b = two_params(3), two_params(1)
+    one, other = FlatMuon(a, matrices=[a.params[0]], lr=0.5), FlatMuon(b, matrices=[b.params[0]], lr=0.25)
+    for opt, bucket in ((one, a), (other, b)):
+        bucket.flat.fill_(2.0)
+        opt.step()
+    before = one.state_dict()
+    with pytest.raises(ValueError, match='shape'):
+        one.load_state_dict(other.state_dict())
+    after = one.state_dict()
+    assert after['param_groups'] == before['param_groups']
+    for i, st in before['state'].items():
+        for k, v in st.items():
+            assert torch.equal(v, after['state'][i][k])
