@@ -287,6 +287,8 @@ class FlatMuon(torch.optim.Optimizer):
             if not lr.is_cuda or lr.numel() != 1:
                 raise RuntimeError('FlatMuon: a tensor learning rate must be one element on the GPU (the kernel reads it there)')
             self._lr_dev[which:which + 1].copy_(lr.detach().reshape(1))
+            if torch.cuda.is_current_stream_capturing():
+                self._captured[which] = lr                      # (what the captured copy reads from here on)
             return self._lr_dev[which:which + 1], 0.0
         if torch.cuda.is_current_stream_capturing():
             self._captured[which] = float(lr)
@@ -333,10 +335,16 @@ class FlatMuon(torch.optim.Optimizer):
         return loss
 
     def check_replay(self):
-        """Called by GraphedElboStep before every replay: a float learning rate was frozen into the captured launches."""
+        """Called by GraphedElboStep before every replay: a float learning rate was frozen into the captured launches, of a
+        tensor its address."""
         for which, group in ((0, self._muon), (1, self._adam)):
             was = self._captured[which]
-            if group is not None and was is not None and not isinstance(group['lr'], torch.Tensor) and float(group['lr']) != was:
+            if group is None or was is None or group['lr'] is was:
+                continue
+            if isinstance(was, torch.Tensor) or isinstance(group['lr'], torch.Tensor):
+                raise RuntimeError('FlatMuon: lr was replaced by another tensor after the step was captured -- change the value '
+                                   'of the one that it was captured with')
+            if float(group['lr']) != was:
                 raise RuntimeError('FlatMuon: lr changed from %g to %g after the step was captured -- a float lr is a constant '
                                    'of the graph; pass a one-element CUDA tensor as lr to change it between replays'
                                    % (was, float(group['lr'])))
@@ -376,7 +384,9 @@ class FlatMuon(torch.optim.Optimizer):
                 to.copy_(v)
             for mine, theirs in zip(have, given):
                 for k, v in theirs.items():
-                    if k != 'params' and k in mine:
+                    if k == 'lr' and isinstance(mine[k], torch.Tensor):
+                        mine[k].fill_(float(v))
+                    elif k != 'params' and k in mine:
                         mine[k] = v
             if steps:
                 self.step_dev.fill_(steps.pop())

@@ -151,3 +151,27 @@ def test_muon_loads_all_of_a_state_or_nothing():
     for i, st in before['state'].items():
         for k, v in st.items():
             assert torch.equal(v, after['state'][i][k])
+
+
+@gpu
+def test_muon_learning_rate_tensors():
+    """A loaded learning rate goes into the tensor that a captured step reads; another tensor in its place is noticed before a
+    replay."""
+    lr, bucket = torch.tensor([0.02], device='cuda'), two_params()
+    opt = FlatMuon(bucket, lr=lr, adam_lr=0.5)
+    bucket.flat.fill_(1.0)
+    opt.step()
+    sd = opt.state_dict()
+    sd['param_groups'][0] = dict(sd['param_groups'][0], lr=torch.tensor([0.125]))
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        opt.step()
+    opt.check_replay()
+    opt.load_state_dict(sd)
+    assert opt.param_groups[0]['lr'] is lr and float(lr) == 0.125
+    opt.check_replay()
+    for group, new in ((0, torch.tensor([0.02], device='cuda')), (0, 0.02), (1, torch.tensor([0.5], device='cuda')), (1, 0.25)):
+        old, opt.param_groups[group]['lr'] = opt.param_groups[group]['lr'], new
+        with pytest.raises(RuntimeError):
+            opt.check_replay()
+        opt.param_groups[group]['lr'] = old
+    opt.check_replay()
