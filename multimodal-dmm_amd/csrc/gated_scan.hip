@@ -468,10 +468,18 @@ Plan plan(const mdmm_gated_scan_t* a) {
   p.waves = (int)(a->T <= ONE ? waves : KEEP / S);
   p.tile = p.waves * S;
   p.tiles = (a->T + p.tile - 1) / p.tile;
-  // fewer than two workgroups a CU: time over workgroups too, two a CU (20011 x 3 x 200 in fp32: 133 us for the four launches
-  // of a training pass, with four a CU 142 -- every split reads through all those before it)
+  // Few workgroups over a long time: time over workgroups too, two a CU (20011 x 3 x 200 in fp32: 130 us for the four launches
+  // of a training pass, with four a CU 140 -- every split reads through all those before it).  The launch that composes the
+  // splits costs 4 to 5 us and reads two of the tensors again, so it pays where a split leaves out most of the tiles and the
+  // workgroups are far from filling the chip.  Training passes in us, one workgroup over all of time and split:
+  //   up to 64 workgroups from 4 tiles on   (1 x 4: 3 tiles 20 and 21, 4 tiles 25 and 22; 64 workgroups, 4 tiles 27 and 24)
+  //   up to 128 from 8 tiles on             (80 workgroups, 4 tiles 28 and 29; 128: 6 tiles 39 and 43, 8 tiles 50 and 48)
+  //   beyond, from 12 on and with narrow types, up to 170 workgroups (bf16, fp32 states) or 192 (bf16): 160 workgroups, 32 tiles
+  //   163 and 122 in bf16, 265 and 262 with its norm in fp32, 187 and 197 all in fp32; 192, 63 tiles 311 and 289, 585 and 642,
+  //   374 and 550; 256 workgroups, 63 tiles 313 and 347 in bf16
   int64_t splits = 1;
-  if (p.wgs < 512 && p.tiles > 1) {
+  const int64_t from = p.wgs <= 64 ? 4 : p.wgs <= 128 ? 8 : 12, most = a->h_bf16 ? 192 : a->gates_bf16 ? 170 : 128;
+  if (p.wgs <= most && p.tiles >= from) {
     splits = (512 + p.wgs - 1) / p.wgs;
     if (splits > p.tiles) splits = p.tiles;
     if (splits > 512) splits = 512;
