@@ -429,3 +429,26 @@ def test_eager_backward_behind_a_capture():
     with torch.no_grad(), torch.cuda.graph(graph):
         rnn(x, h0, None, False, torch.bfloat16)
     assert torch.equal(torch.autograd.grad(y, xd, g)[0], want)
+
+
+@gpu
+@pytest.mark.parametrize('skip', [True, False])
+def test_fused_step_with_bf16_operands(skip):
+    """MultiDKS.step at a width whose products take bf16 operands (512 rows), the left-out modality's rows too few for them,
+    against one forward per pass, which takes them for both: three roundings of 2^-8 a layer on each element of two layers'
+    states, 2.4e-2 of a gradient's norm (test_bf16_operands), and on the loss, an average over them, 1e-3."""
+    dev = torch.device('cuda:0')
+    torch.manual_seed(6)
+    m = models.MultiDKS(['a', 'b'], [3, 4], h_dim=256, z_dim=256, rnn_layers=2, rnn_skip=skip, device=dev, rnn_cell='linear')
+    m.sweep_dtype = torch.bfloat16
+    x, mask, lengths = batch(T=16, lengths=(16,) * 20 + (9,) * 12)
+    found = []
+    for step in (m.step, lambda *a, **k: MultiDGTS.step(m, *a, **k)):
+        m.zero_grad()
+        loss = step(x, mask, 0.7, {'a': 1.0, 'b': 0.5}, lengths=lengths, sample=False)
+        loss.backward()
+        found.append((float(loss), {k: p.grad.clone() for k, p in m.named_parameters()}))
+    assert abs(found[0][0] - found[1][0]) <= 1e-3 * abs(found[1][0])
+    for k in found[0][1]:
+        a, b = found[0][1][k], found[1][1][k]
+        assert float((a - b).norm()) <= 2.4e-2 * float(b.norm()) + 1e-6, k

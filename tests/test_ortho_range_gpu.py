@@ -175,3 +175,12 @@ def test_muon_learning_rate_tensors():
             opt.check_replay()
         opt.param_groups[group]['lr'] = old
     opt.check_replay()
+
+
+@gpu
+def test_large_class_with_slices():
+    """A matrix whose P X takes large tiles and whose A is summed in slices."""
+    gen = torch.Generator().manual_seed(13)
+    m = (0.01 * torch.randn(512, 8192, generator=gen)).cuda()
+    check(m, ops.orthogonalise([m])[0])
+    check(m.t(), ops.orthogonalise([m.t().contiguous()])[0])

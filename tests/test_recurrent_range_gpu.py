@@ -151,3 +151,21 @@ def test_steps_in_place_and_beside():
     gates = make(gen, 2, 2 * H).cuda()
     with pytest.raises(native.MdmmError, match='shares memory'):
         ops.gated_scan_step(gates, start, new_state=gates.view(4, H)[1:3])
+
+
+@gpu
+@pytest.mark.parametrize('T,B,H', [(101, 64, 1024), (301, 8, 2048), (333, 40, 515)])
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('reverse', [False, True])
+def test_scan_over_several_tiles(T, B, H, dtype, reverse):
+    """Workgroups that walk over several tiles of time, alone over it and with it split (a ragged last split too)."""
+    gen = torch.Generator().manual_seed(T + B)
+    gates = torch.cat([make(gen, T, B, H, std=1.5, mean=2.0), make(gen, T, B, H)], -1).to(dtype)
+    m = torch.rand(T, B, generator=gen) > 0.2
+    h0, g_h, g_last = make(gen, H), make(gen, T, B, H, dtype=dtype), make(gen, B, H)
+    want = scan_ref(gates, h0, m, reverse, g_h, g_last)
+    x, hd = gates.cuda().requires_grad_(True), h0.cuda().requires_grad_(True)
+    h, last = ops.gated_scan(x, hd, mask=m.cuda(), reverse=reverse)
+    grads = torch.autograd.grad([h, last], [x, hd], [g_h.cuda(), g_last.cuda()])
+    for got, name in ((h, 'h'), (last, 'last'), (grads[0], 'gates'), (grads[1], 'h0')):
+        close(got, want[name], name)
