@@ -195,7 +195,8 @@ __device__ __forceinline__ float src_at(const mdmm_ortho_t& p, const mdmm_ortho_
 }
 
 // momentum, and the sum of squares in SUMS pieces (in 64 bits: an error of the norm is a scale of X and grows like one).
-// LONG: eight loads of a thread on their way at once (two of 2048 x 2048 25 -> 12 us; eleven small matrices 6.4 -> 10)
+// LONG: eight loads of a thread on their way at once, where most elements lie in rows that have them (one 2048 x 2048 20 -> 9 us,
+// 1000 x 4096 21 -> 9; four 1000 x 1000 8 -> 14, eleven small matrices 6.4 -> 10)
 template <bool LONG> __global__ __launch_bounds__(NT) void ortho_sums_kernel(Call call, Call* keep) {
   const mdmm_ortho_t& p = call.p;
   const int k = blockIdx.y;
@@ -660,15 +661,25 @@ int check(const mdmm_ortho_t* a) {
 constexpr int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 constexpr int64_t KEPT = up(sizeof(Call) + sizeof(Bounds), 256);         // of a size class in the workspace
 
-// A call's larger matrices (more than 384 rows) take 128 x 128 tiles in P X, where those are 256 or more, one for each CU: the
-// larger tile halves what a product loads.  Fewer leave CUs idle and the others alone with one workgroup, whose loads and
-// products then hardly overlap.  Five steps with it and with the small tile: 1000 x 4096 (256 tiles) 482 us and 513, one
-// 2048 x 2048 (256) 892 and 945, two (512) 1470 and 1676; with A and P on large tiles too, two of 2048 x 2048 1553, one 971, one
-// 400 x 400 373 where small ones take 141
+// A call's larger matrices (more than 384 rows) can take 128 x 128 tiles in P X: they halve what a product loads, but both
+// sides are then padded to 128 for all three products, and a CU's two places have to be filled.  Five steps with them and with
+// small tiles:
+//   full rounds of the 256 CUs: one 2048 x 2048 (256 tiles) 902 us and 957, two (512) 1462 and 1687, 1000 x 4096 (256) 479 and
+//   514, sixteen 1024 x 1024 (1024) 1667 and 1806; half a round more: two 768 x 4096 (384) 528 and 552, eleven 768 x 768 (396)
+//   620 and 637, ten 1024 x 1024 (640) 1146 and 1130; less of it: eleven 640 x 640 (275) 495 and 463, two 1500 x 1500 (288) 831
+//   and 798, nine 1024 x 1024 (576) 1064 and 1022
+//   padding: four 640 x 2060 (1.03 of the small tiles' work) 483 and 492, two 900 x 2001 (1.15) 472 and 434, four 520 x 2060
+//   (1.28) 469 and 413, eleven 520 x 520 (1.37) 485 and 333, sixteen 390 x 390 (1.49) 368 and 290
+// So they are taken by matrices that they pad by no more than a twentieth, where those have a round of tiles and the last
+// round is at least half full.  A and P take small ones always (two of 2048 x 2048 on large ones 1553, one 971).
 int64_t large_tiles(const mdmm_ortho_item_t& t) {
   const int64_t n = t.rows < t.cols ? t.rows : t.cols, m = t.rows < t.cols ? t.cols : t.rows;
-  return n > 384 ? up(n, Large::BM) / Large::BM * (up(m, Large::BN) / Large::BN) : 0;
+  if (n <= 384) return 0;
+  auto work = [&](int64_t pad) { return up(n, pad) * up(n, pad) * (3 * up(m, pad) + up(n, pad)); };
+  if (20 * work(Large::BM) > 21 * work(Small::BM)) return 0;
+  return up(n, Large::BM) / Large::BM * (up(m, Large::BN) / Large::BN);
 }
+bool fills(int64_t tiles) { return tiles >= 256 && (tiles - 1) % 256 >= 127; }
 
 // the workspace: fills both size classes' lists (base NULL: sizes only), returns the bytes used
 int64_t lay_out(const mdmm_ortho_t* a, Items (&q)[2], mdmm_ortho_item_t (*items)[MDMM_ORTHO_MAX] = nullptr) {
@@ -680,7 +691,7 @@ int64_t lay_out(const mdmm_ortho_t* a, Items (&q)[2], mdmm_ortho_item_t (*items)
   for (int i = 0; i < a->n; ++i) total += large_tiles(a->item[i]);
   for (int i = 0; i < a->n; ++i) {
     const mdmm_ortho_item_t& t = a->item[i];
-    const bool big = total >= 256 && large_tiles(t) > 0;
+    const bool big = fills(total) && large_tiles(t) > 0;
     Items& l = q[big];
     if (items) items[big][l.n] = t;
     Item& w = l.it[l.n++];
@@ -752,7 +763,14 @@ template <class C, class D> void launch(const mdmm_ortho_t* a, const Items& item
   int64_t fold = 0;
   for (int i = 0; i < q.n; ++i)
     if (q.it[i].splits > 1 && (int64_t)q.it[i].n * q.it[i].n > fold) fold = (int64_t)q.it[i].n * q.it[i].n;
-  hipLaunchKernelGGL((ortho_sums_kernel<D::BM == Large::BM>), dim3(SUMS, q.n), dim3(NT), 0, s, c, keep);
+  int64_t all = 0, wide = 0;               // elements, those in rows of eight workgroups' widths
+  for (int i = 0; i < q.n; ++i) {
+    const int64_t size = (int64_t)mats[i].rows * mats[i].cols;
+    all += size;
+    if (mats[i].cols >= 8 * NT) wide += size;
+  }
+  if (2 * wide > all) hipLaunchKernelGGL(ortho_sums_kernel<true>, dim3(SUMS, q.n), dim3(NT), 0, s, c, keep);
+  else hipLaunchKernelGGL(ortho_sums_kernel<false>, dim3(SUMS, q.n), dim3(NT), 0, s, c, keep);
   hipLaunchKernelGGL(ortho_pack_kernel, dim3(packs), dim3(NT), 0, s, keep);
   if (a->steps == 0) hipLaunchKernelGGL(ortho_copy_kernel, dim3(256, q.n), dim3(NT), 0, s, keep);
   for (int k = 0; k < a->steps; ++k) {

@@ -184,3 +184,13 @@ def test_large_class_with_slices():
     m = (0.01 * torch.randn(512, 8192, generator=gen)).cuda()
     check(m, ops.orthogonalise([m])[0])
     check(m.t(), ops.orthogonalise([m.t().contiguous()])[0])
+
+
+@gpu
+def test_odd_sizes_on_large_tiles():
+    """Both orientations in the large class, beside matrices that its padding or their size keep out of it."""
+    gen = torch.Generator().manual_seed(14)
+    mats = [(0.01 * torch.randn(s, generator=gen)).cuda() for s in ((1100, 1500), (20, 30), (1500, 1101), (900, 2001), (1099, 1497),
+                                                                   (1500, 1100))]
+    for m, o in zip(mats, ops.orthogonalise(mats)):
+        check(m, o)
