@@ -106,9 +106,9 @@ __device__ __forceinline__ double rsqrt_(double v) { return 1.0 / sqrt(v); }
 // act = silu(g) = g a and slope = silu'(g) = a (1 + g k), a = sigmoid(g), k = 1 - a formed apart: as a difference from 1 it
 // would leave the slope of large gates, which is 1, off by 6e-8 |g|
 __device__ __forceinline__ void gate_(float g, float& act, float& slope) {
-  const Gate y(g);
-  act = g * y.a;
-  slope = fmaf(act, y.k, y.a);
+  const float e = exp_neg(g), a = __builtin_amdgcn_rcpf(1.0f + e);
+  act = g * a;
+  slope = fmaf(act, fminf(e * a, 1.0f), a);            // (e infinite, a 0: k is 1)
 }
 __device__ __forceinline__ void gate_(double g, double& act, double& slope) {
   const double a = 1.0 / (1.0 + exp(-g));

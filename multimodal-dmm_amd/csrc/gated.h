@@ -29,8 +29,16 @@ struct Gate {
   }
 };
 
-// sigmoid alone, to the same accuracy wherever x lies (1 / (1 + 2^(-x log2(e))) is off by 6e-8 (1 + |x|) of itself)
-__device__ __forceinline__ float sigmoid_(float x) { return Gate(x).a; }
+// exp(-x) as 2^y (1 + d ln(2)) with Gate's y and d, of any size (infinite from x = -89 on); an infinite x, which has no d, as 200
+__device__ __forceinline__ float exp_neg(float x) {
+  x = __builtin_amdgcn_fmed3f(x, -200.0f, 200.0f);
+  const float y = x * -1.44269504088896341f;
+  const float d = fmaf(x, -1.44269504088896341f, -y);
+  return __builtin_amdgcn_exp2f(y) * fmaf(x, -1.92596299e-8f * 0.69314718055994531f, fmaf(d, 0.69314718055994531f, 1.0f));
+}
+
+// sigmoid alone, accurate wherever x lies (1 / (1 + 2^(-x log2(e))) is off by 6e-8 (1 + |x|) of itself)
+__device__ __forceinline__ float sigmoid_(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_neg(x)); }
 
 // Host side.  The bytes that `rows` rows of n elements of `size` bytes take, `step` elements apart; whether two regions meet
 struct Region { const char* at; int64_t bytes; };
