@@ -406,7 +406,7 @@ __global__ __launch_bounds__(64 * WMAX) void scan_bwd_kernel(mdmm_gated_scan_t p
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float G = gv[s][e] + d[e];
-        dc[e] = G * k[s][e];
+        dc[e] = on >> s & 1 ? G * k[s][e] : 0.0f;          // (whatever G is)
         df[e] = dc[e] * a[s][e] * cv[s][e];
         d[e] = a[s][e] * G;
       }

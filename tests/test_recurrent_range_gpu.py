@@ -169,3 +169,23 @@ def test_scan_over_several_tiles(T, B, H, dtype, reverse):
     grads = torch.autograd.grad([h, last], [x, hd], [g_h.cuda(), g_last.cuda()])
     for got, name in ((h, 'h'), (last, 'last'), (grads[0], 'gates'), (grads[1], 'h0')):
         close(got, want[name], name)
+
+
+@gpu
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+def test_masked_steps_get_zero_gradients_whatever_comes_in(bad):
+    """The gradient of a state that a masked step left as it is belongs to the states before it: f and c of that step get
+    zeros, also where it is not finite."""
+    gen = torch.Generator().manual_seed(6)
+    T, B, H = 70, 2, 6
+    x, g = make(gen, T, B, 2 * H).cuda().requires_grad_(True), make(gen, T, B, H).cuda()
+    mask = torch.ones(T, B, dtype=torch.bool, device='cuda')
+    mask[:3, 0] = False
+    mask[40, 1] = False
+    h, _ = ops.gated_scan(x, mask=mask)
+    want = torch.autograd.grad(h, x, g, retain_graph=True)[0]
+    g[2, 0] = bad                          # (no step of this sequence lies before it)
+    g[40, 1] = bad
+    got = torch.autograd.grad(h, x, g)[0]
+    assert torch.equal(got[:, 0], want[:, 0]) and not got[:3, 0].any()
+    assert torch.equal(got[40:, 1], want[40:, 1]) and not got[40, 1].any() and not torch.isfinite(got[:40, 1]).any()
