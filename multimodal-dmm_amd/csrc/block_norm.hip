@@ -7,8 +7,9 @@
 // sum); a longer one a workgroup's, 4 columns a thread (8 from 2049 on), whose waves meet in LDS once a sum.  Rows that are
 // not aligned to 4 elements take columns one by one.  The three column sums of the backward pass stay in a thread over all
 // of its rows and leave as one slab a workgroup; norm_fold_kernel adds the slabs up in a fixed order, without atomics.
-// 65536 x 1280 in bf16: forward 159 us (840 MB, 5.3 TB/s, a copy's rate), backward 312 (1.34 GB, 4.3 TB/s: three sums a
-// row between its loads and its last store), fold 7.  A row or two: the launch, 4 to 5 us.
+// 65536 x 1280 in bf16: forward 167 us (840 MB, 5.0 TB/s; a copy's 5.35 but for the gate's exponential), backward 300 (1.34 GB,
+// 4.5 TB/s: three sums a row between its loads and its last store), fold 8; in fp32 forward 331, both 877.  Eight rows: 2.6 us,
+// a launch (1.8 for one that fills a word).
 #include <type_traits>
 #include "gated.h"
 

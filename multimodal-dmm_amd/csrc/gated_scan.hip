@@ -10,8 +10,8 @@
 // tile's are used up.  Where the channels alone do not fill the chip, time is also split over workgroups: a first launch
 // composes each split (reading f, c once more; backward f, g), the second starts each split from the splits in front of it.
 // Nothing waits for another workgroup, and no sum is formed by atomics: results do not depend on the schedule.
-// 512 x 256 x 512 in bf16: forward 96 us (403 MB, 4.2 TB/s), backward 153 (672 MB, 4.4 TB/s).  20011 x 3 x 200 in fp32, split:
-// 22 + 32 forward, 22 + 52 backward.
+// 512 x 256 x 512 in bf16: forward 97 us (403 MB, 4.2 TB/s), backward 155 (672 MB, 4.3 TB/s).  20011 x 3 x 200 in fp32, split:
+// 22 + 32 forward, 22 + 51 backward.  One step of 16 x 256: 4.7 us in fp32, 5.0 in bf16.
 #include "gated.h"
 
 namespace mdmm {
@@ -456,14 +456,15 @@ Plan plan(const mdmm_gated_scan_t* a) {
            a->g_gates_st % v == 0 && a->g_gates_sb % v == 0 && ((uintptr_t)a->states & m4) == 0 &&
            ((uintptr_t)a->h_last & m4) == 0 && ((uintptr_t)a->g_h0 & m4) == 0;
   };
-  // (four channels a thread spill in the forward pass: 123 us at 512 x 256 x 512 in bf16, with two 94)
+  // (four channels a thread spill in the forward pass: 123 us at 512 x 256 x 512 in bf16, with two 97)
   p.vec = fits(2) ? 2 : 1;
   auto reach = [&](int64_t sb) { return (sb < 0 ? 0x80000000ll : (a->B - 1) * sb + 2 * (int64_t)a->H) * 4 < 0x7fffffffll; };
   p.buf = reach(a->gates_sb) && reach(a->g_gates_sb) && reach(a->H) && reach(a->mask_sb);
   p.chunks = a->H / p.vec;
   p.wgs = (p.chunks * a->B + 63) / 64;
   // up to ONE steps one tile; beyond, tiles of 4 waves (at 512 x 256 x 512 in bf16 94 us forward and 155 backward, of 8
-  // waves 98 and 179: of the backward pass three workgroups of 4 waves fit a CU's registers, but one of 8)
+  // waves 98 and 179, before the masked steps' zeros cost the backward pass 2: three workgroups of 4 waves fit a CU's registers
+  // there, but one of 8)
   const int64_t waves = (a->T + S - 1) / S;
   p.waves = (int)(a->T <= ONE ? waves : KEEP / S);
   p.tile = p.waves * S;

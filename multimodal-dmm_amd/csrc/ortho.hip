@@ -18,11 +18,12 @@
 // two 2048 x 2048 products 142 us); fp32 rows take the same bytes.  Tiles come straight into LDS, a step or more ahead, chunks
 // of 16 bytes swapped within a row so that the matrix instruction's reads meet all banks; neighbouring tiles go to one XCD,
 // whose L2 then holds their rows.  A and P are symmetric: tiles at and above the diagonal only, stored twice.  Sizes are rounded up to whole tiles with
-// zeros, which every product keeps.  All matrices of a call share each launch.
+// zeros, which every product keeps.  All matrices of a size class share each launch: with large and small tiles in one call
+// there are two chains of launches, one behind the other.
 //
-// Large matrices are bound by feeding the matrix instruction: P X of two 2048 x 2048 takes 115 us (900 TFLOP/s of fp16, the
+// Large matrices are bound by feeding the matrix instruction: P X of two 2048 x 2048 takes 118 us (880 TFLOP/s of fp16, the
 // library's own fp16 product of that size 640), without its loads 78, without its matrix instructions 76.  Small ones are
-// bound by the seventeen launches of five steps, 6 to 11 us each.
+// bound by the seventeen launches of five steps, 7 to 11 us each.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -77,8 +78,8 @@ struct Items {
   int32_t first[LISTS][MDMM_ORTHO_MAX + 1];       // first tile of each matrix in a launch (past the last one: INT32_MAX)
   int32_t n, reserved;
 };
-// What the launches of one size class share (p.item: that class's matrices alone, in q.it's order).  The first launch takes it as its argument and leaves it in the workspace; the
-// others read it there: arguments live in host memory, where each of the dependent loads that find a tile's matrix would
+// What the launches of one size class share (p.item: that class's matrices alone, in q.it's order).  The first launch takes it
+// as its argument and leaves it in the workspace; the others read it there: arguments live in host memory, where each of the dependent loads that find a tile's matrix would
 // wait for the bus
 // |x (ca + cb x^2 + cc x^4)| at its extrema, value[i] at x^2 = at[i] (none: infinity), and q, with which |cb| + |cc| / 4 stays
 // below P's 15.5: what a step needs to bound its result and to scale P

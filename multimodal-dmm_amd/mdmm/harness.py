@@ -212,7 +212,7 @@ class FlatMuon(torch.optim.Optimizer):
         O = ops.orthogonalise(U, ns_steps)
         W <- (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) O
 
-    all matrices sharing the launches (csrc/ortho.hip: momentum in the first, the update in the last).  The other parameters
+    24 to a call and those of a size class sharing its launches (csrc/ortho.hip: momentum in the first, the update in the last).  The other parameters
     take mdmm_adam_flat's update with adam_lr, betas, eps, adam_weight_decay, one launch for all of them.
 
     matrices: the parameters to treat as matrices; by default every one of two or more dimensions whose rows and columns both

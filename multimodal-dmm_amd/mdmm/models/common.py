@@ -106,7 +106,8 @@ class GatedLinearRNN(nn.Module):
                     x = x + scale * silu(g) * rms_norm(h, post);  n = rms_norm(x, norms[next])
 
     Runs on ops.rms_norm and ops.gated_block (GPU only).  forward(x (T,B,in_dim), h0 (num_layers, h_dim), mask (T,B) or None,
-    reverse, precision) -> (T,B,h_dim) in fp32; a step whose mask is 0 leaves every layer's state as it is.  `step` takes one
+    reverse, precision) -> (T,B,h_dim) in fp32; a step whose mask is 0 leaves every layer's state as it is, but still has an
+    output of its own, through the residual path of whatever x holds there (a GRU's is its old state).  `step` takes one
     time step of streams whose states the caller keeps.  Forget biases start between 1 and 4: states that reach over 4 to 50
     steps."""
 

@@ -43,7 +43,9 @@ class MultiDKS(MultiDGTS):
                  rnn_dir='bwd', rnn_skip=True, rnn_layers=1, rnn_bias=True,
                  device=torch.device('cuda:0'), rnn_cell='gru'):
         """Arguments as in the reference (dks.py:27-67), and rnn_cell: 'gru', or 'linear' for inference RNNs of gated
-        linear recurrences (common.GatedLinearRNN), parallel in time."""
+        linear recurrences (common.GatedLinearRNN), parallel in time.  With rnn_skip a missing step leaves both cells' states
+        alone; the GRU's output there is the old state, the linear cell's also carries the placeholder's features (the
+        residual path), so a combiner sees them."""
         super().__init__()
         if rnn_cell not in ('gru', 'linear'):
             raise ValueError('MultiDKS: rnn_cell must be "gru" or "linear", got %r' % (rnn_cell,))
@@ -271,7 +273,8 @@ class MultiDKS(MultiDGTS):
                     gone = torch.zeros(t_max, b_dim, device=dev, dtype=torch.bool)
                     if self.rnn_skip and isinstance(self.rnn[m], nn.GRU):   # never updated: the top layer's initial state
                         h = self.h0[m][-1].reshape(1, 1, -1).expand(t_max, b_dim, -1)
-                    elif self.rnn_skip:     # (states never updated, one row of features: one row for every step)
+                    elif self.rnn_skip:     # (states never updated, one row of features: one row for every step, with fp32
+                                            #  operands where those of a whole batch are bf16)
                         h = self._rnn(m, feat[:1, :1].contiguous(), gone[:1, :1]).expand(t_max, b_dim, -1)
                     else:                   # zero-masked inputs: every sequence sees the same features
                         h = self._rnn(m, feat[:, :1].contiguous(), gone[:, :1]).expand(-1, b_dim, -1)

@@ -431,7 +431,8 @@ def _check_width(name, H):
 
 
 def rms_norm(x, weight, eps=1e-6, dtype=None):
-    """x rsqrt(mean(x^2) + eps) weight over the last dimension: the norm before a block.  x fp32 or bf16, weight (H,) fp32;
+    """x rsqrt(mean(x^2) + eps) weight over the last dimension: the norm before a block.  x fp32 or bf16 (below 1e19, whose
+    squares fp32 holds), weight (H,) fp32;
     dtype: the output's type (x's by default; bf16 from fp32 is the other one there is).  Differentiable, once."""
     if x.dim() < 1:
         raise ValueError('rms_norm: a tensor with rows, got a scalar')
