@@ -78,15 +78,15 @@ struct Items {
   int32_t first[LISTS][MDMM_ORTHO_MAX + 1];       // first tile of each matrix in a launch (past the last one: INT32_MAX)
   int32_t n, reserved;
 };
-// What the launches of one size class share (p.item: that class's matrices alone, in q.it's order).  The first launch takes it
-// as its argument and leaves it in the workspace; the others read it there: arguments live in host memory, where each of the dependent loads that find a tile's matrix would
-// wait for the bus
 // |x (ca + cb x^2 + cc x^4)| at its extrema, value[i] at x^2 = at[i] (none: infinity), and q, with which |cb| + |cc| / 4 stays
 // below P's 15.5: what a step needs to bound its result and to scale P
 struct Range {
   float at[2], value[2];
   int32_t q;
 };
+// What the launches of one size class share (p.item: that class's matrices alone, in q.it's order).  The first launch takes it
+// as its argument and leaves it in the workspace; the others read it there: arguments live in host memory, where each of the
+// dependent loads that find a tile's matrix would wait for the bus
 struct Call {
   mdmm_ortho_t p;
   Items q;

@@ -212,15 +212,16 @@ class FlatMuon(torch.optim.Optimizer):
         O = ops.orthogonalise(U, ns_steps)
         W <- (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) O
 
-    24 to a call and those of a size class sharing its launches (csrc/ortho.hip: momentum in the first, the update in the last).  The other parameters
-    take mdmm_adam_flat's update with adam_lr, betas, eps, adam_weight_decay, one launch for all of them.
+    24 to a call and those of a size class sharing its launches (csrc/ortho.hip: momentum in the first, the update in the
+    last).  The other parameters take mdmm_adam_flat's update with adam_lr, betas, eps, adam_weight_decay, one launch for all
+    of them.
 
     matrices: the parameters to treat as matrices; by default every one of two or more dimensions whose rows and columns both
     exceed one and do not exceed 65536, but for (layers, 1, width) tensors: those are the models' initial RNN states (and
-    the kernels of 1-D convolutions with a single channel on one side), rows that no product mixes.  (Embeddings and output layers are better left to Adam: pass the rest.)  lr and
-    adam_lr are the 'lr' of the two parameter groups (0: matrices, 1: the others); as a one-element CUDA tensor either may change between the replays of
-    a captured step, a float is a constant of the capture.  `step()` needs every gradient to be the bucket's view, as
-    FlatAdam's.  state_dict(): {'momentum_buffer'} per matrix, {'step', 'exp_avg', 'exp_avg_sq'} per other parameter."""
+    the kernels of 1-D convolutions with a single channel on one side), rows that no product mixes.  (Embeddings and output
+    layers are better left to Adam: pass the rest.)  lr and adam_lr are the 'lr' of the two parameter groups (0: matrices, 1:
+    the others); as a one-element CUDA tensor either may change between the replays of a captured step, a float is a constant
+    of the capture.  `step()` needs every gradient to be the bucket's view, as FlatAdam's.  state_dict(): {'momentum_buffer'} per matrix, {'step', 'exp_avg', 'exp_avg_sq'} per other parameter."""
 
     def __init__(self, bucket, lr=0.02, momentum=0.95, nesterov=True, ns_steps=5, weight_decay=0.0, matrices=None,
                  adam_lr=1e-3, betas=(0.9, 0.999), eps=1e-8, adam_weight_decay=0.0):
